@@ -42,6 +42,12 @@ extern "C" {
 
 #define PDEKAN_ACT_IDENTITY 0
 #define PDEKAN_ACT_SILU 1
+#define PDEKAN_ACT_TANH 2          /* pdekan_group_norm_* only */
+
+/* Element types of the tensors of pdekan_group_norm_* (every other tensor is fp32). */
+#define PDEKAN_DTYPE_FP 0          /* fp32 */
+#define PDEKAN_DTYPE_BF 1          /* bfloat16 */
+#define PDEKAN_DTYPE_HALF 2        /* fp16 */
 
 /* Parameters and buffers of one KANLinear (kan.py:27-45):
  *   grid [in][grid_size+2*spline_order+1], base_weight [out][in],
@@ -179,6 +185,37 @@ int pdekan_deeponet_step(const PdekanNet* nets, const float* u1, const float* u2
                          const float* x_pde, const float* t_pde, const float* out_pde, int64_t n_pde,
                          float sigma, float rate, float bc_weight, float* losses, float* s_pred, float* res_out,
                          void* ws, size_t ws_bytes, void* stream);
+
+/* Group norm followed by an activation, channels last - what keeps the values of a deep KAN stack on the range of the
+ * next layer's knots (no counterpart in the reference).  x [n][s][channels] of `dtype`; the statistics of a group run
+ * over the s positions and the channels / groups channels of one sample:
+ *   z = (x - mean) / sqrt(var + eps) (biased variance),  y = f(weight[c] z + bias[c])
+ * weight and bias are fp32 [channels] or NULL (1 and 0).  Sums and statistics are fp32 whatever dtype; y is rounded
+ * once.  `stats` [n][groups][2] (mean, 1 / sqrt(var + eps)) is written by the forward where
+ * pdekan_group_norm_stats_floats is not 0 (NULL: not wanted) and read by the backward.  Backward: gx, and gweight / gbias
+ * (fp32, overwritten) summed over all samples in a fixed order; gweight and gbias may be NULL.
+ * channels <= 8192.  ws: pdekan_group_norm_workspace_bytes (0 for some shapes: ws may be NULL then); 256-byte aligned.
+ * A NaN or infinity stays within its group of its sample, and in gweight / gbias within the channels of its group. */
+size_t pdekan_group_norm_workspace_bytes(int64_t n, int64_t s, int32_t channels, int32_t groups, int32_t backward);
+int64_t pdekan_group_norm_stats_floats(int64_t n, int64_t s, int32_t channels, int32_t groups);
+int pdekan_group_norm_forward(const void* x, int32_t dtype, int64_t n, int64_t s, int32_t channels, int32_t groups,
+                              const float* weight, const float* bias, float eps, int32_t act_kind, void* y, float* stats,
+                              void* ws, size_t ws_bytes, void* stream);
+int pdekan_group_norm_backward(const void* x, const void* gy, int32_t dtype, int64_t n, int64_t s, int32_t channels,
+                               int32_t groups, const float* weight, const float* bias, float eps, int32_t act_kind,
+                               const float* stats, void* gx, float* gweight, float* gbias, void* ws, size_t ws_bytes,
+                               void* stream);
+
+/* The same per point on jets x_jet [n][channels][J] (fp32, 16-byte aligned; (n_dir, n_second) = (2, 1) or (6, 5); at
+ * most 512 channels a group): the derivative slots of y_jet are those of the normalised, activated value.  The
+ * backward takes the cotangent of every slot; workspace as above with s = 1. */
+int pdekan_group_norm_jet_forward(const float* x_jet, int64_t n, int32_t channels, int32_t groups, int32_t n_dir,
+                                  int32_t n_second, const float* weight, const float* bias, float eps, int32_t act_kind,
+                                  float* y_jet, void* stream);
+int pdekan_group_norm_jet_backward(const float* x_jet, const float* gy_jet, int64_t n, int32_t channels, int32_t groups,
+                                   int32_t n_dir, int32_t n_second, const float* weight, const float* bias, float eps,
+                                   int32_t act_kind, float* gx_jet, float* gweight, float* gbias, void* ws,
+                                   size_t ws_bytes, void* stream);
 
 /* Optional per-kernel timing for benchmarks (no counterpart in the reference,
  * which only prints a whole-script wall time, run1.py:524-526).  Between

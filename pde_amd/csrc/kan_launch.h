@@ -181,4 +181,24 @@ void launch_bwd_weight_f16_blocks(const LayerView& L, const float* a, const floa
                                   int64_t chunk, int nx, int ny, int nmain, const unsigned* act_in,
                                   const unsigned* cot_in, hipStream_t st);
 
+
+// kan_norm.hip: group norm with an activation, channels last, on values and on jets
+constexpr int kNormActIdentity = 0, kNormActSilu = 1, kNormActTanh = 2;
+constexpr int kNormF32 = 0, kNormBf16 = 1, kNormF16 = 2;
+constexpr int kNormChannelsMax = 8192;
+struct NormShape { int64_t n, s; int C, G; };                    // samples, positions of a sample, channels, groups
+const char* norm_refusal(const NormShape& p, int n_dir, int n_second);   // nullptr: taken
+size_t norm_ws_bytes(const NormShape& p, bool backward);
+bool norm_wants_stats(const NormShape& p);                       // the backward reads mean and r of the forward
+void launch_norm_forward(int dtype, const NormShape& p, const void* x, const float* w, const float* b, float eps, int act,
+                         void* y, float* stats, void* ws, hipStream_t st);
+void launch_norm_backward(int dtype, const NormShape& p, const void* x, const void* gy, const float* w, const float* b,
+                          float eps, int act, const float* stats, void* gx, float* gw, float* gb, void* ws,
+                          hipStream_t st);
+void launch_norm_jet_forward(const NormShape& p, int n_dir, const float* x, const float* w, const float* b, float eps,
+                             int act, float* y, hipStream_t st);
+void launch_norm_jet_backward(const NormShape& p, int n_dir, const float* x, const float* gy, const float* w,
+                              const float* b, float eps, int act, float* gx, float* gw, float* gb, void* ws,
+                              hipStream_t st);
+
 }  // namespace pdekan

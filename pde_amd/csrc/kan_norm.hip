@@ -1,0 +1,1008 @@
+// Group norm followed by an activation, channels last: on plain values [n][s][C] in fp32, bf16 or fp16 (statistics of a
+// group run over the s positions and the C / groups channels of a sample) and on derivative jets [n][C][J] in fp32
+// (statistics per point).  Sums, statistics and every intermediate are fp32; a 16-bit tensor is rounded once, at the store.
+//
+//   z = (x - mean) r,  r = (var + eps)^-1/2,  y = f(w z + b)
+//   backward: p = gy f',  gb = sum p,  gw = sum p z,  q = w p,  gx = r (q - mean(q) - z mean(q z))
+//
+// Two families of kernels:
+//   rows (norm_rows_*, norm_jet_*): one point at a time, a group of a point = L adjacent lanes, K vectors a lane.  The
+//     data of a group stays in registers between the statistics and the result: x is read once, y written once.
+//   grids (norm_grid_*): samples of many positions.  Launch 1 leaves partial statistics per chunk of positions, launch 2
+//     merges them (Chan's formula) and applies; the second reading of x comes mostly from the caches.
+#include <hip/hip_runtime.h>
+#include <cstdint>
+
+#include "kan_launch.h"
+#include "kan_wave.h"
+
+namespace pdekan {
+namespace {
+
+constexpr int kThreads = 256;
+
+template <typename T, int N> struct VecOf { typedef T type __attribute__((ext_vector_type(N))); };
+template <typename T> struct VecOf<T, 1> { typedef T type; };
+
+template <typename T, int N>
+__device__ __forceinline__ void load_vec(const T* p, float (&v)[N]) {
+  const typename VecOf<T, N>::type r = *reinterpret_cast<const typename VecOf<T, N>::type*>(p);
+  if constexpr (N == 1) v[0] = (float)r;
+  else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = (float)r[i];
+  }
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_vec(T* p, const float (&v)[N]) {
+  typename VecOf<T, N>::type r;
+  if constexpr (N == 1) r = (T)v[0];
+  else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) r[i] = (T)v[i];
+  }
+  *reinterpret_cast<typename VecOf<T, N>::type*>(p) = r;
+}
+
+// sum over the L adjacent lanes of a group (L a power of two, groups aligned to L), in every lane of the group
+template <int L>
+__device__ __forceinline__ float group_sum(float v) {
+  if constexpr (L >= 2) v += dpp_move<0xB1>(v);
+  if constexpr (L >= 4) v += dpp_move<0x4E>(v);
+  if constexpr (L >= 8) v += dpp_move<0x141>(v);
+  if constexpr (L >= 16) v += dpp_move<0x140>(v);
+  if constexpr (L >= 32) v = sum_xor16(v);
+  if constexpr (L >= 64) v = sum_xor32(v);
+  return v;
+}
+
+// f and its first ORDER derivatives at u.
+//   tanh: 1 - 2 / (exp(2u) + 1), which loses relative accuracy near 0, and below |u| = 0.25 the Taylor polynomial of
+//   degree 9 (the first term left out is 9e-9 of the result there)
+template <int ORDER>
+__device__ __forceinline__ void activation(int act, float u, float (&f)[ORDER + 1]) {
+  if (act == kNormActTanh) {
+    const float u2 = u * u;
+    const float far = 1.0f - 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(u * 2.885390081777927f) + 1.0f);
+    const float near =
+        u + u * u2 * fmaf(u2, fmaf(u2, fmaf(u2, 62.0f / 2835.0f, -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f);
+    const float t = u2 < 0.0625f ? near : far;
+    f[0] = t;
+    if constexpr (ORDER >= 1) f[1] = 1.0f - t * t;
+    if constexpr (ORDER >= 2) f[2] = -2.0f * t * f[1];
+    if constexpr (ORDER >= 3) f[3] = f[1] * (6.0f * t * t - 2.0f);
+  } else if (act == kNormActSilu) {
+    const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(u * -1.4426950408889634f));
+    f[0] = u * s;
+    if constexpr (ORDER >= 1) {
+      const float d = s * (1.0f - s), h = 1.0f - 2.0f * s;
+      f[1] = fmaf(u, d, s);
+      if constexpr (ORDER >= 2) f[2] = d * fmaf(u, h, 2.0f);
+      if constexpr (ORDER >= 3) f[3] = d * (3.0f * h + u * (1.0f - 6.0f * d));
+    }
+  } else {
+    f[0] = u;
+    if constexpr (ORDER >= 1) f[1] = 1.0f;
+    if constexpr (ORDER >= 2) f[2] = 0.0f;
+    if constexpr (ORDER >= 3) f[3] = 0.0f;
+  }
+}
+
+// Which (point, group) a lane group of a rows kernel takes.  A block holds 256 / L lane groups: `gpb` groups of `ppb`
+// points; blocks that share a range of groups walk the points with stride npb * ppb, so a lane keeps its channels (their
+// weights and the sums of their gradients stay in registers).
+struct RowMap { int64_t n; int C, G, cpg, gpb, ppb, gchunks, npb; };
+
+struct RowPlace { int g, pi; int64_t p, step; bool on; };
+template <int L>
+__device__ __forceinline__ RowPlace row_place(const RowMap& m) {
+  const int slot = threadIdx.x / L;
+  const int gi = slot % m.gpb, pi = slot / m.gpb;
+  const int gc = blockIdx.x % m.gchunks, pb = blockIdx.x / m.gchunks;
+  RowPlace r;
+  r.g = gc * m.gpb + gi;
+  r.pi = pi;
+  r.on = pi < m.ppb && r.g < m.G;
+  r.p = (int64_t)pb * m.ppb + pi;
+  r.step = (int64_t)m.npb * m.ppb;
+  return r;
+}
+
+// The block's sums of gw / gb over its points, in a fixed order: row npb of part [npb][2][C] (npb = 1: gw and gb
+// themselves).  Lane groups of the same group of channels sit gpb slots apart.
+template <int N, int L>
+__device__ __forceinline__ void row_grad_out(const RowMap& m, const RowPlace& r, const float (&gw)[N], const float (&gb)[N],
+                                             int c0, bool valid, float* part_w, float* part_b, float (*red)[N + 1]) {
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) red[threadIdx.x][i] = which ? gb[i] : gw[i];
+    __syncthreads();
+    float* part = which ? part_b : part_w;
+    if (part && r.on && r.pi == 0 && valid) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        float s = red[threadIdx.x][i];
+        for (int k = 1; k < m.ppb; ++k) s += red[threadIdx.x + k * m.gpb * L][i];
+        part[c0 + i] = s;
+      }
+    }
+  }
+}
+
+template <typename T, int VEC, int L, int K, bool BWD>
+__global__ void __launch_bounds__(kThreads) norm_rows_kernel(RowMap m, const T* __restrict__ x, const T* __restrict__ gy,
+                                                             const float* __restrict__ w, const float* __restrict__ b,
+                                                             float eps, int act, T* __restrict__ out,
+                                                             float* part_w, float* part_b, int part_stride) {
+  const RowPlace r = row_place<L>(m);
+  const int lane = threadIdx.x % L;
+  const float inv = 1.0f / (float)m.cpg;
+  bool valid[K];
+  float wv[K][VEC], bv[K][VEC], gwv[K][VEC], gbv[K][VEC];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    valid[k] = r.on && (lane + L * k) * VEC < m.cpg;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      const int c = r.g * m.cpg + (lane + L * k) * VEC + i;
+      wv[k][i] = valid[k] && w ? w[c] : 1.0f;
+      bv[k][i] = valid[k] && b ? b[c] : 0.0f;
+      gwv[k][i] = gbv[k][i] = 0.0f;
+    }
+  }
+  if (r.on) {
+    for (int64_t p = r.p; p < m.n; p += r.step) {
+      const int64_t at = p * m.C + (int64_t)r.g * m.cpg + lane * VEC;
+      float e[K][VEC], q[K][VEC];
+      float s = 0.0f;
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) e[k][i] = q[k][i] = 0.0f;
+        if (valid[k]) {
+          load_vec<T, VEC>(x + at + L * k * VEC, e[k]);
+          if constexpr (BWD) load_vec<T, VEC>(gy + at + L * k * VEC, q[k]);
+        }
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) s += e[k][i];
+      }
+      const float mean = group_sum<L>(s) * inv;
+      float v = 0.0f;
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          e[k][i] = valid[k] ? e[k][i] - mean : 0.0f;
+          v = fmaf(e[k][i], e[k][i], v);
+        }
+      const float rs = rsqrtf(fmaf(group_sum<L>(v), inv, eps));
+      if constexpr (!BWD) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            float f[1];
+            activation<0>(act, fmaf(e[k][i] * rs, wv[k][i], bv[k][i]), f);
+            e[k][i] = f[0];
+          }
+          if (valid[k]) store_vec<T, VEC>(out + at + L * k * VEC, e[k]);
+        }
+      } else {
+        float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            const float z = e[k][i] * rs;
+            float f[2];
+            activation<1>(act, fmaf(z, wv[k][i], bv[k][i]), f);
+            const float pv = q[k][i] * f[1];
+            gbv[k][i] += pv;
+            gwv[k][i] = fmaf(pv, z, gwv[k][i]);
+            q[k][i] = pv * wv[k][i];
+            s1 += q[k][i];
+            s2 = fmaf(q[k][i], z, s2);
+            e[k][i] = z;
+          }
+        s1 = group_sum<L>(s1) * inv;
+        s2 = group_sum<L>(s2) * inv;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) e[k][i] = rs * (q[k][i] - s1 - e[k][i] * s2);
+          if (valid[k]) store_vec<T, VEC>(out + at + L * k * VEC, e[k]);
+        }
+      }
+    }
+  }
+  if constexpr (BWD) {
+    if (part_w || part_b) {
+      __shared__ float red[kThreads][VEC + 1];
+      const int64_t row = (int64_t)(blockIdx.x / m.gchunks) * part_stride;
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+        row_grad_out<VEC, L>(m, r, gwv[k], gbv[k], r.g * m.cpg + (lane + L * k) * VEC, valid[k],
+                             part_w ? part_w + row : nullptr, part_b ? part_b + row : nullptr, red);
+    }
+  }
+}
+
+// Jets.  Slots of a channel: value x, first derivatives x'_d (d < ND), second derivatives x''_d (d < NS), along each
+// direction d the chain rule of the norm and of the activation.  With e, f, s the slots less their means over the group,
+// V = mean(e^2) + eps, A = mean(e f), B = mean(f^2 + e s):
+//   r = V^-1/2,  r' = -r^3 A,  r'' = -r^3 B + 3 r^5 A^2
+//   z = e r,  z' = f r + e r',  z'' = s r + 2 f r' + e r'',  u = w z + b, u' = w z', u'' = w z''
+//   y = F(u),  y' = F1 u',  y'' = F2 u'^2 + F1 u''
+// Backward (h = cotangent times w, on z, z', z''):
+//   gu'' = F1 gy'', gu' = F1 gy' + 2 F2 u' gy'', gu = F1 gy + sum_d F2 u' gy' + (F3 u'^2 + F2 u'') gy''
+//   gr = sum e h + sum_d (f h' + s h''),  gr' = sum (e h' + 2 f h''),  gr'' = sum e h''
+//   gV = -r^3 gr / 2 + sum_d 3/2 r^5 A gr' + (3/2 r^5 B - 15/2 r^7 A^2) gr'',  gA = -r^3 gr' + 6 r^5 A gr'', gB = -r^3 gr''
+//   ge = r h + 2 e gV / M + sum_d (r' h' + r'' h'' + (f gA + s gB) / M),  gf = r h' + 2 r' h'' + (e gA + 2 f gB) / M,
+//   gs = r h'' + e gB / M, each less its mean over the group (the means of e, f, s vanish: only h's remain)
+template <int ND, int NS, int L, int K, bool BWD>
+__global__ void __launch_bounds__(kThreads) norm_jet_kernel(RowMap m, const float* __restrict__ x,
+                                                            const float* __restrict__ gy, const float* __restrict__ w,
+                                                            const float* __restrict__ b, float eps, int act,
+                                                            float* __restrict__ out, float* part_w, float* part_b,
+                                                            int part_stride) {
+  constexpr int J = 1 + ND + NS;
+  const RowPlace r = row_place<L>(m);
+  const int lane = threadIdx.x % L;
+  const float inv = 1.0f / (float)m.cpg;
+  bool valid[K];
+  float wv[K], bv[K], gwv[K], gbv[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    valid[k] = r.on && lane + L * k < m.cpg;
+    const int c = r.g * m.cpg + lane + L * k;
+    wv[k] = valid[k] && w ? w[c] : 1.0f;
+    bv[k] = valid[k] && b ? b[c] : 0.0f;
+    gwv[k] = gbv[k] = 0.0f;
+  }
+  if (r.on) {
+    for (int64_t p = r.p; p < m.n; p += r.step) {
+      const int64_t at = (p * m.C + (int64_t)r.g * m.cpg + lane) * J;
+      float e[K][J], h[K][J];
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+#pragma unroll
+        for (int j = 0; j < J; ++j) e[k][j] = h[k][j] = 0.0f;
+        if (valid[k]) {
+          if constexpr (J % 4 == 0) {
+#pragma unroll
+            for (int j = 0; j < J; j += 4) {
+              float t[4];
+              load_vec<float, 4>(x + at + (int64_t)L * k * J + j, t);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) e[k][j + i] = t[i];
+              if constexpr (BWD) {
+                load_vec<float, 4>(gy + at + (int64_t)L * k * J + j, t);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) h[k][j + i] = t[i];
+              }
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        float s = 0.0f;
+#pragma unroll
+        for (int k = 0; k < K; ++k) s += e[k][j];
+        s = group_sum<L>(s) * inv;
+#pragma unroll
+        for (int k = 0; k < K; ++k) e[k][j] = valid[k] ? e[k][j] - s : 0.0f;
+      }
+      float V = 0.0f, A[ND], B[NS];
+#pragma unroll
+      for (int k = 0; k < K; ++k) V = fmaf(e[k][0], e[k][0], V);
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        A[d] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < K; ++k) A[d] = fmaf(e[k][0], e[k][1 + d], A[d]);
+        A[d] = group_sum<L>(A[d]) * inv;
+      }
+#pragma unroll
+      for (int d = 0; d < NS; ++d) {
+        B[d] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+          B[d] = fmaf(e[k][1 + d], e[k][1 + d], fmaf(e[k][0], e[k][1 + ND + d], B[d]));
+        B[d] = group_sum<L>(B[d]) * inv;
+      }
+      const float rs = rsqrtf(fmaf(group_sum<L>(V), inv, eps));
+      const float r3 = rs * rs * rs, r5 = r3 * rs * rs;
+      float r1[ND], r2[NS];
+#pragma unroll
+      for (int d = 0; d < ND; ++d) r1[d] = -r3 * A[d];
+#pragma unroll
+      for (int d = 0; d < NS; ++d) r2[d] = fmaf(3.0f * r5 * A[d], A[d], -r3 * B[d]);
+      if constexpr (!BWD) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          float f[3], y[J];
+          activation<2>(act, fmaf(e[k][0] * rs, wv[k], bv[k]), f);
+          y[0] = f[0];
+#pragma unroll
+          for (int d = 0; d < ND; ++d) {
+            const float u1 = wv[k] * fmaf(e[k][0], r1[d], e[k][1 + d] * rs);
+            y[1 + d] = f[1] * u1;
+            if (d < NS) {
+              const float u2 = wv[k] * fmaf(e[k][0], r2[d], fmaf(2.0f * e[k][1 + d], r1[d], e[k][1 + ND + d] * rs));
+              y[1 + ND + d] = fmaf(f[2] * u1, u1, f[1] * u2);
+            }
+          }
+          if (valid[k]) {
+#pragma unroll
+            for (int j = 0; j < J; j += 4) {
+              const float t[4] = {y[j], y[j + 1], y[j + 2], y[j + 3]};
+              store_vec<float, 4>(out + at + (int64_t)L * k * J + j, t);
+            }
+          }
+        }
+      } else {
+        float gr = 0.0f, gr1[ND], gr2[NS], hm[J];
+#pragma unroll
+        for (int d = 0; d < ND; ++d) gr1[d] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < NS; ++d) gr2[d] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < J; ++j) hm[j] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          const float z = e[k][0] * rs;
+          float f[4];
+          activation<3>(act, fmaf(z, wv[k], bv[k]), f);
+          float gu = f[1] * h[k][0], gw = 0.0f;
+#pragma unroll
+          for (int d = 0; d < ND; ++d) {
+            const float z1 = fmaf(e[k][0], r1[d], e[k][1 + d] * rs), u1 = wv[k] * z1;
+            float gu1 = f[1] * h[k][1 + d];
+            gu = fmaf(f[2] * u1, h[k][1 + d], gu);
+            if (d < NS) {
+              const float z2 = fmaf(e[k][0], r2[d], fmaf(2.0f * e[k][1 + d], r1[d], e[k][1 + ND + d] * rs));
+              const float u2 = wv[k] * z2, g2 = h[k][1 + ND + d];
+              gu = fmaf(fmaf(f[3] * u1, u1, f[2] * u2), g2, gu);
+              gu1 = fmaf(2.0f * f[2] * u1, g2, gu1);
+              const float gu2 = f[1] * g2;
+              gw = fmaf(gu2, z2, gw);
+              h[k][1 + ND + d] = wv[k] * gu2;
+              gr2[d] = fmaf(e[k][0], h[k][1 + ND + d], gr2[d]);
+              gr1[d] = fmaf(2.0f * e[k][1 + d], h[k][1 + ND + d], gr1[d]);
+              gr = fmaf(e[k][1 + ND + d], h[k][1 + ND + d], gr);
+            }
+            gw = fmaf(gu1, z1, gw);
+            h[k][1 + d] = wv[k] * gu1;
+            gr1[d] = fmaf(e[k][0], h[k][1 + d], gr1[d]);
+            gr = fmaf(e[k][1 + d], h[k][1 + d], gr);
+          }
+          gbv[k] += gu;
+          gwv[k] += fmaf(gu, z, gw);
+          h[k][0] = wv[k] * gu;
+          gr = fmaf(e[k][0], h[k][0], gr);
+#pragma unroll
+          for (int j = 0; j < J; ++j) hm[j] += h[k][j];
+        }
+        gr = group_sum<L>(gr);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) gr1[d] = group_sum<L>(gr1[d]);
+#pragma unroll
+        for (int d = 0; d < NS; ++d) gr2[d] = group_sum<L>(gr2[d]);
+#pragma unroll
+        for (int j = 0; j < J; ++j) hm[j] = group_sum<L>(hm[j]) * inv;
+        // gA, gB and gV, each already divided by the number of channels
+        float gA[ND], gB[NS], gV = -0.5f * r3 * gr;
+        const float r7 = r5 * rs * rs;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+          gA[d] = -r3 * gr1[d];
+          gV = fmaf(1.5f * r5 * A[d], gr1[d], gV);
+          if (d < NS) {
+            gA[d] = fmaf(6.0f * r5 * A[d], gr2[d], gA[d]);
+            gB[d] = -r3 * gr2[d] * inv;
+            gV = fmaf(fmaf(1.5f * r5, B[d], -7.5f * r7 * A[d] * A[d]), gr2[d], gV);
+          }
+          gA[d] *= inv;
+        }
+        gV *= 2.0f * inv;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          float g[J];
+          g[0] = fmaf(rs, h[k][0] - hm[0], e[k][0] * gV);
+#pragma unroll
+          for (int d = 0; d < ND; ++d) {
+            g[0] = fmaf(r1[d], h[k][1 + d] - hm[1 + d], fmaf(e[k][1 + d], gA[d], g[0]));
+            g[1 + d] = fmaf(rs, h[k][1 + d] - hm[1 + d], e[k][0] * gA[d]);
+            if (d < NS) {
+              const float h2 = h[k][1 + ND + d] - hm[1 + ND + d];
+              g[0] = fmaf(r2[d], h2, fmaf(e[k][1 + ND + d], gB[d], g[0]));
+              g[1 + d] = fmaf(2.0f * r1[d], h2, fmaf(2.0f * e[k][1 + d], gB[d], g[1 + d]));
+              g[1 + ND + d] = fmaf(rs, h2, e[k][0] * gB[d]);
+            }
+          }
+          if (valid[k]) {
+#pragma unroll
+            for (int j = 0; j < J; j += 4) {
+              const float t[4] = {g[j], g[j + 1], g[j + 2], g[j + 3]};
+              store_vec<float, 4>(out + at + (int64_t)L * k * J + j, t);
+            }
+          }
+        }
+      }
+    }
+  }
+  if constexpr (BWD) {
+    if (part_w || part_b) {
+      __shared__ float red[kThreads][2];
+      const int64_t row = (int64_t)(blockIdx.x / m.gchunks) * part_stride;
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const float gw1[1] = {gwv[k]}, gb1[1] = {gbv[k]};
+        row_grad_out<1, L>(m, r, gw1, gb1, r.g * m.cpg + lane + L * k, valid[k], part_w ? part_w + row : nullptr,
+                           part_b ? part_b + row : nullptr, red);
+      }
+    }
+  }
+}
+
+// out_w[c], out_b[c] = sums over the rows of part [rows][2][C], in a fixed order: 32 columns x 32 row slices a block
+constexpr int kFinishCols = 32, kFinishSlices = 32;
+__device__ __forceinline__ void finish_columns(int col_block, const float* __restrict__ part, int64_t rows, int C,
+                                               float* out_w, float* out_b, int threads) {
+  __shared__ float red[kFinishSlices][kFinishCols + 1];
+  const int cl = threadIdx.x % kFinishCols, slices = threads / kFinishCols, sl = threadIdx.x / kFinishCols;
+  const int col = col_block * kFinishCols + cl;
+  float s = 0.0f;
+  if (col < 2 * C)
+    for (int64_t i = sl; i < rows; i += slices) s += part[i * 2 * C + col];
+  red[sl][cl] = s;
+  __syncthreads();
+  if (sl == 0 && col < 2 * C) {
+    for (int i = 1; i < slices; ++i) s += red[i][cl];
+    float* out = col < C ? out_w : out_b;
+    if (out) out[col < C ? col : col - C] = s;
+  }
+}
+__global__ void __launch_bounds__(1024) norm_finish_kernel(const float* __restrict__ part, int64_t rows, int C,
+                                                           float* out_w, float* out_b) {
+  finish_columns(blockIdx.x, part, rows, C, out_w, out_b, 1024);
+}
+
+// ---- samples of many positions ------------------------------------------------------------------------------------
+
+// A block takes one chunk of positions of one sample and all its channels: thread = (vector of channels, row slot).
+struct GridMap { int64_t n, s, rows; int C, G, cpg, chunks; };   // rows: positions a chunk (the last may have fewer)
+
+template <int VEC>
+struct GridThread {
+  int nv, txn, tyn, tx, ty;
+  int64_t sample, row0, row1;
+  int chunk;
+  __device__ __forceinline__ GridThread(const GridMap& m, int64_t block) {
+    nv = m.C / VEC;
+    txn = nv < kThreads ? nv : kThreads;
+    tyn = kThreads / txn;
+    tx = threadIdx.x % txn;
+    ty = threadIdx.x / txn;
+    sample = block / m.chunks;
+    chunk = (int)(block % m.chunks);
+    row0 = chunk * m.rows;
+    row1 = row0 + m.rows < m.s ? row0 + m.rows : m.s;
+  }
+};
+
+// Partial statistics of a chunk: per channel the sums of x - k and (x - k)^2 with k the chunk's first value of that
+// channel.  As k is one of the values, the squared deviations are at least about (k - mean)^2, so subtracting the
+// square of the sum loses no more than eps * (positions a chunk) relative, however far the values lie from zero.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kThreads) norm_grid_stats_kernel(GridMap m, const T* __restrict__ x,
+                                                                   float2* __restrict__ part) {
+  extern __shared__ float chan[];                     // [2][C]: mean and sum of squared deviations of each channel
+  __shared__ float red[2][kThreads][VEC + 1];
+  const GridThread<VEC> t(m, blockIdx.x);
+  const T* base = x + t.sample * m.s * m.C;
+  const float cnt = (float)(t.row1 - t.row0);
+  for (int tile = 0; tile < t.nv; tile += t.txn) {
+    const int vec = tile + t.tx;
+    const bool on = t.ty < t.tyn && vec < t.nv;
+    float k[VEC], s1[VEC], s2[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) k[i] = s1[i] = s2[i] = 0.0f;
+    if (on) {
+      load_vec<T, VEC>(base + t.row0 * m.C + vec * VEC, k);
+#pragma unroll 4
+      for (int64_t row = t.row0 + t.ty; row < t.row1; row += t.tyn) {
+        float v[VEC];
+        load_vec<T, VEC>(base + row * m.C + vec * VEC, v);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          const float d = v[i] - k[i];
+          s1[i] += d;
+          s2[i] = fmaf(d, d, s2[i]);
+        }
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) { red[0][threadIdx.x][i] = s1[i]; red[1][threadIdx.x][i] = s2[i]; }
+    __syncthreads();
+    if (on && t.ty == 0) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        for (int j = 1; j < t.tyn; ++j) {
+          s1[i] += red[0][threadIdx.x + j * t.txn][i];
+          s2[i] += red[1][threadIdx.x + j * t.txn][i];
+        }
+        const float d = s1[i] / cnt;
+        chan[vec * VEC + i] = k[i] + d;
+        chan[m.C + vec * VEC + i] = fmaxf(fmaf(-d, s1[i], s2[i]), 0.0f);
+      }
+    }
+  }
+  __syncthreads();
+  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+  for (int g = wave; g < m.G; g += kThreads / 64) {
+    float s = 0.0f, q = 0.0f;
+    for (int c = lane; c < m.cpg; c += 64) s += chan[g * m.cpg + c];
+    const float mean = wave_sum(s) / (float)m.cpg;
+    for (int c = lane; c < m.cpg; c += 64) {
+      const float d = chan[g * m.cpg + c] - mean;
+      q += fmaf(cnt * d, d, chan[m.C + g * m.cpg + c]);
+    }
+    q = wave_sum(q);
+    if (lane == 0) part[(int64_t)blockIdx.x * m.G + g] = make_float2(mean, q);
+  }
+}
+
+// mean and r of every group of a sample from its chunks' partial statistics, into LDS (and to stats, from one block)
+__device__ __forceinline__ void merge_stats(const GridMap& m, int64_t sample, const float2* __restrict__ part, float eps,
+                                            float* mu, float* rs, float2* stats) {
+  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+  for (int g = wave; g < m.G; g += kThreads / 64) {
+    float mean = 0.0f, q = 0.0f, cnt = 0.0f;
+    if (lane < m.chunks) {
+      const float2 v = part[(sample * m.chunks + lane) * m.G + g];
+      const int64_t left = m.s - lane * m.rows;
+      cnt = (float)(left < m.rows ? left : m.rows);
+      mean = v.x;
+      q = v.y;
+    }
+    const float total = (float)m.s;
+    // about the first chunk's mean: the sum of the differences carries no offset
+    const float first = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(mean)));
+    const float all = first + wave_sum(lane < m.chunks ? cnt * (mean - first) : 0.0f) / total;
+    const float d = mean - all;
+    q = wave_sum(lane < m.chunks ? fmaf(cnt * (float)m.cpg * d, d, q) : 0.0f);
+    const float r = rsqrtf(q / (total * (float)m.cpg) + eps);
+    if (lane == 0) {
+      mu[g] = all;
+      rs[g] = r;
+      if (stats) stats[sample * m.G + g] = make_float2(all, r);
+    }
+  }
+}
+
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kThreads) norm_grid_apply_kernel(GridMap m, const T* __restrict__ x,
+                                                                   const float* __restrict__ w,
+                                                                   const float* __restrict__ b, float eps, int act,
+                                                                   const float2* __restrict__ part, T* __restrict__ y,
+                                                                   float2* stats) {
+  extern __shared__ float chan[];                     // [2][G]
+  float *mu = chan, *rs = chan + m.G;
+  const GridThread<VEC> t(m, blockIdx.x);
+  merge_stats(m, t.sample, part, eps, mu, rs, t.chunk == 0 ? stats : nullptr);
+  __syncthreads();
+  const int64_t base = t.sample * m.s * m.C;
+  for (int tile = 0; tile < t.nv; tile += t.txn) {
+    const int vec = tile + t.tx;
+    if (t.ty >= t.tyn || vec >= t.nv) continue;
+    float wr[VEC], bv[VEC], mean[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      const int c = vec * VEC + i, g = c / m.cpg;
+      wr[i] = (w ? w[c] : 1.0f) * rs[g];
+      bv[i] = b ? b[c] : 0.0f;
+      mean[i] = mu[g];
+    }
+#pragma unroll 4
+    for (int64_t row = t.row0 + t.ty; row < t.row1; row += t.tyn) {
+      float v[VEC];
+      load_vec<T, VEC>(x + base + row * m.C + vec * VEC, v);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        float f[1];
+        activation<0>(act, fmaf(v[i] - mean[i], wr[i], bv[i]), f);
+        v[i] = f[0];
+      }
+      store_vec<T, VEC>(y + base + row * m.C + vec * VEC, v);
+    }
+  }
+}
+
+// Backward, launch 1: per chunk and channel the sums of p = gy f' and of p z (part_c [n * chunks][2][C], p z first),
+// and per group the sums of w p and w p z (part_g [n * chunks][G])
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kThreads) norm_grid_sums_kernel(GridMap m, const T* __restrict__ x,
+                                                                  const T* __restrict__ gy, const float* __restrict__ w,
+                                                                  const float* __restrict__ b, int act,
+                                                                  const float2* __restrict__ stats,
+                                                                  float* __restrict__ part_c, float2* __restrict__ part_g) {
+  extern __shared__ float chan[];                     // [2][C]: sums of w p z, w p
+  __shared__ float red[2][kThreads][VEC + 1];
+  const GridThread<VEC> t(m, blockIdx.x);
+  const int64_t base = t.sample * m.s * m.C;
+  float* mine = part_c + (int64_t)blockIdx.x * 2 * m.C;
+  for (int tile = 0; tile < t.nv; tile += t.txn) {
+    const int vec = tile + t.tx;
+    const bool on = t.ty < t.tyn && vec < t.nv;
+    float s1[VEC], s2[VEC], wv[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) s1[i] = s2[i] = wv[i] = 0.0f;
+    if (on) {
+      float bv[VEC], mean[VEC], rs[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const int c = vec * VEC + i;
+        const float2 st = stats[t.sample * m.G + c / m.cpg];
+        wv[i] = w ? w[c] : 1.0f;
+        bv[i] = b ? b[c] : 0.0f;
+        mean[i] = st.x;
+        rs[i] = st.y;
+      }
+#pragma unroll 2
+      for (int64_t row = t.row0 + t.ty; row < t.row1; row += t.tyn) {
+        float v[VEC], g[VEC];
+        load_vec<T, VEC>(x + base + row * m.C + vec * VEC, v);
+        load_vec<T, VEC>(gy + base + row * m.C + vec * VEC, g);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          const float z = (v[i] - mean[i]) * rs[i];
+          float f[2];
+          activation<1>(act, fmaf(z, wv[i], bv[i]), f);
+          const float p = g[i] * f[1];
+          s1[i] += p;
+          s2[i] = fmaf(p, z, s2[i]);
+        }
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) { red[0][threadIdx.x][i] = s1[i]; red[1][threadIdx.x][i] = s2[i]; }
+    __syncthreads();
+    if (on && t.ty == 0) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        for (int j = 1; j < t.tyn; ++j) {
+          s1[i] += red[0][threadIdx.x + j * t.txn][i];
+          s2[i] += red[1][threadIdx.x + j * t.txn][i];
+        }
+        const int c = vec * VEC + i;
+        mine[c] = s2[i];
+        mine[m.C + c] = s1[i];
+        chan[c] = wv[i] * s2[i];
+        chan[m.C + c] = wv[i] * s1[i];
+      }
+    }
+  }
+  __syncthreads();
+  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+  for (int g = wave; g < m.G; g += kThreads / 64) {
+    float a = 0.0f, q = 0.0f;
+    for (int c = lane; c < m.cpg; c += 64) {
+      q += chan[g * m.cpg + c];
+      a += chan[m.C + g * m.cpg + c];
+    }
+    a = wave_sum(a);
+    q = wave_sum(q);
+    if (lane == 0) part_g[(int64_t)blockIdx.x * m.G + g] = make_float2(a, q);
+  }
+}
+
+// Backward, launch 2: gx from the merged sums of the sample; blocks past the last chunk sum gw and gb over all chunks
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kThreads) norm_grid_grad_kernel(GridMap m, const T* __restrict__ x,
+                                                                  const T* __restrict__ gy, const float* __restrict__ w,
+                                                                  const float* __restrict__ b, int act,
+                                                                  const float2* __restrict__ stats,
+                                                                  const float* __restrict__ part_c,
+                                                                  const float2* __restrict__ part_g, T* __restrict__ gx,
+                                                                  float* gw, float* gb, int64_t main_blocks) {
+  extern __shared__ float chan[];                     // [2][G]
+  if ((int64_t)blockIdx.x >= main_blocks) {
+    finish_columns((int)(blockIdx.x - main_blocks), part_c, m.n * m.chunks, m.C, gw, gb, kThreads);
+    return;
+  }
+  const GridThread<VEC> t(m, blockIdx.x);
+  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+  const float inv = 1.0f / ((float)m.s * (float)m.cpg);
+  for (int g = wave; g < m.G; g += kThreads / 64) {
+    float2 v = make_float2(0.0f, 0.0f);
+    if (lane < m.chunks) v = part_g[(t.sample * m.chunks + lane) * m.G + g];
+    const float a = wave_sum(v.x) * inv, q = wave_sum(v.y) * inv;
+    if (lane == 0) { chan[g] = a; chan[m.G + g] = q; }
+  }
+  __syncthreads();
+  const int64_t base = t.sample * m.s * m.C;
+  for (int tile = 0; tile < t.nv; tile += t.txn) {
+    const int vec = tile + t.tx;
+    if (t.ty >= t.tyn || vec >= t.nv) continue;
+    float wv[VEC], bv[VEC], mean[VEC], rs[VEC], a[VEC], q[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      const int c = vec * VEC + i, g = c / m.cpg;
+      const float2 st = stats[t.sample * m.G + g];
+      wv[i] = w ? w[c] : 1.0f;
+      bv[i] = b ? b[c] : 0.0f;
+      mean[i] = st.x;
+      rs[i] = st.y;
+      a[i] = chan[g];
+      q[i] = chan[m.G + g];
+    }
+#pragma unroll 2
+    for (int64_t row = t.row0 + t.ty; row < t.row1; row += t.tyn) {
+      float v[VEC], g[VEC];
+      load_vec<T, VEC>(x + base + row * m.C + vec * VEC, v);
+      load_vec<T, VEC>(gy + base + row * m.C + vec * VEC, g);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const float z = (v[i] - mean[i]) * rs[i];
+        float f[2];
+        activation<1>(act, fmaf(z, wv[i], bv[i]), f);
+        v[i] = rs[i] * (g[i] * f[1] * wv[i] - a[i] - z * q[i]);
+      }
+      store_vec<T, VEC>(gx + base + row * m.C + vec * VEC, v);
+    }
+  }
+}
+
+// ---- host -----------------------------------------------------------------------------------------------------------
+
+constexpr int kRowBlocks = 2048;       // 8 blocks of 4 waves a compute unit
+constexpr int kGridBlocks = 1024, kChunksMax = 64;
+constexpr size_t kStaticLds = 20 * 1024;   // at least what the grid kernels declare besides the per-channel sums
+
+int pow2_at_least(int v) { int p = 1; while (p < v) p *= 2; return p; }
+
+RowMap row_map(int64_t n, int C, int G, int L) {
+  RowMap m;
+  m.n = n; m.C = C; m.G = G; m.cpg = C / G;
+  const int rpb = kThreads / L;
+  if (G <= rpb) { m.gpb = G; m.ppb = rpb / G; m.gchunks = 1; }
+  else { m.gpb = rpb; m.ppb = 1; m.gchunks = (G + rpb - 1) / rpb; }
+  if (m.ppb > n) m.ppb = (int)n;
+  const int64_t need = (n + m.ppb - 1) / m.ppb, most = kRowBlocks / m.gchunks > 0 ? kRowBlocks / m.gchunks : 1;
+  m.npb = (int)(need < most ? need : most);
+  return m;
+}
+
+// vector width, lanes and vectors a lane of a group of cpg channels; K = 0: too many channels for the rows kernels
+struct RowShape { int vec, L, K; };
+RowShape row_shape(int cpg, int vec) {
+  const int nv = cpg / vec;
+  int L = pow2_at_least(nv);
+  if (L < 4) L = 4;
+  if (L > 64) L = 64;
+  const int K = pow2_at_least((nv + L - 1) / L);
+  return {vec, L, K > 8 ? 0 : K};
+}
+
+int elem_size(int dtype) { return dtype == kNormF32 ? 4 : 2; }
+
+// the widest vector that divides the rows' addresses: 16 bytes, 4 bytes (16-bit types) or one element
+int vec_width(int dtype, int unit, const void* a, const void* b, const void* c) {
+  const int es = elem_size(dtype);
+  const uintptr_t low = (uintptr_t)a | (uintptr_t)b | (uintptr_t)c;
+  for (const int bytes : {16, 4}) {
+    const int v = bytes / es;
+    if (v > 1 && unit % v == 0 && low % bytes == 0) return v;
+  }
+  return 1;
+}
+
+GridMap grid_map(int64_t n, int64_t s, int C, int G) {
+  GridMap m;
+  m.n = n; m.s = s; m.C = C; m.G = G; m.cpg = C / G;
+  int64_t chunks = (kGridBlocks + n - 1) / n;
+  // a chunk of at least 16 KB at two bytes a value: shorter ones cost more in their partial results than they spread
+  const int64_t least = (8192 + C - 1) / C;
+  if (chunks > s / least) chunks = s / least;
+  if (chunks > kChunksMax) chunks = kChunksMax;
+  if (chunks < 1) chunks = 1;
+  m.rows = (s + chunks - 1) / chunks;
+  m.chunks = (int)((s + m.rows - 1) / m.rows);
+  return m;
+}
+
+// 512 channels: with one element a vector (the least aligned tensors) the 64 lanes of a wave still hold a group
+bool rows_kernel_takes(int64_t s, int cpg) { return s == 1 && cpg <= 512; }
+
+template <typename T, int VEC, bool BWD>
+void run_rows(const RowShape& sh, const RowMap& m, const T* x, const T* gy, const float* w, const float* b, float eps,
+              int act, T* out, float* pw, float* pb, int stride, hipStream_t st) {
+  const dim3 grid(m.npb * m.gchunks), block(kThreads);
+#define PDEKAN_ROWS(LL, KK)                                                                                         \
+  if (sh.L == LL && sh.K == KK) {                                                                                   \
+    hipLaunchKernelGGL((norm_rows_kernel<T, VEC, LL, KK, BWD>), grid, block, 0, st, m, x, gy, w, b, eps, act, out, \
+                       pw, pb, stride);                                                                             \
+    return;                                                                                                         \
+  }
+  PDEKAN_ROWS(4, 1) PDEKAN_ROWS(8, 1) PDEKAN_ROWS(16, 1) PDEKAN_ROWS(32, 1) PDEKAN_ROWS(64, 1)
+  if constexpr (VEC <= 4) { PDEKAN_ROWS(64, 2) }
+  if constexpr (VEC <= 2) { PDEKAN_ROWS(64, 4) }
+  if constexpr (VEC <= 1) { PDEKAN_ROWS(64, 8) }
+#undef PDEKAN_ROWS
+}
+
+template <typename T, bool BWD>
+void run_rows_vec(int vec, const RowShape& sh, const RowMap& m, const void* x, const void* gy, const float* w,
+                  const float* b, float eps, int act, void* out, float* pw, float* pb, int stride, hipStream_t st) {
+  constexpr int kWide = 16 / sizeof(T);
+  const T *xt = static_cast<const T*>(x), *gt = static_cast<const T*>(gy);
+  T* ot = static_cast<T*>(out);
+  if (vec == kWide) run_rows<T, kWide, BWD>(sh, m, xt, gt, w, b, eps, act, ot, pw, pb, stride, st);
+  else if (sizeof(T) == 2 && vec == 2) run_rows<T, 2, BWD>(sh, m, xt, gt, w, b, eps, act, ot, pw, pb, stride, st);
+  else run_rows<T, 1, BWD>(sh, m, xt, gt, w, b, eps, act, ot, pw, pb, stride, st);
+}
+
+template <bool BWD>
+void rows_any(int dtype, const NormShape& p, const void* x, const void* gy, const float* w, const float* b, float eps,
+              int act, void* out, float* gw, float* gb, float* part, hipStream_t st) {
+  const int vec = vec_width(dtype, p.C / p.G, x, gy, out);
+  const RowShape sh = row_shape(p.C / p.G, vec);
+  const RowMap m = row_map(p.n, p.C, p.G, sh.L);
+  float *pw = nullptr, *pb = nullptr;
+  const bool direct = m.npb == 1;
+  if (BWD && (gw || gb)) { pw = direct ? gw : part; pb = direct ? gb : part + p.C; }
+  const int stride = 2 * p.C;
+  switch (dtype) {
+    case kNormF32: run_rows_vec<float, BWD>(vec, sh, m, x, gy, w, b, eps, act, out, pw, pb, stride, st); break;
+    case kNormBf16: run_rows_vec<__bf16, BWD>(vec, sh, m, x, gy, w, b, eps, act, out, pw, pb, stride, st); break;
+    default: run_rows_vec<_Float16, BWD>(vec, sh, m, x, gy, w, b, eps, act, out, pw, pb, stride, st); break;
+  }
+  if (BWD && (gw || gb) && !direct)
+    hipLaunchKernelGGL(norm_finish_kernel, dim3((2 * p.C + kFinishCols - 1) / kFinishCols), dim3(1024), 0, st, part,
+                       (int64_t)m.npb, p.C, gw, gb);
+}
+
+template <int ND, int NS, bool BWD>
+void run_jet(const RowShape& sh, const RowMap& m, const float* x, const float* gy, const float* w, const float* b,
+             float eps, int act, float* out, float* pw, float* pb, int stride, hipStream_t st) {
+  const dim3 grid(m.npb * m.gchunks), block(kThreads);
+#define PDEKAN_JETS(LL, KK)                                                                                          \
+  if (sh.L == LL && sh.K == KK) {                                                                                    \
+    hipLaunchKernelGGL((norm_jet_kernel<ND, NS, LL, KK, BWD>), grid, block, 0, st, m, x, gy, w, b, eps, act, out, pw, \
+                       pb, stride);                                                                                  \
+    return;                                                                                                          \
+  }
+  PDEKAN_JETS(4, 1) PDEKAN_JETS(8, 1) PDEKAN_JETS(16, 1) PDEKAN_JETS(32, 1) PDEKAN_JETS(64, 1) PDEKAN_JETS(64, 2)
+  PDEKAN_JETS(64, 4) PDEKAN_JETS(64, 8)
+#undef PDEKAN_JETS
+}
+
+template <bool BWD>
+void jet_any(const NormShape& p, int n_dir, const float* x, const float* gy, const float* w, const float* b, float eps,
+             int act, float* out, float* gw, float* gb, float* part, hipStream_t st) {
+  const RowShape sh = row_shape(p.C / p.G, 1);
+  const RowMap m = row_map(p.n, p.C, p.G, sh.L);
+  float *pw = nullptr, *pb = nullptr;
+  const bool direct = m.npb == 1;
+  if (BWD && (gw || gb)) { pw = direct ? gw : part; pb = direct ? gb : part + p.C; }
+  const int stride = 2 * p.C;
+  if (n_dir == 2) run_jet<2, 1, BWD>(sh, m, x, gy, w, b, eps, act, out, pw, pb, stride, st);
+  else run_jet<6, 5, BWD>(sh, m, x, gy, w, b, eps, act, out, pw, pb, stride, st);
+  if (BWD && (gw || gb) && !direct)
+    hipLaunchKernelGGL(norm_finish_kernel, dim3((2 * p.C + kFinishCols - 1) / kFinishCols), dim3(1024), 0, st, part,
+                       (int64_t)m.npb, p.C, gw, gb);
+}
+
+template <typename T, int VEC>
+void grid_forward(const GridMap& m, const T* x, const float* w, const float* b, float eps, int act, T* y, float2* stats,
+                  float2* part, hipStream_t st) {
+  const unsigned blocks = (unsigned)(m.n * m.chunks);
+  const size_t lds = 2 * (size_t)m.C * sizeof(float), lds_g = 2 * (size_t)m.G * sizeof(float);
+  ensure_dynamic_lds((const void*)norm_grid_stats_kernel<T, VEC>, lds + kStaticLds);
+  ensure_dynamic_lds((const void*)norm_grid_apply_kernel<T, VEC>, lds_g + kStaticLds);
+  hipLaunchKernelGGL((norm_grid_stats_kernel<T, VEC>), dim3(blocks), dim3(kThreads), lds, st, m, x, part);
+  hipLaunchKernelGGL((norm_grid_apply_kernel<T, VEC>), dim3(blocks), dim3(kThreads), lds_g, st, m, x, w, b, eps, act,
+                     part, y, stats);
+}
+template <typename T, int VEC>
+void grid_backward(const GridMap& m, const T* x, const T* gy, const float* w, const float* b, int act,
+                   const float2* stats, T* gx, float* gw, float* gb, float* part_c, float2* part_g, hipStream_t st) {
+  const unsigned blocks = (unsigned)(m.n * m.chunks);
+  const size_t lds = 2 * (size_t)m.C * sizeof(float), lds_g = 2 * (size_t)m.G * sizeof(float);
+  ensure_dynamic_lds((const void*)norm_grid_sums_kernel<T, VEC>, lds + kStaticLds);
+  ensure_dynamic_lds((const void*)norm_grid_grad_kernel<T, VEC>, lds_g + kStaticLds);
+  hipLaunchKernelGGL((norm_grid_sums_kernel<T, VEC>), dim3(blocks), dim3(kThreads), lds, st, m, x, gy, w, b, act, stats,
+                     part_c, part_g);
+  const unsigned extra = gw || gb ? (2 * m.C + kFinishCols - 1) / kFinishCols : 0;
+  hipLaunchKernelGGL((norm_grid_grad_kernel<T, VEC>), dim3(blocks + extra), dim3(kThreads), lds_g, st, m, x, gy, w, b,
+                     act, stats, part_c, part_g, gx, gw, gb, (int64_t)blocks);
+}
+
+}  // namespace
+
+const char* norm_refusal(const NormShape& p, int n_dir, int n_second) {
+  if (p.n < 1 || p.s < 1 || p.C < 1 || p.G < 1) return "empty or negative sizes";
+  if (p.C % p.G) return "the channels do not divide into the groups";
+  if (p.C > kNormChannelsMax) return "more than 8192 channels";
+  if (p.n > (int64_t)1 << 40 || p.s > (int64_t)1 << 24 || p.n * p.s > ((int64_t)1 << 46) / p.C) return "too many values";
+  const bool jets = n_dir || n_second;
+  if (jets && !((n_dir == 2 && n_second == 1) || (n_dir == 6 && n_second == 5))) return "jets of (2, 1) or (6, 5) derivatives only";
+  if (jets && (p.s != 1 || p.C / p.G > 512)) return "jets take one position and at most 512 channels a group";
+  // one block of 256 threads a sample at least, and a launch holds fewer than 2^32 threads
+  if (!rows_kernel_takes(p.s, p.C / p.G) && p.n > (int64_t)1 << 23) return "more than 2^23 samples of many positions";
+  return nullptr;
+}
+
+size_t norm_ws_bytes(const NormShape& p, bool backward) {
+  if (rows_kernel_takes(p.s, p.C / p.G)) {
+    if (!backward) return 0;
+    // lane groups differ with the tensors' alignment: the widest spread of blocks over points any of them gives
+    size_t most = 0;
+    for (int L = 4; L <= 64; L *= 2) {
+      const RowMap m = row_map(p.n, p.C, p.G, L);
+      if (m.npb > 1 && (size_t)m.npb > most) most = m.npb;
+    }
+    return most * 2 * p.C * sizeof(float);
+  }
+  const GridMap m = grid_map(p.n, p.s, p.C, p.G);
+  const size_t blocks = (size_t)m.n * m.chunks;
+  return blocks * m.G * sizeof(float2) + (backward ? blocks * 2 * m.C * sizeof(float) : 0);
+}
+
+bool norm_wants_stats(const NormShape& p) { return !rows_kernel_takes(p.s, p.C / p.G); }
+
+#define PDEKAN_GRID(call)                                                                                      \
+  do {                                                                                                         \
+    switch (dtype) {                                                                                           \
+      case kNormF32: { using T = float; if (vec == 4) { constexpr int V = 4; call; } else { constexpr int V = 1; call; } break; } \
+      case kNormBf16: { using T = __bf16; if (vec == 8) { constexpr int V = 8; call; } else if (vec == 2) { constexpr int V = 2; call; } else { constexpr int V = 1; call; } break; } \
+      default: { using T = _Float16; if (vec == 8) { constexpr int V = 8; call; } else if (vec == 2) { constexpr int V = 2; call; } else { constexpr int V = 1; call; } break; } \
+    }                                                                                                          \
+  } while (0)
+
+void launch_norm_forward(int dtype, const NormShape& p, const void* x, const float* w, const float* b, float eps, int act,
+                         void* y, float* stats, void* ws, hipStream_t st) {
+  if (rows_kernel_takes(p.s, p.C / p.G)) {
+    rows_any<false>(dtype, p, x, nullptr, w, b, eps, act, y, nullptr, nullptr, nullptr, st);
+    return;
+  }
+  const GridMap m = grid_map(p.n, p.s, p.C, p.G);
+  const int vec = vec_width(dtype, p.C, x, y, nullptr);
+  float2* part = static_cast<float2*>(ws);
+  float2* s2 = reinterpret_cast<float2*>(stats);
+  PDEKAN_GRID((grid_forward<T, V>(m, (const T*)x, w, b, eps, act, (T*)y, s2, part, st)));
+}
+
+void launch_norm_backward(int dtype, const NormShape& p, const void* x, const void* gy, const float* w, const float* b,
+                          float eps, int act, const float* stats, void* gx, float* gw, float* gb, void* ws,
+                          hipStream_t st) {
+  if (rows_kernel_takes(p.s, p.C / p.G)) {
+    rows_any<true>(dtype, p, x, gy, w, b, eps, act, gx, gw, gb, static_cast<float*>(ws), st);
+    return;
+  }
+  const GridMap m = grid_map(p.n, p.s, p.C, p.G);
+  const int vec = vec_width(dtype, p.C, x, gy, gx);
+  float2* part_g = static_cast<float2*>(ws);
+  float* part_c = reinterpret_cast<float*>(part_g + (size_t)m.n * m.chunks * m.G);
+  const float2* s2 = reinterpret_cast<const float2*>(stats);
+  PDEKAN_GRID((grid_backward<T, V>(m, (const T*)x, (const T*)gy, w, b, act, s2, (T*)gx, gw, gb, part_c, part_g, st)));
+}
+
+void launch_norm_jet_forward(const NormShape& p, int n_dir, const float* x, const float* w, const float* b, float eps,
+                             int act, float* y, hipStream_t st) {
+  jet_any<false>(p, n_dir, x, nullptr, w, b, eps, act, y, nullptr, nullptr, nullptr, st);
+}
+
+void launch_norm_jet_backward(const NormShape& p, int n_dir, const float* x, const float* gy, const float* w,
+                              const float* b, float eps, int act, float* gx, float* gw, float* gb, void* ws,
+                              hipStream_t st) {
+  jet_any<true>(p, n_dir, x, gy, w, b, eps, act, gx, gw, gb, static_cast<float*>(ws), st);
+}
+
+}  // namespace pdekan

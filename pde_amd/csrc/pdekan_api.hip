@@ -106,6 +106,22 @@ int to_view(const PdekanLayer* l, pdekan::LayerView& v) {
   return PDEKAN_OK;
 }
 
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+// the checks the group-norm entry points share; jets: n_dir or n_second not 0
+int norm_args(const char* what, const pdekan::NormShape& p, int n_dir, int n_second, int dtype, float eps, int act,
+              bool pointers, void* ws, size_t ws_bytes, size_t (*need)(const pdekan::NormShape&, bool), bool backward) {
+  if (!pointers) return fail(PDEKAN_ERR_ARG, "%s: NULL tensor", what);
+  if (dtype < PDEKAN_DTYPE_FP || dtype > PDEKAN_DTYPE_HALF) return fail(PDEKAN_ERR_ARG, "%s: dtype %d unknown", what, dtype);
+  if (act < PDEKAN_ACT_IDENTITY || act > PDEKAN_ACT_TANH) return fail(PDEKAN_ERR_ARG, "%s: act_kind %d unsupported", what, act);
+  if (!(eps >= 0.0f) || eps > 3.0e38f) return fail(PDEKAN_ERR_ARG, "%s: eps must be finite and not negative", what);
+  if (const char* why = pdekan::norm_refusal(p, n_dir, n_second)) return fail(PDEKAN_ERR_ARG, "%s: %s", what, why);
+  const size_t bytes = need ? need(p, backward) : 0;
+  if (bytes && (!ws || ws_bytes < bytes || ((uintptr_t)ws & 255)))
+    return fail(PDEKAN_ERR_WORKSPACE, "%s: workspace of %zu bytes (256-byte aligned) needed, %zu given", what, bytes, ws_bytes);
+  return PDEKAN_OK;
+}
+
 size_t align_up(size_t v, size_t a = 256) { return (v + a - 1) / a * a; }
 
 // the four networks of pdekan_deeponet_step as the kernels' launcher takes them
@@ -1077,6 +1093,77 @@ int pdekan_profile_entry(int idx, char* name, size_t name_cap, double* total_ms,
   if (total_ms) *total_ms = g_prof_sums[idx].ms;
   if (launches) *launches = g_prof_sums[idx].launches;
   return PDEKAN_OK;
+}
+
+size_t pdekan_group_norm_workspace_bytes(int64_t n, int64_t s, int32_t channels, int32_t groups, int32_t backward) {
+  const pdekan::NormShape p{n, s, channels, groups};
+  if (const char* why = pdekan::norm_refusal(p, 0, 0)) { (void)fail(PDEKAN_ERR_ARG, "group_norm: %s", why); return 0; }
+  return pdekan::norm_ws_bytes(p, backward != 0);
+}
+
+int64_t pdekan_group_norm_stats_floats(int64_t n, int64_t s, int32_t channels, int32_t groups) {
+  const pdekan::NormShape p{n, s, channels, groups};
+  if (const char* why = pdekan::norm_refusal(p, 0, 0)) return fail(PDEKAN_ERR_ARG, "group_norm: %s", why);
+  return pdekan::norm_wants_stats(p) ? 2 * n * groups : 0;
+}
+
+int pdekan_group_norm_forward(const void* x, int32_t dtype, int64_t n, int64_t s, int32_t channels, int32_t groups,
+                              const float* weight, const float* bias, float eps, int32_t act_kind, void* y, float* stats,
+                              void* ws, size_t ws_bytes, void* stream) {
+  const pdekan::NormShape p{n, s, channels, groups};
+  const int rc = norm_args("group_norm_forward", p, 0, 0, dtype, eps, act_kind, x && y, ws, ws_bytes,
+                           pdekan::norm_ws_bytes, false);
+  if (rc) return rc;
+  ProfScope prof((hipStream_t)stream, "norm.fwd", 0);
+  pdekan::launch_norm_forward(dtype, p, x, weight, bias, eps, act_kind, y, stats, ws, (hipStream_t)stream);
+  return check_launch("group_norm_forward");
+}
+
+int pdekan_group_norm_backward(const void* x, const void* gy, int32_t dtype, int64_t n, int64_t s, int32_t channels,
+                               int32_t groups, const float* weight, const float* bias, float eps, int32_t act_kind,
+                               const float* stats, void* gx, float* gweight, float* gbias, void* ws, size_t ws_bytes,
+                               void* stream) {
+  const pdekan::NormShape p{n, s, channels, groups};
+  const int rc = norm_args("group_norm_backward", p, 0, 0, dtype, eps, act_kind, x && gy && gx, ws, ws_bytes,
+                           pdekan::norm_ws_bytes, true);
+  if (rc) return rc;
+  if (pdekan::norm_wants_stats(p) && !stats)
+    return fail(PDEKAN_ERR_ARG, "group_norm_backward: this shape needs the statistics of the forward");
+  ProfScope prof((hipStream_t)stream, "norm.bwd", 0);
+  pdekan::launch_norm_backward(dtype, p, x, gy, weight, bias, eps, act_kind, stats, gx, gweight, gbias, ws,
+                               (hipStream_t)stream);
+  return check_launch("group_norm_backward");
+}
+
+int pdekan_group_norm_jet_forward(const float* x_jet, int64_t n, int32_t channels, int32_t groups, int32_t n_dir,
+                                  int32_t n_second, const float* weight, const float* bias, float eps, int32_t act_kind,
+                                  float* y_jet, void* stream) {
+  const pdekan::NormShape p{n, 1, channels, groups};
+  if (n_dir == 0) return fail(PDEKAN_ERR_ARG, "group_norm_jet_forward: jets of (2, 1) or (6, 5) derivatives only");
+  const int rc = norm_args("group_norm_jet_forward", p, n_dir, n_second, PDEKAN_DTYPE_FP, eps, act_kind, x_jet && y_jet,
+                           nullptr, 0, nullptr, false);
+  if (rc) return rc;
+  if (!aligned16(x_jet) || !aligned16(y_jet)) return fail(PDEKAN_ERR_ARG, "group_norm_jet_forward: jets must be 16-byte aligned");
+  ProfScope prof((hipStream_t)stream, "norm_jet.fwd", 0);
+  pdekan::launch_norm_jet_forward(p, n_dir, x_jet, weight, bias, eps, act_kind, y_jet, (hipStream_t)stream);
+  return check_launch("group_norm_jet_forward");
+}
+
+int pdekan_group_norm_jet_backward(const float* x_jet, const float* gy_jet, int64_t n, int32_t channels, int32_t groups,
+                                   int32_t n_dir, int32_t n_second, const float* weight, const float* bias, float eps,
+                                   int32_t act_kind, float* gx_jet, float* gweight, float* gbias, void* ws,
+                                   size_t ws_bytes, void* stream) {
+  const pdekan::NormShape p{n, 1, channels, groups};
+  if (n_dir == 0) return fail(PDEKAN_ERR_ARG, "group_norm_jet_backward: jets of (2, 1) or (6, 5) derivatives only");
+  const int rc = norm_args("group_norm_jet_backward", p, n_dir, n_second, PDEKAN_DTYPE_FP, eps, act_kind,
+                           x_jet && gy_jet && gx_jet, ws, ws_bytes, pdekan::norm_ws_bytes, true);
+  if (rc) return rc;
+  if (!aligned16(x_jet) || !aligned16(gy_jet) || !aligned16(gx_jet))
+    return fail(PDEKAN_ERR_ARG, "group_norm_jet_backward: jets must be 16-byte aligned");
+  ProfScope prof((hipStream_t)stream, "norm_jet.bwd", 0);
+  pdekan::launch_norm_jet_backward(p, n_dir, x_jet, gy_jet, weight, bias, eps, act_kind, gx_jet, gweight, gbias, ws,
+                                   (hipStream_t)stream);
+  return check_launch("group_norm_jet_backward");
 }
 
 }  // extern "C"

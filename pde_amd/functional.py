@@ -16,6 +16,9 @@ from ._lib import PdekanLayer, PdekanLayerGrad
 
 ACT_IDENTITY = 0
 ACT_SILU = 1
+ACT_TANH = 2                      # group norm only
+
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # element types of the group norm and orthogonalize
 
 
 def _require_gpu(t: torch.Tensor, what: str) -> None:
@@ -25,6 +28,20 @@ def _require_gpu(t: torch.Tensor, what: str) -> None:
             "(there is no CPU implementation in this package)")
     if t.dtype != torch.float32:
         raise TypeError(f"pde_amd: {what} must be float32, got {t.dtype}")
+
+
+def _require_gpu_float(t: torch.Tensor, what: str) -> None:
+    if not t.is_cuda:
+        raise RuntimeError(f"pde_amd: {what} is on {t.device}; this operator runs only on a ROCm GPU "
+                           "(there is no CPU implementation in this package)")
+    if t.dtype not in DTYPES:
+        raise TypeError(f"pde_amd: {what} must be float32, bfloat16 or float16, got {t.dtype}")
+
+
+def under_func_transform(*tensors) -> bool:
+    """True while one of the tensors is a torch.func wrapper (grad / vmap / jvp level)."""
+    fn = getattr(torch._C._functorch, "is_functorch_wrapped_tensor", None)
+    return bool(fn and any(t is not None and fn(t) for t in tensors))
 
 
 def _ptr(t: Optional[torch.Tensor]):
@@ -275,3 +292,189 @@ def fit_coefficients(x: torch.Tensor, grid: torch.Tensor, grid_size: int, spline
 def fit_on_device(x: torch.Tensor, grid_size: int, spline_order: int) -> bool:
     """Whether ``fit_coefficients`` takes these samples (float32 on a GPU, cubic splines, at most 20 intervals)."""
     return x.is_cuda and x.dtype == torch.float32 and spline_order == 3 and 1 <= grid_size <= 20 and x.size(0) > 0
+
+
+# ---- group norm with an activation, channels last ---------------------------------------------------------------------
+
+def _norm_check(channels: int, groups: int, weight, bias, eps: float, act: int) -> None:
+    if groups < 1 or channels < 1 or channels % groups:
+        raise ValueError(f"pde_amd: {channels} channels do not divide into {groups} groups")
+    for t, what in ((weight, "weight"), (bias, "bias")):
+        if t is not None and tuple(t.shape) != (channels,):
+            raise ValueError(f"pde_amd: the norm's {what} must have shape ({channels},), got {tuple(t.shape)}")
+    if not 0.0 <= eps < float("inf"):
+        raise ValueError(f"pde_amd: eps must be finite and not negative, got {eps}")
+    if act not in (ACT_IDENTITY, ACT_SILU, ACT_TANH):
+        raise ValueError(f"pde_amd: activation kind {act} unknown")
+
+
+def _group_norm_expression(x, groups, weight, bias, eps, act):
+    """``group_norm_act`` as its defining expression, differentiable to any order and under ``torch.func``."""
+    v = x.reshape(x.size(0), -1, groups, x.size(-1) // groups)
+    if v.dtype in (torch.bfloat16, torch.float16):
+        v = v.float()
+    v = v - v.mean((1, 3), keepdim=True)
+    z = (v * torch.rsqrt((v * v).mean((1, 3), keepdim=True) + eps)).reshape(x.shape)
+    z = z if weight is None else z * weight
+    z = z if bias is None else z + bias
+    z = torch.nn.functional.silu(z) if act == ACT_SILU else torch.tanh(z) if act == ACT_TANH else z
+    return z.to(x.dtype)
+
+
+class _GroupNormAct(torch.autograd.Function):
+    """First-order backward on the kernels; a recorded backward (``create_graph=True``) differentiates the expression."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, groups, eps, act):
+        lib = _lib.load()
+        xd = x.detach().contiguous()
+        w, b = _prep(weight, "weight"), _prep(bias, "bias")
+        n, c = xd.size(0), xd.size(-1)
+        y = torch.empty_like(xd)
+        stats = None
+        if xd.numel():
+            s = xd.numel() // (n * c)
+            with torch.cuda.device(x.device):
+                floats = lib.pdekan_group_norm_stats_floats(n, s, c, groups)
+                if floats < 0:
+                    _lib.check(int(floats))
+                if floats and any(ctx.needs_input_grad[:3]):
+                    stats = torch.empty(floats, dtype=torch.float32, device=x.device)
+                need = lib.pdekan_group_norm_workspace_bytes(n, s, c, groups, 0)
+                ws = _workspace(need, x.device) if need else None
+                _lib.check(lib.pdekan_group_norm_forward(_ptr(xd), DTYPES[xd.dtype], n, s, c, groups, _ptr(w), _ptr(b),
+                                                         eps, act, _ptr(y), _ptr(stats), _ptr(ws), need,
+                                                         _stream(x.device)))
+        ctx.save_for_backward(x, weight, bias, stats)
+        ctx.meta = (groups, eps, act)
+        return y
+
+    @staticmethod
+    def backward(ctx, gy):
+        x, weight, bias, stats = ctx.saved_tensors
+        groups, eps, act = ctx.meta
+        if torch.is_grad_enabled():                    # this backward is being recorded (create_graph=True)
+            with torch.enable_grad():
+                y = _group_norm_expression(x, groups, weight, bias, eps, act)
+                wanted = [i for i in range(3) if ctx.needs_input_grad[i]]
+                got = torch.autograd.grad(y, [(x, weight, bias)[i] for i in wanted], gy, create_graph=True,
+                                          allow_unused=True)
+            out = [None] * 6
+            for i, g in zip(wanted, got):
+                out[i] = g
+            return tuple(out)
+        lib = _lib.load()
+        xd, gd = x.detach().contiguous(), gy.detach().contiguous()
+        w, b = _prep(weight, "weight"), _prep(bias, "bias")
+        n, c = xd.size(0), xd.size(-1)
+        gx = torch.empty_like(xd)
+        gw = torch.empty_like(w) if w is not None and ctx.needs_input_grad[1] else None
+        gb = torch.empty_like(b) if b is not None and ctx.needs_input_grad[2] else None
+        if xd.numel():
+            s = xd.numel() // (n * c)
+            with torch.cuda.device(x.device):
+                need = lib.pdekan_group_norm_workspace_bytes(n, s, c, groups, 1)
+                ws = _workspace(need, x.device) if need else None
+                _lib.check(lib.pdekan_group_norm_backward(_ptr(xd), _ptr(gd), DTYPES[xd.dtype], n, s, c, groups, _ptr(w),
+                                                          _ptr(b), eps, act, _ptr(stats), _ptr(gx), _ptr(gw), _ptr(gb),
+                                                          _ptr(ws), need, _stream(x.device)))
+        else:
+            for g in (gw, gb):
+                if g is not None:
+                    g.zero_()
+        return gx if ctx.needs_input_grad[0] else None, gw, gb, None, None, None
+
+
+def group_norm_act(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] = None,
+                   bias: Optional[torch.Tensor] = None, eps: float = 1e-5, act: int = ACT_IDENTITY) -> torch.Tensor:
+    """``act(group_norm(x) * weight + bias)`` with the channels last.
+
+    ``x`` is ``[N, C]`` or ``[N, ..., C]`` in float32, bfloat16 or float16; the statistics of a group run over the
+    positions of a sample and the ``C / groups`` channels of the group (biased variance), in float32 whatever the type.
+    ``weight`` and ``bias`` are ``[C]`` or None; other types than float32 are converted.  ``act`` is one of
+    ``ACT_IDENTITY``, ``ACT_SILU``, ``ACT_TANH``.  Differentiable in ``x``, ``weight`` and ``bias`` (to any order; beyond the
+    first on tensor code) and usable under ``torch.func`` transforms (tensor code).  At most 8192 channels."""
+    if x.dim() < 2:
+        raise ValueError(f"pde_amd: the norm takes [N, ..., channels], got {tuple(x.shape)}")
+    _norm_check(x.size(-1), groups, weight, bias, eps, act)
+    if under_func_transform(x, weight, bias):
+        return _group_norm_expression(x, groups, weight, bias, eps, act)
+    _require_gpu_float(x, "x")
+    weight = weight if weight is None else weight.to(torch.float32)
+    bias = bias if bias is None else bias.to(torch.float32)
+    _same_device(x, weight, bias)
+    return _GroupNormAct.apply(x, weight, bias, int(groups), float(eps), int(act))
+
+
+def _same_device(x, *others) -> None:
+    for t in others:
+        if t is not None and t.device != x.device:
+            raise RuntimeError(f"pde_amd: tensors on {x.device} and {t.device} in one call")
+
+
+class _GroupNormActJet(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x_jet, weight, bias, groups, eps, act, n_dir, n_second):
+        lib = _lib.load()
+        xd = _aligned(_prep(x_jet, "input"))
+        w, b = _prep(weight, "weight"), _prep(bias, "bias")
+        n, c, _ = xd.shape
+        y = torch.empty_like(xd)
+        if n:
+            with torch.cuda.device(xd.device):
+                _lib.check(lib.pdekan_group_norm_jet_forward(_ptr(xd), n, c, groups, n_dir, n_second, _ptr(w), _ptr(b),
+                                                             eps, act, _ptr(y), _stream(xd.device)))
+        ctx.save_for_backward(x_jet, weight, bias)
+        ctx.meta = (groups, eps, act, n_dir, n_second)
+        return y
+
+    @staticmethod
+    def backward(ctx, gy):
+        if torch.is_grad_enabled():
+            raise RuntimeError("pde_amd: a differentiable backward (create_graph=True) through a norm on jets is not "
+                               "provided; KAN.forward_jet already returns the input derivatives")
+        x_jet, weight, bias = ctx.saved_tensors
+        groups, eps, act, n_dir, n_second = ctx.meta
+        lib = _lib.load()
+        xd, gd = _aligned(_prep(x_jet, "input")), _aligned(_prep(gy, "grad_output"))
+        w, b = _prep(weight, "weight"), _prep(bias, "bias")
+        n, c, _ = xd.shape
+        gx = torch.empty_like(xd)
+        gw = torch.empty_like(w) if w is not None and ctx.needs_input_grad[1] else None
+        gb = torch.empty_like(b) if b is not None and ctx.needs_input_grad[2] else None
+        if n:
+            with torch.cuda.device(xd.device):
+                need = lib.pdekan_group_norm_workspace_bytes(n, 1, c, groups, 1)
+                ws = _workspace(need, xd.device) if need else None
+                _lib.check(lib.pdekan_group_norm_jet_backward(_ptr(xd), _ptr(gd), n, c, groups, n_dir, n_second, _ptr(w),
+                                                              _ptr(b), eps, act, _ptr(gx), _ptr(gw), _ptr(gb), _ptr(ws),
+                                                              need, _stream(xd.device)))
+        else:
+            for g in (gw, gb):
+                if g is not None:
+                    g.zero_()
+        return (gx if ctx.needs_input_grad[0] else None, gw, gb) + (None,) * 5
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """A view at an odd offset as a tensor of its own: the jet kernels read 16 bytes at a time."""
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def group_norm_act_jet(x_jet: torch.Tensor, groups: int, weight: Optional[torch.Tensor] = None,
+                       bias: Optional[torch.Tensor] = None, eps: float = 1e-5, act: int = ACT_IDENTITY, n_dir: int = 2,
+                       n_second: int = 1) -> torch.Tensor:
+    """:func:`group_norm_act` of points ``[N, C]`` on their jets ``[N, C, 1 + n_dir + n_second]`` (float32): the value and,
+    by the chain rule through the statistics, its derivatives, as ``KAN.forward_jet`` carries them.
+    (``n_dir``, ``n_second``) is (0, 0), (2, 1) or (6, 5); at most 512 channels a group for the latter two."""
+    if x_jet.dim() != 3 or x_jet.size(2) != 1 + n_dir + n_second or (n_dir, n_second) not in ((0, 0), (2, 1), (6, 5)):
+        raise ValueError(f"pde_amd: jets [N, C, 1 + n_dir + n_second] of (0, 0), (2, 1) or (6, 5) derivatives wanted, got "
+                         f"{tuple(x_jet.shape)} with ({n_dir}, {n_second})")
+    if n_dir == 0:
+        return group_norm_act(x_jet.squeeze(-1), groups, weight, bias, eps, act).unsqueeze(-1)
+    _norm_check(x_jet.size(1), groups, weight, bias, eps, act)
+    _require_gpu(x_jet, "x_jet")
+    weight = weight if weight is None else weight.to(torch.float32)
+    bias = bias if bias is None else bias.to(torch.float32)
+    _same_device(x_jet, weight, bias)
+    return _GroupNormActJet.apply(x_jet, weight, bias, int(groups), float(eps), int(act), int(n_dir), int(n_second))
