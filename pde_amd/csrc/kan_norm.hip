@@ -25,13 +25,16 @@ template <typename T, int N> struct VecOf { typedef T type __attribute__((ext_ve
 template <typename T> struct VecOf<T, 1> { typedef T type; };
 
 template <typename T, int N>
-__device__ __forceinline__ void load_vec(const T* p, float (&v)[N]) {
-  const typename VecOf<T, N>::type r = *reinterpret_cast<const typename VecOf<T, N>::type*>(p);
+__device__ __forceinline__ void widen(const typename VecOf<T, N>::type& r, float (&v)[N]) {
   if constexpr (N == 1) v[0] = (float)r;
   else {
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = (float)r[i];
   }
+}
+template <typename T, int N>
+__device__ __forceinline__ void load_vec(const T* p, float (&v)[N]) {
+  widen<T, N>(*reinterpret_cast<const typename VecOf<T, N>::type*>(p), v);
 }
 template <typename T, int N>
 __device__ __forceinline__ void store_vec(T* p, const float (&v)[N]) {
@@ -59,9 +62,9 @@ __device__ __forceinline__ float group_sum(float v) {
 // f and its first ORDER derivatives at u.
 //   tanh: 1 - 2 / (exp(2u) + 1), which loses relative accuracy near 0, and below |u| = 0.25 the Taylor polynomial of
 //   degree 9 (the first term left out is 9e-9 of the result there)
-template <int ORDER>
-__device__ __forceinline__ void activation(int act, float u, float (&f)[ORDER + 1]) {
-  if (act == kNormActTanh) {
+template <int ACT, int ORDER>
+__device__ __forceinline__ void activation(float u, float (&f)[ORDER + 1]) {
+  if constexpr (ACT == kNormActTanh) {
     const float u2 = u * u;
     const float far = 1.0f - 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(u * 2.885390081777927f) + 1.0f);
     const float near =
@@ -71,7 +74,7 @@ __device__ __forceinline__ void activation(int act, float u, float (&f)[ORDER + 
     if constexpr (ORDER >= 1) f[1] = 1.0f - t * t;
     if constexpr (ORDER >= 2) f[2] = -2.0f * t * f[1];
     if constexpr (ORDER >= 3) f[3] = f[1] * (6.0f * t * t - 2.0f);
-  } else if (act == kNormActSilu) {
+  } else if constexpr (ACT == kNormActSilu) {
     const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(u * -1.4426950408889634f));
     f[0] = u * s;
     if constexpr (ORDER >= 1) {
@@ -88,10 +91,19 @@ __device__ __forceinline__ void activation(int act, float u, float (&f)[ORDER + 
   }
 }
 
-// Which (point, group) a lane group of a rows kernel takes.  A block holds 256 / L lane groups: `gpb` groups of `ppb`
-// points; blocks that share a range of groups walk the points with stride npb * ppb, so a lane keeps its channels (their
-// weights and the sums of their gradients stay in registers).
-struct RowMap { int64_t n; int C, G, cpg, gpb, ppb, gchunks, npb; };
+// body(IntC<kind>) for the activation `act`, which is the same in the whole grid: one branch a kernel, not one a value
+template <int V> struct IntC { static constexpr int value = V; };
+template <typename F>
+__device__ __forceinline__ void by_activation(int act, F&& body) {
+  if (act == kNormActTanh) body(IntC<kNormActTanh>{});
+  else if (act == kNormActSilu) body(IntC<kNormActSilu>{});
+  else body(IntC<kNormActIdentity>{});
+}
+
+// Which (sample, group) a lane group of a rows kernel takes.  A block holds 256 / L lane groups: `gpb` groups of `ppb`
+// samples; blocks that share a range of groups walk the samples with stride npb * ppb, so a lane keeps its channels
+// (their weights and the sums of their gradients stay in registers).  A sample has s positions (jets: one).
+struct RowMap { int64_t n; int s, C, G, cpg, gpb, ppb, gchunks, npb; };
 
 struct RowPlace { int g, pi; int64_t p, step; bool on; };
 template <int L>
@@ -108,8 +120,8 @@ __device__ __forceinline__ RowPlace row_place(const RowMap& m) {
   return r;
 }
 
-// The block's sums of gw / gb over its points, in a fixed order: row npb of part [npb][2][C] (npb = 1: gw and gb
-// themselves).  Lane groups of the same group of channels sit gpb slots apart.
+// The block's sums of gw / gb over its samples, in a fixed order, into a row of part [npb * s][2][C] for each position
+// (npb * s = 1: gw and gb themselves).  Lane groups of the same group of channels sit gpb slots apart.
 template <int N, int L>
 __device__ __forceinline__ void row_grad_out(const RowMap& m, const RowPlace& r, const float (&gw)[N], const float (&gb)[N],
                                              int c0, bool valid, float* part_w, float* part_b, float (*red)[N + 1]) {
@@ -136,25 +148,33 @@ __global__ void __launch_bounds__(kThreads) norm_rows_kernel(RowMap m, const T* 
                                                              const float* __restrict__ w, const float* __restrict__ b,
                                                              float eps, int act, T* __restrict__ out,
                                                              float* part_w, float* part_b, int part_stride) {
+  __shared__ float red[BWD ? kThreads : 1][VEC + 1];
   const RowPlace r = row_place<L>(m);
   const int lane = threadIdx.x % L;
-  const float inv = 1.0f / (float)m.cpg;
+  const float inv = 1.0f / (float)(m.cpg * m.s);
+  const int nvg = m.cpg / VEC, nv = nvg * m.s;
   bool valid[K];
+  int off[K], pos[K];
   float wv[K][VEC], bv[K][VEC], gwv[K][VEC], gbv[K][VEC];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    valid[k] = r.on && (lane + L * k) * VEC < m.cpg;
+    const int v = lane + L * k;
+    valid[k] = r.on && v < nv;
+    pos[k] = m.s == 1 ? 0 : v / nvg;
+    const int c0 = r.g * m.cpg + (v - pos[k] * nvg) * VEC;
+    off[k] = pos[k] * m.C + c0;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
-      const int c = r.g * m.cpg + (lane + L * k) * VEC + i;
-      wv[k][i] = valid[k] && w ? w[c] : 1.0f;
-      bv[k][i] = valid[k] && b ? b[c] : 0.0f;
+      wv[k][i] = valid[k] && w ? w[c0 + i] : 1.0f;
+      bv[k][i] = valid[k] && b ? b[c0 + i] : 0.0f;
       gwv[k][i] = gbv[k][i] = 0.0f;
     }
   }
-  if (r.on) {
+  by_activation(act, [&](auto kind) {
+    constexpr int ACT = decltype(kind)::value;
+    if (!r.on) return;
     for (int64_t p = r.p; p < m.n; p += r.step) {
-      const int64_t at = p * m.C + (int64_t)r.g * m.cpg + lane * VEC;
+      const int64_t at = p * m.s * m.C;
       float e[K][VEC], q[K][VEC];
       float s = 0.0f;
 #pragma unroll
@@ -162,8 +182,8 @@ __global__ void __launch_bounds__(kThreads) norm_rows_kernel(RowMap m, const T* 
 #pragma unroll
         for (int i = 0; i < VEC; ++i) e[k][i] = q[k][i] = 0.0f;
         if (valid[k]) {
-          load_vec<T, VEC>(x + at + L * k * VEC, e[k]);
-          if constexpr (BWD) load_vec<T, VEC>(gy + at + L * k * VEC, q[k]);
+          load_vec<T, VEC>(x + at + off[k], e[k]);
+          if constexpr (BWD) load_vec<T, VEC>(gy + at + off[k], q[k]);
         }
 #pragma unroll
         for (int i = 0; i < VEC; ++i) s += e[k][i];
@@ -184,10 +204,10 @@ __global__ void __launch_bounds__(kThreads) norm_rows_kernel(RowMap m, const T* 
 #pragma unroll
           for (int i = 0; i < VEC; ++i) {
             float f[1];
-            activation<0>(act, fmaf(e[k][i] * rs, wv[k][i], bv[k][i]), f);
+            activation<ACT, 0>(fmaf(e[k][i] * rs, wv[k][i], bv[k][i]), f);
             e[k][i] = f[0];
           }
-          if (valid[k]) store_vec<T, VEC>(out + at + L * k * VEC, e[k]);
+          if (valid[k]) store_vec<T, VEC>(out + at + off[k], e[k]);
         }
       } else {
         float s1 = 0.0f, s2 = 0.0f;
@@ -197,7 +217,7 @@ __global__ void __launch_bounds__(kThreads) norm_rows_kernel(RowMap m, const T* 
           for (int i = 0; i < VEC; ++i) {
             const float z = e[k][i] * rs;
             float f[2];
-            activation<1>(act, fmaf(z, wv[k][i], bv[k][i]), f);
+            activation<ACT, 1>(fmaf(z, wv[k][i], bv[k][i]), f);
             const float pv = q[k][i] * f[1];
             gbv[k][i] += pv;
             gwv[k][i] = fmaf(pv, z, gwv[k][i]);
@@ -212,19 +232,20 @@ __global__ void __launch_bounds__(kThreads) norm_rows_kernel(RowMap m, const T* 
         for (int k = 0; k < K; ++k) {
 #pragma unroll
           for (int i = 0; i < VEC; ++i) e[k][i] = rs * (q[k][i] - s1 - e[k][i] * s2);
-          if (valid[k]) store_vec<T, VEC>(out + at + L * k * VEC, e[k]);
+          if (valid[k]) store_vec<T, VEC>(out + at + off[k], e[k]);
         }
       }
     }
-  }
+  });
   if constexpr (BWD) {
     if (part_w || part_b) {
-      __shared__ float red[kThreads][VEC + 1];
-      const int64_t row = (int64_t)(blockIdx.x / m.gchunks) * part_stride;
+      const int64_t row = (int64_t)(blockIdx.x / m.gchunks) * m.s;
 #pragma unroll
-      for (int k = 0; k < K; ++k)
-        row_grad_out<VEC, L>(m, r, gwv[k], gbv[k], r.g * m.cpg + (lane + L * k) * VEC, valid[k],
-                             part_w ? part_w + row : nullptr, part_b ? part_b + row : nullptr, red);
+      for (int k = 0; k < K; ++k) {
+        const int64_t at = (row + pos[k]) * part_stride;
+        row_grad_out<VEC, L>(m, r, gwv[k], gbv[k], off[k] - pos[k] * m.C, valid[k], part_w ? part_w + at : nullptr,
+                             part_b ? part_b + at : nullptr, red);
+      }
     }
   }
 }
@@ -261,7 +282,9 @@ __global__ void __launch_bounds__(kThreads) norm_jet_kernel(RowMap m, const floa
     bv[k] = valid[k] && b ? b[c] : 0.0f;
     gwv[k] = gbv[k] = 0.0f;
   }
-  if (r.on) {
+  by_activation(act, [&](auto kind) {
+    constexpr int ACT = decltype(kind)::value;
+    if (!r.on) return;
     for (int64_t p = r.p; p < m.n; p += r.step) {
       const int64_t at = (p * m.C + (int64_t)r.g * m.cpg + lane) * J;
       float e[K][J], h[K][J];
@@ -324,7 +347,7 @@ __global__ void __launch_bounds__(kThreads) norm_jet_kernel(RowMap m, const floa
 #pragma unroll
         for (int k = 0; k < K; ++k) {
           float f[3], y[J];
-          activation<2>(act, fmaf(e[k][0] * rs, wv[k], bv[k]), f);
+          activation<ACT, 2>(fmaf(e[k][0] * rs, wv[k], bv[k]), f);
           y[0] = f[0];
 #pragma unroll
           for (int d = 0; d < ND; ++d) {
@@ -355,7 +378,7 @@ __global__ void __launch_bounds__(kThreads) norm_jet_kernel(RowMap m, const floa
         for (int k = 0; k < K; ++k) {
           const float z = e[k][0] * rs;
           float f[4];
-          activation<3>(act, fmaf(z, wv[k], bv[k]), f);
+          activation<ACT, 3>(fmaf(z, wv[k], bv[k]), f);
           float gu = f[1] * h[k][0], gw = 0.0f;
 #pragma unroll
           for (int d = 0; d < ND; ++d) {
@@ -433,10 +456,10 @@ __global__ void __launch_bounds__(kThreads) norm_jet_kernel(RowMap m, const floa
         }
       }
     }
-  }
+  });
   if constexpr (BWD) {
+    __shared__ float red[kThreads][2];
     if (part_w || part_b) {
-      __shared__ float red[kThreads][2];
       const int64_t row = (int64_t)(blockIdx.x / m.gchunks) * part_stride;
 #pragma unroll
       for (int k = 0; k < K; ++k) {
@@ -448,30 +471,38 @@ __global__ void __launch_bounds__(kThreads) norm_jet_kernel(RowMap m, const floa
   }
 }
 
-// out_w[c], out_b[c] = sums over the rows of part [rows][2][C], in a fixed order: 32 columns x 32 row slices a block
-constexpr int kFinishCols = 32, kFinishSlices = 32;
+// out_w[c], out_b[c] = sums over the rows of part [rows][2][C], in a fixed order: a block takes COLS columns, THREADS / COLS
+// threads a column, eight loads of a thread in flight
+template <int COLS, int THREADS>
 __device__ __forceinline__ void finish_columns(int col_block, const float* __restrict__ part, int64_t rows, int C,
-                                               float* out_w, float* out_b, int threads) {
-  __shared__ float red[kFinishSlices][kFinishCols + 1];
-  const int cl = threadIdx.x % kFinishCols, slices = threads / kFinishCols, sl = threadIdx.x / kFinishCols;
-  const int col = col_block * kFinishCols + cl;
+                                               float* out_w, float* out_b) {
+  constexpr int kSlices = THREADS / COLS;
+  __shared__ float red[kSlices][COLS + 1];
+  const int cl = threadIdx.x % COLS, sl = threadIdx.x / COLS;
+  const int col = col_block * COLS + cl;
   float s = 0.0f;
-  if (col < 2 * C)
-    for (int64_t i = sl; i < rows; i += slices) s += part[i * 2 * C + col];
+  if (col < 2 * C) {
+#pragma unroll 8
+    for (int64_t i = sl; i < rows; i += kSlices) s += part[i * 2 * C + col];
+  }
   red[sl][cl] = s;
   __syncthreads();
   if (sl == 0 && col < 2 * C) {
-    for (int i = 1; i < slices; ++i) s += red[i][cl];
+#pragma unroll
+    for (int i = 1; i < kSlices; ++i) s += red[i][cl];
     float* out = col < C ? out_w : out_b;
     if (out) out[col < C ? col : col - C] = s;
   }
 }
+constexpr int kFinishCols = 32, kGridFinishCols = 8;
 __global__ void __launch_bounds__(1024) norm_finish_kernel(const float* __restrict__ part, int64_t rows, int C,
                                                            float* out_w, float* out_b) {
-  finish_columns(blockIdx.x, part, rows, C, out_w, out_b, 1024);
+  finish_columns<kFinishCols, 1024>(blockIdx.x, part, rows, C, out_w, out_b);
 }
 
 // ---- samples of many positions ------------------------------------------------------------------------------------
+
+constexpr int kAhead = 4;              // rows a thread of the second launches loads before the sums are merged
 
 // A block takes one chunk of positions of one sample and all its channels: thread = (vector of channels, row slot).
 struct GridMap { int64_t n, s, rows; int C, G, cpg, chunks; };   // rows: positions a chunk (the last may have fewer)
@@ -513,7 +544,7 @@ __global__ void __launch_bounds__(kThreads) norm_grid_stats_kernel(GridMap m, co
     for (int i = 0; i < VEC; ++i) k[i] = s1[i] = s2[i] = 0.0f;
     if (on) {
       load_vec<T, VEC>(base + t.row0 * m.C + vec * VEC, k);
-#pragma unroll 4
+#pragma unroll 8
       for (int64_t row = t.row0 + t.ty; row < t.row1; row += t.tyn) {
         float v[VEC];
         load_vec<T, VEC>(base + row * m.C + vec * VEC, v);
@@ -557,30 +588,37 @@ __global__ void __launch_bounds__(kThreads) norm_grid_stats_kernel(GridMap m, co
   }
 }
 
-// mean and r of every group of a sample from its chunks' partial statistics, into LDS (and to stats, from one block)
-__device__ __forceinline__ void merge_stats(const GridMap& m, int64_t sample, const float2* __restrict__ part, float eps,
-                                            float* mu, float* rs, float2* stats) {
-  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
-  for (int g = wave; g < m.G; g += kThreads / 64) {
-    float mean = 0.0f, q = 0.0f, cnt = 0.0f;
-    if (lane < m.chunks) {
-      const float2 v = part[(sample * m.chunks + lane) * m.G + g];
-      const int64_t left = m.s - lane * m.rows;
-      cnt = (float)(left < m.rows ? left : m.rows);
-      mean = v.x;
-      q = v.y;
+__device__ __forceinline__ float chunk_rows(const GridMap& m, int chunk) {
+  const int64_t left = m.s - chunk * m.rows;
+  return (float)(left < m.rows ? left : m.rows);
+}
+
+// Sums over a sample's chunks of two numbers a (chunk, group), part [chunks][G], each group's by 256 / G threads (loads of
+// all chunks in flight at once, neighbouring threads on neighbouring groups): term(chunk, value, first chunk's value)
+// adds to s.  take(g, s, first) gets the totals, one thread a group.
+template <typename Term, typename Take>
+__device__ __forceinline__ void merge_chunks(const GridMap& m, const float2* __restrict__ part, float2 (*red), Term term,
+                                             Take take) {
+  const int gw = m.G < kThreads ? m.G : kThreads, per = kThreads / gw;
+  const int gl = threadIdx.x % gw, sub = threadIdx.x / gw;
+  for (int g0 = 0; g0 < m.G; g0 += gw) {
+    const int g = g0 + gl;
+    float2 s = make_float2(0.0f, 0.0f), first = s;
+    if (g < m.G && sub < per) {
+      first = part[g];
+#pragma unroll 8
+      for (int k = sub; k < m.chunks; k += per) term(k, part[(int64_t)k * m.G + g], first, s);
     }
-    const float total = (float)m.s;
-    // about the first chunk's mean: the sum of the differences carries no offset
-    const float first = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(mean)));
-    const float all = first + wave_sum(lane < m.chunks ? cnt * (mean - first) : 0.0f) / total;
-    const float d = mean - all;
-    q = wave_sum(lane < m.chunks ? fmaf(cnt * (float)m.cpg * d, d, q) : 0.0f);
-    const float r = rsqrtf(q / (total * (float)m.cpg) + eps);
-    if (lane == 0) {
-      mu[g] = all;
-      rs[g] = r;
-      if (stats) stats[sample * m.G + g] = make_float2(all, r);
+    __syncthreads();
+    red[threadIdx.x] = s;
+    __syncthreads();
+    if (g < m.G && sub == 0) {
+      for (int i = 1; i < per; ++i) {
+        const float2 o = red[gl + i * gw];
+        s.x += o.x;
+        s.y += o.y;
+      }
+      take(g, s, first);
     }
   }
 }
@@ -592,11 +630,34 @@ __global__ void __launch_bounds__(kThreads) norm_grid_apply_kernel(GridMap m, co
                                                                    const float2* __restrict__ part, T* __restrict__ y,
                                                                    float2* stats) {
   extern __shared__ float chan[];                     // [2][G]
+  __shared__ float2 red[kThreads];
   float *mu = chan, *rs = chan + m.G;
   const GridThread<VEC> t(m, blockIdx.x);
-  merge_stats(m, t.sample, part, eps, mu, rs, t.chunk == 0 ? stats : nullptr);
-  __syncthreads();
   const int64_t base = t.sample * m.s * m.C;
+  // a thread's first rows are on their way while the statistics are merged
+  typedef typename VecOf<T, VEC>::type Raw;
+  Raw ahead[kAhead];
+  const bool first_on = t.ty < t.tyn && t.tx < t.nv;
+#pragma unroll
+  for (int j = 0; j < kAhead; ++j) {
+    const int64_t row = t.row0 + t.ty + j * t.tyn;
+    if (first_on && row < t.row1) ahead[j] = *reinterpret_cast<const Raw*>(x + base + row * m.C + t.tx * VEC);
+  }
+  // mean and r of the sample's groups, about the first chunk's mean (one of the means: see the stats kernel)
+  const float total = (float)m.s, width = (float)m.cpg;
+  merge_chunks(m, part + t.sample * m.chunks * m.G, red,
+               [&](int k, float2 v, float2 first, float2& s) {
+                 const float cnt = chunk_rows(m, k), d = v.x - first.x;
+                 s.x = fmaf(cnt, d, s.x);
+                 s.y += fmaf(cnt * width * d, d, v.y);
+               },
+               [&](int g, float2 s, float2 first) {
+                 const float d = s.x / total, var = fmaxf(fmaf(-d * width, s.x, s.y), 0.0f) / (total * width);
+                 mu[g] = first.x + d;
+                 rs[g] = rsqrtf(var + eps);
+                 if (t.chunk == 0 && stats) stats[t.sample * m.G + g] = make_float2(mu[g], rs[g]);
+               });
+  __syncthreads();
   for (int tile = 0; tile < t.nv; tile += t.txn) {
     const int vec = tile + t.tx;
     if (t.ty >= t.tyn || vec >= t.nv) continue;
@@ -608,18 +669,28 @@ __global__ void __launch_bounds__(kThreads) norm_grid_apply_kernel(GridMap m, co
       bv[i] = b ? b[c] : 0.0f;
       mean[i] = mu[g];
     }
-#pragma unroll 4
-    for (int64_t row = t.row0 + t.ty; row < t.row1; row += t.tyn) {
-      float v[VEC];
-      load_vec<T, VEC>(x + base + row * m.C + vec * VEC, v);
+    by_activation(act, [&](auto kind) {
+      constexpr int ACT = decltype(kind)::value;
+      auto one = [&](int64_t row, const Raw& raw) {
+        float v[VEC];
+        widen<T, VEC>(raw, v);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        float f[1];
-        activation<0>(act, fmaf(v[i] - mean[i], wr[i], bv[i]), f);
-        v[i] = f[0];
+        for (int i = 0; i < VEC; ++i) {
+          float f[1];
+          activation<ACT, 0>(fmaf(v[i] - mean[i], wr[i], bv[i]), f);
+          v[i] = f[0];
+        }
+        store_vec<T, VEC>(y + base + row * m.C + vec * VEC, v);
+      };
+      int64_t row = t.row0 + t.ty;
+      if (tile == 0) {
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j, row += t.tyn)
+          if (row < t.row1) one(row, ahead[j]);
       }
-      store_vec<T, VEC>(y + base + row * m.C + vec * VEC, v);
-    }
+#pragma unroll 4
+      for (; row < t.row1; row += t.tyn) one(row, *reinterpret_cast<const Raw*>(x + base + row * m.C + vec * VEC));
+    });
   }
 }
 
@@ -653,21 +724,24 @@ __global__ void __launch_bounds__(kThreads) norm_grid_sums_kernel(GridMap m, con
         mean[i] = st.x;
         rs[i] = st.y;
       }
+      by_activation(act, [&](auto kind) {
+        constexpr int ACT = decltype(kind)::value;
 #pragma unroll 2
-      for (int64_t row = t.row0 + t.ty; row < t.row1; row += t.tyn) {
-        float v[VEC], g[VEC];
-        load_vec<T, VEC>(x + base + row * m.C + vec * VEC, v);
-        load_vec<T, VEC>(gy + base + row * m.C + vec * VEC, g);
+        for (int64_t row = t.row0 + t.ty; row < t.row1; row += t.tyn) {
+          float v[VEC], g[VEC];
+          load_vec<T, VEC>(x + base + row * m.C + vec * VEC, v);
+          load_vec<T, VEC>(gy + base + row * m.C + vec * VEC, g);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const float z = (v[i] - mean[i]) * rs[i];
-          float f[2];
-          activation<1>(act, fmaf(z, wv[i], bv[i]), f);
-          const float p = g[i] * f[1];
-          s1[i] += p;
-          s2[i] = fmaf(p, z, s2[i]);
+          for (int i = 0; i < VEC; ++i) {
+            const float z = (v[i] - mean[i]) * rs[i];
+            float f[2];
+            activation<ACT, 1>(fmaf(z, wv[i], bv[i]), f);
+            const float p = g[i] * f[1];
+            s1[i] += p;
+            s2[i] = fmaf(p, z, s2[i]);
+          }
         }
-      }
+      });
     }
     __syncthreads();
 #pragma unroll
@@ -702,7 +776,7 @@ __global__ void __launch_bounds__(kThreads) norm_grid_sums_kernel(GridMap m, con
   }
 }
 
-// Backward, launch 2: gx from the merged sums of the sample; blocks past the last chunk sum gw and gb over all chunks
+// Backward, launch 2: gx from the merged sums of the sample; the first blocks sum gw and gb over all chunks instead
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kThreads) norm_grid_grad_kernel(GridMap m, const T* __restrict__ x,
                                                                   const T* __restrict__ gy, const float* __restrict__ w,
@@ -710,23 +784,31 @@ __global__ void __launch_bounds__(kThreads) norm_grid_grad_kernel(GridMap m, con
                                                                   const float2* __restrict__ stats,
                                                                   const float* __restrict__ part_c,
                                                                   const float2* __restrict__ part_g, T* __restrict__ gx,
-                                                                  float* gw, float* gb, int64_t main_blocks) {
+                                                                  float* gw, float* gb, int finish_blocks) {
   extern __shared__ float chan[];                     // [2][G]
-  if ((int64_t)blockIdx.x >= main_blocks) {
-    finish_columns((int)(blockIdx.x - main_blocks), part_c, m.n * m.chunks, m.C, gw, gb, kThreads);
+  __shared__ float2 red[kThreads];
+  if ((int)blockIdx.x < finish_blocks) {
+    finish_columns<kGridFinishCols, kThreads>(blockIdx.x, part_c, m.n * m.chunks, m.C, gw, gb);
     return;
   }
-  const GridThread<VEC> t(m, blockIdx.x);
-  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
-  const float inv = 1.0f / ((float)m.s * (float)m.cpg);
-  for (int g = wave; g < m.G; g += kThreads / 64) {
-    float2 v = make_float2(0.0f, 0.0f);
-    if (lane < m.chunks) v = part_g[(t.sample * m.chunks + lane) * m.G + g];
-    const float a = wave_sum(v.x) * inv, q = wave_sum(v.y) * inv;
-    if (lane == 0) { chan[g] = a; chan[m.G + g] = q; }
-  }
-  __syncthreads();
+  const GridThread<VEC> t(m, blockIdx.x - finish_blocks);
   const int64_t base = t.sample * m.s * m.C;
+  typedef typename VecOf<T, VEC>::type Raw;
+  Raw ahead_x[kAhead], ahead_g[kAhead];
+  const bool first_on = t.ty < t.tyn && t.tx < t.nv;
+#pragma unroll
+  for (int j = 0; j < kAhead; ++j) {
+    const int64_t row = t.row0 + t.ty + j * t.tyn;
+    if (first_on && row < t.row1) {
+      ahead_x[j] = *reinterpret_cast<const Raw*>(x + base + row * m.C + t.tx * VEC);
+      ahead_g[j] = *reinterpret_cast<const Raw*>(gy + base + row * m.C + t.tx * VEC);
+    }
+  }
+  const float inv = 1.0f / ((float)m.s * (float)m.cpg);
+  merge_chunks(m, part_g + t.sample * m.chunks * m.G, red,
+               [&](int, float2 v, float2, float2& s) { s.x += v.x; s.y += v.y; },
+               [&](int g, float2 s, float2) { chan[g] = s.x * inv; chan[m.G + g] = s.y * inv; });
+  __syncthreads();
   for (int tile = 0; tile < t.nv; tile += t.txn) {
     const int vec = tile + t.tx;
     if (t.ty >= t.tyn || vec >= t.nv) continue;
@@ -742,52 +824,66 @@ __global__ void __launch_bounds__(kThreads) norm_grid_grad_kernel(GridMap m, con
       a[i] = chan[g];
       q[i] = chan[m.G + g];
     }
-#pragma unroll 2
-    for (int64_t row = t.row0 + t.ty; row < t.row1; row += t.tyn) {
-      float v[VEC], g[VEC];
-      load_vec<T, VEC>(x + base + row * m.C + vec * VEC, v);
-      load_vec<T, VEC>(gy + base + row * m.C + vec * VEC, g);
+    by_activation(act, [&](auto kind) {
+      constexpr int ACT = decltype(kind)::value;
+      auto one = [&](int64_t row, const Raw& rx, const Raw& rg) {
+        float v[VEC], g[VEC];
+        widen<T, VEC>(rx, v);
+        widen<T, VEC>(rg, g);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const float z = (v[i] - mean[i]) * rs[i];
-        float f[2];
-        activation<1>(act, fmaf(z, wv[i], bv[i]), f);
-        v[i] = rs[i] * (g[i] * f[1] * wv[i] - a[i] - z * q[i]);
+        for (int i = 0; i < VEC; ++i) {
+          const float z = (v[i] - mean[i]) * rs[i];
+          float f[2];
+          activation<ACT, 1>(fmaf(z, wv[i], bv[i]), f);
+          v[i] = rs[i] * (g[i] * f[1] * wv[i] - a[i] - z * q[i]);
+        }
+        store_vec<T, VEC>(gx + base + row * m.C + vec * VEC, v);
+      };
+      int64_t row = t.row0 + t.ty;
+      if (tile == 0) {
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j, row += t.tyn)
+          if (row < t.row1) one(row, ahead_x[j], ahead_g[j]);
       }
-      store_vec<T, VEC>(gx + base + row * m.C + vec * VEC, v);
-    }
+#pragma unroll 2
+      for (; row < t.row1; row += t.tyn)
+        one(row, *reinterpret_cast<const Raw*>(x + base + row * m.C + vec * VEC),
+            *reinterpret_cast<const Raw*>(gy + base + row * m.C + vec * VEC));
+    });
   }
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------------
 
 constexpr int kRowBlocks = 2048;       // 8 blocks of 4 waves a compute unit
-constexpr int kGridBlocks = 1024, kChunksMax = 64;
+constexpr int kGridBlocks = 1024, kChunksMax = 128;
 constexpr size_t kStaticLds = 20 * 1024;   // at least what the grid kernels declare besides the per-channel sums
 
 int pow2_at_least(int v) { int p = 1; while (p < v) p *= 2; return p; }
 
-RowMap row_map(int64_t n, int C, int G, int L) {
+RowMap row_map(int64_t n, int s, int C, int G, int L) {
   RowMap m;
-  m.n = n; m.C = C; m.G = G; m.cpg = C / G;
+  m.n = n; m.s = s; m.C = C; m.G = G; m.cpg = C / G;
   const int rpb = kThreads / L;
   if (G <= rpb) { m.gpb = G; m.ppb = rpb / G; m.gchunks = 1; }
   else { m.gpb = rpb; m.ppb = 1; m.gchunks = (G + rpb - 1) / rpb; }
   if (m.ppb > n) m.ppb = (int)n;
-  const int64_t need = (n + m.ppb - 1) / m.ppb, most = kRowBlocks / m.gchunks > 0 ? kRowBlocks / m.gchunks : 1;
+  // with several positions the partial gradients take a row each: fewer blocks, but one a compute unit at least
+  const int blocks = s == 1 ? kRowBlocks : kRowBlocks / s > 256 ? kRowBlocks / s : 256;
+  const int64_t need = (n + m.ppb - 1) / m.ppb, most = blocks / m.gchunks > 0 ? blocks / m.gchunks : 1;
   m.npb = (int)(need < most ? need : most);
   return m;
 }
 
-// vector width, lanes and vectors a lane of a group of cpg channels; K = 0: too many channels for the rows kernels
+// lanes and vectors a lane of a group of `values` values
 struct RowShape { int vec, L, K; };
-RowShape row_shape(int cpg, int vec) {
-  const int nv = cpg / vec;
+RowShape row_shape(int values, int vec) {
+  const int nv = values / vec;
   int L = pow2_at_least(nv);
   if (L < 4) L = 4;
   if (L > 64) L = 64;
   const int K = pow2_at_least((nv + L - 1) / L);
-  return {vec, L, K > 8 ? 0 : K};
+  return {vec, L, K};
 }
 
 int elem_size(int dtype) { return dtype == kNormF32 ? 4 : 2; }
@@ -807,8 +903,8 @@ GridMap grid_map(int64_t n, int64_t s, int C, int G) {
   GridMap m;
   m.n = n; m.s = s; m.C = C; m.G = G; m.cpg = C / G;
   int64_t chunks = (kGridBlocks + n - 1) / n;
-  // a chunk of at least 16 KB at two bytes a value: shorter ones cost more in their partial results than they spread
-  const int64_t least = (8192 + C - 1) / C;
+  // a chunk of at least 4096 values: shorter ones cost more in their partial results than they spread
+  const int64_t least = (4096 + C - 1) / C;
   if (chunks > s / least) chunks = s / least;
   if (chunks > kChunksMax) chunks = kChunksMax;
   if (chunks < 1) chunks = 1;
@@ -817,8 +913,8 @@ GridMap grid_map(int64_t n, int64_t s, int C, int G) {
   return m;
 }
 
-// 512 channels: with one element a vector (the least aligned tensors) the 64 lanes of a wave still hold a group
-bool rows_kernel_takes(int64_t s, int cpg) { return s == 1 && cpg <= 512; }
+// 512 values a group: with one element a vector (the least aligned tensors) the 64 lanes of a wave still hold it
+bool rows_kernel_takes(int64_t s, int cpg) { return s <= 32 && s * cpg <= 512; }
 
 template <typename T, int VEC, bool BWD>
 void run_rows(const RowShape& sh, const RowMap& m, const T* x, const T* gy, const float* w, const float* b, float eps,
@@ -852,10 +948,10 @@ template <bool BWD>
 void rows_any(int dtype, const NormShape& p, const void* x, const void* gy, const float* w, const float* b, float eps,
               int act, void* out, float* gw, float* gb, float* part, hipStream_t st) {
   const int vec = vec_width(dtype, p.C / p.G, x, gy, out);
-  const RowShape sh = row_shape(p.C / p.G, vec);
-  const RowMap m = row_map(p.n, p.C, p.G, sh.L);
+  const RowShape sh = row_shape(p.C / p.G * (int)p.s, vec);
+  const RowMap m = row_map(p.n, (int)p.s, p.C, p.G, sh.L);
   float *pw = nullptr, *pb = nullptr;
-  const bool direct = m.npb == 1;
+  const bool direct = m.npb * m.s == 1;
   if (BWD && (gw || gb)) { pw = direct ? gw : part; pb = direct ? gb : part + p.C; }
   const int stride = 2 * p.C;
   switch (dtype) {
@@ -865,7 +961,7 @@ void rows_any(int dtype, const NormShape& p, const void* x, const void* gy, cons
   }
   if (BWD && (gw || gb) && !direct)
     hipLaunchKernelGGL(norm_finish_kernel, dim3((2 * p.C + kFinishCols - 1) / kFinishCols), dim3(1024), 0, st, part,
-                       (int64_t)m.npb, p.C, gw, gb);
+                       (int64_t)m.npb * m.s, p.C, gw, gb);
 }
 
 template <int ND, int NS, bool BWD>
@@ -887,7 +983,7 @@ template <bool BWD>
 void jet_any(const NormShape& p, int n_dir, const float* x, const float* gy, const float* w, const float* b, float eps,
              int act, float* out, float* gw, float* gb, float* part, hipStream_t st) {
   const RowShape sh = row_shape(p.C / p.G, 1);
-  const RowMap m = row_map(p.n, p.C, p.G, sh.L);
+  const RowMap m = row_map(p.n, 1, p.C, p.G, sh.L);
   float *pw = nullptr, *pb = nullptr;
   const bool direct = m.npb == 1;
   if (BWD && (gw || gb)) { pw = direct ? gw : part; pb = direct ? gb : part + p.C; }
@@ -919,9 +1015,9 @@ void grid_backward(const GridMap& m, const T* x, const T* gy, const float* w, co
   ensure_dynamic_lds((const void*)norm_grid_grad_kernel<T, VEC>, lds_g + kStaticLds);
   hipLaunchKernelGGL((norm_grid_sums_kernel<T, VEC>), dim3(blocks), dim3(kThreads), lds, st, m, x, gy, w, b, act, stats,
                      part_c, part_g);
-  const unsigned extra = gw || gb ? (2 * m.C + kFinishCols - 1) / kFinishCols : 0;
+  const unsigned extra = gw || gb ? (2 * m.C + kGridFinishCols - 1) / kGridFinishCols : 0;
   hipLaunchKernelGGL((norm_grid_grad_kernel<T, VEC>), dim3(blocks + extra), dim3(kThreads), lds_g, st, m, x, gy, w, b,
-                     act, stats, part_c, part_g, gx, gw, gb, (int64_t)blocks);
+                     act, stats, part_c, part_g, gx, gw, gb, (int)extra);
 }
 
 }  // namespace
@@ -945,8 +1041,8 @@ size_t norm_ws_bytes(const NormShape& p, bool backward) {
     // lane groups differ with the tensors' alignment: the widest spread of blocks over points any of them gives
     size_t most = 0;
     for (int L = 4; L <= 64; L *= 2) {
-      const RowMap m = row_map(p.n, p.C, p.G, L);
-      if (m.npb > 1 && (size_t)m.npb > most) most = m.npb;
+      const RowMap m = row_map(p.n, (int)p.s, p.C, p.G, L);
+      if (m.npb * m.s > 1 && (size_t)m.npb * m.s > most) most = (size_t)m.npb * m.s;
     }
     return most * 2 * p.C * sizeof(float);
   }

@@ -6,7 +6,9 @@ live on a ROCm device - a CPU tensor raises instead of taking another path.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
+import functools
 from typing import Optional
 
 import torch
@@ -50,6 +52,18 @@ def _ptr(t: Optional[torch.Tensor]):
 
 def _stream(device) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+_NO_SWITCH = contextlib.nullcontext()
+
+
+def _on(device):
+    """The tensors' device as the current one; switching costs host time, so only where it is not already."""
+    return _NO_SWITCH if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _raw_stream(device) -> int:
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def layer_struct(grid, base_weight, spline_weight, spline_scaler, act_kind, grid_size, spline_order) -> PdekanLayer:
@@ -321,30 +335,44 @@ def _group_norm_expression(x, groups, weight, bias, eps, act):
     return z.to(x.dtype)
 
 
+@functools.lru_cache(maxsize=1024)
+def _norm_sizes(n: int, s: int, c: int, groups: int):
+    """(floats of statistics, workspace bytes of the forward, of the backward) of a shape the library takes."""
+    lib = _lib.load()
+    floats = lib.pdekan_group_norm_stats_floats(n, s, c, groups)
+    if floats < 0:
+        _lib.check(int(floats))
+    return (floats, lib.pdekan_group_norm_workspace_bytes(n, s, c, groups, 0),
+            lib.pdekan_group_norm_workspace_bytes(n, s, c, groups, 1))
+
+
+def _address(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
 class _GroupNormAct(torch.autograd.Function):
     """First-order backward on the kernels; a recorded backward (``create_graph=True``) differentiates the expression."""
 
     @staticmethod
     def forward(ctx, x, weight, bias, groups, eps, act):
-        lib = _lib.load()
-        xd = x.detach().contiguous()
-        w, b = _prep(weight, "weight"), _prep(bias, "bias")
-        n, c = xd.size(0), xd.size(-1)
+        xd = x if x.is_contiguous() else x.contiguous()
+        w = weight if weight is None or weight.is_contiguous() else weight.contiguous()
+        b = bias if bias is None or bias.is_contiguous() else bias.contiguous()
         y = torch.empty_like(xd)
         stats = None
-        if xd.numel():
-            s = xd.numel() // (n * c)
-            with torch.cuda.device(x.device):
-                floats = lib.pdekan_group_norm_stats_floats(n, s, c, groups)
-                if floats < 0:
-                    _lib.check(int(floats))
-                if floats and any(ctx.needs_input_grad[:3]):
-                    stats = torch.empty(floats, dtype=torch.float32, device=x.device)
-                need = lib.pdekan_group_norm_workspace_bytes(n, s, c, groups, 0)
-                ws = _workspace(need, x.device) if need else None
-                _lib.check(lib.pdekan_group_norm_forward(_ptr(xd), DTYPES[xd.dtype], n, s, c, groups, _ptr(w), _ptr(b),
-                                                         eps, act, _ptr(y), _ptr(stats), _ptr(ws), need,
-                                                         _stream(x.device)))
+        n, c = xd.shape[0], xd.shape[-1]
+        if y.numel():
+            s = y.numel() // (n * c)
+            floats, need, _ = _norm_sizes(n, s, c, groups)
+            device = x.device
+            if floats and any(ctx.needs_input_grad):
+                stats = torch.empty(floats, dtype=torch.float32, device=device)
+            ws = _workspace(need, device) if need else None
+            with _on(device):
+                rc = _lib.load().pdekan_group_norm_forward(xd.data_ptr(), DTYPES[xd.dtype], n, s, c, groups, _address(w),
+                                                           _address(b), eps, act, y.data_ptr(), _address(stats),
+                                                           _address(ws), need, _raw_stream(device))
+            _lib.check(rc)
         ctx.save_for_backward(x, weight, bias, stats)
         ctx.meta = (groups, eps, act)
         return y
@@ -354,35 +382,38 @@ class _GroupNormAct(torch.autograd.Function):
         x, weight, bias, stats = ctx.saved_tensors
         groups, eps, act = ctx.meta
         if torch.is_grad_enabled():                    # this backward is being recorded (create_graph=True)
-            with torch.enable_grad():
-                y = _group_norm_expression(x, groups, weight, bias, eps, act)
-                wanted = [i for i in range(3) if ctx.needs_input_grad[i]]
-                got = torch.autograd.grad(y, [(x, weight, bias)[i] for i in wanted], gy, create_graph=True,
-                                          allow_unused=True)
+            y = _group_norm_expression(x, groups, weight, bias, eps, act)
+            wanted = [i for i in range(3) if ctx.needs_input_grad[i]]
+            got = torch.autograd.grad(y, [(x, weight, bias)[i] for i in wanted], gy, create_graph=True, allow_unused=True)
             out = [None] * 6
             for i, g in zip(wanted, got):
                 out[i] = g
             return tuple(out)
-        lib = _lib.load()
-        xd, gd = x.detach().contiguous(), gy.detach().contiguous()
-        w, b = _prep(weight, "weight"), _prep(bias, "bias")
-        n, c = xd.size(0), xd.size(-1)
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        xd = x if x.is_contiguous() else x.contiguous()
+        gd = gy if gy.is_contiguous() else gy.contiguous()
+        w = weight if weight is None or weight.is_contiguous() else weight.contiguous()
+        b = bias if bias is None or bias.is_contiguous() else bias.contiguous()
+        n, c = xd.shape[0], xd.shape[-1]
         gx = torch.empty_like(xd)
-        gw = torch.empty_like(w) if w is not None and ctx.needs_input_grad[1] else None
-        gb = torch.empty_like(b) if b is not None and ctx.needs_input_grad[2] else None
-        if xd.numel():
-            s = xd.numel() // (n * c)
-            with torch.cuda.device(x.device):
-                need = lib.pdekan_group_norm_workspace_bytes(n, s, c, groups, 1)
-                ws = _workspace(need, x.device) if need else None
-                _lib.check(lib.pdekan_group_norm_backward(_ptr(xd), _ptr(gd), DTYPES[xd.dtype], n, s, c, groups, _ptr(w),
-                                                          _ptr(b), eps, act, _ptr(stats), _ptr(gx), _ptr(gw), _ptr(gb),
-                                                          _ptr(ws), need, _stream(x.device)))
+        gw = torch.empty_like(w) if need_w else None
+        gb = torch.empty_like(b) if need_b else None
+        if gx.numel():
+            s = gx.numel() // (n * c)
+            need = _norm_sizes(n, s, c, groups)[2]
+            device = x.device
+            ws = _workspace(need, device) if need else None
+            with _on(device):
+                rc = _lib.load().pdekan_group_norm_backward(xd.data_ptr(), gd.data_ptr(), DTYPES[xd.dtype], n, s, c, groups,
+                                                            _address(w), _address(b), eps, act, _address(stats),
+                                                            gx.data_ptr(), _address(gw), _address(gb), _address(ws), need,
+                                                            _raw_stream(device))
+            _lib.check(rc)
         else:
             for g in (gw, gb):
                 if g is not None:
                     g.zero_()
-        return gx if ctx.needs_input_grad[0] else None, gw, gb, None, None, None
+        return gx if need_x else None, gw, gb, None, None, None
 
 
 def group_norm_act(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] = None,
@@ -400,8 +431,8 @@ def group_norm_act(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] 
     if under_func_transform(x, weight, bias):
         return _group_norm_expression(x, groups, weight, bias, eps, act)
     _require_gpu_float(x, "x")
-    weight = weight if weight is None else weight.to(torch.float32)
-    bias = bias if bias is None else bias.to(torch.float32)
+    weight = weight if weight is None or weight.dtype == torch.float32 else weight.to(torch.float32)
+    bias = bias if bias is None or bias.dtype == torch.float32 else bias.to(torch.float32)
     _same_device(x, weight, bias)
     return _GroupNormAct.apply(x, weight, bias, int(groups), float(eps), int(act))
 
@@ -415,15 +446,17 @@ def _same_device(x, *others) -> None:
 class _GroupNormActJet(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x_jet, weight, bias, groups, eps, act, n_dir, n_second):
-        lib = _lib.load()
-        xd = _aligned(_prep(x_jet, "input"))
-        w, b = _prep(weight, "weight"), _prep(bias, "bias")
+        xd = _aligned(x_jet if x_jet.is_contiguous() else x_jet.contiguous())
+        w = weight if weight is None or weight.is_contiguous() else weight.contiguous()
+        b = bias if bias is None or bias.is_contiguous() else bias.contiguous()
         n, c, _ = xd.shape
         y = torch.empty_like(xd)
         if n:
-            with torch.cuda.device(xd.device):
-                _lib.check(lib.pdekan_group_norm_jet_forward(_ptr(xd), n, c, groups, n_dir, n_second, _ptr(w), _ptr(b),
-                                                             eps, act, _ptr(y), _stream(xd.device)))
+            device = x_jet.device
+            with _on(device):
+                rc = _lib.load().pdekan_group_norm_jet_forward(xd.data_ptr(), n, c, groups, n_dir, n_second, _address(w),
+                                                               _address(b), eps, act, y.data_ptr(), _raw_stream(device))
+            _lib.check(rc)
         ctx.save_for_backward(x_jet, weight, bias)
         ctx.meta = (groups, eps, act, n_dir, n_second)
         return y
@@ -435,25 +468,30 @@ class _GroupNormActJet(torch.autograd.Function):
                                "provided; KAN.forward_jet already returns the input derivatives")
         x_jet, weight, bias = ctx.saved_tensors
         groups, eps, act, n_dir, n_second = ctx.meta
-        lib = _lib.load()
-        xd, gd = _aligned(_prep(x_jet, "input")), _aligned(_prep(gy, "grad_output"))
-        w, b = _prep(weight, "weight"), _prep(bias, "bias")
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        xd = _aligned(x_jet if x_jet.is_contiguous() else x_jet.contiguous())
+        gd = _aligned(gy if gy.is_contiguous() else gy.contiguous())
+        w = weight if weight is None or weight.is_contiguous() else weight.contiguous()
+        b = bias if bias is None or bias.is_contiguous() else bias.contiguous()
         n, c, _ = xd.shape
         gx = torch.empty_like(xd)
-        gw = torch.empty_like(w) if w is not None and ctx.needs_input_grad[1] else None
-        gb = torch.empty_like(b) if b is not None and ctx.needs_input_grad[2] else None
+        gw = torch.empty_like(w) if need_w else None
+        gb = torch.empty_like(b) if need_b else None
         if n:
-            with torch.cuda.device(xd.device):
-                need = lib.pdekan_group_norm_workspace_bytes(n, 1, c, groups, 1)
-                ws = _workspace(need, xd.device) if need else None
-                _lib.check(lib.pdekan_group_norm_jet_backward(_ptr(xd), _ptr(gd), n, c, groups, n_dir, n_second, _ptr(w),
-                                                              _ptr(b), eps, act, _ptr(gx), _ptr(gw), _ptr(gb), _ptr(ws),
-                                                              need, _stream(xd.device)))
+            device = x_jet.device
+            need = _norm_sizes(n, 1, c, groups)[2]
+            ws = _workspace(need, device) if need else None
+            with _on(device):
+                rc = _lib.load().pdekan_group_norm_jet_backward(xd.data_ptr(), gd.data_ptr(), n, c, groups, n_dir, n_second,
+                                                                _address(w), _address(b), eps, act, gx.data_ptr(),
+                                                                _address(gw), _address(gb), _address(ws), need,
+                                                                _raw_stream(device))
+            _lib.check(rc)
         else:
             for g in (gw, gb):
                 if g is not None:
                     g.zero_()
-        return (gx if ctx.needs_input_grad[0] else None, gw, gb) + (None,) * 5
+        return (gx if need_x else None, gw, gb) + (None,) * 5
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
@@ -474,7 +512,7 @@ def group_norm_act_jet(x_jet: torch.Tensor, groups: int, weight: Optional[torch.
         return group_norm_act(x_jet.squeeze(-1), groups, weight, bias, eps, act).unsqueeze(-1)
     _norm_check(x_jet.size(1), groups, weight, bias, eps, act)
     _require_gpu(x_jet, "x_jet")
-    weight = weight if weight is None else weight.to(torch.float32)
-    bias = bias if bias is None else bias.to(torch.float32)
+    weight = weight if weight is None or weight.dtype == torch.float32 else weight.to(torch.float32)
+    bias = bias if bias is None or bias.dtype == torch.float32 else bias.to(torch.float32)
     _same_device(x_jet, weight, bias)
     return _GroupNormActJet.apply(x_jet, weight, bias, int(groups), float(eps), int(act), int(n_dir), int(n_second))

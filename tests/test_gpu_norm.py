@@ -83,7 +83,8 @@ def _check(got, want, bound, dtype):
 SHAPES = [((1, 1), 1), ((3, 1), 1), ((7, 2), 1), ((5, 6), 6), ((1, 8), 2), ((33, 64), 8), ((1001, 64), 8), ((257, 90), 6),
           ((64, 96), 1), ((19, 320), 32), ((9, 512), 1), ((5, 1024), 2), ((3, 513), 1), ((2, 4097), 1), ((70, 384), 384),
           ((2, 1, 8), 2), ((1, 2, 4), 4), ((3, 5, 6), 3), ((2, 4096, 64), 8), ((3, 1999, 90), 6), ((1, 777, 1), 1),
-          ((130, 9, 24), 3), ((2, 16, 16, 40), 4), ((1, 20000, 10), 5), ((2, 33, 2050), 1), ((4, 300, 257), 257)]
+          ((130, 9, 24), 3), ((2, 16, 16, 40), 4), ((1, 20000, 10), 5), ((2, 33, 2050), 1), ((4, 300, 257), 257),
+          ((300, 32, 16), 1), ((70, 31, 5), 1), ((5000, 3, 7), 7), ((1, 70000, 6), 2), ((2000, 5, 64), 64), ((9, 33, 15), 3)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
