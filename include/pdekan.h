@@ -44,7 +44,7 @@ extern "C" {
 #define PDEKAN_ACT_SILU 1
 #define PDEKAN_ACT_TANH 2          /* pdekan_group_norm_* only */
 
-/* Element types of the tensors of pdekan_group_norm_* (every other tensor is fp32). */
+/* Element types of the tensors of pdekan_group_norm_* and of orthogonalised matrices (every other tensor is fp32). */
 #define PDEKAN_DTYPE_FP 0          /* fp32 */
 #define PDEKAN_DTYPE_BF 1          /* bfloat16 */
 #define PDEKAN_DTYPE_HALF 2        /* fp16 */
@@ -216,6 +216,40 @@ int pdekan_group_norm_jet_backward(const float* x_jet, const float* gy_jet, int6
                                    int32_t n_dir, int32_t n_second, const float* weight, const float* bias, float eps,
                                    int32_t act_kind, float* gx_jet, float* gweight, float* gbias, void* ws,
                                    size_t ws_bytes, void* stream);
+
+/* Orthogonalised updates (no counterpart in the reference, whose scripts train with AdamW and LBFGS): the polar factor
+ * of a matrix, nearly, by `steps` Newton-Schulz products.  With X = g / (|g|_F + eps), its short side first:
+ *   steps times:  S = X X^T,  X <- c[0] X + (c[1] S + c[2] S S) X
+ * out = X, so every singular value of g well above |g|_F c[0]^-steps is carried close to 1.  coefficients: 3 floats on
+ * the HOST ((3.4445, -4.7750, 2.0315) are the usual ones); refused if they carry singular values of [0, 1] past 64.
+ * Products have fp32 accuracy, the norm is summed in 64 bits; out is rounded to dtype once.  1 <= steps <= 100,
+ * eps >= 1e-30.  A stack of `batch` contiguous matrices [batch][rows][cols] counts as one entry; `out` may be `g`.  A matrix
+ * that holds a NaN or an infinity becomes NaN, the others are not touched by it; one of zeros stays zero. */
+typedef struct PdekanMatrix {
+  const void* g;
+  void* out;
+  int64_t rows, cols, batch;
+} PdekanMatrix;
+size_t pdekan_orthogonalize_workspace_bytes(const PdekanMatrix* mats, int32_t n_mats);
+int pdekan_orthogonalize(const PdekanMatrix* mats, int32_t n_mats, int32_t dtype, int32_t steps,
+                         const float* coefficients, float eps, void* ws, size_t ws_bytes, void* stream);
+
+/* One step of the Muon optimiser on fp32 weights [rows][cols] (a vector is a matrix of one row):
+ *   momentum <- mu momentum + (1 - mu) grad;  u = nesterov ? (1 - mu) grad + mu momentum : momentum
+ *   param <- (1 - lr weight_decay) param - lr gain orthogonalize(u)
+ * lr_device, if not NULL, is read on the device instead of lr (a captured step then follows a schedule). */
+typedef struct PdekanMuonParam {
+  float* param;
+  const float* grad;
+  float* momentum;
+  int64_t rows, cols;
+  float gain;
+  int32_t reserved;
+} PdekanMuonParam;
+size_t pdekan_muon_workspace_bytes(const PdekanMuonParam* params, int32_t n_params);
+int pdekan_muon_step(const PdekanMuonParam* params, int32_t n_params, float lr, const float* lr_device, float momentum,
+                     int32_t nesterov, float weight_decay, int32_t steps, const float* coefficients, float eps, void* ws,
+                     size_t ws_bytes, void* stream);
 
 /* Optional per-kernel timing for benchmarks (no counterpart in the reference,
  * which only prints a whole-script wall time, run1.py:524-526).  Between

@@ -49,6 +49,28 @@ class PdekanNet(ctypes.Structure):
     ]
 
 
+class PdekanMatrix(ctypes.Structure):
+    _fields_ = [
+        ("g", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("rows", ctypes.c_int64),
+        ("cols", ctypes.c_int64),
+        ("batch", ctypes.c_int64),
+    ]
+
+
+class PdekanMuonParam(ctypes.Structure):
+    _fields_ = [
+        ("param", ctypes.c_void_p),
+        ("grad", ctypes.c_void_p),
+        ("momentum", ctypes.c_void_p),
+        ("rows", ctypes.c_int64),
+        ("cols", ctypes.c_int64),
+        ("gain", ctypes.c_float),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
 # name -> (restype, argtypes); every symbol include/pdekan.h declares
 SIGNATURES = {
     "pdekan_version": (ctypes.c_int, []),
@@ -117,6 +139,14 @@ SIGNATURES = {
                                                       ctypes.c_void_p, ctypes.c_float, ctypes.c_int32, ctypes.c_void_p,
                                                       ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
                                                       ctypes.c_size_t, ctypes.c_void_p]),
+    "pdekan_orthogonalize_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(PdekanMatrix), ctypes.c_int32]),
+    "pdekan_orthogonalize": (ctypes.c_int, [ctypes.POINTER(PdekanMatrix), ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,
+                                            c_float_p, ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t,
+                                            ctypes.c_void_p]),
+    "pdekan_muon_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(PdekanMuonParam), ctypes.c_int32]),
+    "pdekan_muon_step": (ctypes.c_int, [ctypes.POINTER(PdekanMuonParam), ctypes.c_int32, ctypes.c_float, ctypes.c_void_p,
+                                        ctypes.c_float, ctypes.c_int32, ctypes.c_float, ctypes.c_int32, c_float_p,
+                                        ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
     "pdekan_profile_begin": (ctypes.c_int, []),
     "pdekan_profile_end": (ctypes.c_int, []),
     "pdekan_profile_count": (ctypes.c_int, []),

@@ -17,13 +17,14 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libpdekan.so")
 SOURCES = ["kan_kernels.hip", "kan_mfma.hip", "kan_head.hip", "kan_sparse.hip", "kan_f16.hip", "kan_small.hip", "kan_deeponet.hip",
-           "kan_norm.hip", "pdekan_api.hip"]
+           "kan_norm.hip", "kan_muon.hip", "pdekan_api.hip"]
 # kan_f16.hip: without the SLP vectorizer.  With it, hipcc 7.2 (-O3, gfx950) builds the 12-jet weight-gradient kernel
 # into code whose expanded columns come out wrong in lanes 48..63 (first element of each packed pair), whatever the
 # source-level form of the expansion; the explicit vector types in the kernels are packed by legalization regardless.
-# kan_norm.hip: no packed fp32 instructions (v_pk_fma_f32 and its kin), which the compiler forms from ordinary float code.
+# kan_norm.hip, kan_muon.hip: no packed fp32 instructions (v_pk_fma_f32 and its kin), which the compiler forms from ordinary float code.
 NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-EXTRA_FLAGS = {"kan_f16.hip": ["-fno-slp-vectorize"], "kan_norm.hip": NO_PACKED_FP32}
+EXTRA_FLAGS = {"kan_f16.hip": ["-fno-slp-vectorize"], "kan_norm.hip": NO_PACKED_FP32,
+               "kan_muon.hip": NO_PACKED_FP32}
 INCLUDE = os.path.join(HERE, "..", "include")
 ARCH = "gfx950"
 

@@ -201,4 +201,29 @@ void launch_norm_jet_backward(const NormShape& p, int n_dir, const float* x, con
                               const float* b, float eps, int act, float* gx, float* gw, float* gb, void* ws,
                               hipStream_t st);
 
+// kan_muon.hip: Newton-Schulz orthogonalisation of matrices and the Muon step around it
+constexpr int kNsItemsMax = 16;           // matrices or stacks of equal matrices a call of launch_ns
+struct NsMatrix {
+  const void* src;                        // [batch][rows][cols]: the matrix, or the optimiser's gradient
+  float* momentum;                        // the optimiser's buffer, or nullptr: orthogonalise src
+  void* out;                              // the result, or the optimiser's weight
+  int64_t rows, cols, batch;
+  float gain;
+};
+struct NsCoefficients { float a, b, c; };
+struct NsPlan {
+  NsCoefficients k;
+  int steps;
+  float eps, momentum;
+  int nesterov;
+  float lr, decay;
+  const float* lr_dev;
+  float scale_x, scale_s, scale_r;        // set by ns_scales, as is
+  int growth;
+};
+const char* ns_refusal(const NsMatrix& M);                       // nullptr: taken
+bool ns_scales(const NsCoefficients& k, int steps, NsPlan* p);   // false: the iteration leaves the fp16 range
+size_t ns_ws_bytes(const NsMatrix* mats, int count);
+void launch_ns(int dtype, const NsMatrix* mats, int count, const NsPlan& p, void* ws, hipStream_t st);
+
 }  // namespace pdekan

@@ -122,6 +122,71 @@ int norm_args(const char* what, const pdekan::NormShape& p, int n_dir, int n_sec
   return PDEKAN_OK;
 }
 
+// the part of a list of matrices one launch takes, as the kernels see it
+struct NsBatch { pdekan::NsMatrix m[pdekan::kNsItemsMax]; int n; };
+int ns_args(const char* what, const PdekanMatrix* mats, int n, int from, NsBatch& B, bool pointers) {
+  B.n = 0;
+  for (int i = from; i < n && B.n < pdekan::kNsItemsMax; ++i) {
+    const PdekanMatrix& M = mats[i];
+    const pdekan::NsMatrix v{M.g, nullptr, M.out, M.rows, M.cols, M.batch, 1.0f};
+    if (pointers && (!M.g || !M.out)) return fail(PDEKAN_ERR_ARG, "%s: matrix %d has a NULL tensor", what, i);
+    if (const char* why = pdekan::ns_refusal(v)) return fail(PDEKAN_ERR_ARG, "%s: matrix %d: %s", what, i, why);
+    B.m[B.n++] = v;
+  }
+  return PDEKAN_OK;
+}
+int ns_args(const char* what, const PdekanMuonParam* params, int n, int from, NsBatch& B, bool pointers) {
+  B.n = 0;
+  for (int i = from; i < n && B.n < pdekan::kNsItemsMax; ++i) {
+    const PdekanMuonParam& M = params[i];
+    const pdekan::NsMatrix v{M.grad, M.momentum, M.param, M.rows, M.cols, 1, M.gain};
+    if (pointers && (!M.grad || !M.momentum || !M.param)) return fail(PDEKAN_ERR_ARG, "%s: parameter %d has a NULL tensor", what, i);
+    if (!(M.gain >= 0.0f && M.gain < 3.0e38f)) return fail(PDEKAN_ERR_ARG, "%s: parameter %d: gain must be finite and not negative", what, i);
+    if (const char* why = pdekan::ns_refusal(v)) return fail(PDEKAN_ERR_ARG, "%s: parameter %d: %s", what, i, why);
+    B.m[B.n++] = v;
+  }
+  return PDEKAN_OK;
+}
+// workspace of a list: the largest launch's, every launch of the call uses it again; 0 with an error set: refused
+template <typename M>
+size_t ns_workspace(const char* what, const M* mats, int n) {
+  if (!mats || n < 1) { (void)fail(PDEKAN_ERR_ARG, "%s: no matrices", what); return 0; }
+  size_t most = 0;
+  NsBatch B;
+  for (int i = 0; i < n; i += pdekan::kNsItemsMax) {
+    if (ns_args(what, mats, n, i, B, false)) return 0;
+    const size_t bytes = pdekan::ns_ws_bytes(B.m, B.n);
+    if (bytes > most) most = bytes;
+  }
+  return most;
+}
+template <typename M>
+int ns_run(const char* what, const M* mats, int n, int dtype, pdekan::NsPlan& p, const float* coefficients, void* ws,
+           size_t ws_bytes, hipStream_t st) {
+  if (!coefficients) return fail(PDEKAN_ERR_ARG, "%s: coefficients is NULL", what);
+  if (p.steps < 1 || p.steps > 100) return fail(PDEKAN_ERR_ARG, "%s: %d steps (1 .. 100)", what, p.steps);
+  if (!(p.eps >= 1e-30f && p.eps < 3.0e38f)) return fail(PDEKAN_ERR_ARG, "%s: eps must be at least 1e-30 and finite", what);
+  p.k = {coefficients[0], coefficients[1], coefficients[2]};
+  if (!pdekan::ns_scales(p.k, p.steps, &p))
+    return fail(PDEKAN_ERR_ARG, "%s: coefficients (%g, %g, %g) carry singular values past 64 within %d steps", what,
+                (double)p.k.a, (double)p.k.b, (double)p.k.c, p.steps);
+  const size_t need = ns_workspace(what, mats, n);
+  if (!need) return PDEKAN_ERR_ARG;
+  if (!ws || ws_bytes < need || ((uintptr_t)ws & 255))
+    return fail(PDEKAN_ERR_WORKSPACE, "%s: workspace of %zu bytes (256-byte aligned) needed, %zu given", what, need, ws_bytes);
+  NsBatch B;
+  for (int i = 0; i < n; i += pdekan::kNsItemsMax) {               // refuse before the first launch
+    const int rc = ns_args(what, mats, n, i, B, true);
+    if (rc) return rc;
+  }
+  ProfScope prof(st, what, 0);
+  for (int i = 0; i < n; i += pdekan::kNsItemsMax) {
+    (void)ns_args(what, mats, n, i, B, true);
+    pdekan::launch_ns(dtype, B.m, B.n, p, ws, st);
+  }
+  return check_launch(what);
+}
+
 size_t align_up(size_t v, size_t a = 256) { return (v + a - 1) / a * a; }
 
 // the four networks of pdekan_deeponet_step as the kernels' launcher takes them
@@ -1164,6 +1229,40 @@ int pdekan_group_norm_jet_backward(const float* x_jet, const float* gy_jet, int6
   pdekan::launch_norm_jet_backward(p, n_dir, x_jet, gy_jet, weight, bias, eps, act_kind, gx_jet, gweight, gbias, ws,
                                    (hipStream_t)stream);
   return check_launch("group_norm_jet_backward");
+}
+
+size_t pdekan_orthogonalize_workspace_bytes(const PdekanMatrix* mats, int32_t n_mats) {
+  return ns_workspace("orthogonalize", mats, n_mats);
+}
+
+int pdekan_orthogonalize(const PdekanMatrix* mats, int32_t n_mats, int32_t dtype, int32_t steps,
+                         const float* coefficients, float eps, void* ws, size_t ws_bytes, void* stream) {
+  if (dtype < PDEKAN_DTYPE_FP || dtype > PDEKAN_DTYPE_HALF) return fail(PDEKAN_ERR_ARG, "orthogonalize: dtype %d unknown", dtype);
+  pdekan::NsPlan p{};
+  p.steps = steps;
+  p.eps = eps;
+  return ns_run("orthogonalize", mats, n_mats, dtype, p, coefficients, ws, ws_bytes, (hipStream_t)stream);
+}
+
+size_t pdekan_muon_workspace_bytes(const PdekanMuonParam* params, int32_t n_params) {
+  return ns_workspace("muon", params, n_params);
+}
+
+int pdekan_muon_step(const PdekanMuonParam* params, int32_t n_params, float lr, const float* lr_device, float momentum,
+                     int32_t nesterov, float weight_decay, int32_t steps, const float* coefficients, float eps, void* ws,
+                     size_t ws_bytes, void* stream) {
+  if (!(momentum >= 0.0f && momentum < 1.0f)) return fail(PDEKAN_ERR_ARG, "muon_step: momentum must lie in [0, 1)");
+  if (!(weight_decay >= 0.0f && weight_decay < 3.0e38f)) return fail(PDEKAN_ERR_ARG, "muon_step: weight_decay must be finite and not negative");
+  if (!lr_device && !(lr >= 0.0f && lr < 3.0e38f)) return fail(PDEKAN_ERR_ARG, "muon_step: lr must be finite and not negative");
+  pdekan::NsPlan p{};
+  p.steps = steps;
+  p.eps = eps;
+  p.momentum = momentum;
+  p.nesterov = nesterov != 0;
+  p.lr = lr;
+  p.lr_dev = lr_device;
+  p.decay = weight_decay;
+  return ns_run("muon_step", params, n_params, PDEKAN_DTYPE_FP, p, coefficients, ws, ws_bytes, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -9,12 +9,12 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import functools
-from typing import Optional
+from typing import Optional, Sequence, Tuple, Union
 
 import torch
 
 from . import _lib
-from ._lib import PdekanLayer, PdekanLayerGrad
+from ._lib import PdekanLayer, PdekanLayerGrad, PdekanMatrix
 
 ACT_IDENTITY = 0
 ACT_SILU = 1
@@ -516,3 +516,63 @@ def group_norm_act_jet(x_jet: torch.Tensor, groups: int, weight: Optional[torch.
     bias = bias if bias is None or bias.dtype == torch.float32 else bias.to(torch.float32)
     _same_device(x_jet, weight, bias)
     return _GroupNormActJet.apply(x_jet, weight, bias, int(groups), float(eps), int(act), int(n_dir), int(n_second))
+
+
+# ---- orthogonalised updates ----------------------------------------------------------------------------------------------
+
+# the usual quintic: slope 3.4445 at zero, singular values end up within 0.7 .. 1.2 after five steps
+NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+
+
+def ns_settings(steps: int, eps: float, coefficients: Sequence[float]):
+    """(steps, eps, coefficients as a C array), checked."""
+    coefficients = tuple(float(c) for c in coefficients)
+    if len(coefficients) != 3:
+        raise ValueError(f"pde_amd: three Newton-Schulz coefficients wanted, got {len(coefficients)}")
+    if not 1 <= int(steps) <= 100:
+        raise ValueError(f"pde_amd: 1 to 100 Newton-Schulz steps, got {steps}")
+    if not 1e-30 <= eps < float("inf"):
+        raise ValueError(f"pde_amd: eps must be at least 1e-30 and finite, got {eps}")
+    return int(steps), float(eps), (ctypes.c_float * 3)(*coefficients)
+
+
+@torch.no_grad()
+def orthogonalize(g: Union[torch.Tensor, Sequence[torch.Tensor]], steps: int = 5, eps: float = 1e-7,
+                  coefficients: Tuple[float, float, float] = NS_COEFFICIENTS):
+    """The nearly orthogonal factor of a matrix ``[rows, cols]``, of each matrix of a stack ``[..., rows, cols]``, or of
+    each tensor of a sequence (one list back), by ``steps`` Newton-Schulz products (the update of the Muon optimiser).
+
+    ``X = g / (|g|_F + eps)`` with its short side first, then ``steps`` times ``X <- a X + (b S + c S S) X``, ``S = X X^T``.
+    float32, bfloat16 or float16 (one type and device a call); the products have float32 accuracy whatever the type.  Not
+    differentiable.  A matrix holding a NaN or an infinity becomes NaN and leaves the others alone."""
+    one = isinstance(g, torch.Tensor)
+    mats = [g] if one else list(g)
+    steps, eps, c = ns_settings(steps, eps, coefficients)
+    if not mats:
+        return []
+    for t in mats:
+        if t.dim() < 2:
+            raise ValueError(f"pde_amd: orthogonalize takes matrices [..., rows, cols], got {tuple(t.shape)}")
+        _require_gpu_float(t, "g")
+        if t.dtype != mats[0].dtype:
+            raise TypeError(f"pde_amd: matrices of types {mats[0].dtype} and {t.dtype} in one call")
+    _same_device(*mats)
+    device = mats[0].device
+    src = [t if t.is_contiguous() else t.contiguous() for t in mats]
+    out = [torch.empty_like(t) for t in src]
+    todo = [(s, o) for s, o in zip(src, out) if s.numel()]
+    if todo:
+        lib = _lib.load()
+        desc = (PdekanMatrix * len(todo))()
+        for d, (s, o) in zip(desc, todo):
+            rows, cols = s.shape[-2:]
+            d.g, d.out, d.rows, d.cols, d.batch = s.data_ptr(), o.data_ptr(), rows, cols, s.numel() // (rows * cols)
+        need = lib.pdekan_orthogonalize_workspace_bytes(desc, len(todo))
+        if need == 0:
+            _lib.check(-1)
+        ws = _workspace(need, device)
+        with _on(device):
+            rc = lib.pdekan_orthogonalize(desc, len(todo), DTYPES[src[0].dtype], steps, c, eps, ws.data_ptr(), need,
+                                          _raw_stream(device))
+        _lib.check(rc)
+    return out[0] if one else out
