@@ -247,6 +247,8 @@ def main():
     ap.add_argument("--graph", action="store_true",
                     help="capture one step (library call + all-reduce + AdamW) in a HIP graph and replay it")
     ap.add_argument("--no-cpu-baseline", action="store_true")
+    ap.add_argument("--optimizer", default="adamw", choices=["adamw", "muon"],
+                    help="adamw = what the scripts use (run1.py:209); muon = pde_amd.optim.Muon")
     ap.add_argument("--no-optimizer", action="store_true", help="diagnostic only: skip the AdamW update")
     ap.add_argument("--no-scaling-reference", action="store_true",
                     help="skip the short extra run at cfg3's per-GPU point count on the default one-GPU line")
@@ -314,7 +316,11 @@ def main():
         step = BlackScholesStep(model, micro_batch=args.micro_batch)
     dp = DataParallelStep(step, dist, sync="check") if dist is not None else None
     # run1.py:209; one launch for all tensors; capturable keeps the step count on the device (graph replay)
-    opt = torch.optim.AdamW(model.parameters(), lr=0.01, fused=True, capturable=args.graph)
+    if args.optimizer == "muon":
+        from pde_amd.optim import Muon
+        opt = Muon(model.parameters(), lr=0.01)
+    else:
+        opt = torch.optim.AdamW(model.parameters(), lr=0.01, fused=True, capturable=args.graph)
 
     def eager_step():
         if dp is not None:
@@ -412,7 +418,7 @@ def main():
         "ms_per_step": ms_per_step, "higher_is_better": True, "scaling": scaling, "vs_baseline": None,
         "dtype": "f32", "arithmetic": ARITHMETIC, "data": "synthetic",
         "config": {"workload": f"{name}: KAN {widths} grid={grid} k=3 {'SiLU' if args.base_activation == 'silu' else 'Identity'}, Black-Scholes PINN step "
-                               f"(fwd + residual + loss + bwd + AdamW), {n_local} points/GPU, {n_global} total",
+                               f"(fwd + residual + loss + bwd + {'Muon' if args.optimizer == 'muon' else 'AdamW'}), {n_local} points/GPU, {n_global} total",
                    "points_per_gpu": n_local, "points_total": n_global, "micro_batch": args.micro_batch,
                    "optimizer_in_step": not args.no_optimizer, "hip_graph": bool(args.graph),
                    "parallelism": f"dp{world}", "ranks": world,

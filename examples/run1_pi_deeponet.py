@@ -88,6 +88,7 @@ def main(argv=None):
     ap.add_argument("--batch", type=int, default=100, help="run1.py:470-471")
     ap.add_argument("--epochs", type=int, default=20, help="the script trains 1500 (run1.py:211)")
     ap.add_argument("--seed", type=int, default=0)
+    ap.add_argument("--optimizer", default="adamw", choices=["adamw", "muon"], help="adamw: run1.py:209")
     ap.add_argument("--graph", action="store_true",
                     help="capture one training step in a HIP graph and replay it")
     args = ap.parse_args(argv)
@@ -109,7 +110,11 @@ def main(argv=None):
     dl2 = DataLoader(TensorDataset(data["x_b"], data["t_b"], data["outputs_b"]), batch_size=args.batch, shuffle=True,
                      generator=gen)
     # run1.py:209 (fused=True: the same update as one launch instead of a dozen)
-    opt = torch.optim.AdamW(net.parameters(), lr=0.01, capturable=args.graph, fused=True)
+    if args.optimizer == "muon":
+        from pde_amd import Muon
+        opt = Muon(net.parameters(), lr=0.01)
+    else:
+        opt = torch.optim.AdamW(net.parameters(), lr=0.01, capturable=args.graph, fused=True)
     u_s1, u_s2 = data["u_1"][:, 2], data["u_2"][:, 2]
 
     step_fn = lambda bc, pde: net.train_step(opt, data["u_1"], data["u_2"], u_s1, u_s2, bc, pde)

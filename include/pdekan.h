@@ -158,6 +158,15 @@ int pdekan_bs_step(const PdekanLayer* layers, int32_t n_layers, const float* x, 
                    float rate, float* loss_out, float* res_out, const PdekanLayerGrad* grads,
                    int32_t accumulate, int64_t micro_batch, void* ws, size_t ws_bytes, void* stream);
 
+/* The residual, its loss and the cotangent of the model's output jets, as pdekan_bs_step forms them, for models that run
+ * layer by layer (group norms between the layers): v_jet[n][1][1 + d + d - 1] of points x[n][d], d = 2 or 6;
+ *   loss (+)= sum((res - target)^2) / n_global,  gv_jet = d loss / d v_jet
+ * target, res_out, gv_jet and loss_out may be NULL.  ws: PDEKAN_BS_RESIDUAL_WORKSPACE_BYTES. */
+#define PDEKAN_BS_RESIDUAL_WORKSPACE_BYTES 4096
+int pdekan_bs_residual(const float* x, int64_t stride_n, int64_t stride_d, int64_t n, int32_t d, const float* v_jet,
+                       const float* target, int64_t n_global, float sigma, float rate, float* loss_out, float* res_out,
+                       float* gv_jet, int32_t accumulate, void* ws, size_t ws_bytes, void* stream);
+
 /* One training step of the physics-informed DeepONet the scripts build around four KANs, without the optimiser
  * update (class PI_DeepONet, run1.py:75-149; loop body run1.py:217-233; networks run1.py:478-482):
  *   v[r]      = model1(u1[r]) * model2(u2[r])            one value per sensor row, run1.py:92-98

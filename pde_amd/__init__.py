@@ -3,10 +3,13 @@ MI355X-native (hand-written gfx950 HIP kernels behind a C ABI).
 
     from pde_amd import KAN, KANLinear          # same interface as efficient_kan
     pde_amd.install_as_efficient_kan()          # `from efficient_kan import KAN` resolves here
+    from pde_amd import GroupNormAct, Muon      # norm between layers, orthogonalising optimiser
 """
 from .kan import KAN, KANLinear  # noqa: F401
+from .norm import GroupNormAct  # noqa: F401
+from .optim import Muon  # noqa: F401
 
-__all__ = ["KAN", "KANLinear", "install_as_efficient_kan"]
+__all__ = ["KAN", "KANLinear", "GroupNormAct", "Muon", "install_as_efficient_kan"]
 
 
 def install_as_efficient_kan() -> None:

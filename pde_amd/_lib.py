@@ -109,6 +109,10 @@ SIGNATURES = {
                                       ctypes.c_int64, ctypes.c_float, ctypes.c_float, ctypes.c_void_p,
                                       ctypes.c_void_p, ctypes.POINTER(PdekanLayerGrad), ctypes.c_int32,
                                       ctypes.c_int64, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
+    "pdekan_bs_residual": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int32,
+                                          ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_float,
+                                          ctypes.c_float, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+                                          ctypes.c_int32, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
     "pdekan_deeponet_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(PdekanNet), ctypes.c_int64, ctypes.c_int64,
                                                           ctypes.c_int64]),
     "pdekan_deeponet_step": (ctypes.c_int, [ctypes.POINTER(PdekanNet), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64,

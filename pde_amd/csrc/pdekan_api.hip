@@ -1160,6 +1160,26 @@ int pdekan_profile_entry(int idx, char* name, size_t name_cap, double* total_ms,
   return PDEKAN_OK;
 }
 
+int pdekan_bs_residual(const float* x, int64_t stride_n, int64_t stride_d, int64_t n, int32_t d, const float* v_jet,
+                       const float* target, int64_t n_global, float sigma, float rate, float* loss_out, float* res_out,
+                       float* gv_jet, int32_t accumulate, void* ws, size_t ws_bytes, void* stream) {
+  static_assert(kLossBlocks * sizeof(float) <= PDEKAN_BS_RESIDUAL_WORKSPACE_BYTES, "one partial sum a block");
+  if (!x || !v_jet || n < 1 || n_global < 1) return fail(PDEKAN_ERR_ARG, "bs_residual: bad arguments");
+  if (!ws || ws_bytes < PDEKAN_BS_RESIDUAL_WORKSPACE_BYTES || ((uintptr_t)ws & 255))
+    return fail(PDEKAN_ERR_WORKSPACE, "bs_residual: workspace of %d bytes (256-byte aligned) needed, %zu given",
+                PDEKAN_BS_RESIDUAL_WORKSPACE_BYTES, ws_bytes);
+  if (d != 2 && d != 6) return fail(PDEKAN_ERR_ARG, "bs_residual: %d input columns unsupported (2 or 6)", d);
+  const int64_t blocks = (n + 255) / 256;
+  const int nblocks = (int)(blocks < kLossBlocks ? blocks : kLossBlocks);
+  const float inv_n = 1.0f / (float)n_global;
+  float* part = static_cast<float*>(ws);
+  ProfScope prof((hipStream_t)stream, "bs_residual_loss", 0);
+  (void)pdekan::launch_bs_residual(d, x, stride_n, stride_d, v_jet, target, sigma, rate, inv_n, res_out, gv_jet, part,
+                                   nblocks, n, (hipStream_t)stream);
+  if (loss_out) pdekan::launch_loss_finish(part, nblocks, inv_n, loss_out, accumulate, (hipStream_t)stream);
+  return check_launch("bs_residual");
+}
+
 size_t pdekan_group_norm_workspace_bytes(int64_t n, int64_t s, int32_t channels, int32_t groups, int32_t backward) {
   const pdekan::NormShape p{n, s, channels, groups};
   if (const char* why = pdekan::norm_refusal(p, 0, 0)) { (void)fail(PDEKAN_ERR_ARG, "group_norm: %s", why); return 0; }

@@ -29,14 +29,15 @@ Everything runs on the library kernels: there is no CPU path.
 from __future__ import annotations
 
 import ctypes
-from typing import List, Optional, Sequence
+from typing import List, Optional, Sequence, Union
 
 import torch
 from torch import nn
 
 from . import _lib, functional as K
 from ._lib import PdekanLayer, PdekanLayerGrad, PdekanNet
-from .kan import KAN, _act_kind
+from .kan import KAN, _act_kind, has_norms
+from .optim import Muon
 from .pinn import BS_RATE, BS_SIGMA
 
 
@@ -69,6 +70,8 @@ class DeepONetStep:
     def supported(self) -> bool:
         """Whether the networks are of a kind the call takes at all (sizes are settled per batch)."""
         for m in self.models:
+            if has_norms(m):
+                return False
             for layer in m.layers:
                 if _act_kind(layer.base_activation) is None or layer.spline_order != 3:
                     return False
@@ -232,8 +235,13 @@ class PI_DeepONet(nn.Module):
         return loss.detach(), pde_loss.detach(), bc_loss.detach()
 
     def fit(self, u1, u2, u_s1, u_s2, dataloader1, dataloader2, epochs: int = 1500, lr: float = 0.01,
-            optimizer: Optional[torch.optim.Optimizer] = None):
-        """run1.py:197-241: AdamW(lr=0.01) over the zipped boundary / collocation loaders."""
+            optimizer: Union[torch.optim.Optimizer, str, None] = None):
+        """run1.py:197-241: AdamW(lr=0.01) over the zipped boundary / collocation loaders; ``optimizer="muon"`` takes
+        :class:`pde_amd.optim.Muon` at ``lr`` instead."""
+        if isinstance(optimizer, str):
+            if optimizer not in ("adamw", "muon"):
+                raise ValueError(f"optimizer must be 'adamw', 'muon' or an optimiser, got {optimizer!r}")
+            optimizer = Muon(self.parameters(), lr=lr) if optimizer == "muon" else None
         opt = optimizer or torch.optim.AdamW(self.parameters(), lr=lr)
         for _ in range(epochs):
             for bc_batch, pde_batch in zip(dataloader1, dataloader2):

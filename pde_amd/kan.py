@@ -23,6 +23,7 @@ import torch
 import torch.nn.functional as F
 
 from . import functional as K
+from .norm import GroupNormAct
 from .spline_host import dense_bsplines, extended_knots, fit_coefficients
 
 __all__ = ["KANLinear", "KAN"]
@@ -32,6 +33,11 @@ def _under_func_transform(t: torch.Tensor) -> bool:
     """True while ``t`` is a torch.func wrapper (grad / vmap / jvp level)."""
     fn = getattr(torch._C._functorch, "is_functorch_wrapped_tensor", None)
     return bool(fn and fn(t))
+
+
+def has_norms(model) -> bool:
+    """Whether a model has norms between its layers: the one-call steps take plain stacks of layers only."""
+    return getattr(model, "norms", None) is not None and len(model.norms) > 0
 
 
 def _act_kind(module: torch.nn.Module) -> Optional[int]:
@@ -204,10 +210,15 @@ class KANLinear(torch.nn.Module):
 
 
 class KAN(torch.nn.Module):
-    """Sequential stack of :class:`KANLinear` (kan.py:240-285)."""
+    """Sequential stack of :class:`KANLinear` (kan.py:240-285).
+
+    ``norm_groups`` (not in the reference) puts a group norm over each point's hidden values, followed by
+    ``norm_activation``, between two layers (:class:`pde_amd.norm.GroupNormAct`, modules ``norms.{l}``): with the default
+    ``tanh`` the next layer's inputs stay inside the knots' default range."""
 
     def __init__(self, layers_hidden, grid_size=5, spline_order=3, scale_noise=0.1, scale_base=1.0,
-                 scale_spline=1.0, base_activation=torch.nn.SiLU, grid_eps=0.02, grid_range=[-1, 1]):
+                 scale_spline=1.0, base_activation=torch.nn.SiLU, grid_eps=0.02, grid_range=[-1, 1],
+                 norm_groups: Optional[int] = None, norm_activation=torch.nn.Tanh):
         super().__init__()
         self.grid_size = grid_size
         self.spline_order = spline_order
@@ -216,12 +227,20 @@ class KAN(torch.nn.Module):
                       scale_base=scale_base, scale_spline=scale_spline, base_activation=base_activation,
                       grid_eps=grid_eps, grid_range=grid_range)
             for n_in, n_out in zip(layers_hidden, layers_hidden[1:]))
+        self.norms = None if norm_groups is None else torch.nn.ModuleList(
+            GroupNormAct(norm_groups, width, activation=norm_activation) for width in layers_hidden[1:-1])
+
+    def _norm_after(self, i: int) -> Optional[GroupNormAct]:
+        return None if self.norms is None or i >= len(self.norms) else self.norms[i]
 
     def forward(self, x: torch.Tensor, update_grid=False):
-        for layer in self.layers:
+        for i, layer in enumerate(self.layers):
             if update_grid:
                 layer.update_grid(x)
             x = layer(x)
+            norm = self._norm_after(i)
+            if norm is not None:
+                x = norm(x.reshape(-1, norm.channels)).view(x.shape)      # point by point, whatever leads
         return x
 
     def forward_jet(self, x: torch.Tensor, n_second: Optional[int] = None):
@@ -239,8 +258,11 @@ class KAN(torch.nn.Module):
         if n_second is None:
             n_second = d - 1
         jet = K.seed_jets(x, d, n_second)
-        for layer in self.layers:
+        for i, layer in enumerate(self.layers):
             jet = layer.forward_jet(jet, d, n_second)
+            norm = self._norm_after(i)
+            if norm is not None:
+                jet = norm.forward_jet(jet, d, n_second)
         return jet
 
     def regularization_loss(self, regularize_activation=1.0, regularize_entropy=1.0):

@@ -127,3 +127,5 @@ class Muon(torch.optim.Optimizer):
             rc = lib.pdekan_muon_step(desc, len(params), lr, lr_ptr, group["momentum"], int(group["nesterov"]),
                                       group["weight_decay"], steps, c, eps, ws.data_ptr(), need, K._raw_stream(device))
         _lib.check(rc)
+        # written through their addresses: an autograd graph that saved them has to know
+        torch.autograd.graph.increment_version([*params, *[self.state[p]["momentum_buffer"] for p in params]])

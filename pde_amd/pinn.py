@@ -4,7 +4,8 @@ What the reference scripts do per minibatch for the PDE part - ``residual_net``
 (run1.py:120-129), ``loss_res`` (:145-149) and ``loss.backward()`` (:225) -
 as one call into libpdekan.so: forward with analytic input derivatives,
 residual, mean-squared loss, every parameter gradient.  The optimiser update
-stays with ``torch.optim`` (the scripts use AdamW / LBFGS).
+stays with ``torch.optim`` (the scripts use AdamW / LBFGS) or ``pde_amd.optim``.
+A model with norms between its layers runs layer by layer on the same kernels.
 """
 from __future__ import annotations
 
@@ -15,7 +16,8 @@ import torch
 
 from . import _lib, functional as K
 from ._lib import PdekanLayer, PdekanLayerGrad
-from .kan import KAN, _act_kind
+from .kan import KAN, _act_kind, has_norms
+from .norm import _norm_act_kind
 
 # run1.py:126-127
 BS_SIGMA = 0.165856529
@@ -56,6 +58,9 @@ class BlackScholesStep:
                 raise NotImplementedError("the kernels implement cubic splines (spline_order=3)")
         if model.layers[-1].out_features != 1:
             raise ValueError("the PINN head must have one output")
+        self.layered = has_norms(model)
+        if self.layered and any(_norm_act_kind(m.activation) is None for m in model.norms):
+            raise NotImplementedError("the step supports Identity, SiLU and Tanh after a norm")
         total = sum(p.numel() for p in params)
         # gradients and the loss share one buffer so that a data-parallel wrapper can all-reduce both in place
         self.grad_and_loss = torch.zeros(total + 1, dtype=torch.float32, device=self.device)
@@ -88,11 +93,20 @@ class BlackScholesStep:
                                        0 if sc is None else by_id[id(sc)].data_ptr())
         return layers, grads, n
 
+    def _bytes(self, lib, layers, n_layers, n, d, mb) -> int:
+        if not self.layered:
+            return lib.pdekan_model_workspace_bytes(layers, n_layers, n, d, d - 1, mb)
+        m = min(mb, n) if mb else n
+        widths = [layer.in_features for layer in layers] + [1]
+        ws = [lib.pdekan_layer_workspace_bytes(ctypes.byref(layer), m, d, d - 1) for layer in layers]
+        # the jets of every layer and norm, two cotangents, a layer's workspace
+        return 0 if 0 in ws else 4 * m * 2 * d * (2 * sum(widths) + 2 * max(widths)) + max(ws)
+
     def _fit_micro_batch(self, lib, layers, n_layers, n, d) -> int:
         """Largest micro-batch (0 = the whole batch) whose workspace fits the budget."""
         mb = 0
         while True:
-            need = lib.pdekan_model_workspace_bytes(layers, n_layers, n, d, d - 1, mb)
+            need = self._bytes(lib, layers, n_layers, n, d, mb)
             if need == 0:
                 raise _lib.PdekanError(lib.pdekan_last_error().decode())
             if need <= self.workspace_budget:
@@ -138,6 +152,11 @@ class BlackScholesStep:
                 p.grad = v
         layers, grads, nl = self._structs()
         xd = x.detach()
+        if self.layered:
+            with torch.cuda.device(self.device):
+                self._run_layered(lib, layers, grads, nl, xd, target, n if n_global is None else int(n_global),
+                                  residual_out)
+            return self.loss
         with torch.cuda.device(self.device):
             ws = self._workspace(lib, layers, nl, n, d)
             _lib.check(lib.pdekan_bs_step(layers, nl, K._ptr(xd), xd.stride(0), xd.stride(1), K._ptr(target), n,
@@ -145,6 +164,75 @@ class BlackScholesStep:
                                           K._ptr(self.loss), K._ptr(residual_out), grads, 0, self.micro_batch,
                                           K._ptr(ws), ws.numel(), K._stream(self.device)))
         return self.loss
+
+
+    def _run_layered(self, lib, layers, grads, nl, x, target, n_global, residual_out):
+        """The step of a model with norms: layers, norms, residual and their backward kernels one after the other, without
+        the autograd tape (so it can be captured like the one-call step); parameter gradients land in the same views."""
+        n, d = x.shape
+        if self.workspace_budget is not None and (self._ws_key is None or self._ws_key[:2] != (n, d)):
+            self.micro_batch = self._fit_micro_batch(lib, layers, nl, n, d)
+            self._ws_key = (n, d, self.micro_batch)
+        st = K._stream(self.device)
+        norms = self.model.norms
+        by_id = {id(p): v for p, v in zip(self.model.parameters(), self._views)}
+        empty = lambda *shape: torch.empty(*shape, dtype=torch.float32, device=self.device)
+        settings = []
+        for m in norms:
+            for t in (m.weight, m.bias):
+                if t is not None and not (t.is_cuda and t.is_contiguous() and t.dtype == torch.float32):
+                    raise RuntimeError("pde_amd: parameters must be contiguous float32 tensors on the GPU")
+            settings.append((K._ptr(m.weight), K._ptr(m.bias), m.eps, _norm_act_kind(m.activation)))
+        step = self.micro_batch or max(n, 1)
+        space = None
+        for lo in range(0, max(n, 1), step):
+            pts = x[lo:lo + step]
+            m, jets, raw = pts.size(0), 2 * d, []
+            more = int(lo > 0)
+            a = [empty(m, d, jets)]
+            _lib.check(lib.pdekan_seed_jets(K._ptr(pts), pts.stride(0), pts.stride(1), m, d, d, d - 1, K._ptr(a[0]), st))
+            if space is None:                              # the layers' workspace, the first micro-batch is the largest
+                space = K._workspace(max(lib.pdekan_layer_workspace_bytes(ctypes.byref(layer), m, d, d - 1)
+                                         for layer in layers), self.device)
+            for i in range(nl):
+                y = empty(m, layers[i].out_features, jets)
+                _lib.check(lib.pdekan_layer_forward(ctypes.byref(layers[i]), K._ptr(a[i]), K._ptr(y), m, d, d - 1,
+                                                    K._ptr(space), space.numel(), st))
+                raw.append(y)
+                if i < len(norms):
+                    w, b, eps, act = settings[i]
+                    y = torch.empty_like(y)
+                    _lib.check(lib.pdekan_group_norm_jet_forward(K._ptr(raw[i]), m, norms[i].channels, norms[i].groups, d,
+                                                                 d - 1, w, b, eps, act, K._ptr(y), st))
+                a.append(y)
+            g = torch.empty_like(a[-1])
+            ws = K._workspace(4096, self.device)
+            t = None if target is None else target[lo:lo + step]
+            r = None if residual_out is None else residual_out.reshape(-1)[lo:lo + step]
+            _lib.check(lib.pdekan_bs_residual(K._ptr(pts), pts.stride(0), pts.stride(1), m, d, K._ptr(a[-1]), K._ptr(t),
+                                              n_global, self.sigma, self.rate, K._ptr(self.loss), K._ptr(r), K._ptr(g), more,
+                                              K._ptr(ws), ws.numel(), st))
+            for i in reversed(range(nl)):
+                if i < len(norms):
+                    w, b, eps, act = settings[i]
+                    into = [None if p is None else by_id[id(p)] for p in (norms[i].weight, norms[i].bias)]
+                    got = [None if v is None else torch.empty_like(v) for v in into] if more else into
+                    gy, g = g, torch.empty_like(g)
+                    need = lib.pdekan_group_norm_workspace_bytes(m, 1, norms[i].channels, norms[i].groups, 1)
+                    ws = K._workspace(need, self.device)
+                    _lib.check(lib.pdekan_group_norm_jet_backward(K._ptr(raw[i]), K._ptr(gy), m, norms[i].channels,
+                                                                  norms[i].groups, d, d - 1, w, b, eps, act, K._ptr(g),
+                                                                  K._ptr(got[0]), K._ptr(got[1]), K._ptr(ws), ws.numel(),
+                                                                  st))
+                    if more:
+                        for v, part in zip(into, got):
+                            if v is not None:
+                                v.add_(part)
+                below = empty(m, layers[i].in_features, jets) if i else None
+                _lib.check(lib.pdekan_layer_backward(ctypes.byref(layers[i]), K._ptr(a[i]), K._ptr(g), m, d, d - 1,
+                                                     K._ptr(below), ctypes.byref(grads[i]), more, K._ptr(space),
+                                                     space.numel(), st))
+                g = below
 
 
 class GraphedStep:

@@ -15,7 +15,7 @@ FAKE = 0x1000        # never dereferenced: every call below is refused before a 
 
 @pytest.mark.parametrize("n,s,c,g,word", [(4, 1, 6, 4, b"divide"), (0, 1, 8, 2, b"empty"), (4, 0, 8, 2, b"empty"),
                                           (4, 1, 8, 0, b"empty"), (4, 1, 8200, 1, b"8192"), (4, 1 << 25, 8, 1, b"many"),
-                                          (1 << 24, 2, 8, 1, b"samples")])
+                                          (1 << 24, 40, 8, 1, b"samples")])
 def test_bad_shapes_are_refused(n, s, c, g, word):
     lib = _lib()
     assert lib.pdekan_group_norm_workspace_bytes(n, s, c, g, 1) == 0
