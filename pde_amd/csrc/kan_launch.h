@@ -218,7 +218,7 @@ struct NsPlan {
   int nesterov;
   float lr, decay;
   const float* lr_dev;
-  float scale_x, scale_s, scale_r;        // set by ns_scales, as is
+  float scale_x, scale_s, scale_r, scale_q, scale_t, scale_p;   // set by ns_scales, as is
   int growth;
 };
 const char* ns_refusal(const NsMatrix& M);                       // nullptr: taken

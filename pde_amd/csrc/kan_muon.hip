@@ -27,7 +27,6 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 constexpr int kThreads = 256;
 constexpr int kItemsMax = kNsItemsMax;    // matrices (or stacks of equal ones) a launch
 constexpr int kSumsMax = 256;             // partial sums of squares a matrix
-constexpr int kTileHalves = 1024;         // a 16 x 32 tile: 512 hi pieces, 512 lo pieces
 
 // One matrix, or a stack of `batch` equal ones, and its share of the workspace.
 struct Item {
@@ -39,6 +38,7 @@ struct Item {
   int64_t size;           // rows * cols
   int rows, cols, m, n, mp, np, batch, tall;
   int nsum;               // partial sums of squares
+  int bt;                 // rows and columns a block of the products takes: 64 or 128
   int chunks, kchunk;     // splits of the long axis in X X^T, inner tiles (of 32) a split
   float gain;
 };
@@ -48,22 +48,24 @@ struct Items {
   int n;
 };
 
-// workspace of a matrix: X [mp][np], X^T twice [np][mp], S and R [mp][mp] as two-piece tiles, then the splits' partial
-// products and the partial sums of squares
+// workspace of a matrix: X [mp][np], X^T twice [np][mp], five square matrices [mp][mp] as two-piece tiles, then the splits'
+// partial products, the partial sums of squares and the numbers of struct Norm
 __device__ __host__ inline int64_t plane_bytes(const Item& I) { return (int64_t)I.mp * I.np * 4; }
 __device__ __host__ inline int64_t square_bytes(const Item& I) { return (int64_t)I.mp * I.mp * 4; }
 __device__ __host__ inline int64_t off_xt(const Item& I, int k) { return plane_bytes(I) * (1 + k); }
-__device__ __host__ inline int64_t off_s(const Item& I) { return plane_bytes(I) * 3; }
-__device__ __host__ inline int64_t off_r(const Item& I) { return off_s(I) + square_bytes(I); }
-__device__ __host__ inline int64_t off_part(const Item& I) { return off_r(I) + square_bytes(I); }
-__device__ __host__ inline int tri_tiles(const Item& I) { const int t = (I.mp + 63) / 64; return t * (t + 1) / 2; }
+enum Square { kS = 0, kQ = 1, kT = 2, kP0 = 3, kP1 = 4, kSquares = 5 };
+__device__ __host__ inline int64_t off_sq(const Item& I, int k) { return plane_bytes(I) * 3 + square_bytes(I) * k; }
+__device__ __host__ inline int64_t off_part(const Item& I) { return off_sq(I, kSquares); }
+__device__ __host__ inline int tri_tiles(const Item& I) { const int t = (I.mp + I.bt - 1) / I.bt; return t * (t + 1) / 2; }
 __device__ __host__ inline int64_t off_sums(const Item& I) {
   if (I.m == 1) return 0;                 // a vector has nothing else
-  return off_part(I) + (I.chunks > 1 ? (int64_t)I.chunks * tri_tiles(I) * 64 * 64 * 4 : 0);
+  return off_part(I) + (I.chunks > 1 ? (int64_t)I.chunks * tri_tiles(I) * I.bt * I.bt * 4 : 0);
 }
 __device__ __host__ inline int64_t item_bytes(const Item& I) {
-  return (off_sums(I) + kSumsMax * (int64_t)sizeof(double) + 8 + 255) / 256 * 256;      // (8: the exponent, see x_scale)
+  return (off_sums(I) + kSumsMax * (int64_t)sizeof(double) + 16 + 255) / 256 * 256;
 }
+template <typename H>
+__device__ __forceinline__ H* at(char* ws, int64_t off) { return reinterpret_cast<H*>(ws + off); }
 
 struct Where { int item, local; };
 __device__ __forceinline__ Where find_item(const Items& L) {
@@ -80,46 +82,56 @@ __device__ __forceinline__ void tri_tile(int t, int& bi, int& bj) {
   bi = t - bj * (bj + 1) / 2;
 }
 
-// ---- exponents of the pieces --------------------------------------------------------------------------------------
-// X has no singular value over the host's bound 2^kx, S none over 2^(2 kx), R none over 2^kr; entries are bounded alike, and
-// pieces are scaled by powers of two to stay below 2^15.  Where eps dominates |U|_F, X starts as small as |U| / eps and its
-// pieces are scaled up by 2^ex0 more, ex0 = the exponent of (|U| + eps) / |U|; a step multiplies X by at most 2^growth, so
-// step k has 2^max(0, ex0 - growth k).
-struct Scales { float x, s, r; int growth; };          // what the entries of X, S, R are multiplied by
+// ---- scales of the pieces -------------------------------------------------------------------------------------------
+// X has no singular value over the host's bound 2^kx, S none over 2^(2 kx), and so on; entries are bounded alike, and pieces
+// are scaled by powers of two to stay below 2^15.  Where eps dominates |U|_F, X starts as small as |U| / eps and its pieces
+// are scaled up by 2^ex more, ex = the exponent of (|U| + eps) / |U|; a step multiplies X by at most 2^growth, so before step
+// k it is 2^max(0, ex - growth k).
+struct Scales { float x, s, q, t, p; int growth; };    // what the entries of X, S, Q (or R), T = Q S, P are multiplied by
 
-__device__ __forceinline__ int* exponent_slot(const Item& I, char* ws) {
-  return reinterpret_cast<int*>(ws + off_sums(I) + kSumsMax * (int64_t)sizeof(double));
+// What the first kernels find out about a matrix.  X = factor U' with U' = U 2^-e: the composed form keeps U' itself, whose
+// entries are those of U to the last bit, in the pieces, and applies the factor to the products; the other form has 1.
+struct Norm { float factor; int ex; };
+__device__ __forceinline__ Norm* norm_slot(const Item& I, char* ws) {
+  return at<Norm>(ws, off_sums(I) + kSumsMax * (int64_t)sizeof(double));
 }
-__device__ __forceinline__ float x_scale(const Item& I, char* ws, const Scales& sc, int step) {
-  const int ex = *exponent_slot(I, ws) - sc.growth * step;
+__device__ __forceinline__ float x_scale(const Norm& n, const Scales& sc, int step) {
+  const int ex = n.ex - sc.growth * step;
   return ldexpf(sc.x, ex > 0 ? ex : 0);
 }
 
-// two pieces of four values
-__device__ __forceinline__ void split4(const float (&v)[4], float scale, f16x4& hi, f16x4& lo) {
+// halves offset of (row, col) of a matrix of PIECES pieces with kt inner tiles a row of tiles; col % 4 == 0 addresses four
+// values
+template <int PIECES>
+__device__ __forceinline__ int64_t piece_at(int row, int col, int kt) {
+  return ((int64_t)(row >> 4) * kt + (col >> 5)) * (512 * PIECES) + ((row & 15) + 16 * ((col & 31) >> 3)) * 8 + (col & 7);
+}
+template <int PIECES>
+__device__ __forceinline__ void store_pieces(_Float16* base, int row, int col, int kt, const float (&v)[4], float scale) {
+  f16x4 hi, lo;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float y = v[i] * scale;
     hi[i] = (_Float16)y;
     lo[i] = (_Float16)(y - (float)hi[i]);
   }
-}
-// halves offset of (row, col) of a matrix with kt inner tiles a row of tiles; col % 4 == 0 addresses four values
-__device__ __forceinline__ int64_t piece_at(int row, int col, int kt) {
-  return ((int64_t)(row >> 4) * kt + (col >> 5)) * kTileHalves + ((row & 15) + 16 * ((col & 31) >> 3)) * 8 + (col & 7);
-}
-__device__ __forceinline__ void store_pieces(_Float16* base, int row, int col, int kt, const float (&v)[4], float scale) {
-  f16x4 hi, lo;
-  split4(v, scale, hi, lo);
-  _Float16* p = base + piece_at(row, col, kt);
+  _Float16* p = base + piece_at<PIECES>(row, col, kt);
   *reinterpret_cast<f16x4*>(p) = hi;
-  *reinterpret_cast<f16x4*>(p + 512) = lo;
+  if constexpr (PIECES == 2) *reinterpret_cast<f16x4*>(p + 512) = lo;
 }
+template <int PIECES>
 __device__ __forceinline__ void load_pieces(const _Float16* base, int row, int col, int kt, float (&v)[4], float unscale) {
-  const _Float16* p = base + piece_at(row, col, kt);
-  const f16x4 hi = *reinterpret_cast<const f16x4*>(p), lo = *reinterpret_cast<const f16x4*>(p + 512);
+  const _Float16* p = base + piece_at<PIECES>(row, col, kt);
+  const f16x4 hi = *reinterpret_cast<const f16x4*>(p);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = ((float)hi[i] + (float)lo[i]) * unscale;
+  for (int i = 0; i < 4; ++i) v[i] = (float)hi[i];
+  if constexpr (PIECES == 2) {
+    const f16x4 lo = *reinterpret_cast<const f16x4*>(p + 512);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] += (float)lo[i];
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] *= unscale;
 }
 
 // v[r] of lane t of a quad -> v[t] of lane r
@@ -183,22 +195,31 @@ __device__ __forceinline__ double matrix_norm(const Item& I, int b) {
   return sqrt(s);
 }
 
-// X and X^T of a 64 x 64 tile as pieces.
-template <typename T>
+// X and X^T of a 64 x 64 tile as pieces; COMPOSED: of U' in one piece (16-bit types: exact).
+template <typename T, bool COMPOSED>
 __global__ void __launch_bounds__(kThreads) ns_split_kernel(Items L, Momentum mo, float eps, Scales sc) {
+  constexpr int PX = COMPOSED ? 1 : 2;
   __shared__ float tile[64][65];
   const Where w = find_item(L);
   const Item& I = L.it[w.item];
   const int tm = (I.mp + 63) / 64, tn = (I.np + 63) / 64;
   const int b = w.local / (tm * tn), t = w.local % (tm * tn), bi = t % tm, bj = t / tm;
   const int64_t base = b * I.size;
-  const double norm = matrix_norm(I, b);
-  const float scale = (float)(1.0 / (norm + (double)eps));
+  char* ws = I.ws + b * I.ws_stride;
+  const double norm = matrix_norm(I, b), whole = norm + (double)eps, small = whole / norm;
+  Norm nm;
   // at most 2^96: entries below 2^-96 |X| lose their low bits; (NaN and 0 norms: no shift)
-  const double small = (norm + (double)eps) / norm;
-  const int ex0 = small > 1.0 && norm > 0.0 ? (small < 7.9e28 ? ilogb(small) : 96) : 0;
-  if (t == 0 && threadIdx.x == 0) *exponent_slot(I, I.ws + b * I.ws_stride) = ex0;
-  const float scx = ldexpf(sc.x, ex0);
+  nm.ex = small > 1.0 && norm > 0.0 ? (small < 7.9e28 ? ilogb(small) : 96) : 0;
+  nm.factor = 1.0f;
+  float scale = (float)(1.0 / whole);
+  if constexpr (COMPOSED) {
+    // U 2^-e with 2^e >= |U| + eps: entries within [-1, 1]; an infinite or NaN norm makes everything NaN
+    const int e = whole < 1.0e300 ? ilogb(whole) + 1 : 0;
+    nm.factor = whole < 1.0e300 ? (float)ldexp(1.0 / whole, e) : __builtin_nanf("");
+    scale = ldexpf(1.0f, -e);
+  }
+  if (t == 0 && threadIdx.x == 0) *norm_slot(I, ws) = nm;
+  const float scx = x_scale(nm, sc, 0);
   for (int k = threadIdx.x; k < 64 * 64; k += kThreads) {
     // neighbouring threads on neighbouring addresses
     const int a = k / 64, c = k % 64;
@@ -209,215 +230,294 @@ __global__ void __launch_bounds__(kThreads) ns_split_kernel(Items L, Momentum mo
     tile[li][lj] = v;
   }
   __syncthreads();
-  char* ws = I.ws + b * I.ws_stride;
-  _Float16 *x = reinterpret_cast<_Float16*>(ws), *xt = reinterpret_cast<_Float16*>(ws + off_xt(I, 0));
+  _Float16 *x = at<_Float16>(ws, 0), *xt = at<_Float16>(ws, off_xt(I, 0));
   const int ktx = I.np / 32, kt = I.mp / 32;
   for (int k = threadIdx.x; k < 64 * 16; k += kThreads) {
     const int r = k % 64, q = k / 64 * 4;
     const int i = bi * 64 + r, j = bj * 64 + q;
     if (i < I.mp && j < I.np) {
       const float v[4] = {tile[r][q], tile[r][q + 1], tile[r][q + 2], tile[r][q + 3]};
-      store_pieces(x, i, j, ktx, v, scx);
+      store_pieces<PX>(x, i, j, ktx, v, scx);
     }
     const int i2 = bi * 64 + q, j2 = bj * 64 + r;
     if (i2 < I.mp && j2 < I.np) {
       const float v[4] = {tile[q][r], tile[q + 1][r], tile[q + 2][r], tile[q + 3][r]};
-      store_pieces(xt, j2, i2, kt, v, scx);
+      store_pieces<PX>(xt, j2, i2, kt, v, scx);
     }
   }
 }
 
 // ---- products -------------------------------------------------------------------------------------------------------
 
-// A wave's 32 x 32 share of a 64 x 64 block of P Q^T over inner tiles [k0, k1): acc[a][c] is the 16 x 16 block at rows
-// 16 a of P and 16 c of Q; lane l holds Q's row l % 16 and P's rows 4 (l / 16) + r.
-struct Acc { f32x4 v[2][2]; };
-__device__ __forceinline__ void product(const _Float16* P, const _Float16* Q, int rp, int rq, int prows, int qrows, int kt,
-                                        int k0, int k1, Acc& acc) {
-  const int lane = threadIdx.x & 63;
+// P Q^T of a BT x BT block over inner tiles [k0, k1), PP and PQ pieces an operand.  Four waves take a quarter each: acc[a][c]
+// is the 16 x 16 block at rows 16 a of P and 16 c of Q; lane l holds Q's row l % 16 and P's rows 4 (l / 16) + r.
+// Operand tiles go from memory to LDS without passing registers, `kStages` inner tiles of the whole block in a ring, and
+// from LDS to registers as contiguous 1 KB reads.
+template <int BT, int PP, int PQ>
+struct Product {
+  static constexpr int kW = BT / 32;                           // 16-row tiles a wave takes of either operand
+  static constexpr int kFrags = BT / 16 * (PP + PQ);           // 1 KB pieces of tiles a stage
+  static constexpr int kLoads = kFrags / 4;                    // a wave's
+  static constexpr int kStages = kFrags * 1024 * 4 <= 64 * 1024 ? 4 : kFrags * 1024 * 3 <= 80 * 1024 ? 3 : 2;
+  static constexpr int kLds = kFrags * 1024 * kStages;
+  f32x4 v[kW][kW];
+
+  __device__ __forceinline__ void run(const _Float16* P, const _Float16* Q, int bp, int bq, int prows, int qrows, int kt,
+                                      int k0, int k1, char* lds) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const _Float16* src[kLoads];
+    int step[kLoads];
 #pragma unroll
-  for (int a = 0; a < 2; ++a)
-#pragma unroll
-    for (int c = 0; c < 2; ++c) acc.v[a][c] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-  for (int k = k0; k < k1; ++k) {
-    f16x8 ph[2], pl[2], qh[2], ql[2];
-#pragma unroll
-    for (int a = 0; a < 2; ++a) {
+    for (int u = 0; u < kLoads; ++u) {
       // tiles past the padded matrix repeat its last one; what they give is never stored
-      const int tp = min(rp / 16 + a, prows / 16 - 1), tq = min(rq / 16 + a, qrows / 16 - 1);
-      const _Float16* p = P + ((int64_t)tp * kt + k) * kTileHalves + lane * 8;
-      const _Float16* q = Q + ((int64_t)tq * kt + k) * kTileHalves + lane * 8;
-      ph[a] = *reinterpret_cast<const f16x8*>(p);
-      pl[a] = *reinterpret_cast<const f16x8*>(p + 512);
-      qh[a] = *reinterpret_cast<const f16x8*>(q);
-      ql[a] = *reinterpret_cast<const f16x8*>(q + 512);
+      const int f = wave * kLoads + u;
+      const bool isp = f < BT / 16 * PP;
+      const int g = isp ? f : f - BT / 16 * PP, pieces = isp ? PP : PQ;
+      const int tile = min((isp ? bp : bq) * (BT / 16) + g / pieces, (isp ? prows : qrows) / 16 - 1);
+      step[u] = 512 * pieces;
+      src[u] = (isp ? P : Q) + ((int64_t)tile * kt + k0) * step[u] + (g % pieces) * 512 + lane * 8;
     }
+    auto fetch = [&](int stage) {
+      char* dst = lds + stage * (kFrags * 1024) + wave * (kLoads * 1024);
 #pragma unroll
-    for (int a = 0; a < 2; ++a)
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        acc.v[a][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl[a], qh[c], acc.v[a][c], 0, 0, 0);
-        acc.v[a][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[a], ql[c], acc.v[a][c], 0, 0, 0);
-        acc.v[a][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[a], qh[c], acc.v[a][c], 0, 0, 0);
+      for (int u = 0; u < kLoads; ++u) {
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src[u],
+                                         (__attribute__((address_space(3))) void*)(dst + u * 1024), 16, 0, 0);
+        src[u] += step[u];
       }
+    };
+#pragma unroll
+    for (int a = 0; a < kW; ++a)
+#pragma unroll
+      for (int c = 0; c < kW; ++c) v[a][c] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+    const int n = k1 - k0;
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i)
+      if (i < n) fetch(i);
+    int stage = 0, free = kStages - 1;
+    for (int i = 0; i < n; ++i) {
+      // this stage has landed (later ones may still be on their way), and every wave is done with the one before
+      if (i + kStages - 2 < n) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kStages - 2) * kLoads) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      if (i + kStages - 1 < n) fetch(free);
+      const char* base = lds + stage * (kFrags * 1024) + lane * 16;
+      f16x8 p[kW][PP], q[kW][PQ];
+#pragma unroll
+      for (int a = 0; a < kW; ++a) {
+#pragma unroll
+        for (int h = 0; h < PP; ++h)
+          p[a][h] = *reinterpret_cast<const f16x8*>(base + (((wave & 1) * kW + a) * PP + h) * 1024);
+#pragma unroll
+        for (int h = 0; h < PQ; ++h)
+          q[a][h] = *reinterpret_cast<const f16x8*>(base + (BT / 16 * PP + ((wave >> 1) * kW + a) * PQ + h) * 1024);
+      }
+#pragma unroll
+      for (int a = 0; a < kW; ++a)
+#pragma unroll
+        for (int c = 0; c < kW; ++c) {
+          if constexpr (PP == 2) v[a][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(p[a][1], q[c][0], v[a][c], 0, 0, 0);
+          if constexpr (PQ == 2) v[a][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(p[a][0], q[c][1], v[a][c], 0, 0, 0);
+          v[a][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(p[a][0], q[c][0], v[a][c], 0, 0, 0);
+        }
+      stage = stage + 1 == kStages ? 0 : stage + 1;
+      free = free + 1 == kStages ? 0 : free + 1;
+    }
+  }
+  // first rows of P and Q of this wave's part
+  static __device__ __forceinline__ int row_p(int bp) { return bp * BT + (threadIdx.x >> 6 & 1) * (BT / 2); }
+  static __device__ __forceinline__ int row_q(int bq) { return bq * BT + (threadIdx.x >> 7) * (BT / 2); }
+
+  // f(16 x 16 block's first row of P, of Q, the lane's four values)
+  template <typename F>
+  __device__ __forceinline__ void each(int bp, int bq, int prows, int qrows, F&& f) {
+#pragma unroll
+    for (int a = 0; a < kW; ++a)
+#pragma unroll
+      for (int c = 0; c < kW; ++c) {
+        const int p0 = row_p(bp) + 16 * a, q0 = row_q(bq) + 16 * c;
+        if (p0 >= prows || q0 >= qrows) continue;
+        float x[4] = {v[a][c][0], v[a][c][1], v[a][c][2], v[a][c][3]};
+        f(p0, q0, x);
+      }
+  }
+};
+
+// A symmetric result: both triangles from one, blocks on the diagonal as they are.
+__device__ __forceinline__ void store_symmetric(_Float16* S, int kt, bool diagonal, int p0, int q0, float (&v)[4], float scale) {
+  const int lane = threadIdx.x & 63;
+  store_pieces<2>(S, q0 + (lane & 15), p0 + 4 * (lane >> 4), kt, v, scale);
+  if (!diagonal) {
+    quad_transpose(v);
+    store_pieces<2>(S, p0 + 4 * (lane >> 4) + (lane & 3), q0 + (lane & 12), kt, v, scale);
   }
 }
 
-// The symmetric m x m result of a wave: both triangles from one, blocks on the diagonal as they are.
-__device__ __forceinline__ void store_symmetric(_Float16* S, int mp, int bi, int bj, int rp, int rq, const Acc& acc,
-                                                float scale) {
-  const int lane = threadIdx.x & 63, kt = mp / 32;
-#pragma unroll
-  for (int a = 0; a < 2; ++a)
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const int p0 = rp + 16 * a, q0 = rq + 16 * c;
-      if (p0 >= mp || q0 >= mp) continue;
-      float v[4] = {acc.v[a][c][0], acc.v[a][c][1], acc.v[a][c][2], acc.v[a][c][3]};
-      store_pieces(S, q0 + (lane & 15), p0 + 4 * (lane >> 4), kt, v, scale);
-      if (bi != bj) {
-        quad_transpose(v);
-        store_pieces(S, p0 + 4 * (lane >> 4) + (lane & 3), q0 + (lane & 12), kt, v, scale);
-      }
-    }
+// Neighbouring blocks go to different XCDs, each with an L2 of its own: renumbered, an XCD's blocks are neighbours.
+__device__ __forceinline__ int xcd_order(int local, int count) {
+  const int per = count / 8;
+  return local < per * 8 ? (local % 8) * per + local / 8 : local;
 }
 
 // S = X X^T: block = (split of the long axis, tile of the upper triangle)
-__global__ void __launch_bounds__(kThreads) ns_gram_kernel(Items L, Scales sc, int step) {
+template <int BT, int PX>
+__global__ void __launch_bounds__(kThreads, 2) ns_gram_kernel(Items L, Scales sc, int step) {
+  extern __shared__ char lds[];
   const Where w = find_item(L);
   const Item& I = L.it[w.item];
   const int tiles = tri_tiles(I), per = tiles * I.chunks;
-  const int b = w.local / per, rest = w.local % per, chunk = rest / tiles, t = rest % tiles;
+  const int local = xcd_order(w.local, per * I.batch), b = local / per, rest = local % per, chunk = rest / tiles, t = rest % tiles;
   int bi, bj;
   tri_tile(t, bi, bj);
   char* ws = I.ws + b * I.ws_stride;
-  const _Float16* x = reinterpret_cast<const _Float16*>(ws);
-  const int wave = threadIdx.x >> 6, rp = bi * 64 + 32 * (wave & 1), rq = bj * 64 + 32 * (wave >> 1);
+  const _Float16* x = at<const _Float16>(ws, 0);
   const int kt = I.np / 32, k0 = chunk * I.kchunk, k1 = min(k0 + I.kchunk, kt);
-  Acc acc;
-  product(x, x, rp, rq, I.mp, I.mp, kt, k0, k1, acc);
-  const float scx = x_scale(I, ws, sc, step), unscale = 1.0f / scx / scx;
+  Product<BT, PX, PX> acc;
+  acc.run(x, x, bi, bj, I.mp, I.mp, kt, k0, k1, lds);
+  const Norm nm = *norm_slot(I, ws);
+  const float scx = x_scale(nm, sc, step), factor = step ? 1.0f : nm.factor, unscale = factor / scx * (factor / scx);
   if (I.chunks == 1) {
-    store_symmetric(reinterpret_cast<_Float16*>(ws + off_s(I)), I.mp, bi, bj, rp, rq, acc, unscale * sc.s);
+    acc.each(bi, bj, I.mp, I.mp, [&](int p0, int q0, float (&v)[4]) {
+      store_symmetric(at<_Float16>(ws, off_sq(I, kS)), I.mp / 32, bi == bj, p0, q0, v, unscale * sc.s);
+    });
     return;
   }
-  f32x4* part = reinterpret_cast<f32x4*>(ws + off_part(I)) + ((int64_t)chunk * tiles + t) * 1024 + threadIdx.x;
+  constexpr int kAcc = BT * BT / 1024;                         // 16 x 16 blocks a wave
+  f32x4* part = at<f32x4>(ws, off_part(I)) + ((int64_t)chunk * tiles + t) * (BT * BT / 4) + threadIdx.x;
 #pragma unroll
-  for (int a = 0; a < 4; ++a) part[a * kThreads] = acc.v[a >> 1][a & 1] * unscale;
+  for (int a = 0; a < kAcc; ++a) part[a * kThreads] = acc.v[a / acc.kW][a % acc.kW] * unscale;
 }
 
-// the sum of the splits, in their order
+// the sum of the splits, in their order: a block sums a quarter (BT = 128: a sixteenth) of a tile's 16 x 16 blocks
+template <int BT>
 __global__ void __launch_bounds__(kThreads) ns_gram_sum_kernel(Items L, Scales sc) {
+  constexpr int kAcc = BT * BT / 1024, kW = BT / 32;
   const Where w = find_item(L);
   const Item& I = L.it[w.item];
-  const int tiles = tri_tiles(I), b = w.local / tiles, t = w.local % tiles;
+  const int tiles = tri_tiles(I), b = w.local / (tiles * kAcc), t = w.local / kAcc % tiles, a = w.local % kAcc;
   int bi, bj;
   tri_tile(t, bi, bj);
   char* ws = I.ws + b * I.ws_stride;
-  const f32x4* part = reinterpret_cast<const f32x4*>(ws + off_part(I)) + (int64_t)t * 1024 + threadIdx.x;
-  Acc acc;
-#pragma unroll
-  for (int a = 0; a < 4; ++a) acc.v[a >> 1][a & 1] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-  for (int k = 0; k < I.chunks; ++k)
-#pragma unroll
-    for (int a = 0; a < 4; ++a) acc.v[a >> 1][a & 1] += part[(int64_t)k * tiles * 1024 + a * kThreads];
-  const int wave = threadIdx.x >> 6;
-  store_symmetric(reinterpret_cast<_Float16*>(ws + off_s(I)), I.mp, bi, bj, bi * 64 + 32 * (wave & 1),
-                  bj * 64 + 32 * (wave >> 1), acc, sc.s);
+  const f32x4* part = at<const f32x4>(ws, off_part(I)) + (int64_t)t * (BT * BT / 4) + a * kThreads + threadIdx.x;
+  f32x4 s = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
+  for (int k = 0; k < I.chunks; ++k) s += part[(int64_t)k * tiles * (BT * BT / 4)];
+  const int p0 = Product<BT, 2, 2>::row_p(bi) + 16 * (a / kW), q0 = Product<BT, 2, 2>::row_q(bj) + 16 * (a % kW);
+  if (p0 >= I.mp || q0 >= I.mp) return;
+  float v[4] = {s[0], s[1], s[2], s[3]};
+  store_symmetric(at<_Float16>(ws, off_sq(I, kS)), I.mp / 32, bi == bj, p0, q0, v, sc.s);
 }
 
-// R = b S + c S S
-__global__ void __launch_bounds__(kThreads) ns_poly_kernel(Items L, Scales sc, float cb, float cc) {
+// Q = a I + b S + c S S  (a = 0: R, the step less its multiple of one)
+template <int BT>
+__global__ void __launch_bounds__(kThreads, 2) ns_poly_kernel(Items L, Scales sc, NsCoefficients k, int out) {
+  extern __shared__ char lds[];
   const Where w = find_item(L);
   const Item& I = L.it[w.item];
-  const int tiles = tri_tiles(I), b = w.local / tiles, t = w.local % tiles;
+  const int tiles = tri_tiles(I), local = xcd_order(w.local, tiles * I.batch), b = local / tiles, t = local % tiles;
   int bi, bj;
   tri_tile(t, bi, bj);
   char* ws = I.ws + b * I.ws_stride;
-  const _Float16* s = reinterpret_cast<const _Float16*>(ws + off_s(I));
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, kt = I.mp / 32;
-  const int rp = bi * 64 + 32 * (wave & 1), rq = bj * 64 + 32 * (wave >> 1);
-  Acc acc;
-  product(s, s, rp, rq, I.mp, I.mp, kt, 0, kt, acc);
+  const _Float16* s = at<const _Float16>(ws, off_sq(I, kS));
+  const int lane = threadIdx.x & 63, kt = I.mp / 32;
+  Product<BT, 2, 2> acc;
+  acc.run(s, s, bi, bj, I.mp, I.mp, kt, 0, kt, lds);
   const float unscale = 1.0f / sc.s;
+  acc.each(bi, bj, I.mp, I.mp, [&](int p0, int q0, float (&v)[4]) {
+    const int q = q0 + (lane & 15), p = p0 + 4 * (lane >> 4);
+    float o[4];
+    load_pieces<2>(s, q, p, kt, o, unscale);
 #pragma unroll
-  for (int a = 0; a < 2; ++a)
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const int p0 = rp + 16 * a, q0 = rq + 16 * c;
-      if (p0 >= I.mp || q0 >= I.mp) continue;
-      float v[4];
-      load_pieces(s, q0 + (lane & 15), p0 + 4 * (lane >> 4), kt, v, unscale);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) acc.v[a][c][r] = fmaf(cc * unscale * unscale, acc.v[a][c][r], cb * v[r]);
-    }
-  store_symmetric(reinterpret_cast<_Float16*>(ws + off_r(I)), I.mp, bi, bj, rp, rq, acc, sc.r);
+    for (int r = 0; r < 4; ++r) v[r] = fmaf(k.c * unscale * unscale, v[r], k.b * o[r]) + (p + r == q ? k.a : 0.0f);
+    store_symmetric(at<_Float16>(ws, off_sq(I, out)), kt, bi == bj, p0, q0, v, sc.q);
+  });
+}
+
+// Products of square matrices that commute (polynomials of one S), up to two in a launch: out = left right
+struct SquareJob { int left, right, out; float scale; };       // scale: out's pieces over the product of the operands' pieces
+struct SquareJobs { SquareJob j[2]; int n; };
+template <int BT>
+__global__ void __launch_bounds__(kThreads, 2) ns_square_kernel(Items L, SquareJobs jobs) {
+  extern __shared__ char lds[];
+  const Where w = find_item(L);
+  const Item& I = L.it[w.item];
+  const int tiles = tri_tiles(I), local = xcd_order(w.local, tiles * I.batch * jobs.n);
+  const int b = local / (tiles * jobs.n), t = local % tiles;
+  const SquareJob job = jobs.j[local / tiles % jobs.n];
+  int bi, bj;
+  tri_tile(t, bi, bj);
+  char* ws = I.ws + b * I.ws_stride;
+  const int kt = I.mp / 32;
+  Product<BT, 2, 2> acc;
+  acc.run(at<const _Float16>(ws, off_sq(I, job.left)), at<const _Float16>(ws, off_sq(I, job.right)), bi, bj, I.mp, I.mp, kt, 0,
+          kt, lds);
+  acc.each(bi, bj, I.mp, I.mp, [&](int p0, int q0, float (&v)[4]) {
+    store_symmetric(at<_Float16>(ws, off_sq(I, job.out)), kt, bi == bj, p0, q0, v, job.scale);
+  });
 }
 
 struct Finish { const float* lr_dev; float lr, decay; };
 
-// what becomes of value x at element `at` of the matrix
+// what becomes of value x at element `e` of the matrices
 template <typename T>
-__device__ __forceinline__ void put(const Item& I, int64_t at, float x, float lr, const Finish& f) {
+__device__ __forceinline__ void put(const Item& I, int64_t e, float x, float lr, const Finish& f) {
   T* out = static_cast<T*>(I.out);
-  if (I.mom) out[at] = (T)fmaf((float)out[at], fmaf(-lr, f.decay, 1.0f), -(lr * I.gain) * x);
-  else out[at] = (T)x;
+  if (I.mom) out[e] = (T)fmaf((float)out[e], fmaf(-lr, f.decay, 1.0f), -(lr * I.gain) * x);
+  else out[e] = (T)x;
 }
 
-// X <- a X + R X, computed as X^T <- a X^T + X^T R: block = 64 of the long axis x 64 of the short; the last step writes the
-// result instead
-template <typename T, bool LAST>
-__global__ void __launch_bounds__(kThreads) ns_update_kernel(Items L, Scales sc, float ca, int step, Finish f) {
-  const int from = step & 1;
+// X <- a X + M X, computed as X^T <- a X^T + X^T M (M symmetric; a = 0: M holds all of the step): block = BT of the long axis x
+// BT of the short; the last one writes the result instead.  PX pieces in, PN out.
+template <typename T, int BT, int PX, int PN, bool LAST>
+__global__ void __launch_bounds__(kThreads, 2) ns_update_kernel(Items L, Scales sc, float ca, int square, float scale_m, int from,
+                                                                int step, int next_step, Finish f) {
+  extern __shared__ char lds[];
   const Where w = find_item(L);
   const Item& I = L.it[w.item];
-  const int tm = (I.mp + 63) / 64, tn = (I.np + 63) / 64;
-  const int b = w.local / (tm * tn), t = w.local % (tm * tn), bi = t % tm, bj = t / tm;
+  const int tm = (I.mp + BT - 1) / BT, tn = (I.np + BT - 1) / BT;
+  const int local = xcd_order(w.local, tm * tn * I.batch), b = local / (tm * tn), t = local % (tm * tn), bi = t % tm, bj = t / tm;
   char* ws = I.ws + b * I.ws_stride;
-  const _Float16* xt = reinterpret_cast<const _Float16*>(ws + off_xt(I, from));
-  const _Float16* rm = reinterpret_cast<const _Float16*>(ws + off_r(I));
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, kt = I.mp / 32;
-  const int rj = bj * 64 + 32 * (wave & 1), ri = bi * 64 + 32 * (wave >> 1);
-  Acc acc;
-  product(xt, rm, rj, ri, I.np, I.mp, kt, 0, kt, acc);
-  const float scx = x_scale(I, ws, sc, step), next = x_scale(I, ws, sc, step + 1);
-  const float unscale = 1.0f / scx / sc.r, own = ca / scx;
+  const _Float16* xt = at<const _Float16>(ws, off_xt(I, from));
+  const int lane = threadIdx.x & 63, kt = I.mp / 32;
+  Product<BT, PX, 2> acc;
+  acc.run(xt, at<const _Float16>(ws, off_sq(I, square)), bj, bi, I.np, I.mp, kt, 0, kt, lds);
+  const Norm nm = *norm_slot(I, ws);
+  const float scx = x_scale(nm, sc, step), next = x_scale(nm, sc, next_step);
+  const float factor = step ? 1.0f : nm.factor, unscale = factor / scx / scale_m, own = ca * factor / scx;
   const float lr = f.lr_dev ? *f.lr_dev : f.lr;
+  acc.each(bj, bi, I.np, I.mp, [&](int j0, int i0, float (&v)[4]) {
+    // after the transpose lane l holds row j0 + 4 (l / 16) + l % 4 of X^T, columns i0 + (l & 12) ..
 #pragma unroll
-  for (int a = 0; a < 2; ++a)
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const int j0 = rj + 16 * a, i0 = ri + 16 * c;
-      if (j0 >= I.np || i0 >= I.mp) continue;
-      // after the transpose lane l holds row j0 + 4 (l / 16) + l % 4 of X^T, columns i0 + (l & 12) ..
-      float v[4], o[4];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) v[r] = acc.v[a][c][r] * unscale;
-      quad_transpose(v);
-      const int j = j0 + 4 * (lane >> 4) + (lane & 3), i = i0 + (lane & 12);
-      load_pieces(xt, j, i, kt, o, own);
+    for (int r = 0; r < 4; ++r) v[r] *= unscale;
+    quad_transpose(v);
+    const int j = j0 + 4 * (lane >> 4) + (lane & 3), i = i0 + (lane & 12);
+    if (ca != 0.0f) {
+      float o[4];
+      load_pieces<PX>(xt, j, i, kt, o, own);
 #pragma unroll
       for (int r = 0; r < 4; ++r) v[r] += o[r];
-      if constexpr (!LAST) {
-        store_pieces(reinterpret_cast<_Float16*>(ws + off_xt(I, from ^ 1)), j, i, kt, v, next);
-        quad_transpose(v);
-        store_pieces(reinterpret_cast<_Float16*>(ws), i0 + (lane & 15), j0 + 4 * (lane >> 4), I.np / 32, v, next);
-      } else if (I.tall) {
-        if (j < I.n) {
+    }
+    if constexpr (!LAST) {
+      store_pieces<PN>(at<_Float16>(ws, off_xt(I, from ^ 1)), j, i, kt, v, next);
+      quad_transpose(v);
+      store_pieces<PN>(at<_Float16>(ws, 0), i0 + (lane & 15), j0 + 4 * (lane >> 4), I.np / 32, v, next);
+    } else if (I.tall) {
+      if (j < I.n) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (i + r < I.m) put<T>(I, b * I.size + (int64_t)j * I.m + i + r, v[r], lr, f);
-        }
-      } else {
-        quad_transpose(v);
-        const int jj = j0 + 4 * (lane >> 4), ii = i0 + (lane & 15);
-        if (ii < I.m) {
+        for (int r = 0; r < 4; ++r)
+          if (i + r < I.m) put<T>(I, b * I.size + (int64_t)j * I.m + i + r, v[r], lr, f);
+      }
+    } else {
+      quad_transpose(v);
+      const int jj = j0 + 4 * (lane >> 4), ii = i0 + (lane & 15);
+      if (ii < I.m) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (jj + r < I.n) put<T>(I, b * I.size + (int64_t)ii * I.n + jj + r, v[r], lr, f);
-        }
+        for (int r = 0; r < 4; ++r)
+          if (jj + r < I.n) put<T>(I, b * I.size + (int64_t)ii * I.n + jj + r, v[r], lr, f);
       }
     }
+  });
 }
 
 // A matrix of one row (a vector): S is the number s = |X|^2 and X keeps its direction, so the whole iteration is one factor.
@@ -456,7 +556,11 @@ Item make_item(const NsMatrix& M) {
   I.size = M.rows * M.cols;
   const int64_t parts = (I.size + kThreads * 16 - 1) / (kThreads * 16);
   I.nsum = (int)(parts < kSumsMax ? parts : kSumsMax);
-  // splits of the long axis: enough blocks for the card, at least four inner tiles each
+  // blocks of 128 x 128 read half as much for a product as blocks of 64 x 64; they need a matrix that gives each of the
+  // 256 compute units one in the products along the long axis
+  const int64_t big = (int64_t)((I.mp + 127) / 128) * ((I.np + 127) / 128) * I.batch;
+  I.bt = I.m > 64 && big >= 192 ? 128 : 64;
+  // splits of the long axis: two blocks a compute unit, at least four inner tiles each
   const int kt = I.np / 32, tiles = tri_tiles(I);
   int64_t chunks = (512 + (int64_t)tiles * I.batch - 1) / ((int64_t)tiles * I.batch);
   if (chunks > kt / 4) chunks = kt / 4;
@@ -467,62 +571,130 @@ Item make_item(const NsMatrix& M) {
   return I;
 }
 
-int blocks_before(Items& L, int (*count)(const Item&)) {
+int blocks_before(Items& L, int (*count)(const Item&), int times = 1) {
   int total = 0;
-  for (int i = 0; i < L.n; ++i) { L.first[i] = total; total += count(L.it[i]) * L.it[i].batch; }
+  for (int i = 0; i < L.n; ++i) { L.first[i] = total; total += count(L.it[i]) * L.it[i].batch * times; }
   L.first[L.n] = total;
   return total;
 }
 int count_sums(const Item& I) { return I.nsum; }
-int count_tiles(const Item& I) { return ((I.mp + 63) / 64) * ((I.np + 63) / 64); }
+int count_split(const Item& I) { return ((I.mp + 63) / 64) * ((I.np + 63) / 64); }
+int count_tiles(const Item& I) { return ((I.mp + I.bt - 1) / I.bt) * ((I.np + I.bt - 1) / I.bt); }
 int count_tri(const Item& I) { return tri_tiles(I); }
 int count_gram(const Item& I) { return tri_tiles(I) * I.chunks; }
-int count_split(const Item& I) { return I.chunks > 1 ? tri_tiles(I) : 0; }
+int count_parts(const Item& I) { return I.chunks > 1 ? tri_tiles(I) * (I.bt * I.bt / 1024) : 0; }
+
+template <typename K, typename... A>
+void launch(K kernel, int blocks, size_t lds, hipStream_t st, A... args) {
+  if (!blocks) return;
+  ensure_dynamic_lds((const void*)kernel, lds);
+  hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kThreads), lds, st, args...);
+}
+
+// the products of all matrices of one block size
+template <typename T, int BT>
+struct Steps {
+  Items& L;
+  const NsPlan& p;
+  const Scales sc;
+  const Finish fin;
+  hipStream_t st;
+
+  template <int PX>
+  void gram(int step) {
+    launch(ns_gram_kernel<BT, PX>, blocks_before(L, count_gram), Product<BT, PX, PX>::kLds, st, L, sc, step);
+    Items S = L;                                       // the matrices whose long axis was split
+    S.n = 0;
+    for (int i = 0; i < L.n; ++i)
+      if (L.it[i].chunks > 1) S.it[S.n++] = L.it[i];
+    launch(ns_gram_sum_kernel<BT>, blocks_before(S, count_parts), 0, st, S, sc);
+  }
+  void poly(float a, int out) {
+    launch(ns_poly_kernel<BT>, blocks_before(L, count_tri), Product<BT, 2, 2>::kLds, st, L, sc, NsCoefficients{a, p.k.b, p.k.c},
+           out);
+  }
+  void squares(const SquareJobs& jobs) {
+    launch(ns_square_kernel<BT>, blocks_before(L, count_tri, jobs.n), Product<BT, 2, 2>::kLds, st, L, jobs);
+  }
+  template <int PX, int PN>
+  void update(float a, int square, float scale_m, int from, int step, int next) {
+    const int blocks = blocks_before(L, count_tiles);
+    constexpr int kLds = Product<BT, PX, 2>::kLds;
+    if (next < p.steps) launch(ns_update_kernel<T, BT, PX, PN, false>, blocks, kLds, st, L, sc, a, square, scale_m, from, step, next, fin);
+    else launch(ns_update_kernel<T, BT, PX, PN, true>, blocks, kLds, st, L, sc, a, square, scale_m, from, step, next, fin);
+  }
+
+  // step by step: S = X X^T, R = b S + c S S, X <- a X + R X
+  void plain() {
+    for (int k = 0; k < p.steps; ++k) {
+      gram<2>(k);
+      poly(0.0f, kQ);
+      update<2, 2>(p.k.a, kQ, sc.q, k & 1, k, k + 1);
+    }
+  }
+
+  // Up to three steps composed in the square matrices, then one product with X: with Q = a I + b S + c S S the step takes X to
+  // Q X and S to Q S Q, and all of these commute.  Three products along the long axis for five steps instead of ten.
+  // Rounding errors of S in the small singular directions grow by a^2 a step, so three steps cost about a factor 4 in
+  // accuracy over fp32, far below the 2^-9 or 2^-12 of a 16-bit result, and a new S is formed after them.
+  // PN: pieces that X keeps between.  In bf16 one: 2^-12 of each value, of random sign, which the remaining steps multiply by at
+  // most a each in the smallest directions only, against the result's own 2^-9.
+  template <int PN>
+  void composed() {
+    for (int k = 0, part = 0; k < p.steps; ++part) {
+      const int start = k, n = p.steps - k < 3 ? p.steps - k : 3;
+      if (part == 0) gram<1>(0);
+      else gram<PN>(start);
+      int cur = kP0;                                     // the composed steps so far; the first one is its own Q
+      float scale = sc.q;
+      for (int i = 0; i < n; ++i, ++k) {
+        const int q = i == 0 ? kP0 : kQ;
+        poly(p.k.a, q);
+        SquareJobs jobs{};
+        if (i > 0) {
+          const int out = cur == kP0 ? kP1 : kP0;
+          jobs.j[jobs.n++] = {kQ, cur, out, sc.p / (sc.q * scale)};
+          cur = out;
+          scale = sc.p;
+        }
+        if (i + 1 < n) jobs.j[jobs.n++] = {q, kS, kT, sc.t / (sc.q * sc.s)};
+        if (jobs.n) squares(jobs);
+        if (i + 1 < n) {
+          SquareJobs next{};
+          next.j[next.n++] = {kT, q, kS, sc.s / (sc.t * sc.q)};
+          squares(next);
+        }
+      }
+      if (part == 0) update<1, PN>(0.0f, cur, scale, 0, 0, k);
+      else update<PN, PN>(0.0f, cur, scale, part & 1, start, k);
+    }
+  }
+};
+
+template <typename T, int BT>
+void run_products(Items& L, const NsPlan& p, const Scales& sc, const Finish& fin, hipStream_t st) {
+  if (!L.n) return;
+  Steps<T, BT> s{L, p, sc, fin, st};
+  if constexpr (sizeof(T) == 4) s.plain();
+  else s.template composed<__is_same(T, __bf16) ? 1 : 2>();
+}
 
 template <typename T>
 void run_items(Items& L, const NsPlan& p, hipStream_t st) {
   const Momentum mo{p.momentum, p.nesterov};
   const Finish fin{p.lr_dev, p.lr, p.decay};
-  const dim3 block(kThreads);
-  auto launch_over = [&](int (*count)(const Item&), auto&& go) {
-    const int blocks = blocks_before(L, count);
-    if (blocks) go(dim3(blocks));
-  };
-  launch_over(count_sums, [&](dim3 g) { hipLaunchKernelGGL((ns_norm_kernel<T>), g, block, 0, st, L, mo); });
-  Items V, M;                                          // vectors and matrices
-  V.n = M.n = 0;
+  launch(ns_norm_kernel<T>, blocks_before(L, count_sums), 0, st, L, mo);
+  Items V, M, B;                                       // vectors, matrices in blocks of 64 and of 128
+  V.n = M.n = B.n = 0;
   for (int i = 0; i < L.n; ++i) {
-    Items& to = L.it[i].m == 1 ? V : M;
+    Items& to = L.it[i].m == 1 ? V : L.it[i].bt == 128 ? B : M;
     to.it[to.n++] = L.it[i];
   }
-  if (V.n) {
-    const int blocks = blocks_before(V, count_sums);
-    hipLaunchKernelGGL((ns_vector_kernel<T>), dim3(blocks), block, 0, st, V, mo, p.eps, p.k, p.steps, fin);
-  }
-  if (!M.n) return;
-  L = M;
-  Scales sc{p.scale_x, p.scale_s, p.scale_r, p.growth};
-  launch_over(count_tiles, [&](dim3 g) { hipLaunchKernelGGL((ns_split_kernel<T>), g, block, 0, st, L, mo, p.eps, sc); });
-  for (int k = 0; k < p.steps; ++k) {
-    launch_over(count_gram, [&](dim3 g) { hipLaunchKernelGGL(ns_gram_kernel, g, block, 0, st, L, sc, k); });
-    Items S = L;                                       // the matrices whose long axis was split
-    S.n = 0;
-    for (int i = 0; i < L.n; ++i)
-      if (L.it[i].chunks > 1) S.it[S.n++] = L.it[i];
-    if (S.n) {
-      const int blocks = blocks_before(S, count_split);
-      hipLaunchKernelGGL(ns_gram_sum_kernel, dim3(blocks), block, 0, st, S, sc);
-    }
-    launch_over(count_tri, [&](dim3 g) { hipLaunchKernelGGL(ns_poly_kernel, g, block, 0, st, L, sc, p.k.b, p.k.c); });
-    if (k + 1 < p.steps)
-      launch_over(count_tiles, [&](dim3 g) {
-        hipLaunchKernelGGL((ns_update_kernel<T, false>), g, block, 0, st, L, sc, p.k.a, k, fin);
-      });
-    else
-      launch_over(count_tiles, [&](dim3 g) {
-        hipLaunchKernelGGL((ns_update_kernel<T, true>), g, block, 0, st, L, sc, p.k.a, k, fin);
-      });
-  }
+  launch(ns_vector_kernel<T>, blocks_before(V, count_sums), 0, st, V, mo, p.eps, p.k, p.steps, fin);
+  const Scales sc{p.scale_x, p.scale_s, sizeof(T) == 4 ? p.scale_r : p.scale_q, p.scale_t, p.scale_p, p.growth};
+  for (Items* X : {&M, &B}) launch(ns_split_kernel<T, sizeof(T) == 2>, blocks_before(*X, count_split), 0, st, *X, mo, p.eps, sc);
+  run_products<T, 64>(M, p, sc, fin, st);
+  run_products<T, 128>(B, p, sc, fin, st);
 }
 
 }  // namespace
@@ -538,11 +710,11 @@ const char* ns_refusal(const NsMatrix& M) {
 }
 
 bool ns_scales(const NsCoefficients& k, int steps, NsPlan* p) {
-  // the largest |x (a + b x^2 + c x^4)| and |b s + c s^2| over the singular values a step can meet, by interval ends and
+  // the largest |x (a + b x^2 + c x^4)|, |b s + c s^2| and |a + b s + c s^2| over the singular values a step can meet, by interval ends and
   // the inner extrema, step by step from [0, 1]
   for (const float v : {k.a, k.b, k.c})
     if (!(std::fabs(v) < 4096.0f)) return false;
-  double top = 1.0, all = 1.0, rmax = 0.0, grow = 1.0;
+  double top = 1.0, all = 1.0, rmax = 0.0, qmax = 1.0;
   for (int i = 0; i < steps; ++i) {
     const double T = top;
     auto f = [&](double x) { return std::fabs(x * (k.a + x * x * (k.b + k.c * x * x))); };
@@ -565,18 +737,26 @@ bool ns_scales(const NsCoefficients& k, int steps, NsPlan* p) {
       const double s = -(double)k.b / (2.0 * k.c);
       if (s > 0.0 && s < T * T) rmax = std::fmax(rmax, r(s));
     }
-    // |a + b s + c s^2| <= |a| + the bound on R: what a step multiplies any singular value by
-    grow = std::fmax(grow, std::fabs(k.a) + rmax);
+    auto q = [&](double s) { return std::fabs(k.a + s * (k.b + k.c * s)); };
+    qmax = std::fmax(qmax, std::fmax(q(0.0), q(T * T)));
+    if (k.c != 0.0f) {
+      const double s = -(double)k.b / (2.0 * k.c);
+      if (s > 0.0 && s < T * T) qmax = std::fmax(qmax, q(s));
+    }
     top = next;
     all = std::fmax(all, top);
-    if (!(all < 64.0) || !(rmax < 4096.0)) return false;
+    if (!(all < 64.0) || !(rmax < 4096.0) || !(qmax < 4096.0)) return false;
   }
   // 1.01: rounding can carry a singular value past the bound
   const int kx = (int)std::ceil(std::log2(all * 1.01)), kr = (int)std::ceil(std::log2(std::fmax(rmax, 1.0) * 1.01));
   p->scale_x = std::ldexp(1.0f, 15 - kx);
   p->scale_s = std::ldexp(1.0f, 15 - 2 * kx);
   p->scale_r = std::ldexp(1.0f, 15 - kr);
-  p->growth = (int)std::ceil(std::log2(grow * 1.01));
+  const int kq = (int)std::ceil(std::log2(qmax * 1.01)), kp = (int)std::ceil(3.0 * std::log2(qmax * 1.01));
+  p->growth = kq;
+  p->scale_q = std::ldexp(1.0f, 15 - kq);
+  p->scale_t = std::ldexp(1.0f, 15 - kq - 2 * kx);
+  p->scale_p = std::ldexp(1.0f, 15 - kp);
   return true;
 }
 
