@@ -26,7 +26,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kThreads = 256;
 constexpr int kItemsMax = kNsItemsMax;    // matrices (or stacks of equal ones) a launch
-constexpr int kSumsMax = 256;             // partial sums of squares a matrix
+constexpr int kSumsMax = 1024;            // partial sums of squares a matrix
 
 // One matrix, or a stack of `batch` equal ones, and its share of the workspace.
 struct Item {
@@ -38,7 +38,7 @@ struct Item {
   int64_t size;           // rows * cols
   int rows, cols, m, n, mp, np, batch, tall;
   int nsum;               // partial sums of squares
-  int bt;                 // rows and columns a block of the products takes: 64 or 128
+  int bt, bts;            // rows and columns a block of the products takes, along the long axis and among squares: 64 or 128
   int chunks, kchunk;     // splits of the long axis in X X^T, inner tiles (of 32) a split
   float gain;
 };
@@ -57,6 +57,7 @@ enum Square { kS = 0, kQ = 1, kT = 2, kP0 = 3, kP1 = 4, kSquares = 5 };
 __device__ __host__ inline int64_t off_sq(const Item& I, int k) { return plane_bytes(I) * 3 + square_bytes(I) * k; }
 __device__ __host__ inline int64_t off_part(const Item& I) { return off_sq(I, kSquares); }
 __device__ __host__ inline int tri_tiles(const Item& I) { const int t = (I.mp + I.bt - 1) / I.bt; return t * (t + 1) / 2; }
+__device__ __host__ inline int tri_squares(const Item& I) { const int t = (I.mp + I.bts - 1) / I.bts; return t * (t + 1) / 2; }
 __device__ __host__ inline int64_t off_sums(const Item& I) {
   if (I.m == 1) return 0;                 // a vector has nothing else
   return off_part(I) + (I.chunks > 1 ? (int64_t)I.chunks * tri_tiles(I) * I.bt * I.bt * 4 : 0);
@@ -157,23 +158,40 @@ __device__ __forceinline__ float source_value(const Item& I, int64_t at, const M
   return mo.nesterov ? (1.0f - mo.mu) * g + mo.mu * m : m;
 }
 
-// Partial sums of squares of U in 64 bits (the squares of gradients as small as 1e-25 vanish in 32), one a block; the
-// optimiser's momentum is updated on the way.
+// Partial sums of squares of U in 64 bits (the squares of gradients as small as 1e-25 vanish in 32), one a block, a block's
+// values contiguous, 16 bytes of G a thread; the optimiser's momentum is updated on the way.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) ns_norm_kernel(Items L, Momentum mo) {
+  constexpr int kVec = 16 / sizeof(T);
+  typedef T Vec __attribute__((ext_vector_type(kVec)));
   __shared__ double red[kThreads / 64];
   const Where w = find_item(L);
   const Item& I = L.it[w.item];
   const int b = w.local / I.nsum, part = w.local % I.nsum;
-  const int64_t base = b * I.size;
+  const int64_t base = b * I.size, per = (I.size + I.nsum - 1) / I.nsum, span = (per + kThreads * kVec - 1) / (kThreads * kVec) * (kThreads * kVec);
+  const int64_t lo = part * span, hi = lo + span < I.size ? lo + span : I.size;
+  const T* src = static_cast<const T*>(I.src) + base;
+  const bool wide = (((uintptr_t)src | (I.mom ? (uintptr_t)(I.mom + base) : 0)) & 15) == 0;
   double s = 0.0;
-  for (int64_t i = (int64_t)part * kThreads + threadIdx.x; i < I.size; i += (int64_t)I.nsum * kThreads) {
-    if (I.mom) {
-      const float g = (float)static_cast<const T*>(I.src)[base + i];
-      I.mom[base + i] = fmaf(mo.mu, I.mom[base + i], (1.0f - mo.mu) * g);
+  if (!I.mom && wide) {
+#pragma unroll 4
+    for (int64_t i = lo + threadIdx.x * kVec; i + kVec <= hi; i += kThreads * kVec) {
+      const Vec v = *reinterpret_cast<const Vec*>(src + i);
+#pragma unroll
+      for (int k = 0; k < kVec; ++k) s = fma((double)(float)v[k], (double)(float)v[k], s);
     }
-    const double u = source_value<T>(I, base + i, mo);
-    s = fma(u, u, s);
+    if (hi == I.size)
+      for (int64_t i = hi - (hi - lo) % kVec + threadIdx.x; i < hi; i += kThreads) s = fma((double)(float)src[i], (double)(float)src[i], s);
+  } else {
+#pragma unroll 4
+    for (int64_t i = lo + threadIdx.x; i < hi; i += kThreads) {
+      if (I.mom) {
+        const float g = (float)src[i];
+        I.mom[base + i] = fmaf(mo.mu, I.mom[base + i], (1.0f - mo.mu) * g);
+      }
+      const double u = source_value<T>(I, base + i, mo);
+      s = fma(u, u, s);
+    }
   }
 #pragma unroll
   for (int d = 32; d >= 1; d >>= 1) s += __shfl_xor(s, d);
@@ -189,6 +207,7 @@ __global__ void __launch_bounds__(kThreads) ns_norm_kernel(Items L, Momentum mo)
 __device__ __forceinline__ double matrix_norm(const Item& I, int b) {
   const double* sums = reinterpret_cast<const double*>(I.ws + b * I.ws_stride + off_sums(I));
   double s = 0.0;
+#pragma unroll 4
   for (int k = threadIdx.x & 63; k < I.nsum; k += 64) s += sums[k];
 #pragma unroll
   for (int d = 32; d >= 1; d >>= 1) s += __shfl_xor(s, d);
@@ -415,7 +434,7 @@ __global__ void __launch_bounds__(kThreads, 2) ns_poly_kernel(Items L, Scales sc
   extern __shared__ char lds[];
   const Where w = find_item(L);
   const Item& I = L.it[w.item];
-  const int tiles = tri_tiles(I), local = xcd_order(w.local, tiles * I.batch), b = local / tiles, t = local % tiles;
+  const int tiles = tri_squares(I), local = xcd_order(w.local, tiles * I.batch), b = local / tiles, t = local % tiles;
   int bi, bj;
   tri_tile(t, bi, bj);
   char* ws = I.ws + b * I.ws_stride;
@@ -442,7 +461,7 @@ __global__ void __launch_bounds__(kThreads, 2) ns_square_kernel(Items L, SquareJ
   extern __shared__ char lds[];
   const Where w = find_item(L);
   const Item& I = L.it[w.item];
-  const int tiles = tri_tiles(I), local = xcd_order(w.local, tiles * I.batch * jobs.n);
+  const int tiles = tri_squares(I), local = xcd_order(w.local, tiles * I.batch * jobs.n);
   const int b = local / (tiles * jobs.n), t = local % tiles;
   const SquareJob job = jobs.j[local / tiles % jobs.n];
   int bi, bj;
@@ -554,12 +573,15 @@ Item make_item(const NsMatrix& M) {
   I.mp = round_up(I.m, 32);
   I.np = round_up(I.n, 32);
   I.size = M.rows * M.cols;
-  const int64_t parts = (I.size + kThreads * 16 - 1) / (kThreads * 16);
-  I.nsum = (int)(parts < kSumsMax ? parts : kSumsMax);
+  // a block of the norm takes at least 4096 values; all matrices together about eight blocks a compute unit
+  const int64_t parts = (I.size + kThreads * 16 - 1) / (kThreads * 16), most = kSumsMax / (I.batch < 4 ? I.batch : 4);
+  I.nsum = (int)(parts < most ? parts : most);
   // blocks of 128 x 128 read half as much for a product as blocks of 64 x 64; they need a matrix that gives each of the
   // 256 compute units one in the products along the long axis
   const int64_t big = (int64_t)((I.mp + 127) / 128) * ((I.np + 127) / 128) * I.batch;
   I.bt = I.m > 64 && big >= 192 ? 128 : 64;
+  const int64_t t128 = (I.mp + 127) / 128, squares = t128 * (t128 + 1) / 2 * I.batch;
+  I.bts = squares >= 512 ? 128 : 64;
   // splits of the long axis: two blocks a compute unit, at least four inner tiles each
   const int kt = I.np / 32, tiles = tri_tiles(I);
   int64_t chunks = (512 + (int64_t)tiles * I.batch - 1) / ((int64_t)tiles * I.batch);
@@ -580,7 +602,7 @@ int blocks_before(Items& L, int (*count)(const Item&), int times = 1) {
 int count_sums(const Item& I) { return I.nsum; }
 int count_split(const Item& I) { return ((I.mp + 63) / 64) * ((I.np + 63) / 64); }
 int count_tiles(const Item& I) { return ((I.mp + I.bt - 1) / I.bt) * ((I.np + I.bt - 1) / I.bt); }
-int count_tri(const Item& I) { return tri_tiles(I); }
+int count_squares(const Item& I) { return tri_squares(I); }
 int count_gram(const Item& I) { return tri_tiles(I) * I.chunks; }
 int count_parts(const Item& I) { return I.chunks > 1 ? tri_tiles(I) * (I.bt * I.bt / 1024) : 0; }
 
@@ -609,12 +631,24 @@ struct Steps {
       if (L.it[i].chunks > 1) S.it[S.n++] = L.it[i];
     launch(ns_gram_sum_kernel<BT>, blocks_before(S, count_parts), 0, st, S, sc);
   }
+  // the matrices whose squares go in blocks of `bts`
+  Items by_squares(int bts) const {
+    Items S = L;
+    S.n = 0;
+    for (int i = 0; i < L.n; ++i)
+      if (L.it[i].bts == bts) S.it[S.n++] = L.it[i];
+    return S;
+  }
   void poly(float a, int out) {
-    launch(ns_poly_kernel<BT>, blocks_before(L, count_tri), Product<BT, 2, 2>::kLds, st, L, sc, NsCoefficients{a, p.k.b, p.k.c},
-           out);
+    const NsCoefficients k{a, p.k.b, p.k.c};
+    Items S = by_squares(64), B = by_squares(128);
+    launch(ns_poly_kernel<64>, blocks_before(S, count_squares), Product<64, 2, 2>::kLds, st, S, sc, k, out);
+    launch(ns_poly_kernel<128>, blocks_before(B, count_squares), Product<128, 2, 2>::kLds, st, B, sc, k, out);
   }
   void squares(const SquareJobs& jobs) {
-    launch(ns_square_kernel<BT>, blocks_before(L, count_tri, jobs.n), Product<BT, 2, 2>::kLds, st, L, jobs);
+    Items S = by_squares(64), B = by_squares(128);
+    launch(ns_square_kernel<64>, blocks_before(S, count_squares, jobs.n), Product<64, 2, 2>::kLds, st, S, jobs);
+    launch(ns_square_kernel<128>, blocks_before(B, count_squares, jobs.n), Product<128, 2, 2>::kLds, st, B, jobs);
   }
   template <int PX, int PN>
   void update(float a, int square, float scale_m, int from, int step, int next) {
@@ -704,8 +738,9 @@ const char* ns_refusal(const NsMatrix& M) {
   const int64_t m = M.rows < M.cols ? M.rows : M.cols, n = M.rows < M.cols ? M.cols : M.rows;
   if (m > 32768 || n > (int64_t)1 << 30 || (m > 1 && n > (int64_t)1 << 24)) return "a side is too long (short side over 32768, or long side over 2^24, 2^30 for a vector)";
   // a launch holds fewer than 2^32 threads: 2^24 blocks of 256, over all the matrices that share it
-  const int64_t tiles = ((m + 63) / 64) * ((n + 63) / 64);
-  if (M.batch > ((int64_t)1 << 19) / (tiles > kSumsMax ? tiles : kSumsMax)) return "too many tiles in one stack";
+  const int64_t tiles = ((m + 63) / 64) * ((n + 63) / 64), values = (m * n + 4095) / 4096;
+  const int64_t sums = values < kSumsMax ? values : kSumsMax, most = m > 1 && tiles > sums ? tiles : sums;
+  if (M.batch > ((int64_t)1 << 19) / most) return "too many tiles in one stack";
   return nullptr;
 }
 
