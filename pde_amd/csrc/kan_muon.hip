@@ -40,8 +40,13 @@ struct Item {
   int nsum;               // partial sums of squares
   int bt, bts;            // rows and columns a block of the products takes, along the long axis and among squares: 64 or 128
   int chunks, kchunk;     // splits of the long axis in X X^T, inner tiles (of 32) a split
+  int path;               // see enum Path
+  int width, strips;      // columns of X a block of the small kernel takes, and how many such blocks there are
   float gain;
 };
+// kVector: one row, too long for one block;  kSingle: one block does everything (vectors too);  kStrips: one block a strip of
+// columns, a launch a step;  kTiles: one launch a product
+enum Path { kVector, kSingle, kStrips, kTiles };
 struct Items {
   Item it[kItemsMax];
   int first[kItemsMax + 1];               // first block of each item in this launch
@@ -59,7 +64,7 @@ __device__ __host__ inline int64_t off_part(const Item& I) { return off_sq(I, kS
 __device__ __host__ inline int tri_tiles(const Item& I) { const int t = (I.mp + I.bt - 1) / I.bt; return t * (t + 1) / 2; }
 __device__ __host__ inline int tri_squares(const Item& I) { const int t = (I.mp + I.bts - 1) / I.bts; return t * (t + 1) / 2; }
 __device__ __host__ inline int64_t off_sums(const Item& I) {
-  if (I.m == 1) return 0;                 // a vector has nothing else
+  if (I.path == kVector) return 0;        // a vector has nothing else
   return off_part(I) + (I.chunks > 1 ? (int64_t)I.chunks * tri_tiles(I) * I.bt * I.bt * 4 : 0);
 }
 __device__ __host__ inline int64_t item_bytes(const Item& I) {
@@ -270,14 +275,16 @@ __global__ void __launch_bounds__(kThreads) ns_split_kernel(Items L, Momentum mo
 
 // P Q^T of a BT x BT block over inner tiles [k0, k1), PP and PQ pieces an operand.  Four waves take a quarter each: acc[a][c]
 // is the 16 x 16 block at rows 16 a of P and 16 c of Q; lane l holds Q's row l % 16 and P's rows 4 (l / 16) + r.
-// Operand tiles go from memory to LDS without passing registers, `kStages` inner tiles of the whole block in a ring, and
+// Operand tiles go from memory to LDS without passing registers, kStages inner tiles of the whole block in a ring, and
 // from LDS to registers as contiguous 1 KB reads.
 template <int BT, int PP, int PQ>
 struct Product {
   static constexpr int kW = BT / 32;                           // 16-row tiles a wave takes of either operand
   static constexpr int kFrags = BT / 16 * (PP + PQ);           // 1 KB pieces of tiles a stage
   static constexpr int kLoads = kFrags / 4;                    // a wave's
-  static constexpr int kStages = kFrags * 1024 * 4 <= 64 * 1024 ? 4 : kFrags * 1024 * 3 <= 80 * 1024 ? 3 : 2;
+  // as many stages as leave room for three blocks of 64 or two of 128 a compute unit
+  static constexpr int kRoom = BT == 64 ? 48 * 1024 : 80 * 1024;
+  static constexpr int kStages = kRoom / (kFrags * 1024) < 4 ? kRoom / (kFrags * 1024) : 4;
   static constexpr int kLds = kFrags * 1024 * kStages;
   f32x4 v[kW][kW];
 
@@ -311,38 +318,65 @@ struct Product {
       for (int c = 0; c < kW; ++c) v[a][c] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
     const int n = k1 - k0;
 #pragma unroll
-    for (int i = 0; i < kStages - 1; ++i)
+    for (int i = 0; i < kStages; ++i)
       if (i < n) fetch(i);
-    int stage = 0, free = kStages - 1;
-    for (int i = 0; i < n; ++i) {
-      // this stage has landed (later ones may still be on their way), and every wave is done with the one before
-      if (i + kStages - 2 < n) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kStages - 2) * kLoads) : "memory");
-      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __builtin_amdgcn_s_barrier();
-      asm volatile("" ::: "memory");
-      if (i + kStages - 1 < n) fetch(free);
+    // Step i multiplies what step i - 1 read from LDS, and reads the next inner tile meanwhile.  Its wait leaves the stages
+    // after the next on their way; behind the barrier every wave has stage i in registers, so its place takes a new one.
+    struct Regs { f16x8 p[kW][PP], q[kW][PQ]; };
+    auto read = [&](Regs& r, int stage) {
       const char* base = lds + stage * (kFrags * 1024) + lane * 16;
-      f16x8 p[kW][PP], q[kW][PQ];
 #pragma unroll
       for (int a = 0; a < kW; ++a) {
 #pragma unroll
         for (int h = 0; h < PP; ++h)
-          p[a][h] = *reinterpret_cast<const f16x8*>(base + (((wave & 1) * kW + a) * PP + h) * 1024);
+          r.p[a][h] = *reinterpret_cast<const f16x8*>(base + (((wave & 1) * kW + a) * PP + h) * 1024);
 #pragma unroll
         for (int h = 0; h < PQ; ++h)
-          q[a][h] = *reinterpret_cast<const f16x8*>(base + (BT / 16 * PP + ((wave >> 1) * kW + a) * PQ + h) * 1024);
+          r.q[a][h] = *reinterpret_cast<const f16x8*>(base + (BT / 16 * PP + ((wave >> 1) * kW + a) * PQ + h) * 1024);
       }
+    };
+    // one kind of product over all blocks, then the next: instructions on one accumulator stand kW^2 apart
+    auto multiply = [&](const Regs& r) {
 #pragma unroll
-      for (int a = 0; a < kW; ++a)
+      for (int kind = 0; kind < 3; ++kind) {
+        const int hp = kind == 0, hq = kind == 1;
+        if ((hp && PP == 1) || (hq && PQ == 1)) continue;
 #pragma unroll
-        for (int c = 0; c < kW; ++c) {
-          if constexpr (PP == 2) v[a][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(p[a][1], q[c][0], v[a][c], 0, 0, 0);
-          if constexpr (PQ == 2) v[a][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(p[a][0], q[c][1], v[a][c], 0, 0, 0);
-          v[a][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(p[a][0], q[c][0], v[a][c], 0, 0, 0);
-        }
-      stage = stage + 1 == kStages ? 0 : stage + 1;
-      free = free + 1 == kStages ? 0 : free + 1;
+        for (int a = 0; a < kW; ++a)
+#pragma unroll
+          for (int c = 0; c < kW; ++c)
+            v[a][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(r.p[a][hp ? PP - 1 : 0], r.q[c][hq ? PQ - 1 : 0], v[a][c], 0, 0, 0);
+      }
+    };
+    auto landed = [&](bool more) {
+      if (more) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((kStages - 2) * kLoads) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+    };
+    // the first stage: up to kStages - 1 younger ones
+    if (n >= kStages) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kStages - 1) * kLoads) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    Regs ra, rb;
+    read(ra, 0);
+    int stage = 0;
+    auto one = [&](int i, const Regs& now, Regs& next) {
+      if (i + 1 < n) {
+        landed(i + kStages <= n);
+        if (i + kStages < n) fetch(stage);
+        stage = stage + 1 == kStages ? 0 : stage + 1;
+        read(next, stage);
+      }
+      multiply(now);
+    };
+    int i = 0;
+    for (; i + 1 < n; i += 2) {
+      one(i, ra, rb);
+      one(i + 1, rb, ra);
     }
+    if (i < n) multiply(ra);
   }
   // first rows of P and Q of this wave's part
   static __device__ __forceinline__ int row_p(int bp) { return bp * BT + (threadIdx.x >> 6 & 1) * (BT / 2); }
@@ -381,7 +415,7 @@ __device__ __forceinline__ int xcd_order(int local, int count) {
 
 // S = X X^T: block = (split of the long axis, tile of the upper triangle)
 template <int BT, int PX>
-__global__ void __launch_bounds__(kThreads, 2) ns_gram_kernel(Items L, Scales sc, int step) {
+__global__ void __launch_bounds__(kThreads, BT == 64 ? 3 : 2) ns_gram_kernel(Items L, Scales sc, int step) {
   extern __shared__ char lds[];
   const Where w = find_item(L);
   const Item& I = L.it[w.item];
@@ -430,7 +464,7 @@ __global__ void __launch_bounds__(kThreads) ns_gram_sum_kernel(Items L, Scales s
 
 // Q = a I + b S + c S S  (a = 0: R, the step less its multiple of one)
 template <int BT>
-__global__ void __launch_bounds__(kThreads, 2) ns_poly_kernel(Items L, Scales sc, NsCoefficients k, int out) {
+__global__ void __launch_bounds__(kThreads, BT == 64 ? 3 : 2) ns_poly_kernel(Items L, Scales sc, NsCoefficients k, int out) {
   extern __shared__ char lds[];
   const Where w = find_item(L);
   const Item& I = L.it[w.item];
@@ -457,7 +491,7 @@ __global__ void __launch_bounds__(kThreads, 2) ns_poly_kernel(Items L, Scales sc
 struct SquareJob { int left, right, out; float scale; };       // scale: out's pieces over the product of the operands' pieces
 struct SquareJobs { SquareJob j[2]; int n; };
 template <int BT>
-__global__ void __launch_bounds__(kThreads, 2) ns_square_kernel(Items L, SquareJobs jobs) {
+__global__ void __launch_bounds__(kThreads, BT == 64 ? 3 : 2) ns_square_kernel(Items L, SquareJobs jobs) {
   extern __shared__ char lds[];
   const Where w = find_item(L);
   const Item& I = L.it[w.item];
@@ -489,7 +523,7 @@ __device__ __forceinline__ void put(const Item& I, int64_t e, float x, float lr,
 // X <- a X + M X, computed as X^T <- a X^T + X^T M (M symmetric; a = 0: M holds all of the step): block = BT of the long axis x
 // BT of the short; the last one writes the result instead.  PX pieces in, PN out.
 template <typename T, int BT, int PX, int PN, bool LAST>
-__global__ void __launch_bounds__(kThreads, 2) ns_update_kernel(Items L, Scales sc, float ca, int square, float scale_m, int from,
+__global__ void __launch_bounds__(kThreads, BT == 64 ? 3 : 2) ns_update_kernel(Items L, Scales sc, float ca, int square, float scale_m, int from,
                                                                 int step, int next_step, Finish f) {
   extern __shared__ char lds[];
   const Where w = find_item(L);
@@ -539,24 +573,317 @@ __global__ void __launch_bounds__(kThreads, 2) ns_update_kernel(Items L, Scales 
   });
 }
 
-// A matrix of one row (a vector): S is the number s = |X|^2 and X keeps its direction, so the whole iteration is one factor.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) ns_vector_kernel(Items L, Momentum mo, float eps, NsCoefficients k, int steps,
-                                                             Finish f) {
-  const Where w = find_item(L);
-  const Item& I = L.it[w.item];
-  const int b = w.local / I.nsum, part = w.local % I.nsum;
-  const double norm = matrix_norm(I, b);
+// what the steps multiply U by where it is a single row: S is the number |X|^2 and X keeps its direction
+__device__ __forceinline__ double vector_factor(double norm, float eps, const NsCoefficients& k, int steps) {
   double factor = 1.0 / (norm + (double)eps), length = norm * factor;
   for (int i = 0; i < steps; ++i) {
     const double s = length * length, q = k.a + s * ((double)k.b + k.c * s);
     factor *= q;
     length *= q;
   }
+  return factor;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) ns_vector_kernel(Items L, Momentum mo, float eps, NsCoefficients k, int steps,
+                                                             Finish f) {
+  const Where w = find_item(L);
+  const Item& I = L.it[w.item];
+  const int b = w.local / I.nsum, part = w.local % I.nsum;
+  const double factor = vector_factor(matrix_norm(I, b), eps, k, steps);
   const float lr = f.lr_dev ? *f.lr_dev : f.lr;
   const int64_t base = b * I.size;
   for (int64_t i = (int64_t)part * kThreads + threadIdx.x; i < I.size; i += (int64_t)I.nsum * kThreads)
     put<T>(I, base + i, (float)((double)source_value<T>(I, base + i, mo) * factor), lr, f);
+}
+
+// ---- small matrices -------------------------------------------------------------------------------------------------
+
+// A block of eight waves holds a strip of X's columns in LDS: X [mp][width] and X^T [width][mp] as two-piece tiles, and S or R
+// [mp][mp], mp <= 128.  Where the strip is the whole matrix the block runs all steps on its own (kSingle); else each block
+// leaves its part of X X^T in memory, and the launch of the next step lets every block of the matrix add up all parts - the
+// sum, S S and R are formed once a block, which costs less than a launch of their own (kStrips).
+constexpr int kSmallThreads = 512, kSmallWaves = kSmallThreads / 64;
+constexpr int kSmallRows = 128;                                // mp at most
+constexpr int kTriMax = 36, kTriWave = (kTriMax + kSmallWaves - 1) / kSmallWaves;
+constexpr int kUpdateWave = 8;                                 // 16 x 16 blocks of X a wave: width * mp / 256 / 8 at most
+constexpr int kSmallLds = 150 * 1024;
+constexpr float kFirst = 16384.0f;                             // what U 2^-e, |.| <= 1, is multiplied by before the first step
+
+__device__ __host__ inline int tri16(int mp) { return mp / 16 * (mp / 16 + 1) / 2; }
+__device__ __host__ inline int64_t strip_bytes(const Item& I) { return (int64_t)I.width * I.mp * 4; }
+__device__ __host__ inline int64_t off_parts(const Item& I, int parity) {
+  return strip_bytes(I) * I.strips + (int64_t)parity * I.strips * tri16(I.mp) * 1024;
+}
+__device__ __host__ inline int64_t off_squares_sum(const Item& I) { return off_parts(I, 2); }           // double [strips]
+__device__ __host__ inline int64_t off_exponents(const Item& I) { return off_squares_sum(I) + I.strips * 8; }   // int [strips]
+__device__ __host__ inline int64_t small_bytes(const Item& I) {
+  return I.path == kSingle ? 256 : (off_exponents(I) + I.strips * 4 + 255) / 256 * 256;
+}
+
+__device__ __forceinline__ double block_sum(double s, double* red) {
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) s += __shfl_xor(s, d);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  s = 0.0;
+  for (int k = 0; k < kSmallWaves; ++k) s += red[k];
+  return s;
+}
+__device__ __forceinline__ float block_max(float v, double* red) {
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = 0.0f;
+  for (int k = 0; k < kSmallWaves; ++k) v = fmaxf(v, (float)red[k]);
+  return v;
+}
+// exponent of (|U| + eps) / |U|, see Scales
+__device__ __forceinline__ int small_exponent(double norm, double eps) {
+  const double small = (norm + eps) / norm;
+  return small > 1.0 && norm > 0.0 ? (small < 7.9e28 ? ilogb(small) : 96) : 0;
+}
+
+// 16 x 16 block of P Q^T from tiles of two pieces in LDS: row of tiles `a` of P and `b` of Q, kp and kq inner tiles a row
+__device__ __forceinline__ f32x4 block_product(const _Float16* P, const _Float16* Q, int a, int b, int kt) {
+  const int lane = threadIdx.x & 63;
+  f32x4 lh = (f32x4){0.0f, 0.0f, 0.0f, 0.0f}, hl = lh, hh = lh;
+  const _Float16 *p = P + a * kt * 1024 + lane * 8, *q = Q + b * kt * 1024 + lane * 8;
+#pragma unroll 2
+  for (int k = 0; k < kt; ++k) {
+    const f16x8 ph = *reinterpret_cast<const f16x8*>(p + k * 1024), pl = *reinterpret_cast<const f16x8*>(p + k * 1024 + 512);
+    const f16x8 qh = *reinterpret_cast<const f16x8*>(q + k * 1024), ql = *reinterpret_cast<const f16x8*>(q + k * 1024 + 512);
+    lh = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl, qh, lh, 0, 0, 0);
+    hl = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, ql, hl, 0, 0, 0);
+    hh = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, qh, hh, 0, 0, 0);
+  }
+  return hh + (lh + hl);
+}
+
+// step < 0: the strips' U, their sums of squares and first parts;  step >= 0: that step of the strips;  SINGLE: everything
+template <typename T, bool SINGLE>
+__global__ void __launch_bounds__(kSmallThreads) ns_small_kernel(Items L, Momentum mo, float eps, NsCoefficients kc, int steps,
+                                                                 int step, Scales sc, Finish f) {
+  extern __shared__ char lds[];
+  __shared__ double red[kSmallWaves];
+  const Where w = find_item(L);
+  const Item& I = L.it[w.item];
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int b = w.local / I.strips, strip = w.local % I.strips;
+  const int64_t base = b * I.size;
+  const float lr = f.lr_dev ? *f.lr_dev : f.lr;
+  if (SINGLE && I.m == 1) {
+    // X keeps the direction of the vector, S is the number |X|^2: the whole iteration is one factor
+    double s = 0.0;
+    for (int i = tid; i < I.n; i += kSmallThreads) {
+      if (I.mom) I.mom[base + i] = fmaf(mo.mu, I.mom[base + i], (1.0f - mo.mu) * (float)static_cast<const T*>(I.src)[base + i]);
+      const double u = source_value<T>(I, base + i, mo);
+      s = fma(u, u, s);
+    }
+    const double norm = sqrt(block_sum(s, red));
+    const double factor = vector_factor(norm, eps, kc, steps);
+    for (int i = tid; i < I.n; i += kSmallThreads)
+      put<T>(I, base + i, (float)((double)source_value<T>(I, base + i, mo) * factor), lr, f);
+    return;
+  }
+  const int mp = I.mp, width = I.width, rb = mp / 16, mt = mp / 32, wb = width / 16, wt = width / 32, ntri = tri16(mp);
+  _Float16* xt = reinterpret_cast<_Float16*>(lds);
+  _Float16* x = xt + width * mp * 2;
+  _Float16* sq = x + width * mp * 2;
+  char* ws = I.ws + b * I.ws_stride;
+  double* sums = at<double>(ws, off_squares_sum(I));
+  int* exps = at<int>(ws, off_exponents(I));
+  double norm = 0.0;
+  float first = 0.0f;                                           // X of the first step = first * (its pieces' values)
+
+  if (SINGLE || step < 0) {
+    // U of the strip, in fp32 where X's pieces go afterwards
+    float* u = reinterpret_cast<float*>(x);                     // [width][mp]
+    const int j0 = strip * width;
+    double s = 0.0;
+    float big = 0.0f;
+    for (int k = tid; k < width * mp; k += kSmallThreads) {
+      // neighbouring threads on neighbouring addresses
+      const int i = I.tall ? k % mp : k / width, j = I.tall ? k / mp : k % width;
+      float v = 0.0f;
+      if (i < I.m && j0 + j < I.n) {
+        const int64_t e = base + (I.tall ? (int64_t)(j0 + j) * I.m + i : (int64_t)i * I.n + j0 + j);
+        if (I.mom) I.mom[e] = fmaf(mo.mu, I.mom[e], (1.0f - mo.mu) * (float)static_cast<const T*>(I.src)[e]);
+        v = source_value<T>(I, e, mo);
+        s = fma((double)v, (double)v, s);
+        big = fmaxf(big, fabsf(v));
+      }
+      u[j * mp + i] = v;
+    }
+    s = block_sum(s, red);
+    big = block_max(big, red);
+    const int e = big > 0.0f && big < 3.4e38f ? ilogbf(big) + 1 : 0;
+    __syncthreads();
+    for (int k = tid; k < width * (mp / 4); k += kSmallThreads) {
+      const int j = k / (mp / 4), i = k % (mp / 4) * 4;
+      const float4 t = *reinterpret_cast<const float4*>(u + j * mp + i);
+      const float v[4] = {ldexpf(t.x, -e), ldexpf(t.y, -e), ldexpf(t.z, -e), ldexpf(t.w, -e)};
+      store_pieces<2>(xt, j, i, mt, v, kFirst);
+    }
+    __syncthreads();
+    for (int k = tid; k < mp * (width / 4); k += kSmallThreads) {
+      const int i = k % mp, j = k / mp * 4;
+      _Float16* to = x + piece_at<2>(i, j, wt);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const _Float16* from = xt + piece_at<2>(j + r, i, mt);
+        to[r] = from[0];
+        to[512 + r] = from[512];
+      }
+    }
+    __syncthreads();
+    if constexpr (SINGLE) {
+      norm = sqrt(s);
+      first = (float)ldexp(1.0 / (norm + (double)eps), e);
+    } else {
+      if (tid == 0) { sums[strip] = s; exps[strip] = e; }
+      // X^T's pieces to memory
+      const f32x4* from = reinterpret_cast<const f32x4*>(xt);
+      f32x4* to = at<f32x4>(ws, strip_bytes(I) * strip);
+      for (int k = tid; k < width * mp / 4; k += kSmallThreads) to[k] = from[k];
+    }
+  } else {
+    const f32x4* from = at<const f32x4>(ws, strip_bytes(I) * strip);
+    f32x4* to = reinterpret_cast<f32x4*>(xt);
+    for (int k = tid; k < width * mp / 4; k += kSmallThreads) to[k] = from[k];
+    double s = 0.0;
+    for (int k = 0; k < I.strips; ++k) s += sums[k];
+    norm = sqrt(s);
+    if (step == 0) first = (float)ldexp(1.0 / (norm + (double)eps), exps[strip]);
+  }
+  Norm nm;
+  nm.factor = 1.0f;
+  nm.ex = small_exponent(norm, eps);
+
+  for (int k = SINGLE ? 0 : step; k >= 0 && k < steps; ++k) {
+    const float inv_x = k == 0 ? first / kFirst : 1.0f / x_scale(nm, sc, k);        // X over its pieces
+    {
+      // S
+      if (SINGLE) {
+        for (int t = wave; t < ntri; t += kSmallWaves) {
+          int ba, bb;
+          tri_tile(t, ba, bb);
+          const f32x4 r = block_product(x, x, ba, bb, wt) * (inv_x * inv_x);
+          float v[4] = {r[0], r[1], r[2], r[3]};
+          store_symmetric(sq, mt, ba == bb, ba * 16, bb * 16, v, sc.s);
+        }
+      } else {
+        const f32x4* part = at<const f32x4>(ws, off_parts(I, k & 1));
+        for (int t = wave; t < ntri; t += kSmallWaves) {
+          int ba, bb;
+          tri_tile(t, ba, bb);
+          f32x4 r = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
+          for (int p = 0; p < I.strips; ++p) {
+            float scale = inv_x * inv_x;
+            if (k == 0) {
+              const float own = (float)ldexp(1.0 / (norm + (double)eps), exps[p]) / kFirst;
+              scale = own * own;
+            }
+            r += part[((int64_t)p * ntri + t) * 64 + lane] * scale;
+          }
+          float v[4] = {r[0], r[1], r[2], r[3]};
+          store_symmetric(sq, mt, ba == bb, ba * 16, bb * 16, v, sc.s);
+        }
+      }
+      __syncthreads();
+      // R = b S + c S S, in the place of S once every wave has read it
+      float rv[kTriWave][4];
+#pragma unroll
+      for (int q = 0; q < kTriWave; ++q) {
+        const int t = wave + q * kSmallWaves;
+        if (t < ntri) {
+          int ba, bb;
+          tri_tile(t, ba, bb);
+          const f32x4 r = block_product(sq, sq, ba, bb, mt);
+          float o[4];
+          load_pieces<2>(sq, bb * 16 + (lane & 15), ba * 16 + 4 * (lane >> 4), mt, o, 1.0f / sc.s);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) rv[q][i] = fmaf(kc.c / (sc.s * sc.s), r[i], kc.b * o[i]);
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int q = 0; q < kTriWave; ++q) {
+        const int t = wave + q * kSmallWaves;
+        if (t < ntri) {
+          int ba, bb;
+          tri_tile(t, ba, bb);
+          store_symmetric(sq, mt, ba == bb, ba * 16, bb * 16, rv[q], sc.q);
+        }
+      }
+      __syncthreads();
+      // X^T <- a X^T + X^T R, likewise
+      const bool last = k + 1 == steps;
+      const float next = x_scale(nm, sc, k + 1), own = kc.a * inv_x, unscale = inv_x / sc.q;
+      float xv[kUpdateWave][4];
+#pragma unroll
+      for (int q = 0; q < kUpdateWave; ++q) {
+        const int t = wave + q * kSmallWaves;
+        if (t < wb * rb) {
+          const int jb = t % wb, ib = t / wb;
+          const f32x4 r = block_product(xt, sq, jb, ib, mt);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) xv[q][i] = r[i] * unscale;
+          quad_transpose(xv[q]);
+          float o[4];
+          load_pieces<2>(xt, jb * 16 + 4 * (lane >> 4) + (lane & 3), ib * 16 + (lane & 12), mt, o, own);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) xv[q][i] += o[i];
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int q = 0; q < kUpdateWave; ++q) {
+        const int t = wave + q * kSmallWaves;
+        if (t < wb * rb) {
+          const int jb = t % wb, ib = t / wb;
+          const int j = jb * 16 + 4 * (lane >> 4) + (lane & 3), i = ib * 16 + (lane & 12);
+          const int j4 = jb * 16 + 4 * (lane >> 4), i1 = ib * 16 + (lane & 15);
+          if (!last) {
+            store_pieces<2>(SINGLE ? xt : at<_Float16>(ws, strip_bytes(I) * strip), j, i, mt, xv[q], next);
+            quad_transpose(xv[q]);
+            store_pieces<2>(x, i1, j4, wt, xv[q], next);
+          } else if (I.tall) {
+            const int jj = strip * width + j;
+            if (jj < I.n) {
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                if (i + r < I.m) put<T>(I, base + (int64_t)jj * I.m + i + r, xv[q][r], lr, f);
+            }
+          } else {
+            quad_transpose(xv[q]);
+            const int jj = strip * width + j4;
+            if (i1 < I.m) {
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                if (jj + r < I.n) put<T>(I, base + (int64_t)i1 * I.n + jj + r, xv[q][r], lr, f);
+            }
+          }
+        }
+      }
+      __syncthreads();
+      if (last) return;
+    }
+    if constexpr (!SINGLE) break;
+  }
+  if constexpr (!SINGLE) {
+    // this strip's part of the next S, as the pieces multiply
+    f32x4* part = at<f32x4>(ws, off_parts(I, (step + 1) & 1)) + (int64_t)strip * ntri * 64;
+    for (int t = wave; t < ntri; t += kSmallWaves) {
+      int ba, bb;
+      tri_tile(t, ba, bb);
+      part[t * 64 + lane] = block_product(x, x, ba, bb, wt);
+    }
+  }
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------------
@@ -580,8 +907,9 @@ Item make_item(const NsMatrix& M) {
   // 256 compute units one in the products along the long axis
   const int64_t big = (int64_t)((I.mp + 127) / 128) * ((I.np + 127) / 128) * I.batch;
   I.bt = I.m > 64 && big >= 192 ? 128 : 64;
-  const int64_t t128 = (I.mp + 127) / 128, squares = t128 * (t128 + 1) / 2 * I.batch;
-  I.bts = squares >= 512 ? 128 : 64;
+  // among squares only the upper triangle's blocks are computed: 128 x 128 ones where they are two a compute unit
+  const int64_t t128 = (I.mp + 127) / 128;
+  I.bts = t128 * (t128 + 1) / 2 * I.batch >= 512 ? 128 : 64;
   // splits of the long axis: two blocks a compute unit, at least four inner tiles each
   const int kt = I.np / 32, tiles = tri_tiles(I);
   int64_t chunks = (512 + (int64_t)tiles * I.batch - 1) / ((int64_t)tiles * I.batch);
@@ -589,7 +917,26 @@ Item make_item(const NsMatrix& M) {
   if (chunks < 1) chunks = 1;
   I.kchunk = (kt + (int)chunks - 1) / (int)chunks;
   I.chunks = (kt + I.kchunk - 1) / I.kchunk;
-  I.ws_stride = I.m == 1 ? (int64_t)kSumsMax * (int64_t)sizeof(double) : item_bytes(I);
+  // the widest strip whose X, X^T and square fit the LDS and the waves' registers
+  const int room = I.mp <= kSmallRows ? (kSmallLds - I.mp * I.mp * 4) / (I.mp * 8) / 32 * 32 : 0;
+  const int hold = kUpdateWave * kSmallWaves * 256 / I.mp, widest = room < hold ? room : hold;
+  I.strips = 1;
+  I.width = I.np;
+  I.path = kTiles;
+  if (I.m == 1) {
+    I.path = I.n <= 65536 ? kSingle : kVector;
+  } else if (I.mp <= kSmallRows) {
+    if (I.np <= widest) {
+      I.path = kSingle;
+    } else {
+      // strips of 64 columns (128 of the narrowest matrices): a block of the next step reads a part of tri16 KB of each, which
+      // has to stay below what the launches that it saves cost
+      const int width = I.mp <= 64 ? 128 : 64;
+      const int strips = (I.np + width - 1) / width;
+      if ((int64_t)strips * tri16(I.mp) <= 1024) { I.path = kStrips; I.width = width; I.strips = strips; }
+    }
+  }
+  I.ws_stride = I.path == kVector ? (int64_t)kSumsMax * (int64_t)sizeof(double) : I.path == kTiles ? item_bytes(I) : small_bytes(I);
   return I;
 }
 
@@ -600,17 +947,18 @@ int blocks_before(Items& L, int (*count)(const Item&), int times = 1) {
   return total;
 }
 int count_sums(const Item& I) { return I.nsum; }
+int count_strips(const Item& I) { return I.strips; }
 int count_split(const Item& I) { return ((I.mp + 63) / 64) * ((I.np + 63) / 64); }
 int count_tiles(const Item& I) { return ((I.mp + I.bt - 1) / I.bt) * ((I.np + I.bt - 1) / I.bt); }
 int count_squares(const Item& I) { return tri_squares(I); }
 int count_gram(const Item& I) { return tri_tiles(I) * I.chunks; }
 int count_parts(const Item& I) { return I.chunks > 1 ? tri_tiles(I) * (I.bt * I.bt / 1024) : 0; }
 
-template <typename K, typename... A>
+template <int THREADS = kThreads, typename K, typename... A>
 void launch(K kernel, int blocks, size_t lds, hipStream_t st, A... args) {
   if (!blocks) return;
   ensure_dynamic_lds((const void*)kernel, lds);
-  hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kThreads), lds, st, args...);
+  hipLaunchKernelGGL(kernel, dim3(blocks), dim3(THREADS), lds, st, args...);
 }
 
 // the products of all matrices of one block size
@@ -631,24 +979,35 @@ struct Steps {
       if (L.it[i].chunks > 1) S.it[S.n++] = L.it[i];
     launch(ns_gram_sum_kernel<BT>, blocks_before(S, count_parts), 0, st, S, sc);
   }
-  // the matrices whose squares go in blocks of `bts`
-  Items by_squares(int bts) const {
+  // go(the matrices whose squares go in blocks of `bts`, their number of blocks), for each block size there is
+  template <int BTS, typename Go>
+  void squares_of(int jobs, Go&& go) {
     Items S = L;
     S.n = 0;
     for (int i = 0; i < L.n; ++i)
-      if (L.it[i].bts == bts) S.it[S.n++] = L.it[i];
-    return S;
+      if (L.it[i].bts == BTS) S.it[S.n++] = L.it[i];
+    const int blocks = blocks_before(S, count_squares, jobs);
+    if (blocks) go(S, blocks);
+  }
+  template <int BTS>
+  void poly_in(const NsCoefficients& k, int out) {
+    squares_of<BTS>(1, [&](const Items& S, int blocks) {
+      launch(ns_poly_kernel<BTS>, blocks, Product<BTS, 2, 2>::kLds, st, S, sc, k, out);
+    });
   }
   void poly(float a, int out) {
-    const NsCoefficients k{a, p.k.b, p.k.c};
-    Items S = by_squares(64), B = by_squares(128);
-    launch(ns_poly_kernel<64>, blocks_before(S, count_squares), Product<64, 2, 2>::kLds, st, S, sc, k, out);
-    launch(ns_poly_kernel<128>, blocks_before(B, count_squares), Product<128, 2, 2>::kLds, st, B, sc, k, out);
+    poly_in<64>({a, p.k.b, p.k.c}, out);
+    poly_in<128>({a, p.k.b, p.k.c}, out);
+  }
+  template <int BTS>
+  void squares_in(const SquareJobs& jobs) {
+    squares_of<BTS>(jobs.n, [&](const Items& S, int blocks) {
+      launch(ns_square_kernel<BTS>, blocks, Product<BTS, 2, 2>::kLds, st, S, jobs);
+    });
   }
   void squares(const SquareJobs& jobs) {
-    Items S = by_squares(64), B = by_squares(128);
-    launch(ns_square_kernel<64>, blocks_before(S, count_squares, jobs.n), Product<64, 2, 2>::kLds, st, S, jobs);
-    launch(ns_square_kernel<128>, blocks_before(B, count_squares, jobs.n), Product<128, 2, 2>::kLds, st, B, jobs);
+    squares_in<64>(jobs);
+    squares_in<128>(jobs);
   }
   template <int PX, int PN>
   void update(float a, int square, float scale_m, int from, int step, int next) {
@@ -714,16 +1073,31 @@ void run_products(Items& L, const NsPlan& p, const Scales& sc, const Finish& fin
 }
 
 template <typename T>
-void run_items(Items& L, const NsPlan& p, hipStream_t st) {
+void run_items(const Items& L, const NsPlan& p, hipStream_t st) {
   const Momentum mo{p.momentum, p.nesterov};
   const Finish fin{p.lr_dev, p.lr, p.decay};
-  launch(ns_norm_kernel<T>, blocks_before(L, count_sums), 0, st, L, mo);
-  Items V, M, B;                                       // vectors, matrices in blocks of 64 and of 128
-  V.n = M.n = B.n = 0;
+  Items V, O, S, M, B, N;         // vectors, single blocks, strips, products in blocks of 64 and of 128; whose norm goes first
+  V.n = O.n = S.n = M.n = B.n = N.n = 0;
+  size_t lds = 0;
   for (int i = 0; i < L.n; ++i) {
-    Items& to = L.it[i].m == 1 ? V : L.it[i].bt == 128 ? B : M;
-    to.it[to.n++] = L.it[i];
+    const Item& I = L.it[i];
+    Items& to = I.path == kVector ? V : I.path == kSingle ? O : I.path == kStrips ? S : I.bt == 128 ? B : M;
+    to.it[to.n++] = I;
+    if (I.path == kVector || I.path == kTiles) N.it[N.n++] = I;
+    else if (I.m > 1) {
+      const size_t need = (size_t)I.width * I.mp * 8 + (size_t)I.mp * I.mp * 4;
+      if (need > lds) lds = need;
+    }
   }
+  // the small kernels form R, the composed products Q
+  const Scales small{p.scale_x, p.scale_s, p.scale_r, p.scale_t, p.scale_p, p.growth};
+  launch<kSmallThreads>(ns_small_kernel<T, true>, blocks_before(O, count_strips), lds, st, O, mo, p.eps, p.k, p.steps, 0, small,
+                        fin);
+  if (S.n)
+    for (int k = -1; k < p.steps; ++k)
+      launch<kSmallThreads>(ns_small_kernel<T, false>, blocks_before(S, count_strips), lds, st, S, mo, p.eps, p.k, p.steps, k,
+                            small, fin);
+  launch(ns_norm_kernel<T>, blocks_before(N, count_sums), 0, st, N, mo);
   launch(ns_vector_kernel<T>, blocks_before(V, count_sums), 0, st, V, mo, p.eps, p.k, p.steps, fin);
   const Scales sc{p.scale_x, p.scale_s, sizeof(T) == 4 ? p.scale_r : p.scale_q, p.scale_t, p.scale_p, p.growth};
   for (Items* X : {&M, &B}) launch(ns_split_kernel<T, sizeof(T) == 2>, blocks_before(*X, count_split), 0, st, *X, mo, p.eps, sc);

@@ -56,7 +56,7 @@ def _matrix(shape, seed, kind="noise", dtype=torch.float32):
 
 SHAPES = [(1, 1), (1, 7), (5, 1), (1, 5000), (2, 2), (2, 64), (3, 40), (16, 16), (33, 65), (64, 2), (64, 64), (64, 832), (100, 31),
           (128, 128), (257, 129), (300, 1000), (1000, 300), (65, 4097), (129, 2000), (512, 512), (2, 70000), (70000, 3),
-          (640, 1500)]
+          (640, 1500), (20, 500), (20, 600), (96, 96), (96, 128), (90, 161), (128, 64), (128, 1664), (40, 4000), (100, 70), (4100, 64)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])

@@ -66,7 +66,7 @@ def test_bad_optimiser_steps_are_refused():
     assert run(p=None) == -1 and run(g=None) == -1 and run(m=None) == -1 and run(gain=-1.0) == -1
     assert run(gain=float("nan")) == -1 and run(lr=-0.1) == -1 and run(lr=float("nan")) == -1 and run(mu=1.0) == -1
     assert run(mu=-0.1) == -1 and run(decay=-1.0) == -1 and run(steps=0) == -1 and run(shape=(0, 8)) == -1
-    assert run(ws=None) == -2 and run(nbytes=256) == -2
+    assert run(ws=None) == -2 and run(nbytes=128) == -2
 
 
 def test_python_entry_points_refuse():
