@@ -599,14 +599,14 @@ __global__ void __launch_bounds__(kThreads) ns_vector_kernel(Items L, Momentum m
 
 // ---- small matrices -------------------------------------------------------------------------------------------------
 
-// A block of eight waves holds a strip of X's columns in LDS: X [mp][width] and X^T [width][mp] as two-piece tiles, and S or R
+// A block of sixteen waves holds a strip of X's columns in LDS: X [mp][width] and X^T [width][mp] as two-piece tiles, and S or R
 // [mp][mp], mp <= 128.  Where the strip is the whole matrix the block runs all steps on its own (kSingle); else each block
 // leaves its part of X X^T in memory, and the launch of the next step lets every block of the matrix add up all parts - the
 // sum, S S and R are formed once a block, which costs less than a launch of their own (kStrips).
-constexpr int kSmallThreads = 512, kSmallWaves = kSmallThreads / 64;
+constexpr int kSmallThreads = 1024, kSmallWaves = kSmallThreads / 64;
 constexpr int kSmallRows = 128;                                // mp at most
 constexpr int kTriMax = 36, kTriWave = (kTriMax + kSmallWaves - 1) / kSmallWaves;
-constexpr int kUpdateWave = 8;                                 // 16 x 16 blocks of X a wave: width * mp / 256 / 8 at most
+constexpr int kUpdateWave = 4;                                 // 16 x 16 blocks of X a wave: width * mp / 256 / 16 at most
 constexpr int kSmallLds = 150 * 1024;
 constexpr float kFirst = 16384.0f;                             // what U 2^-e, |.| <= 1, is multiplied by before the first step
 
@@ -696,53 +696,72 @@ __global__ void __launch_bounds__(kSmallThreads) ns_small_kernel(Items L, Moment
   char* ws = I.ws + b * I.ws_stride;
   double* sums = at<double>(ws, off_squares_sum(I));
   int* exps = at<int>(ws, off_exponents(I));
+  // the blocks of the upper triangle and of X that this wave computes, the same in every step
+  int ta[kTriWave], tb[kTriWave], tj[kUpdateWave], ti[kUpdateWave];
+#pragma unroll
+  for (int q = 0; q < kTriWave; ++q) {
+    const int t = wave + q * kSmallWaves;
+    ta[q] = tb[q] = -1;
+    if (t < ntri) tri_tile(t, ta[q], tb[q]);
+  }
+#pragma unroll
+  for (int q = 0; q < kUpdateWave; ++q) {
+    const int t = wave + q * kSmallWaves;
+    ti[q] = t / wb;
+    tj[q] = t - ti[q] * wb;
+  }
   double norm = 0.0;
-  float first = 0.0f;                                           // X of the first step = first * (its pieces' values)
+  int own_e = 0;
 
   if (SINGLE || step < 0) {
-    // U of the strip, in fp32 where X's pieces go afterwards
-    float* u = reinterpret_cast<float*>(x);                     // [width][mp]
-    const int j0 = strip * width;
+    // U of the strip, in fp32 where X's pieces go afterwards; a wave takes rows of memory, its lanes neighbouring values
+    float* u = reinterpret_cast<float*>(x);                     // [width][mp + 1]: lanes along either side hit other banks
+    const int j0 = strip * width, rows = I.tall ? width : mp, across = I.tall ? mp : width;
     double s = 0.0;
     float big = 0.0f;
-    for (int k = tid; k < width * mp; k += kSmallThreads) {
-      // neighbouring threads on neighbouring addresses
-      const int i = I.tall ? k % mp : k / width, j = I.tall ? k / mp : k % width;
-      float v = 0.0f;
-      if (i < I.m && j0 + j < I.n) {
-        const int64_t e = base + (I.tall ? (int64_t)(j0 + j) * I.m + i : (int64_t)i * I.n + j0 + j);
-        if (I.mom) I.mom[e] = fmaf(mo.mu, I.mom[e], (1.0f - mo.mu) * (float)static_cast<const T*>(I.src)[e]);
-        v = source_value<T>(I, e, mo);
-        s = fma((double)v, (double)v, s);
-        big = fmaxf(big, fabsf(v));
+    for (int a = wave; a < rows; a += kSmallWaves) {
+      for (int c = lane; c < across; c += 64) {
+        const int i = I.tall ? c : a, j = I.tall ? a : c;
+        float v = 0.0f;
+        if (i < I.m && j0 + j < I.n) {
+          const int64_t e = base + (I.tall ? (int64_t)(j0 + j) * I.m + i : (int64_t)i * I.n + j0 + j);
+          if (I.mom) I.mom[e] = fmaf(mo.mu, I.mom[e], (1.0f - mo.mu) * (float)static_cast<const T*>(I.src)[e]);
+          v = source_value<T>(I, e, mo);
+          s = fma((double)v, (double)v, s);
+          big = fmaxf(big, fabsf(v));
+        }
+        u[j * (mp + 1) + i] = v;
       }
-      u[j * mp + i] = v;
     }
     s = block_sum(s, red);
     big = block_max(big, red);
     const int e = big > 0.0f && big < 3.4e38f ? ilogbf(big) + 1 : 0;
-    __syncthreads();
-    for (int k = tid; k < width * (mp / 4); k += kSmallThreads) {
-      const int j = k / (mp / 4), i = k % (mp / 4) * 4;
-      const float4 t = *reinterpret_cast<const float4*>(u + j * mp + i);
-      const float v[4] = {ldexpf(t.x, -e), ldexpf(t.y, -e), ldexpf(t.z, -e), ldexpf(t.w, -e)};
-      store_pieces<2>(xt, j, i, mt, v, kFirst);
-    }
-    __syncthreads();
-    for (int k = tid; k < mp * (width / 4); k += kSmallThreads) {
-      const int i = k % mp, j = k / mp * 4;
-      _Float16* to = x + piece_at<2>(i, j, wt);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const _Float16* from = xt + piece_at<2>(j + r, i, mt);
-        to[r] = from[0];
-        to[512 + r] = from[512];
+    for (int j = wave; j < width; j += kSmallWaves) {
+      const int i = lane * 4;
+      if (i < mp) {
+        const float* t = u + j * (mp + 1) + i;
+        const float v[4] = {ldexpf(t[0], -e), ldexpf(t[1], -e), ldexpf(t[2], -e), ldexpf(t[3], -e)};
+        store_pieces<2>(xt, j, i, mt, v, kFirst);
       }
     }
     __syncthreads();
+    for (int jb = wave; jb < width / 4; jb += kSmallWaves) {
+      for (int i = lane; i < mp; i += 64) {
+        _Float16* to = x + piece_at<2>(i, jb * 4, wt);
+        const _Float16* from = xt + piece_at<2>(jb * 4, i, mt);        // rows of X^T lie 8 halves apart
+        f16x4 hi, lo;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          hi[r] = from[8 * r];
+          lo[r] = from[8 * r + 512];
+        }
+        *reinterpret_cast<f16x4*>(to) = hi;
+        *reinterpret_cast<f16x4*>(to + 512) = lo;
+      }
+    }
+    own_e = e;
     if constexpr (SINGLE) {
       norm = sqrt(s);
-      first = (float)ldexp(1.0 / (norm + (double)eps), e);
     } else {
       if (tid == 0) { sums[strip] = s; exps[strip] = e; }
       // X^T's pieces to memory
@@ -757,132 +776,126 @@ __global__ void __launch_bounds__(kSmallThreads) ns_small_kernel(Items L, Moment
     double s = 0.0;
     for (int k = 0; k < I.strips; ++k) s += sums[k];
     norm = sqrt(s);
-    if (step == 0) first = (float)ldexp(1.0 / (norm + (double)eps), exps[strip]);
+    if (step == 0) own_e = exps[strip];
   }
+  const double inv_norm = 1.0 / (norm + (double)eps);
   Norm nm;
   nm.factor = 1.0f;
   nm.ex = small_exponent(norm, eps);
+  const float inv_s = 1.0f / sc.s, inv_q = 1.0f / sc.q;
+  if (SINGLE || step < 0) __syncthreads();
 
   for (int k = SINGLE ? 0 : step; k >= 0 && k < steps; ++k) {
-    const float inv_x = k == 0 ? first / kFirst : 1.0f / x_scale(nm, sc, k);        // X over its pieces
-    {
-      // S
-      if (SINGLE) {
-        for (int t = wave; t < ntri; t += kSmallWaves) {
-          int ba, bb;
-          tri_tile(t, ba, bb);
-          const f32x4 r = block_product(x, x, ba, bb, wt) * (inv_x * inv_x);
-          float v[4] = {r[0], r[1], r[2], r[3]};
-          store_symmetric(sq, mt, ba == bb, ba * 16, bb * 16, v, sc.s);
-        }
+    // X over its pieces; U 2^-e holds the first step's
+    const float inv_x = k == 0 ? (float)ldexp(inv_norm, own_e) / kFirst : 1.0f / x_scale(nm, sc, k);
+    // S
+#pragma unroll
+    for (int q = 0; q < kTriWave; ++q) {
+      if (ta[q] < 0) continue;
+      f32x4 r = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+      if constexpr (SINGLE) {
+        r = block_product(x, x, ta[q], tb[q], wt) * (inv_x * inv_x);
       } else {
-        const f32x4* part = at<const f32x4>(ws, off_parts(I, k & 1));
-        for (int t = wave; t < ntri; t += kSmallWaves) {
-          int ba, bb;
-          tri_tile(t, ba, bb);
-          f32x4 r = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 8
+        const f32x4* part = at<const f32x4>(ws, off_parts(I, k & 1)) + (wave + q * kSmallWaves) * 64 + lane;
+        if (k == 0) {
           for (int p = 0; p < I.strips; ++p) {
-            float scale = inv_x * inv_x;
-            if (k == 0) {
-              const float own = (float)ldexp(1.0 / (norm + (double)eps), exps[p]) / kFirst;
-              scale = own * own;
-            }
-            r += part[((int64_t)p * ntri + t) * 64 + lane] * scale;
+            const float own = (float)ldexp(inv_norm, exps[p]) / kFirst;
+            r += part[(int64_t)p * ntri * 64] * (own * own);
           }
-          float v[4] = {r[0], r[1], r[2], r[3]};
-          store_symmetric(sq, mt, ba == bb, ba * 16, bb * 16, v, sc.s);
+        } else {
+#pragma unroll 8
+          for (int p = 0; p < I.strips; ++p) r += part[(int64_t)p * ntri * 64];
+          r *= inv_x * inv_x;
         }
       }
-      __syncthreads();
-      // R = b S + c S S, in the place of S once every wave has read it
-      float rv[kTriWave][4];
-#pragma unroll
-      for (int q = 0; q < kTriWave; ++q) {
-        const int t = wave + q * kSmallWaves;
-        if (t < ntri) {
-          int ba, bb;
-          tri_tile(t, ba, bb);
-          const f32x4 r = block_product(sq, sq, ba, bb, mt);
-          float o[4];
-          load_pieces<2>(sq, bb * 16 + (lane & 15), ba * 16 + 4 * (lane >> 4), mt, o, 1.0f / sc.s);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) rv[q][i] = fmaf(kc.c / (sc.s * sc.s), r[i], kc.b * o[i]);
-        }
-      }
-      __syncthreads();
-#pragma unroll
-      for (int q = 0; q < kTriWave; ++q) {
-        const int t = wave + q * kSmallWaves;
-        if (t < ntri) {
-          int ba, bb;
-          tri_tile(t, ba, bb);
-          store_symmetric(sq, mt, ba == bb, ba * 16, bb * 16, rv[q], sc.q);
-        }
-      }
-      __syncthreads();
-      // X^T <- a X^T + X^T R, likewise
-      const bool last = k + 1 == steps;
-      const float next = x_scale(nm, sc, k + 1), own = kc.a * inv_x, unscale = inv_x / sc.q;
-      float xv[kUpdateWave][4];
-#pragma unroll
-      for (int q = 0; q < kUpdateWave; ++q) {
-        const int t = wave + q * kSmallWaves;
-        if (t < wb * rb) {
-          const int jb = t % wb, ib = t / wb;
-          const f32x4 r = block_product(xt, sq, jb, ib, mt);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) xv[q][i] = r[i] * unscale;
-          quad_transpose(xv[q]);
-          float o[4];
-          load_pieces<2>(xt, jb * 16 + 4 * (lane >> 4) + (lane & 3), ib * 16 + (lane & 12), mt, o, own);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) xv[q][i] += o[i];
-        }
-      }
-      __syncthreads();
-#pragma unroll
-      for (int q = 0; q < kUpdateWave; ++q) {
-        const int t = wave + q * kSmallWaves;
-        if (t < wb * rb) {
-          const int jb = t % wb, ib = t / wb;
-          const int j = jb * 16 + 4 * (lane >> 4) + (lane & 3), i = ib * 16 + (lane & 12);
-          const int j4 = jb * 16 + 4 * (lane >> 4), i1 = ib * 16 + (lane & 15);
-          if (!last) {
-            store_pieces<2>(SINGLE ? xt : at<_Float16>(ws, strip_bytes(I) * strip), j, i, mt, xv[q], next);
-            quad_transpose(xv[q]);
-            store_pieces<2>(x, i1, j4, wt, xv[q], next);
-          } else if (I.tall) {
-            const int jj = strip * width + j;
-            if (jj < I.n) {
-#pragma unroll
-              for (int r = 0; r < 4; ++r)
-                if (i + r < I.m) put<T>(I, base + (int64_t)jj * I.m + i + r, xv[q][r], lr, f);
-            }
-          } else {
-            quad_transpose(xv[q]);
-            const int jj = strip * width + j4;
-            if (i1 < I.m) {
-#pragma unroll
-              for (int r = 0; r < 4; ++r)
-                if (jj + r < I.n) put<T>(I, base + (int64_t)i1 * I.n + jj + r, xv[q][r], lr, f);
-            }
-          }
-        }
-      }
-      __syncthreads();
-      if (last) return;
+      float v[4] = {r[0], r[1], r[2], r[3]};
+      store_symmetric(sq, mt, ta[q] == tb[q], ta[q] * 16, tb[q] * 16, v, sc.s);
     }
+    __syncthreads();
+    // R = b S + c S S, in the place of S once every wave has read it
+    float rv[kTriWave][4];
+#pragma unroll
+    for (int q = 0; q < kTriWave; ++q) {
+      if (ta[q] < 0) continue;
+      const f32x4 r = block_product(sq, sq, ta[q], tb[q], mt);
+      float o[4];
+      load_pieces<2>(sq, tb[q] * 16 + (lane & 15), ta[q] * 16 + 4 * (lane >> 4), mt, o, inv_s);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) rv[q][i] = fmaf(kc.c * inv_s * inv_s, r[i], kc.b * o[i]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < kTriWave; ++q)
+      if (ta[q] >= 0) store_symmetric(sq, mt, ta[q] == tb[q], ta[q] * 16, tb[q] * 16, rv[q], sc.q);
+    __syncthreads();
+    // X^T <- a X^T + X^T R, likewise
+    const bool last = k + 1 == steps;
+    const float next = x_scale(nm, sc, k + 1), own = kc.a * inv_x, unscale = inv_x * inv_q;
+    float xv[kUpdateWave][4];
+#pragma unroll
+    for (int q = 0; q < kUpdateWave; ++q) {
+      if (ti[q] >= rb) continue;
+      const f32x4 r = block_product(xt, sq, tj[q], ti[q], mt);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) xv[q][i] = r[i] * unscale;
+      quad_transpose(xv[q]);
+      float o[4];
+      load_pieces<2>(xt, tj[q] * 16 + 4 * (lane >> 4) + (lane & 3), ti[q] * 16 + (lane & 12), mt, o, own);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) xv[q][i] += o[i];
+    }
+    if (last) {
+#pragma unroll 1
+      for (int q = 0; q < kUpdateWave; ++q) {
+        if (ti[0] >= rb) break;
+        const int j = tj[0] * 16 + 4 * (lane >> 4) + (lane & 3), i = ti[0] * 16 + (lane & 12);
+        const int j4 = tj[0] * 16 + 4 * (lane >> 4), i1 = ti[0] * 16 + (lane & 15);
+        if (I.tall) {
+          const int jj = strip * width + j;
+          if (jj < I.n) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (i + r < I.m) put<T>(I, base + (int64_t)jj * I.m + i + r, xv[0][r], lr, f);
+          }
+        } else {
+          quad_transpose(xv[0]);
+          const int jj = strip * width + j4;
+          if (i1 < I.m) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (jj + r < I.n) put<T>(I, base + (int64_t)i1 * I.n + jj + r, xv[0][r], lr, f);
+          }
+        }
+        // the next block moves up, so that this code is there once
+#pragma unroll
+        for (int n = 0; n + 1 < kUpdateWave; ++n) {
+          ti[n] = ti[n + 1];
+          tj[n] = tj[n + 1];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) xv[n][r] = xv[n + 1][r];
+        }
+        ti[kUpdateWave - 1] = rb;
+      }
+      return;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < kUpdateWave; ++q) {
+      if (ti[q] >= rb) continue;
+      store_pieces<2>(SINGLE ? xt : at<_Float16>(ws, strip_bytes(I) * strip), tj[q] * 16 + 4 * (lane >> 4) + (lane & 3),
+                      ti[q] * 16 + (lane & 12), mt, xv[q], next);
+      quad_transpose(xv[q]);
+      store_pieces<2>(x, ti[q] * 16 + (lane & 15), tj[q] * 16 + 4 * (lane >> 4), wt, xv[q], next);
+    }
+    __syncthreads();
     if constexpr (!SINGLE) break;
   }
   if constexpr (!SINGLE) {
     // this strip's part of the next S, as the pieces multiply
     f32x4* part = at<f32x4>(ws, off_parts(I, (step + 1) & 1)) + (int64_t)strip * ntri * 64;
-    for (int t = wave; t < ntri; t += kSmallWaves) {
-      int ba, bb;
-      tri_tile(t, ba, bb);
-      part[t * 64 + lane] = block_product(x, x, ba, bb, wt);
-    }
+#pragma unroll
+    for (int q = 0; q < kTriWave; ++q)
+      if (ta[q] >= 0) part[(wave + q * kSmallWaves) * 64 + lane] = block_product(x, x, ta[q], tb[q], wt);
   }
 }
 
