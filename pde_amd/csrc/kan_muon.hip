@@ -140,6 +140,24 @@ __device__ __forceinline__ void load_pieces(const _Float16* base, int row, int c
   for (int i = 0; i < 4; ++i) v[i] *= unscale;
 }
 
+// the two pieces of four values, hi | lo << 16 each: what a quad of lanes can transpose and store twice
+__device__ __forceinline__ void split_pieces(const float (&v)[4], float scale, float (&p)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float y = v[i] * scale;
+    const _Float16 hi = (_Float16)y, lo = (_Float16)(y - (float)hi);
+    p[i] = __uint_as_float((unsigned)__builtin_bit_cast(unsigned short, hi) |
+                           (unsigned)__builtin_bit_cast(unsigned short, lo) << 16);
+  }
+}
+__device__ __forceinline__ void store_packed(_Float16* base, int row, int col, int kt, const float (&p)[4]) {
+  // hi halves of a pair: bytes 0, 1 of each; lo halves: bytes 2, 3
+  const unsigned a = __float_as_uint(p[0]), b = __float_as_uint(p[1]), c = __float_as_uint(p[2]), d = __float_as_uint(p[3]);
+  _Float16* to = base + piece_at<2>(row, col, kt);
+  *reinterpret_cast<uint2*>(to) = make_uint2(__builtin_amdgcn_perm(b, a, 0x05040100u), __builtin_amdgcn_perm(d, c, 0x05040100u));
+  *reinterpret_cast<uint2*>(to + 512) = make_uint2(__builtin_amdgcn_perm(b, a, 0x07060302u), __builtin_amdgcn_perm(d, c, 0x07060302u));
+}
+
 // v[r] of lane t of a quad -> v[t] of lane r
 __device__ __forceinline__ void quad_transpose(float (&v)[4]) {
   const bool odd = threadIdx.x & 1, high = threadIdx.x & 2;
@@ -398,12 +416,15 @@ struct Product {
 };
 
 // A symmetric result: both triangles from one, blocks on the diagonal as they are.
-__device__ __forceinline__ void store_symmetric(_Float16* S, int kt, bool diagonal, int p0, int q0, float (&v)[4], float scale) {
+__device__ __forceinline__ void store_symmetric(_Float16* S, int kt, bool diagonal, int p0, int q0, const float (&v)[4],
+                                                float scale) {
   const int lane = threadIdx.x & 63;
-  store_pieces<2>(S, q0 + (lane & 15), p0 + 4 * (lane >> 4), kt, v, scale);
+  float p[4];
+  split_pieces(v, scale, p);
+  store_packed(S, q0 + (lane & 15), p0 + 4 * (lane >> 4), kt, p);
   if (!diagonal) {
-    quad_transpose(v);
-    store_pieces<2>(S, p0 + 4 * (lane >> 4) + (lane & 3), q0 + (lane & 12), kt, v, scale);
+    quad_transpose(p);
+    store_packed(S, p0 + 4 * (lane >> 4) + (lane & 3), q0 + (lane & 12), kt, p);
   }
 }
 
@@ -552,9 +573,17 @@ __global__ void __launch_bounds__(kThreads, BT == 64 ? 3 : 2) ns_update_kernel(I
       for (int r = 0; r < 4; ++r) v[r] += o[r];
     }
     if constexpr (!LAST) {
-      store_pieces<PN>(at<_Float16>(ws, off_xt(I, from ^ 1)), j, i, kt, v, next);
-      quad_transpose(v);
-      store_pieces<PN>(at<_Float16>(ws, 0), i0 + (lane & 15), j0 + 4 * (lane >> 4), I.np / 32, v, next);
+      if constexpr (PN == 2) {
+        float p[4];
+        split_pieces(v, next, p);
+        store_packed(at<_Float16>(ws, off_xt(I, from ^ 1)), j, i, kt, p);
+        quad_transpose(p);
+        store_packed(at<_Float16>(ws, 0), i0 + (lane & 15), j0 + 4 * (lane >> 4), I.np / 32, p);
+      } else {
+        store_pieces<1>(at<_Float16>(ws, off_xt(I, from ^ 1)), j, i, kt, v, next);
+        quad_transpose(v);
+        store_pieces<1>(at<_Float16>(ws, 0), i0 + (lane & 15), j0 + 4 * (lane >> 4), I.np / 32, v, next);
+      }
     } else if (I.tall) {
       if (j < I.n) {
 #pragma unroll
@@ -621,25 +650,35 @@ __device__ __host__ inline int64_t small_bytes(const Item& I) {
   return I.path == kSingle ? 256 : (off_exponents(I) + I.strips * 4 + 255) / 256 * 256;
 }
 
-__device__ __forceinline__ double block_sum(double s, double* red) {
-#pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) s += __shfl_xor(s, d);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
-  __syncthreads();
-  s = 0.0;
-  for (int k = 0; k < kSmallWaves; ++k) s += red[k];
-  return s;
+template <int kCtrl>
+__device__ __forceinline__ double dpp_move64(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const unsigned lo = __builtin_amdgcn_update_dpp(0u, (unsigned)u, kCtrl, 0xf, 0xf, false);
+  const unsigned hi = __builtin_amdgcn_update_dpp(0u, (unsigned)(u >> 32), kCtrl, 0xf, 0xf, false);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
-__device__ __forceinline__ float block_max(float v, double* red) {
+// sum and maximum (not of NaNs) over the block, in every thread; red: a double and a float a wave
+struct SumMax { double sum; float max; };
+__device__ __forceinline__ SumMax block_sum_max(double s, float v, double* red, float* redf) {
+  // over a row of 16 lanes as in wave_sum; the four rows through LDS with the waves
+  s += dpp_move64<0xB1>(s);
+  s += dpp_move64<0x4E>(s);
+  s += dpp_move64<0x141>(s);
+  s += dpp_move64<0x140>(s);
+  v = fmaxf(v, dpp_move<0xB1>(v));
+  v = fmaxf(v, dpp_move<0x4E>(v));
+  v = fmaxf(v, dpp_move<0x141>(v));
+  v = fmaxf(v, dpp_move<0x140>(v));
+  if ((threadIdx.x & 15) == 0) { red[threadIdx.x >> 4] = s; redf[threadIdx.x >> 4] = v; }
+  __syncthreads();
+  s = red[threadIdx.x & 63];
+  v = redf[threadIdx.x & 63];
 #pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = 0.0f;
-  for (int k = 0; k < kSmallWaves; ++k) v = fmaxf(v, (float)red[k]);
-  return v;
+  for (int d = 32; d >= 1; d >>= 1) {
+    s += __shfl_xor(s, d);
+    v = fmaxf(v, __shfl_xor(v, d));
+  }
+  return {s, v};
 }
 // exponent of (|U| + eps) / |U|, see Scales
 __device__ __forceinline__ int small_exponent(double norm, double eps) {
@@ -668,7 +707,8 @@ template <typename T, bool SINGLE>
 __global__ void __launch_bounds__(kSmallThreads) ns_small_kernel(Items L, Momentum mo, float eps, NsCoefficients kc, int steps,
                                                                  int step, Scales sc, Finish f) {
   extern __shared__ char lds[];
-  __shared__ double red[kSmallWaves];
+  __shared__ double red[kSmallThreads / 16];
+  __shared__ float redf[kSmallThreads / 16];
   const Where w = find_item(L);
   const Item& I = L.it[w.item];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
@@ -683,7 +723,7 @@ __global__ void __launch_bounds__(kSmallThreads) ns_small_kernel(Items L, Moment
       const double u = source_value<T>(I, base + i, mo);
       s = fma(u, u, s);
     }
-    const double norm = sqrt(block_sum(s, red));
+    const double norm = sqrt(block_sum_max(s, 0.0f, red, redf).sum);
     const double factor = vector_factor(norm, eps, kc, steps);
     for (int i = tid; i < I.n; i += kSmallThreads)
       put<T>(I, base + i, (float)((double)source_value<T>(I, base + i, mo) * factor), lr, f);
@@ -733,8 +773,9 @@ __global__ void __launch_bounds__(kSmallThreads) ns_small_kernel(Items L, Moment
         u[j * (mp + 1) + i] = v;
       }
     }
-    s = block_sum(s, red);
-    big = block_max(big, red);
+    const SumMax all = block_sum_max(s, big, red, redf);
+    s = all.sum;
+    big = all.max;
     const int e = big > 0.0f && big < 3.4e38f ? ilogbf(big) + 1 : 0;
     for (int j = wave; j < width; j += kSmallWaves) {
       const int i = lane * 4;
@@ -882,10 +923,12 @@ __global__ void __launch_bounds__(kSmallThreads) ns_small_kernel(Items L, Moment
 #pragma unroll
     for (int q = 0; q < kUpdateWave; ++q) {
       if (ti[q] >= rb) continue;
-      store_pieces<2>(SINGLE ? xt : at<_Float16>(ws, strip_bytes(I) * strip), tj[q] * 16 + 4 * (lane >> 4) + (lane & 3),
-                      ti[q] * 16 + (lane & 12), mt, xv[q], next);
-      quad_transpose(xv[q]);
-      store_pieces<2>(x, ti[q] * 16 + (lane & 15), tj[q] * 16 + 4 * (lane >> 4), wt, xv[q], next);
+      float v[4];
+      split_pieces(xv[q], next, v);
+      store_packed(SINGLE ? xt : at<_Float16>(ws, strip_bytes(I) * strip), tj[q] * 16 + 4 * (lane >> 4) + (lane & 3),
+                   ti[q] * 16 + (lane & 12), mt, v);
+      quad_transpose(v);
+      store_packed(x, ti[q] * 16 + (lane & 15), tj[q] * 16 + 4 * (lane >> 4), wt, v);
     }
     __syncthreads();
     if constexpr (!SINGLE) break;
@@ -942,10 +985,10 @@ Item make_item(const NsMatrix& M) {
     if (I.np <= widest) {
       I.path = kSingle;
     } else {
-      // strips of 64 columns (128 of the narrowest matrices): a block of the next step reads a part of tri16 KB of each, which
+      // strips of 64 columns, of 128 where there would be many: a block of the next step reads a part of tri16 KB of each, which
       // has to stay below what the launches that it saves cost
-      const int width = I.mp <= 64 ? 128 : 64;
-      const int strips = (I.np + width - 1) / width;
+      int width = 64, strips = (I.np + 63) / 64;
+      if (I.mp <= 64 && strips * tri16(I.mp) > 512) { width = 128; strips = (I.np + 127) / 128; }
       if ((int64_t)strips * tri16(I.mp) <= 1024) { I.path = kStrips; I.width = width; I.strips = strips; }
     }
   }
