@@ -826,6 +826,9 @@ __global__ void __launch_bounds__(kSmallThreads) ns_small_kernel(Items L, Moment
   const float inv_s = 1.0f / sc.s, inv_q = 1.0f / sc.q;
   if (SINGLE || step < 0) __syncthreads();
 
+  // this wave's blocks of X in fp32: lane l holds row 16 ti + l % 16, columns 16 tj + 4 (l / 16) ..
+  float xv[kUpdateWave][4];
+
   for (int k = SINGLE ? 0 : step; k >= 0 && k < steps; ++k) {
     // X over its pieces; U 2^-e holds the first step's
     const float inv_x = k == 0 ? (float)ldexp(inv_norm, own_e) / kFirst : 1.0f / x_scale(nm, sc, k);
@@ -869,21 +872,23 @@ __global__ void __launch_bounds__(kSmallThreads) ns_small_kernel(Items L, Moment
     for (int q = 0; q < kTriWave; ++q)
       if (ta[q] >= 0) store_symmetric(sq, mt, ta[q] == tb[q], ta[q] * 16, tb[q] * 16, rv[q], sc.q);
     __syncthreads();
-    // X^T <- a X^T + X^T R, likewise
+    // X <- a X + R X, likewise
     const bool last = k + 1 == steps;
-    const float next = x_scale(nm, sc, k + 1), own = kc.a * inv_x, unscale = inv_x * inv_q;
-    float xv[kUpdateWave][4];
+    const float next = x_scale(nm, sc, k + 1), unscale = inv_x * inv_q;
+    if (!SINGLE || k == 0) {
+#pragma unroll
+      for (int q = 0; q < kUpdateWave; ++q) {
+        if (ti[q] >= rb) continue;
+        load_pieces<2>(xt, tj[q] * 16 + 4 * (lane >> 4) + (lane & 3), ti[q] * 16 + (lane & 12), mt, xv[q], inv_x);
+        quad_transpose(xv[q]);
+      }
+    }
 #pragma unroll
     for (int q = 0; q < kUpdateWave; ++q) {
       if (ti[q] >= rb) continue;
       const f32x4 r = block_product(xt, sq, tj[q], ti[q], mt);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) xv[q][i] = r[i] * unscale;
-      quad_transpose(xv[q]);
-      float o[4];
-      load_pieces<2>(xt, tj[q] * 16 + 4 * (lane >> 4) + (lane & 3), ti[q] * 16 + (lane & 12), mt, o, own);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) xv[q][i] += o[i];
+      for (int i = 0; i < 4; ++i) xv[q][i] = fmaf(kc.a, xv[q][i], r[i] * unscale);
     }
     if (last) {
 #pragma unroll 1
@@ -892,6 +897,7 @@ __global__ void __launch_bounds__(kSmallThreads) ns_small_kernel(Items L, Moment
         const int j = tj[0] * 16 + 4 * (lane >> 4) + (lane & 3), i = ti[0] * 16 + (lane & 12);
         const int j4 = tj[0] * 16 + 4 * (lane >> 4), i1 = ti[0] * 16 + (lane & 15);
         if (I.tall) {
+          quad_transpose(xv[0]);
           const int jj = strip * width + j;
           if (jj < I.n) {
 #pragma unroll
@@ -899,7 +905,6 @@ __global__ void __launch_bounds__(kSmallThreads) ns_small_kernel(Items L, Moment
               if (i + r < I.m) put<T>(I, base + (int64_t)jj * I.m + i + r, xv[0][r], lr, f);
           }
         } else {
-          quad_transpose(xv[0]);
           const int jj = strip * width + j4;
           if (i1 < I.m) {
 #pragma unroll
@@ -925,10 +930,10 @@ __global__ void __launch_bounds__(kSmallThreads) ns_small_kernel(Items L, Moment
       if (ti[q] >= rb) continue;
       float v[4];
       split_pieces(xv[q], next, v);
+      store_packed(x, ti[q] * 16 + (lane & 15), tj[q] * 16 + 4 * (lane >> 4), wt, v);
+      quad_transpose(v);
       store_packed(SINGLE ? xt : at<_Float16>(ws, strip_bytes(I) * strip), tj[q] * 16 + 4 * (lane >> 4) + (lane & 3),
                    ti[q] * 16 + (lane & 12), mt, v);
-      quad_transpose(v);
-      store_packed(x, ti[q] * 16 + (lane & 15), tj[q] * 16 + 4 * (lane >> 4), wt, v);
     }
     __syncthreads();
     if constexpr (!SINGLE) break;
