@@ -951,6 +951,8 @@ __global__ void __launch_bounds__(kSmallThreads) ns_small_kernel(Items L, Moment
 
 int round_up(int64_t v, int a) { return (int)((v + a - 1) / a * a); }
 
+void choose_path(Item& I, Path least);
+
 Item make_item(const NsMatrix& M) {
   Item I{};
   I.src = M.src; I.mom = M.momentum; I.out = M.out; I.gain = M.gain;
@@ -978,6 +980,12 @@ Item make_item(const NsMatrix& M) {
   if (chunks < 1) chunks = 1;
   I.kchunk = (kt + (int)chunks - 1) / (int)chunks;
   I.chunks = (kt + I.kchunk - 1) / I.kchunk;
+  choose_path(I, kSingle);
+  return I;
+}
+
+// The small kernels' path of a matrix, or a slower-starting one: `least` is kSingle, kStrips or kTiles.
+void choose_path(Item& I, Path least) {
   // the widest strip whose X, X^T and square fit the LDS and the waves' registers
   const int room = I.mp <= kSmallRows ? (kSmallLds - I.mp * I.mp * 4) / (I.mp * 8) / 32 * 32 : 0;
   const int hold = kUpdateWave * kSmallWaves * 256 / I.mp, widest = room < hold ? room : hold;
@@ -986,8 +994,8 @@ Item make_item(const NsMatrix& M) {
   I.path = kTiles;
   if (I.m == 1) {
     I.path = I.n <= 65536 ? kSingle : kVector;
-  } else if (I.mp <= kSmallRows) {
-    if (I.np <= widest) {
+  } else if (I.mp <= kSmallRows && least < kTiles) {
+    if (I.np <= widest && least == kSingle) {
       I.path = kSingle;
     } else {
       // strips of 64 columns, of 128 where there would be many: a block of the next step reads a part of tri16 KB of each, which
@@ -998,7 +1006,19 @@ Item make_item(const NsMatrix& M) {
     }
   }
   I.ws_stride = I.path == kVector ? (int64_t)kSumsMax * (int64_t)sizeof(double) : I.path == kTiles ? item_bytes(I) : small_bytes(I);
-  return I;
+}
+
+// The matrices of one list.  Those that could go alone in fewer launches join the launches of the others that take more of
+// them: beside those they cost next to nothing, on their own their whole time.
+void make_items(const NsMatrix* mats, int count, Items& L) {
+  L.n = 0;
+  Path most = kSingle;
+  for (int j = 0; j < count && j < kItemsMax; ++j) {
+    const Item& I = L.it[L.n++] = make_item(mats[j]);
+    if (I.m > 1 && I.path > most) most = (Path)I.path;
+  }
+  for (int j = 0; j < L.n; ++j)
+    if (L.it[j].m > 1 && L.it[j].path < most) choose_path(L.it[j], most);
 }
 
 int blocks_before(Items& L, int (*count)(const Item&), int times = 1) {
@@ -1231,23 +1251,20 @@ bool ns_scales(const NsCoefficients& k, int steps, NsPlan* p) {
 }
 
 size_t ns_ws_bytes(const NsMatrix* mats, int count) {
+  Items L;
+  make_items(mats, count, L);
   size_t sum = 0;
-  for (int j = 0; j < count; ++j) {
-    const Item I = make_item(mats[j]);
-    sum += (size_t)I.ws_stride * I.batch;
-  }
+  for (int j = 0; j < L.n; ++j) sum += (size_t)L.it[j].ws_stride * L.it[j].batch;
   return sum;
 }
 
 void launch_ns(int dtype, const NsMatrix* mats, int count, const NsPlan& p, void* ws, hipStream_t st) {
   Items L;
-  L.n = 0;
+  make_items(mats, count, L);
   char* at = static_cast<char*>(ws);
-  for (int j = 0; j < count && j < kItemsMax; ++j) {
-    Item I = make_item(mats[j]);
-    I.ws = at;
-    at += I.ws_stride * I.batch;
-    L.it[L.n++] = I;
+  for (int j = 0; j < L.n; ++j) {
+    L.it[j].ws = at;
+    at += L.it[j].ws_stride * L.it[j].batch;
   }
   switch (dtype) {
     case kNormF32: run_items<float>(L, p, st); break;
