@@ -125,6 +125,20 @@ __device__ __forceinline__ void store_pieces(_Float16* base, int row, int col, i
   *reinterpret_cast<f16x4*>(p) = hi;
   if constexpr (PIECES == 2) *reinterpret_cast<f16x4*>(p + 512) = lo;
 }
+// eight values of a row, col % 8 == 0
+template <int PIECES>
+__device__ __forceinline__ void store_pieces8(_Float16* base, int row, int col, int kt, const float (&v)[8], float scale) {
+  f16x8 hi, lo;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float y = v[i] * scale;
+    hi[i] = (_Float16)y;
+    lo[i] = (_Float16)(y - (float)hi[i]);
+  }
+  _Float16* p = base + piece_at<PIECES>(row, col, kt);
+  *reinterpret_cast<f16x8*>(p) = hi;
+  if constexpr (PIECES == 2) *reinterpret_cast<f16x8*>(p + 512) = lo;
+}
 template <int PIECES>
 __device__ __forceinline__ void load_pieces(const _Float16* base, int row, int col, int kt, float (&v)[4], float unscale) {
   const _Float16* p = base + piece_at<PIECES>(row, col, kt);
@@ -274,17 +288,20 @@ __global__ void __launch_bounds__(kThreads) ns_split_kernel(Items L, Momentum mo
   __syncthreads();
   _Float16 *x = at<_Float16>(ws, 0), *xt = at<_Float16>(ws, off_xt(I, 0));
   const int ktx = I.np / 32, kt = I.mp / 32;
-  for (int k = threadIdx.x; k < 64 * 16; k += kThreads) {
-    const int r = k % 64, q = k / 64 * 4;
+  for (int k = threadIdx.x; k < 64 * 8; k += kThreads) {
+    const int r = k % 64, q = k / 64 * 8;
+    float v[8];
     const int i = bi * 64 + r, j = bj * 64 + q;
     if (i < I.mp && j < I.np) {
-      const float v[4] = {tile[r][q], tile[r][q + 1], tile[r][q + 2], tile[r][q + 3]};
-      store_pieces<PX>(x, i, j, ktx, v, scx);
+#pragma unroll
+      for (int n = 0; n < 8; ++n) v[n] = tile[r][q + n];
+      store_pieces8<PX>(x, i, j, ktx, v, scx);
     }
     const int i2 = bi * 64 + q, j2 = bj * 64 + r;
     if (i2 < I.mp && j2 < I.np) {
-      const float v[4] = {tile[q][r], tile[q + 1][r], tile[q + 2][r], tile[q + 3][r]};
-      store_pieces<PX>(xt, j2, i2, kt, v, scx);
+#pragma unroll
+      for (int n = 0; n < 8; ++n) v[n] = tile[q + n][r];
+      store_pieces8<PX>(xt, j2, i2, kt, v, scx);
     }
   }
 }
@@ -463,23 +480,33 @@ __global__ void __launch_bounds__(kThreads, BT == 64 ? 3 : 2) ns_gram_kernel(Ite
   for (int a = 0; a < kAcc; ++a) part[a * kThreads] = acc.v[a / acc.kW][a % acc.kW] * unscale;
 }
 
-// the sum of the splits, in their order: a block sums a quarter (BT = 128: a sixteenth) of a tile's 16 x 16 blocks
-template <int BT>
-__global__ void __launch_bounds__(kThreads) ns_gram_sum_kernel(Items L, Scales sc) {
+// the sum of the splits, in a fixed order: a block sums a quarter (BT = 128: a sixteenth) of a tile's 16 x 16 blocks, GROUPS
+// groups of four waves every GROUPS-th split each
+template <int BT, int GROUPS>
+__global__ void __launch_bounds__(GROUPS * kThreads) ns_gram_sum_kernel(Items L, Scales sc) {
   constexpr int kAcc = BT * BT / 1024, kW = BT / 32;
+  __shared__ f32x4 red[GROUPS][kThreads];
   const Where w = find_item(L);
   const Item& I = L.it[w.item];
   const int tiles = tri_tiles(I), b = w.local / (tiles * kAcc), t = w.local / kAcc % tiles, a = w.local % kAcc;
   int bi, bj;
   tri_tile(t, bi, bj);
   char* ws = I.ws + b * I.ws_stride;
-  const f32x4* part = at<const f32x4>(ws, off_part(I)) + (int64_t)t * (BT * BT / 4) + a * kThreads + threadIdx.x;
+  const int tid = threadIdx.x % kThreads, group = threadIdx.x / kThreads;
+  const f32x4* part = at<const f32x4>(ws, off_part(I)) + (int64_t)t * (BT * BT / 4) + a * kThreads + tid;
   f32x4 s = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 8
-  for (int k = 0; k < I.chunks; ++k) s += part[(int64_t)k * tiles * (BT * BT / 4)];
+  for (int k = group; k < I.chunks; k += GROUPS) s += part[(int64_t)k * tiles * (BT * BT / 4)];
+  if constexpr (GROUPS > 1) {
+    red[group][tid] = s;
+    __syncthreads();
+    if (group) return;
+#pragma unroll
+    for (int g = 1; g < GROUPS; ++g) s += red[g][tid];
+  }
   const int p0 = Product<BT, 2, 2>::row_p(bi) + 16 * (a / kW), q0 = Product<BT, 2, 2>::row_q(bj) + 16 * (a % kW);
   if (p0 >= I.mp || q0 >= I.mp) return;
-  float v[4] = {s[0], s[1], s[2], s[3]};
+  const float v[4] = {s[0], s[1], s[2], s[3]};
   store_symmetric(at<_Float16>(ws, off_sq(I, kS)), I.mp / 32, bi == bj, p0, q0, v, sc.s);
 }
 
@@ -1058,7 +1085,12 @@ struct Steps {
     S.n = 0;
     for (int i = 0; i < L.n; ++i)
       if (L.it[i].chunks > 1) S.it[S.n++] = L.it[i];
-    launch(ns_gram_sum_kernel<BT>, blocks_before(S, count_parts), 0, st, S, sc);
+    // with many splits four groups of waves share them (46 splits of 256 x 5888: 7.0 -> 6.1 us; 4 splits: 11 -> 17 us)
+    int most = 0;
+    for (int i = 0; i < S.n; ++i) most = S.it[i].chunks > most ? S.it[i].chunks : most;
+    const int sums = blocks_before(S, count_parts);
+    if (most >= 16) launch<4 * kThreads>(ns_gram_sum_kernel<BT, 4>, sums, 0, st, S, sc);
+    else launch(ns_gram_sum_kernel<BT, 1>, sums, 0, st, S, sc);
   }
   // go(the matrices whose squares go in blocks of `bts`, their number of blocks), for each block size there is
   template <int BTS, typename Go>
