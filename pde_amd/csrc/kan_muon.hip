@@ -700,17 +700,34 @@ __device__ __forceinline__ SumMax block_sum_max(double s, float v, double* red, 
   __syncthreads();
   s = red[threadIdx.x & 63];
   v = redf[threadIdx.x & 63];
-#pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) {
-    s += __shfl_xor(s, d);
-    v = fmaxf(v, __shfl_xor(v, d));
-  }
+  s += dpp_move64<0xB1>(s);
+  s += dpp_move64<0x4E>(s);
+  s += dpp_move64<0x141>(s);
+  s += dpp_move64<0x140>(s);
+  v = fmaxf(v, dpp_move<0xB1>(v));
+  v = fmaxf(v, dpp_move<0x4E>(v));
+  v = fmaxf(v, dpp_move<0x141>(v));
+  v = fmaxf(v, dpp_move<0x140>(v));
+  s += __shfl_xor(s, 16);
+  s += __shfl_xor(s, 32);
+  v = fmaxf(v, __shfl_xor(v, 16));
+  v = fmaxf(v, __shfl_xor(v, 32));
   return {s, v};
 }
-// exponent of (|U| + eps) / |U|, see Scales
-__device__ __forceinline__ int small_exponent(double norm, double eps) {
-  const double small = (norm + eps) / norm;
-  return small > 1.0 && norm > 0.0 ? (small < 7.9e28 ? ilogb(small) : 96) : 0;
+// From the sum of squares, in 32 bits: everything over 2^e, so that nothing overflows.  first: 2^e / (|U| + eps);
+// ex: the exponent of (|U| + eps) / |U|, see Scales
+constexpr int kNoExponent = -1000;                             // of a strip of zeros
+struct Start { float first; int ex; };
+__device__ __forceinline__ Start start_of(double squares, float eps, int e) {
+  const float norm = sqrtf((float)ldexp(squares, -2 * e)), eps_e = ldexpf(eps, -e);
+  Start r;
+  r.first = 1.0f / (norm + eps_e);
+  r.ex = 0;
+  if (norm < eps_e && norm > 0.0f) {
+    const float small = 1.0f + eps_e / norm;
+    r.ex = small < 7.9e28f ? ilogbf(small) : 96;
+  }
+  return r;
 }
 
 // 16 x 16 block of P Q^T from tiles of two pieces in LDS: row of tiles `a` of P and `b` of Q, kp and kq inner tiles a row
@@ -777,12 +794,16 @@ __global__ void __launch_bounds__(kSmallThreads) ns_small_kernel(Items L, Moment
     ti[q] = t / wb;
     tj[q] = t - ti[q] * wb;
   }
-  double norm = 0.0;
-  int own_e = 0;
+  double squares = 0.0;
+  int own_e = 0, all_e = 0;
 
   if (SINGLE || step < 0) {
-    // U of the strip, in fp32 where X's pieces go afterwards; a wave takes rows of memory, its lanes neighbouring values
-    float* u = reinterpret_cast<float*>(x);                     // [width][mp + 1]: lanes along either side hit other banks
+    // U of the strip in fp32; a wave takes rows of memory, its lanes neighbouring values
+    // (behind the square where there is room, so that X and X^T are made in one go)
+    const int plane = width * mp * 2;                           // halves
+    const bool apart = plane * 4 + mp * mp * 4 + width * (mp + 1) * 4 <= kSmallLds;
+    float* u = apart ? reinterpret_cast<float*>(sq + mp * mp * 2) : reinterpret_cast<float*>(x);
+    // [width][mp + 1]: lanes along either side hit other banks
     const int j0 = strip * width, rows = I.tall ? width : mp, across = I.tall ? mp : width;
     double s = 0.0;
     float big = 0.0f;
@@ -803,34 +824,40 @@ __global__ void __launch_bounds__(kSmallThreads) ns_small_kernel(Items L, Moment
     const SumMax all = block_sum_max(s, big, red, redf);
     s = all.sum;
     big = all.max;
-    const int e = big > 0.0f && big < 3.4e38f ? ilogbf(big) + 1 : 0;
-    for (int j = wave; j < width; j += kSmallWaves) {
-      const int i = lane * 4;
-      if (i < mp) {
-        const float* t = u + j * (mp + 1) + i;
+    const int e = big > 0.0f ? (big < 3.4e38f ? ilogbf(big) + 1 : 0) : kNoExponent;
+    const int per = mp / 4, across4 = 64 / per, jl = lane / per, il = (lane - jl * per) * 4;       // lanes a column of X, columns a wave
+    if (jl < across4) {
+      for (int j = wave * across4 + jl; j < width; j += kSmallWaves * across4) {
+        const float* t = u + j * (mp + 1) + il;
         const float v[4] = {ldexpf(t[0], -e), ldexpf(t[1], -e), ldexpf(t[2], -e), ldexpf(t[3], -e)};
-        store_pieces<2>(xt, j, i, mt, v, kFirst);
+        store_pieces<2>(xt, j, il, mt, v, kFirst);
       }
     }
-    __syncthreads();
+    if (!apart) __syncthreads();
     for (int jb = wave; jb < width / 4; jb += kSmallWaves) {
       for (int i = lane; i < mp; i += 64) {
-        _Float16* to = x + piece_at<2>(i, jb * 4, wt);
-        const _Float16* from = xt + piece_at<2>(jb * 4, i, mt);        // rows of X^T lie 8 halves apart
-        f16x4 hi, lo;
+        if (apart) {
+          const float* t = u + jb * 4 * (mp + 1) + i;
+          const float v[4] = {ldexpf(t[0], -e), ldexpf(t[mp + 1], -e), ldexpf(t[2 * (mp + 1)], -e), ldexpf(t[3 * (mp + 1)], -e)};
+          store_pieces<2>(x, i, jb * 4, wt, v, kFirst);
+        } else {
+          _Float16* to = x + piece_at<2>(i, jb * 4, wt);
+          const _Float16* from = xt + piece_at<2>(jb * 4, i, mt);        // rows of X^T lie 8 halves apart
+          f16x4 hi, lo;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          hi[r] = from[8 * r];
-          lo[r] = from[8 * r + 512];
+          for (int r = 0; r < 4; ++r) {
+            hi[r] = from[8 * r];
+            lo[r] = from[8 * r + 512];
+          }
+          *reinterpret_cast<f16x4*>(to) = hi;
+          *reinterpret_cast<f16x4*>(to + 512) = lo;
         }
-        *reinterpret_cast<f16x4*>(to) = hi;
-        *reinterpret_cast<f16x4*>(to + 512) = lo;
       }
     }
     own_e = e;
-    if constexpr (SINGLE) {
-      norm = sqrt(s);
-    } else {
+    squares = s;
+    if constexpr (!SINGLE) {
+      __syncthreads();
       if (tid == 0) { sums[strip] = s; exps[strip] = e; }
       // X^T's pieces to memory
       const f32x4* from = reinterpret_cast<const f32x4*>(xt);
@@ -842,14 +869,19 @@ __global__ void __launch_bounds__(kSmallThreads) ns_small_kernel(Items L, Moment
     f32x4* to = reinterpret_cast<f32x4*>(xt);
     for (int k = tid; k < width * mp / 4; k += kSmallThreads) to[k] = from[k];
     double s = 0.0;
-    for (int k = 0; k < I.strips; ++k) s += sums[k];
-    norm = sqrt(s);
-    if (step == 0) own_e = exps[strip];
+    int most = kNoExponent;
+    for (int k = 0; k < I.strips; ++k) {
+      s += sums[k];
+      most = max(most, exps[k]);
+    }
+    squares = s;
+    own_e = exps[strip];
+    all_e = most;
   }
-  const double inv_norm = 1.0 / (norm + (double)eps);
+  const Start start = start_of(squares, eps, own_e);
   Norm nm;
   nm.factor = 1.0f;
-  nm.ex = small_exponent(norm, eps);
+  nm.ex = SINGLE ? start.ex : start_of(squares, eps, all_e).ex;        // the same in all strips
   const float inv_s = 1.0f / sc.s, inv_q = 1.0f / sc.q;
   if (SINGLE || step < 0) __syncthreads();
 
@@ -858,7 +890,7 @@ __global__ void __launch_bounds__(kSmallThreads) ns_small_kernel(Items L, Moment
 
   for (int k = SINGLE ? 0 : step; k >= 0 && k < steps; ++k) {
     // X over its pieces; U 2^-e holds the first step's
-    const float inv_x = k == 0 ? (float)ldexp(inv_norm, own_e) / kFirst : 1.0f / x_scale(nm, sc, k);
+    const float inv_x = k == 0 ? start.first * (1.0f / kFirst) : 1.0f / x_scale(nm, sc, k);
     // S
 #pragma unroll
     for (int q = 0; q < kTriWave; ++q) {
@@ -870,7 +902,7 @@ __global__ void __launch_bounds__(kSmallThreads) ns_small_kernel(Items L, Moment
         const f32x4* part = at<const f32x4>(ws, off_parts(I, k & 1)) + (wave + q * kSmallWaves) * 64 + lane;
         if (k == 0) {
           for (int p = 0; p < I.strips; ++p) {
-            const float own = (float)ldexp(inv_norm, exps[p]) / kFirst;
+            const float own = start_of(squares, eps, exps[p]).first * (1.0f / kFirst);
             r += part[(int64_t)p * ntri * 64] * (own * own);
           }
         } else {
@@ -1198,7 +1230,9 @@ void run_items(const Items& L, const NsPlan& p, hipStream_t st) {
     to.it[to.n++] = I;
     if (I.path == kVector || I.path == kTiles) N.it[N.n++] = I;
     else if (I.m > 1) {
-      const size_t need = (size_t)I.width * I.mp * 8 + (size_t)I.mp * I.mp * 4;
+      size_t need = (size_t)I.width * I.mp * 8 + (size_t)I.mp * I.mp * 4;
+      const size_t apart = need + (size_t)I.width * (I.mp + 1) * 4;
+      if (apart <= kSmallLds) need = apart;
       if (need > lds) lds = need;
     }
   }

@@ -119,9 +119,22 @@ def test_scales(shape, scale):
     _check(K.orthogonalize(g), want, off + 1e-37)
 
 
+def test_strips_of_zeros_and_tiny_values():
+    """Columns of zeros and of far smaller values than the rest: a block that holds only those takes part as the others do."""
+    from pde_amd import functional as K
+    for shape in ((50, 900), (900, 50), (120, 700), (30, 60)):
+        for scale in (1.0, 1e-25):
+            g = _matrix(shape, 12) * scale
+            long = g if shape[1] > shape[0] else g.t()
+            long[:, :len(long[0]) // 3] = 0
+            long[:, -len(long[0]) // 3:] *= 1e-9
+            want, off = _definition(g)
+            _check(K.orthogonalize(g), want, off + 1e-37)
+
+
 def test_zero_and_non_finite_matrices():
     from pde_amd import functional as K
-    for shape in ((3, 40, 70), (3, 1, 50), (3, 200, 140)):
+    for shape in ((3, 40, 70), (3, 1, 50), (3, 200, 140), (3, 60, 1000)):
         g = _matrix(shape, 4)
         clean = K.orthogonalize(g)
         g[0] = 0
