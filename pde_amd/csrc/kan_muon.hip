@@ -796,6 +796,9 @@ __global__ void __launch_bounds__(kSmallThreads) ns_small_kernel(Items L, Moment
   }
   double squares = 0.0;
   int own_e = 0, all_e = 0;
+  f32x4 parts[kTriWave];
+#pragma unroll
+  for (int q = 0; q < kTriWave; ++q) parts[q] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
 
   if (SINGLE || step < 0) {
     // U of the strip in fp32; a wave takes rows of memory, its lanes neighbouring values
@@ -865,14 +868,31 @@ __global__ void __launch_bounds__(kSmallThreads) ns_small_kernel(Items L, Moment
       for (int k = tid; k < width * mp / 4; k += kSmallThreads) to[k] = from[k];
     }
   } else {
-    const f32x4* from = at<const f32x4>(ws, strip_bytes(I) * strip);
-    f32x4* to = reinterpret_cast<f32x4*>(xt);
-    for (int k = tid; k < width * mp / 4; k += kSmallThreads) to[k] = from[k];
+    // X^T's pieces on their way to LDS, 1 KB a wave and turn, while the sums and the parts below are read
+    const char* from = ws + strip_bytes(I) * strip + lane * 16;
+    for (int k = wave * 1024; k < width * mp * 4; k += kSmallWaves * 1024)
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + k),
+                                       (__attribute__((address_space(3))) void*)(lds + k), 16, 0, 0);
+    if (step > 0) {
+      // the strips' parts of S; the first step's have a factor each, see below
+#pragma unroll
+      for (int q = 0; q < kTriWave; ++q) {
+        if (ta[q] < 0) continue;
+        const f32x4* part = at<const f32x4>(ws, off_parts(I, step & 1)) + (wave + q * kSmallWaves) * 64 + lane;
+#pragma unroll 8
+        for (int p = 0; p < I.strips; ++p) parts[q] += part[(int64_t)p * ntri * 64];
+      }
+    }
     double s = 0.0;
     int most = kNoExponent;
-    for (int k = 0; k < I.strips; ++k) {
+    for (int k = lane; k < I.strips; k += 64) {
       s += sums[k];
       most = max(most, exps[k]);
+    }
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) {
+      s += __shfl_xor(s, d);
+      most = max(most, __shfl_xor(most, d));
     }
     squares = s;
     own_e = exps[strip];
@@ -899,21 +919,26 @@ __global__ void __launch_bounds__(kSmallThreads) ns_small_kernel(Items L, Moment
       if constexpr (SINGLE) {
         r = block_product(x, x, ta[q], tb[q], wt) * (inv_x * inv_x);
       } else {
-        const f32x4* part = at<const f32x4>(ws, off_parts(I, k & 1)) + (wave + q * kSmallWaves) * 64 + lane;
         if (k == 0) {
-          for (int p = 0; p < I.strips; ++p) {
-            const float own = start_of(squares, eps, exps[p]).first * (1.0f / kFirst);
-            r += part[(int64_t)p * ntri * 64] * (own * own);
+          // a strip's factor by a lane of its own
+          const f32x4* part = at<const f32x4>(ws, off_parts(I, 0)) + (wave + q * kSmallWaves) * 64 + lane;
+          for (int p0 = 0; p0 < I.strips; p0 += 64) {
+            const float own = p0 + lane < I.strips ? start_of(squares, eps, exps[p0 + lane]).first * (1.0f / kFirst) : 0.0f;
+            const int n = min(64, I.strips - p0);
+#pragma unroll 4
+            for (int p = 0; p < n; ++p) {
+              const float f1 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(own), p));
+              r += part[(int64_t)(p0 + p) * ntri * 64] * (f1 * f1);
+            }
           }
         } else {
-#pragma unroll 8
-          for (int p = 0; p < I.strips; ++p) r += part[(int64_t)p * ntri * 64];
-          r *= inv_x * inv_x;
+          r = parts[q] * (inv_x * inv_x);
         }
       }
       float v[4] = {r[0], r[1], r[2], r[3]};
       store_symmetric(sq, mt, ta[q] == tb[q], ta[q] * 16, tb[q] * 16, v, sc.s);
     }
+    if constexpr (!SINGLE) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");          // X^T has landed
     __syncthreads();
     // R = b S + c S S, in the place of S once every wave has read it
     float rv[kTriWave][4];
