@@ -664,6 +664,7 @@ constexpr int kSmallRows = 128;                                // mp at most
 constexpr int kTriMax = 36, kTriWave = (kTriMax + kSmallWaves - 1) / kSmallWaves;
 constexpr int kUpdateWave = 4;                                 // 16 x 16 blocks of X a wave: width * mp / 256 / 16 at most
 constexpr int kSmallLds = 150 * 1024;
+constexpr int kPartsAhead = 16;                                // strips' parts a thread has on their way at once
 constexpr float kFirst = 16384.0f;                             // what U 2^-e, |.| <= 1, is multiplied by before the first step
 
 __device__ __host__ inline int tri16(int mp) { return mp / 16 * (mp / 16 + 1) / 2; }
@@ -879,8 +880,14 @@ __global__ void __launch_bounds__(kSmallThreads) ns_small_kernel(Items L, Moment
       for (int q = 0; q < kTriWave; ++q) {
         if (ta[q] < 0) continue;
         const f32x4* part = at<const f32x4>(ws, off_parts(I, step & 1)) + (wave + q * kSmallWaves) * 64 + lane;
-#pragma unroll 8
-        for (int p = 0; p < I.strips; ++p) parts[q] += part[(int64_t)p * ntri * 64];
+        for (int p0 = 0; p0 < I.strips; p0 += kPartsAhead) {
+          f32x4 v[kPartsAhead];
+#pragma unroll
+          for (int p = 0; p < kPartsAhead; ++p) v[p] = part[(int64_t)min(p0 + p, I.strips - 1) * ntri * 64];
+#pragma unroll
+          for (int p = 0; p < kPartsAhead; ++p)
+            if (p0 + p < I.strips) parts[q] += v[p];
+        }
       }
     }
     double s = 0.0;
@@ -925,10 +932,16 @@ __global__ void __launch_bounds__(kSmallThreads) ns_small_kernel(Items L, Moment
           for (int p0 = 0; p0 < I.strips; p0 += 64) {
             const float own = p0 + lane < I.strips ? start_of(squares, eps, exps[p0 + lane]).first * (1.0f / kFirst) : 0.0f;
             const int n = min(64, I.strips - p0);
-#pragma unroll 4
-            for (int p = 0; p < n; ++p) {
-              const float f1 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(own), p));
-              r += part[(int64_t)(p0 + p) * ntri * 64] * (f1 * f1);
+            for (int p1 = 0; p1 < n; p1 += kPartsAhead) {
+              f32x4 v[kPartsAhead];
+#pragma unroll
+              for (int p = 0; p < kPartsAhead; ++p) v[p] = part[(int64_t)(p0 + min(p1 + p, n - 1)) * ntri * 64];
+#pragma unroll
+              for (int p = 0; p < kPartsAhead; ++p) {
+                if (p1 + p >= n) continue;
+                const float f1 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(own), p1 + p));
+                r += v[p] * (f1 * f1);
+              }
             }
           }
         } else {
