@@ -1296,10 +1296,10 @@ const char* ns_refusal(const NsMatrix& M) {
   if (M.rows < 1 || M.cols < 1 || M.batch < 1) return "empty or negative sizes";
   const int64_t m = M.rows < M.cols ? M.rows : M.cols, n = M.rows < M.cols ? M.cols : M.rows;
   if (m > 32768 || n > (int64_t)1 << 30 || (m > 1 && n > (int64_t)1 << 24)) return "a side is too long (short side over 32768, or long side over 2^24, 2^30 for a vector)";
-  // a launch holds fewer than 2^32 threads: 2^24 blocks of 256, over all the matrices that share it
+  // a launch holds fewer than 2^32 threads, over the 16 entries that may share it in blocks of up to 1024
   const int64_t tiles = ((m + 63) / 64) * ((n + 63) / 64), values = (m * n + 4095) / 4096;
   const int64_t sums = values < kSumsMax ? values : kSumsMax, most = m > 1 && tiles > sums ? tiles : sums;
-  if (M.batch > ((int64_t)1 << 19) / most) return "too many tiles in one stack";
+  if (most > (int64_t)1 << 18 || M.batch > (most < 1 << 17 ? ((int64_t)1 << 17) / most : 1)) return "too many tiles in one stack";
   return nullptr;
 }
 

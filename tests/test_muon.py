@@ -19,7 +19,7 @@ def _mats(*shapes, g=FAKE, out=FAKE):
 
 
 @pytest.mark.parametrize("shape", [(0, 4, 1), (4, 0, 1), (4, 4, 0), (40000, 40000, 1), (2, 1 << 25, 1), (1 << 31, 1, 1),
-                                   (64, 64, 1 << 20)])
+                                   (64, 64, 1 << 20), (64, 64, (1 << 17) + 1), (1, 4, (1 << 17) + 1), (32768, 32768, 2)])
 def test_bad_matrices_are_refused(shape):
     lib = _lib()
     mats = _mats((8, 8, 1), shape)
