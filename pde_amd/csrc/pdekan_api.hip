@@ -106,6 +106,16 @@ int to_view(const PdekanLayer* l, pdekan::LayerView& v) {
   return PDEKAN_OK;
 }
 
+// Nothing throws across the ABI: what host allocations (kernel attributes, profile records) could throw becomes an error.
+template <typename F>
+int guarded(const char* what, F&& body) {
+  try {
+    return body();
+  } catch (...) {
+    return fail(PDEKAN_ERR_HIP, "%s: out of host memory", what);
+  }
+}
+
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 // the checks the group-norm entry points share; jets: n_dir or n_second not 0
@@ -179,12 +189,14 @@ int ns_run(const char* what, const M* mats, int n, int dtype, pdekan::NsPlan& p,
     const int rc = ns_args(what, mats, n, i, B, true);
     if (rc) return rc;
   }
-  ProfScope prof(st, what, 0);
-  for (int i = 0; i < n; i += pdekan::kNsItemsMax) {
-    (void)ns_args(what, mats, n, i, B, true);
-    pdekan::launch_ns(dtype, B.m, B.n, p, ws, st);
-  }
-  return check_launch(what);
+  return guarded(what, [&] {
+    ProfScope prof(st, what, 0);
+    for (int i = 0; i < n; i += pdekan::kNsItemsMax) {
+      (void)ns_args(what, mats, n, i, B, true);
+      pdekan::launch_ns(dtype, B.m, B.n, p, ws, st);
+    }
+    return check_launch(what);
+  });
 }
 
 size_t align_up(size_t v, size_t a = 256) { return (v + a - 1) / a * a; }
@@ -1173,11 +1185,13 @@ int pdekan_bs_residual(const float* x, int64_t stride_n, int64_t stride_d, int64
   const int nblocks = (int)(blocks < kLossBlocks ? blocks : kLossBlocks);
   const float inv_n = 1.0f / (float)n_global;
   float* part = static_cast<float*>(ws);
-  ProfScope prof((hipStream_t)stream, "bs_residual_loss", 0);
-  (void)pdekan::launch_bs_residual(d, x, stride_n, stride_d, v_jet, target, sigma, rate, inv_n, res_out, gv_jet, part,
-                                   nblocks, n, (hipStream_t)stream);
-  if (loss_out) pdekan::launch_loss_finish(part, nblocks, inv_n, loss_out, accumulate, (hipStream_t)stream);
-  return check_launch("bs_residual");
+  return guarded("bs_residual", [&] {
+    ProfScope prof((hipStream_t)stream, "bs_residual_loss", 0);
+    (void)pdekan::launch_bs_residual(d, x, stride_n, stride_d, v_jet, target, sigma, rate, inv_n, res_out, gv_jet, part,
+                                     nblocks, n, (hipStream_t)stream);
+    if (loss_out) pdekan::launch_loss_finish(part, nblocks, inv_n, loss_out, accumulate, (hipStream_t)stream);
+    return check_launch("bs_residual");
+  });
 }
 
 size_t pdekan_group_norm_workspace_bytes(int64_t n, int64_t s, int32_t channels, int32_t groups, int32_t backward) {
@@ -1199,9 +1213,11 @@ int pdekan_group_norm_forward(const void* x, int32_t dtype, int64_t n, int64_t s
   const int rc = norm_args("group_norm_forward", p, 0, 0, dtype, eps, act_kind, x && y, ws, ws_bytes,
                            pdekan::norm_ws_bytes, false);
   if (rc) return rc;
-  ProfScope prof((hipStream_t)stream, "norm.fwd", 0);
-  pdekan::launch_norm_forward(dtype, p, x, weight, bias, eps, act_kind, y, stats, ws, (hipStream_t)stream);
-  return check_launch("group_norm_forward");
+  return guarded("group_norm_forward", [&] {
+    ProfScope prof((hipStream_t)stream, "norm.fwd", 0);
+    pdekan::launch_norm_forward(dtype, p, x, weight, bias, eps, act_kind, y, stats, ws, (hipStream_t)stream);
+    return check_launch("group_norm_forward");
+  });
 }
 
 int pdekan_group_norm_backward(const void* x, const void* gy, int32_t dtype, int64_t n, int64_t s, int32_t channels,
@@ -1214,10 +1230,12 @@ int pdekan_group_norm_backward(const void* x, const void* gy, int32_t dtype, int
   if (rc) return rc;
   if (pdekan::norm_wants_stats(p) && !stats)
     return fail(PDEKAN_ERR_ARG, "group_norm_backward: this shape needs the statistics of the forward");
-  ProfScope prof((hipStream_t)stream, "norm.bwd", 0);
-  pdekan::launch_norm_backward(dtype, p, x, gy, weight, bias, eps, act_kind, stats, gx, gweight, gbias, ws,
-                               (hipStream_t)stream);
-  return check_launch("group_norm_backward");
+  return guarded("group_norm_backward", [&] {
+    ProfScope prof((hipStream_t)stream, "norm.bwd", 0);
+    pdekan::launch_norm_backward(dtype, p, x, gy, weight, bias, eps, act_kind, stats, gx, gweight, gbias, ws,
+                                 (hipStream_t)stream);
+    return check_launch("group_norm_backward");
+  });
 }
 
 int pdekan_group_norm_jet_forward(const float* x_jet, int64_t n, int32_t channels, int32_t groups, int32_t n_dir,
@@ -1229,9 +1247,11 @@ int pdekan_group_norm_jet_forward(const float* x_jet, int64_t n, int32_t channel
                            nullptr, 0, nullptr, false);
   if (rc) return rc;
   if (!aligned16(x_jet) || !aligned16(y_jet)) return fail(PDEKAN_ERR_ARG, "group_norm_jet_forward: jets must be 16-byte aligned");
-  ProfScope prof((hipStream_t)stream, "norm_jet.fwd", 0);
-  pdekan::launch_norm_jet_forward(p, n_dir, x_jet, weight, bias, eps, act_kind, y_jet, (hipStream_t)stream);
-  return check_launch("group_norm_jet_forward");
+  return guarded("group_norm_jet_forward", [&] {
+    ProfScope prof((hipStream_t)stream, "norm_jet.fwd", 0);
+    pdekan::launch_norm_jet_forward(p, n_dir, x_jet, weight, bias, eps, act_kind, y_jet, (hipStream_t)stream);
+    return check_launch("group_norm_jet_forward");
+  });
 }
 
 int pdekan_group_norm_jet_backward(const float* x_jet, const float* gy_jet, int64_t n, int32_t channels, int32_t groups,
@@ -1245,10 +1265,12 @@ int pdekan_group_norm_jet_backward(const float* x_jet, const float* gy_jet, int6
   if (rc) return rc;
   if (!aligned16(x_jet) || !aligned16(gy_jet) || !aligned16(gx_jet))
     return fail(PDEKAN_ERR_ARG, "group_norm_jet_backward: jets must be 16-byte aligned");
-  ProfScope prof((hipStream_t)stream, "norm_jet.bwd", 0);
-  pdekan::launch_norm_jet_backward(p, n_dir, x_jet, gy_jet, weight, bias, eps, act_kind, gx_jet, gweight, gbias, ws,
-                                   (hipStream_t)stream);
-  return check_launch("group_norm_jet_backward");
+  return guarded("group_norm_jet_backward", [&] {
+    ProfScope prof((hipStream_t)stream, "norm_jet.bwd", 0);
+    pdekan::launch_norm_jet_backward(p, n_dir, x_jet, gy_jet, weight, bias, eps, act_kind, gx_jet, gweight, gbias, ws,
+                                     (hipStream_t)stream);
+    return check_launch("group_norm_jet_backward");
+  });
 }
 
 size_t pdekan_orthogonalize_workspace_bytes(const PdekanMatrix* mats, int32_t n_mats) {
