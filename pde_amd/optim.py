@@ -109,6 +109,8 @@ class Muon(torch.optim.Optimizer):
             rows, cols = _matrix_shape(p)
             d.param, d.grad, d.momentum, d.rows, d.cols = p.data_ptr(), g.data_ptr(), m.data_ptr(), rows, cols
             d.gain = self._gain(rows, cols, group["adjust_lr"])
+        if len({d.param for d in desc}) < len(params):
+            raise RuntimeError("pde_amd: two parameters of one group share their memory")
         lr, lr_ptr = group["lr"], None
         if isinstance(lr, torch.Tensor):
             if lr.is_cuda:

@@ -266,6 +266,36 @@ def test_muon_in_a_graph():
         assert all(torch.equal(p, q) for p, q in zip(a, b)), k
 
 
+def test_muon_refusals_on_the_gpu():
+    from pde_amd.optim import Muon
+    base = torch.ones(6, 4, device="cuda")
+    p, q = torch.nn.Parameter(base), torch.nn.Parameter(base.view(4, 6))
+    p.grad, q.grad = torch.ones_like(p), torch.ones_like(q)
+    with pytest.raises(RuntimeError):
+        Muon([p, q]).step()                                      # one memory, two updates
+    h = torch.nn.Parameter(base.half())
+    h.grad = torch.ones_like(h)
+    with pytest.raises(TypeError):
+        Muon([h]).step()
+    t = torch.nn.Parameter(torch.ones(4, 6, device="cuda").t())
+    t.grad = torch.ones_like(t)
+    with pytest.raises(RuntimeError):
+        Muon([t]).step()
+    s = torch.nn.Parameter(torch.ones(4, 6, device="cuda"))
+    s.grad = torch.ones(4, 6, device="cuda").to_sparse()
+    with pytest.raises(RuntimeError):
+        Muon([s]).step()
+    ok = torch.nn.Parameter(torch.ones(4, 6, device="cuda"))
+    ok.grad = torch.ones_like(ok)
+    for lr in (torch.tensor([0.1, 0.2], device="cuda"), torch.tensor(0.1, device="cuda", dtype=torch.float64)):
+        with pytest.raises(RuntimeError):
+            Muon([ok], lr=lr).step()
+    assert torch.equal(ok, torch.ones(4, 6, device="cuda"))
+    opt = Muon([ok], lr=torch.tensor(0.1))                       # a number on the host
+    opt.step()
+    assert opt.step(lambda: torch.tensor(3.0)) == 3.0
+
+
 def test_streams():
     from pde_amd import functional as K
     g = [_matrix((300, 400), 10), _matrix((64, 64), 11)]
