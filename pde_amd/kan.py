@@ -231,7 +231,8 @@ class KAN(torch.nn.Module):
             GroupNormAct(norm_groups, width, activation=norm_activation) for width in layers_hidden[1:-1])
 
     def _norm_after(self, i: int) -> Optional[GroupNormAct]:
-        return None if self.norms is None or i >= len(self.norms) else self.norms[i]
+        norms = getattr(self, "norms", None)             # (a module pickled before there were norms has none)
+        return None if norms is None or i >= len(norms) else norms[i]
 
     def forward(self, x: torch.Tensor, update_grid=False):
         for i, layer in enumerate(self.layers):

@@ -101,13 +101,14 @@ def _loss(f, params, x, target, n_global):
     return ((res[:, 0] - target) ** 2).sum() / n_global, res[:, 0]
 
 
-@pytest.mark.parametrize("groups", [4, 2])
-@pytest.mark.parametrize("widths", [[2, 8, 8, 1], [2, 64, 64, 1], [6, 32, 16, 1]])
-def test_step_matches_the_definition(widths, groups):
+@pytest.mark.parametrize("widths,groups,grid", [([2, 8, 8, 1], 4, 5), ([2, 8, 8, 1], 2, 5), ([2, 64, 64, 1], 4, 5), ([2, 64, 64, 1], 2, 5),
+                                                ([6, 32, 16, 1], 4, 5), ([6, 32, 16, 1], 2, 5), ([2, 64, 64, 1], 8, 10),
+                                                ([6, 64, 64, 1], 8, 10), ([2, 64, 1], 1, 20)])
+def test_step_matches_the_definition(widths, groups, grid):
     """Loss, residual and every gradient of the layer-by-layer step against 64-bit differentiation of the tensor code, in
     one pass, in micro-batches and within a workspace budget."""
     from pde_amd.pinn import BlackScholesStep
-    model = _model(widths, groups).cuda()
+    model = _model(widths, groups, grid).cuda()
     n = 97
     x = torch.rand(n, widths[0], generator=torch.Generator().manual_seed(2)) * 1.6 - 0.8
     target = torch.randn(n, generator=torch.Generator().manual_seed(3))
