@@ -185,6 +185,7 @@ class BlackScholesStep:
             settings.append((K._ptr(m.weight), K._ptr(m.bias), m.eps, _norm_act_kind(m.activation)))
         step = self.micro_batch or max(n, 1)
         space = None
+        written = set()                                    # norm parameters whose gradient holds a part already
         for lo in range(0, max(n, 1), step):
             pts = x[lo:lo + step]
             m, jets, raw = pts.size(0), 2 * d, []
@@ -215,8 +216,9 @@ class BlackScholesStep:
             for i in reversed(range(nl)):
                 if i < len(norms):
                     w, b, eps, act = settings[i]
-                    into = [None if p is None else by_id[id(p)] for p in (norms[i].weight, norms[i].bias)]
-                    got = [None if v is None else torch.empty_like(v) for v in into] if more else into
+                    own = [norms[i].weight, norms[i].bias]
+                    into = [None if p is None else by_id[id(p)] for p in own]
+                    got = [torch.empty_like(v) if id(p) in written else v for p, v in zip(own, into)]
                     gy, g = g, torch.empty_like(g)
                     need = lib.pdekan_group_norm_workspace_bytes(m, 1, norms[i].channels, norms[i].groups, 1)
                     ws = K._workspace(need, self.device)
@@ -224,10 +226,10 @@ class BlackScholesStep:
                                                                   norms[i].groups, d, d - 1, w, b, eps, act, K._ptr(g),
                                                                   K._ptr(got[0]), K._ptr(got[1]), K._ptr(ws), ws.numel(),
                                                                   st))
-                    if more:
-                        for v, part in zip(into, got):
-                            if v is not None:
-                                v.add_(part)
+                    for p, v, part in zip(own, into, got):
+                        if part is not v:
+                            v.add_(part)
+                    written.update(id(p) for p in own if p is not None)
                 below = empty(m, layers[i].in_features, jets) if i else None
                 _lib.check(lib.pdekan_layer_backward(ctypes.byref(layers[i]), K._ptr(a[i]), K._ptr(g), m, d, d - 1,
                                                      K._ptr(below), ctypes.byref(grads[i]), more, K._ptr(space),

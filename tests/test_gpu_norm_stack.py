@@ -136,6 +136,23 @@ def test_step_matches_the_definition(widths, groups, grid):
         assert _rel(g, p.grad.double()) < 2 * tol[k], k
 
 
+def test_shared_norms():
+    """One norm between several layers gets the sum of its gradients."""
+    from pde_amd.pinn import BlackScholesStep, bs_residual_from_jet
+    model = _model([2, 8, 8, 8, 1], 2)
+    model.norms[2] = model.norms[0]
+    model = model.cuda()
+    x = torch.rand(97, 2, device="cuda", generator=torch.Generator(device="cuda").manual_seed(2))
+    r = bs_residual_from_jet(x, model.forward_jet(x))
+    want = torch.autograd.grad((r ** 2).sum() / 97, list(model.parameters()))
+    for kw in ({}, {"micro_batch": 40}):
+        BlackScholesStep(model, **kw)(x)
+        for (k, p), g in zip(model.named_parameters(), want):
+            # the same kernels and other orders of the sums: 1e-4 is over a hundred roundings of sums of 97 points times
+            # the conditions (below 10) that the tolerances of the other tests of this model come out at
+            assert _rel(p.grad, g.double()) < 1e-4, (k, kw)
+
+
 def test_gradient_against_differences():
     """The step's gradient along a direction against central differences of the 64-bit loss."""
     from pde_amd.pinn import BlackScholesStep
