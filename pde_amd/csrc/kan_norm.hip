@@ -472,18 +472,19 @@ __global__ void __launch_bounds__(kThreads) norm_jet_kernel(RowMap m, const floa
 }
 
 // out_w[c], out_b[c] = sums over the rows of part [rows][2][C], in a fixed order: a block takes COLS columns, THREADS / COLS
-// threads a column, eight loads of a thread in flight
+// threads a column, eight loads of a thread in flight.  In 64 bits: a thread's chain is rows / (THREADS / COLS) long, up to
+// 2^18 where there are millions of samples, and the additions hide behind the loads.
 template <int COLS, int THREADS>
 __device__ __forceinline__ void finish_columns(int col_block, const float* __restrict__ part, int64_t rows, int C,
                                                float* out_w, float* out_b) {
   constexpr int kSlices = THREADS / COLS;
-  __shared__ float red[kSlices][COLS + 1];
+  __shared__ double red[kSlices][COLS + 1];
   const int cl = threadIdx.x % COLS, sl = threadIdx.x / COLS;
   const int col = col_block * COLS + cl;
-  float s = 0.0f;
+  double s = 0.0;
   if (col < 2 * C) {
 #pragma unroll 8
-    for (int64_t i = sl; i < rows; i += kSlices) s += part[i * 2 * C + col];
+    for (int64_t i = sl; i < rows; i += kSlices) s += (double)part[i * 2 * C + col];
   }
   red[sl][cl] = s;
   __syncthreads();
@@ -491,7 +492,7 @@ __device__ __forceinline__ void finish_columns(int col_block, const float* __res
 #pragma unroll
     for (int i = 1; i < kSlices; ++i) s += red[i][cl];
     float* out = col < C ? out_w : out_b;
-    if (out) out[col < C ? col : col - C] = s;
+    if (out) out[col < C ? col : col - C] = (float)s;
   }
 }
 constexpr int kFinishCols = 32, kGridFinishCols = 8;

@@ -40,10 +40,9 @@ def _require_gpu_float(t: torch.Tensor, what: str) -> None:
         raise TypeError(f"pde_amd: {what} must be float32, bfloat16 or float16, got {t.dtype}")
 
 
-def under_func_transform(*tensors) -> bool:
-    """True while one of the tensors is a torch.func wrapper (grad / vmap / jvp level)."""
-    fn = getattr(torch._C._functorch, "is_functorch_wrapped_tensor", None)
-    return bool(fn and any(t is not None and fn(t) for t in tensors))
+def under_func_transform() -> bool:
+    """True inside a torch.func transform (grad / vmap / jvp level), also where a call's own tensors are not wrapped."""
+    return torch._C._are_functorch_transforms_active()
 
 
 def _ptr(t: Optional[torch.Tensor]):
@@ -428,7 +427,7 @@ def group_norm_act(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] 
     if x.dim() < 2:
         raise ValueError(f"pde_amd: the norm takes [N, ..., channels], got {tuple(x.shape)}")
     _norm_check(x.size(-1), groups, weight, bias, eps, act)
-    if under_func_transform(x, weight, bias):
+    if under_func_transform():
         return _group_norm_expression(x, groups, weight, bias, eps, act)
     _require_gpu_float(x, "x")
     weight = weight if weight is None or weight.dtype == torch.float32 else weight.to(torch.float32)
@@ -511,6 +510,8 @@ def group_norm_act_jet(x_jet: torch.Tensor, groups: int, weight: Optional[torch.
     if n_dir == 0:
         return group_norm_act(x_jet.squeeze(-1), groups, weight, bias, eps, act).unsqueeze(-1)
     _norm_check(x_jet.size(1), groups, weight, bias, eps, act)
+    if under_func_transform():
+        raise RuntimeError("pde_amd: a norm on jets does not run inside torch.func transforms")
     _require_gpu(x_jet, "x_jet")
     weight = weight if weight is None or weight.dtype == torch.float32 else weight.to(torch.float32)
     bias = bias if bias is None or bias.dtype == torch.float32 else bias.to(torch.float32)

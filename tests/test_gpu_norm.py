@@ -221,6 +221,13 @@ def test_second_order_and_transforms():
     assert torch.allclose(v, K.group_norm_act(x.detach(), 3, w, b), atol=1e-5)
 
 
+def _with_gradients(f, x, gy):
+    """(f(x), its gradient in x along gy)"""
+    x = x.detach().requires_grad_()
+    y = f(x)
+    return y.detach(), torch.autograd.grad(y, x, gy)[0]
+
+
 def _jet_definition(jet, w, b, groups, eps, act, n_dir, n_second):
     """Derivatives along x + t x'_d + t^2 x''_d / 2 of the values' definition, by nested forward differentiation."""
     from torch.func import jvp
@@ -315,3 +322,83 @@ def test_results_repeat_on_streams_and_in_graphs():
             torch.cuda.synchronize()
             assert all(torch.equal(a, e) for a, e in zip(held, eager))
         x.copy_(source)
+
+
+def _repeats_match(y, want, tol=None):
+    """Every copy of a block [rows, ...] along y's leading axis: the same bits, or off by at most ``tol`` elementwise."""
+    copies = y.view(-1, *want.shape)
+    for part in copies.split(max(1, (1 << 28) // want.numel())):
+        ok = part == want if tol is None else (part.double() - want).abs() <= tol
+        if not bool(ok.all()):
+            return False
+    return True
+
+
+def test_offsets_beyond_32_bits():
+    """2^32 values and more: one block of points over and over has to give the same bits everywhere."""
+    from pde_amd import functional as K
+    x, w, b, gy = _make((1 << 15, 128), torch.bfloat16, 8)
+    gy = gy.abs()
+    copies = (1 << 10) + 1
+    want = [t.clone() for t in _with_gradients(lambda t: K.group_norm_act(t, 8, w, b, 1e-5, K.ACT_TANH), x, gy)]
+    got = _with_gradients(lambda t: K.group_norm_act(t, 8, w, b, 1e-5, K.ACT_TANH), x.repeat(copies, 1), gy.repeat(copies, 1))
+    assert got[0].numel() > 1 << 32
+    assert all(_repeats_match(a, e) for a, e in zip(got, want))
+    del got
+    torch.cuda.empty_cache()
+    # gradients of the parameters: 2^25 points over 2048 blocks of 8 points at a time are chains of 2^11 additions of
+    # one sign: at most 2^11 (and the 64-bit finish) times 2^-24
+    bias = b.clone().requires_grad_()
+    K.group_norm_act(x.repeat(copies, 1), 8, w, bias).backward(gy.repeat(copies, 1))
+    assert torch.allclose(bias.grad.double(), copies * gy.double().sum(0), rtol=2.0 ** -12, atol=0)
+    torch.cuda.empty_cache()
+    jets, copies = torch.randn(1 << 14, 64, 4, device="cuda", generator=torch.Generator(device="cuda").manual_seed(9)), (1 << 10) + 1
+    w, b = w[:64].contiguous(), b[:64].contiguous()
+    cot = torch.randn_like(jets)
+    f = lambda t: K.group_norm_act_jet(t, 8, w, b, 1e-5, K.ACT_TANH)
+    want = [t.clone() for t in _with_gradients(f, jets, cot)]
+    got = _with_gradients(f, jets.repeat(copies, 1, 1), cot.repeat(copies, 1, 1))
+    assert got[0].numel() > 1 << 32
+    assert all(_repeats_match(a, e) for a, e in zip(got, want))
+    del got
+    torch.cuda.empty_cache()
+
+
+def test_long_samples_beyond_32_bits():
+    """Three samples of 2^31 values: positions over and over have the statistics of one round of them."""
+    from pde_amd import functional as K
+    s, c, groups, copies = 1 << 14, 128, 8, 1 << 10
+    x, w, b, gy = _make((3, s, c), torch.bfloat16, 10)
+    gy = gy.abs()
+    long = lambda t: t.unsqueeze(1).expand(3, copies, s, c).reshape(3, copies * s, c)
+    got = _with_gradients(lambda t: K.group_norm_act(t, groups, w, b, 1e-5, K.ACT_SILU), long(x), long(gy))
+    assert got[0].numel() > 1 << 32
+    xd = x.double().requires_grad_()
+    y = _definition(xd, w.double(), b.double(), groups, 1e-5, "silu")
+    gx, = torch.autograd.grad(y, xd, gy.double())
+    # a thread adds 2^24 / 128 chunks / 16 rows = 2^13 values of a channel, so the sums are off by D = 2^13 + 2^8 steps of
+    # 2^-24 relative to the sums of the magnitudes; values and gradients take that times slopes and normalised values: of
+    # data of spread 1 and |z| < 6, (1 + |z|) |w| 1.1 D u for the value and twice r (|w| max|gy|) (1 + |z|)^2 D u for the gradient
+    d = (2 ** 13 + 2 ** 8) * 2.0 ** -24
+    half = 2.0 ** -8
+    z = _definition(x.double(), torch.ones(c, device="cuda").double(), torch.zeros(c, device="cuda").double(), groups, 1e-5, "identity")
+    spread = x.double().reshape(3, s, groups, -1).std((1, 3), keepdim=True)
+    r = (1 / spread).expand(3, s, groups, c // groups).reshape(3, s, c)
+    shift = 1 + x.double().abs() * r                              # sums of magnitudes against the spread
+    tol_y = 2.2 * d * (1 + z.abs()) * w.double().abs() * shift + half * y.detach().abs() + 1e-30
+    tol_g = 4 * d * r * (1 + z.abs()) ** 2 * (w.double().abs() * gy.double().abs()).amax() * shift + half * gx.abs() + 1e-30
+    for i in range(3):
+        assert _repeats_match(got[0][i], y.detach()[i], tol_y[i])
+        assert _repeats_match(got[1][i], gx[i], tol_g[i])
+    del got
+    torch.cuda.empty_cache()
+
+
+def test_under_transforms_of_something_else():
+    """Inside a transform a call whose own tensors are constants takes the tensor code; a norm on jets refuses."""
+    from pde_amd import functional as K
+    x, w, b, _ = _make((5, 12), torch.float32, 12)
+    g = torch.func.grad(lambda t: (K.group_norm_act(x, 3, w, b) * t).sum())(torch.ones(5, 12, device="cuda"))
+    assert torch.allclose(g, K.group_norm_act(x, 3, w, b), atol=1e-5)
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda t: K.group_norm_act_jet(t, 2))(torch.ones(3, 2, 4, 4, device="cuda"))
