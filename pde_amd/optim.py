@@ -97,7 +97,9 @@ class Muon(torch.optim.Optimizer):
             state = self.state[p]
             m = state.get("momentum_buffer")
             if m is None:
-                if torch.cuda.is_current_stream_capturing():
+                with K._on(device):
+                    capturing = torch.cuda.is_current_stream_capturing()
+                if capturing:
                     raise RuntimeError("pde_amd: run one eager Muon step before capturing one (its momentum buffers "
                                        "would be cleared at every replay)")
                 m = state["momentum_buffer"] = torch.zeros_like(p, memory_format=torch.contiguous_format)

@@ -309,3 +309,35 @@ def test_streams():
                 out.append(K.orthogonalize(g))
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for o in out for a, b in zip(o, want))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_the_largest_matrix(dtype):
+    """2^30 values, workspaces beyond 2^32 bytes: [B B ... B] of 2^10 copies has the factor [O O ... O] / 2^5 of B's O."""
+    from pde_amd import functional as K
+    base = _matrix((1024, 1024), 14, "noise", dtype)
+    copies = 1 << 10
+    out = K.orthogonalize(base.repeat(1, copies))
+    assert out.numel() == 1 << 30
+    want, off = _definition(base, eps=0.0)
+    # the rounding errors of the sums over the long axis add like the root of its length
+    off, want, half = off * copies ** 0.5, want / 32, torch.finfo(dtype).eps / 2
+    for k in range(0, copies, 32):
+        d = (out[:, k * 1024:(k + 32) * 1024].reshape(1024, 32, 1024).double() - want.unsqueeze(1)).square().sum((0, 2)).sqrt()
+        assert bool((d <= off / 32 * (1 + half) + half * want.square().sum().sqrt()).all()), k
+    with pytest.raises(RuntimeError):
+        K.orthogonalize(torch.empty(1025, 1 << 20, device="cuda", dtype=dtype))
+    del out
+    torch.cuda.empty_cache()
+
+
+def test_a_vector_of_two_to_the_30():
+    from pde_amd.optim import Muon
+    p = torch.nn.Parameter(torch.zeros(1 << 30, device="cuda"))
+    p.grad = torch.randn(1 << 30, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3))
+    Muon([p], lr=1.0, momentum=0.0, ns_steps=1, ns_coefficients=(1.0, 0.0, 0.0), adjust_lr="none").step()
+    norm = sum(float(t.double().square().sum()) for t in p.grad.split(1 << 27)) ** 0.5
+    for a, g in zip(p.detach().split(1 << 27), p.grad.split(1 << 27)):
+        assert torch.allclose(a, -g / norm, rtol=2e-6, atol=0)
+    del p
+    torch.cuda.empty_cache()
