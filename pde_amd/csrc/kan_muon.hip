@@ -195,6 +195,12 @@ __device__ __forceinline__ float source_value(const Item& I, int64_t at, const M
   return mo.nesterov ? (1.0f - mo.mu) * g + mo.mu * m : m;
 }
 
+// the momentum takes in g;  what U has there
+__device__ __forceinline__ float moved(float g, float& m, const Momentum& mo) {
+  m = fmaf(mo.mu, m, (1.0f - mo.mu) * g);
+  return mo.nesterov ? (1.0f - mo.mu) * g + mo.mu * m : m;
+}
+
 // Partial sums of squares of U in 64 bits (the squares of gradients as small as 1e-25 vanish in 32), one a block, a block's
 // values contiguous, 16 bytes of G a thread; the optimiser's momentum is updated on the way.
 template <typename T>
@@ -210,23 +216,51 @@ __global__ void __launch_bounds__(kThreads) ns_norm_kernel(Items L, Momentum mo)
   const T* src = static_cast<const T*>(I.src) + base;
   const bool wide = (((uintptr_t)src | (I.mom ? (uintptr_t)(I.mom + base) : 0)) & 15) == 0;
   double s = 0.0;
-  if (!I.mom && wide) {
-#pragma unroll 4
-    for (int64_t i = lo + threadIdx.x * kVec; i + kVec <= hi; i += kThreads * kVec) {
-      const Vec v = *reinterpret_cast<const Vec*>(src + i);
+  if (wide) {
+    constexpr int kTurns = 4;                            // a thread's loads on their way at once
+    constexpr int64_t kTurn = kThreads * kVec;
+    float* mom = I.mom ? I.mom + base : nullptr;
+    for (int64_t at = lo + threadIdx.x * kVec; at + kVec <= hi; at += kTurns * kTurn) {
+      Vec g[kTurns];
+      float m[kTurns][kVec];
 #pragma unroll
-      for (int k = 0; k < kVec; ++k) s = fma((double)(float)v[k], (double)(float)v[k], s);
+      for (int t = 0; t < kTurns; ++t) {
+        const int64_t i = at + t * kTurn;
+        if (i + kVec > hi) continue;
+        g[t] = *reinterpret_cast<const Vec*>(src + i);
+        if (mom) {
+#pragma unroll
+          for (int q = 0; q < kVec; q += 4) *reinterpret_cast<f32x4*>(m[t] + q) = *reinterpret_cast<const f32x4*>(mom + i + q);
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < kTurns; ++t) {
+        const int64_t i = at + t * kTurn;
+        if (i + kVec > hi) continue;
+        double u[kVec];
+#pragma unroll
+        for (int q = 0; q < kVec; ++q) {
+          u[q] = (float)g[t][q];
+          if (mom) u[q] = moved((float)g[t][q], m[t][q], mo);
+          s = fma(u[q], u[q], s);
+        }
+        if (mom) {
+#pragma unroll
+          for (int q = 0; q < kVec; q += 4) *reinterpret_cast<f32x4*>(mom + i + q) = *reinterpret_cast<const f32x4*>(m[t] + q);
+        }
+      }
     }
     if (hi == I.size)
-      for (int64_t i = hi - (hi - lo) % kVec + threadIdx.x; i < hi; i += kThreads) s = fma((double)(float)src[i], (double)(float)src[i], s);
+      for (int64_t i = hi - (hi - lo) % kVec + threadIdx.x; i < hi; i += kThreads) {
+        const float g = (float)src[i];
+        const double u = mom ? moved(g, mom[i], mo) : g;
+        s = fma(u, u, s);
+      }
   } else {
 #pragma unroll 4
     for (int64_t i = lo + threadIdx.x; i < hi; i += kThreads) {
-      if (I.mom) {
-        const float g = (float)src[i];
-        I.mom[base + i] = fmaf(mo.mu, I.mom[base + i], (1.0f - mo.mu) * g);
-      }
-      const double u = source_value<T>(I, base + i, mo);
+      const float g = (float)src[i];
+      const double u = I.mom ? moved(g, I.mom[base + i], mo) : g;
       s = fma(u, u, s);
     }
   }
@@ -251,17 +285,71 @@ __device__ __forceinline__ double matrix_norm(const Item& I, int b) {
   return sqrt(s);
 }
 
-// X and X^T of a 64 x 64 tile as pieces; COMPOSED: of U' in one piece (16-bit types: exact).
+struct Finish { const float* lr_dev; float lr, decay; };
+
+// what becomes of value x at element `e` of the matrices (weights are fp32)
+template <typename T>
+__device__ __forceinline__ void put(const Item& I, int64_t e, float x, float lr, const Finish& f) {
+  T* out = static_cast<T*>(I.out);
+  if (sizeof(T) == 4 && I.mom) out[e] = (T)fmaf((float)out[e], fmaf(-lr, f.decay, 1.0f), -(lr * I.gain) * x);
+  else out[e] = (T)x;
+}
+
+// what the steps multiply U by where it is a single row: S is the number |X|^2 and X keeps its direction
+__device__ __forceinline__ double vector_factor(double norm, float eps, const NsCoefficients& k, int steps) {
+  double factor = 1.0 / (norm + (double)eps), length = norm * factor;
+  for (int i = 0; i < steps; ++i) {
+    const double s = length * length, q = k.a + s * ((double)k.b + k.c * s);
+    factor *= q;
+    length *= q;
+  }
+  return factor;
+}
+
+// a block's share of a vector
+template <typename T>
+__device__ __forceinline__ void vector_share(const Item& I, int local, const Momentum& mo, float eps, const NsCoefficients& k, int steps,
+                                             const Finish& f) {
+  const int b = local / I.nsum, part = local % I.nsum;
+  const double factor = vector_factor(matrix_norm(I, b), eps, k, steps);
+  const float lr = f.lr_dev ? *f.lr_dev : f.lr;
+  const int64_t base = b * I.size;
+  for (int64_t i = (int64_t)part * kThreads + threadIdx.x; i < I.size; i += (int64_t)I.nsum * kThreads)
+    put<T>(I, base + i, (float)((double)source_value<T>(I, base + i, mo) * factor), lr, f);
+}
+template <typename T>
+__global__ void __launch_bounds__(kThreads) ns_vector_kernel(Items L, Momentum mo, float eps, NsCoefficients k, int steps,
+                                                             Finish f) {
+  const Where w = find_item(L);
+  vector_share<T>(L.it[w.item], w.local, mo, eps, k, steps, f);
+}
+
+// X and X^T of a 64 x 64 tile as pieces, and the vectors of the list; COMPOSED: of U' in one piece (16-bit types: exact).
 template <typename T, bool COMPOSED>
-__global__ void __launch_bounds__(kThreads) ns_split_kernel(Items L, Momentum mo, float eps, Scales sc) {
+__global__ void __launch_bounds__(kThreads) ns_split_kernel(Items L, Momentum mo, float eps, Scales sc, NsCoefficients k, int steps,
+                                                            Finish f) {
   constexpr int PX = COMPOSED ? 1 : 2;
   __shared__ float tile[64][65];
   const Where w = find_item(L);
   const Item& I = L.it[w.item];
+  if (I.path == kVector) {
+    vector_share<T>(I, w.local, mo, eps, k, steps, f);
+    return;
+  }
   const int tm = (I.mp + 63) / 64, tn = (I.np + 63) / 64;
   const int b = w.local / (tm * tn), t = w.local % (tm * tn), bi = t % tm, bj = t / tm;
   const int64_t base = b * I.size;
   char* ws = I.ws + b * I.ws_stride;
+  // all of a thread's values on their way before the norm is put together
+  float raw[16];
+#pragma unroll
+  for (int u = 0; u < 16; ++u) {
+    // neighbouring threads on neighbouring addresses
+    const int k = threadIdx.x + u * kThreads, a = k / 64, c = k % 64;
+    const int i = bi * 64 + (I.tall ? c : a), j = bj * 64 + (I.tall ? a : c);
+    raw[u] = 0.0f;
+    if (i < I.m && j < I.n) raw[u] = source_value<T>(I, base + (I.tall ? (int64_t)j * I.m + i : (int64_t)i * I.n + j), mo);
+  }
   const double norm = matrix_norm(I, b), whole = norm + (double)eps, small = whole / norm;
   Norm nm;
   // at most 2^96: entries below 2^-96 |X| lose their low bits; (NaN and 0 norms: no shift)
@@ -276,14 +364,10 @@ __global__ void __launch_bounds__(kThreads) ns_split_kernel(Items L, Momentum mo
   }
   if (t == 0 && threadIdx.x == 0) *norm_slot(I, ws) = nm;
   const float scx = x_scale(nm, sc, 0);
-  for (int k = threadIdx.x; k < 64 * 64; k += kThreads) {
-    // neighbouring threads on neighbouring addresses
-    const int a = k / 64, c = k % 64;
-    const int li = I.tall ? c : a, lj = I.tall ? a : c;
-    const int i = bi * 64 + li, j = bj * 64 + lj;
-    float v = 0.0f;
-    if (i < I.m && j < I.n) v = source_value<T>(I, base + (I.tall ? (int64_t)j * I.m + i : (int64_t)i * I.n + j), mo) * scale;
-    tile[li][lj] = v;
+#pragma unroll
+  for (int u = 0; u < 16; ++u) {
+    const int k = threadIdx.x + u * kThreads, a = k / 64, c = k % 64;
+    tile[I.tall ? c : a][I.tall ? a : c] = raw[u] * scale;
   }
   __syncthreads();
   _Float16 *x = at<_Float16>(ws, 0), *xt = at<_Float16>(ws, off_xt(I, 0));
@@ -558,14 +642,21 @@ __global__ void __launch_bounds__(kThreads, BT == 64 ? 3 : 2) ns_square_kernel(I
   });
 }
 
-struct Finish { const float* lr_dev; float lr, decay; };
-
-// what becomes of value x at element `e` of the matrices
+// four values next to each other, all inside and aligned
 template <typename T>
-__device__ __forceinline__ void put(const Item& I, int64_t e, float x, float lr, const Finish& f) {
-  T* out = static_cast<T*>(I.out);
-  if (I.mom) out[e] = (T)fmaf((float)out[e], fmaf(-lr, f.decay, 1.0f), -(lr * I.gain) * x);
-  else out[e] = (T)x;
+__device__ __forceinline__ void put4(const Item& I, int64_t e, const float (&x)[4], float lr, const Finish& f) {
+  typedef T Four __attribute__((ext_vector_type(4)));
+  Four* out = reinterpret_cast<Four*>(static_cast<T*>(I.out) + e);
+  Four v;
+  if (sizeof(T) == 4 && I.mom) {
+    v = *out;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] = (T)fmaf((float)v[r], fmaf(-lr, f.decay, 1.0f), -(lr * I.gain) * x[r]);
+  } else {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] = (T)x[r];
+  }
+  *out = v;
 }
 
 // X <- a X + M X, computed as X^T <- a X^T + X^T M (M symmetric; a = 0: M holds all of the step): block = BT of the long axis x
@@ -587,6 +678,7 @@ __global__ void __launch_bounds__(kThreads, BT == 64 ? 3 : 2) ns_update_kernel(I
   const float scx = x_scale(nm, sc, step), next = x_scale(nm, sc, next_step);
   const float factor = step ? 1.0f : nm.factor, unscale = factor / scx / scale_m, own = ca * factor / scx;
   const float lr = f.lr_dev ? *f.lr_dev : f.lr;
+  const bool quads = (I.tall ? I.m : I.n) % 4 == 0 && (uintptr_t)I.out % (4 * sizeof(T)) == 0;
   acc.each(bj, bi, I.np, I.mp, [&](int j0, int i0, float (&v)[4]) {
     // after the transpose lane l holds row j0 + 4 (l / 16) + l % 4 of X^T, columns i0 + (l & 12) ..
 #pragma unroll
@@ -612,7 +704,9 @@ __global__ void __launch_bounds__(kThreads, BT == 64 ? 3 : 2) ns_update_kernel(I
         store_pieces<1>(at<_Float16>(ws, 0), i0 + (lane & 15), j0 + 4 * (lane >> 4), I.np / 32, v, next);
       }
     } else if (I.tall) {
-      if (j < I.n) {
+      if (quads) {
+        if (j < I.n && i < I.m) put4<T>(I, b * I.size + (int64_t)j * I.m + i, v, lr, f);
+      } else if (j < I.n) {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
           if (i + r < I.m) put<T>(I, b * I.size + (int64_t)j * I.m + i + r, v[r], lr, f);
@@ -620,37 +714,15 @@ __global__ void __launch_bounds__(kThreads, BT == 64 ? 3 : 2) ns_update_kernel(I
     } else {
       quad_transpose(v);
       const int jj = j0 + 4 * (lane >> 4), ii = i0 + (lane & 15);
-      if (ii < I.m) {
+      if (quads) {
+        if (ii < I.m && jj < I.n) put4<T>(I, b * I.size + (int64_t)ii * I.n + jj, v, lr, f);
+      } else if (ii < I.m) {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
           if (jj + r < I.n) put<T>(I, b * I.size + (int64_t)ii * I.n + jj + r, v[r], lr, f);
       }
     }
   });
-}
-
-// what the steps multiply U by where it is a single row: S is the number |X|^2 and X keeps its direction
-__device__ __forceinline__ double vector_factor(double norm, float eps, const NsCoefficients& k, int steps) {
-  double factor = 1.0 / (norm + (double)eps), length = norm * factor;
-  for (int i = 0; i < steps; ++i) {
-    const double s = length * length, q = k.a + s * ((double)k.b + k.c * s);
-    factor *= q;
-    length *= q;
-  }
-  return factor;
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kThreads) ns_vector_kernel(Items L, Momentum mo, float eps, NsCoefficients k, int steps,
-                                                             Finish f) {
-  const Where w = find_item(L);
-  const Item& I = L.it[w.item];
-  const int b = w.local / I.nsum, part = w.local % I.nsum;
-  const double factor = vector_factor(matrix_norm(I, b), eps, k, steps);
-  const float lr = f.lr_dev ? *f.lr_dev : f.lr;
-  const int64_t base = b * I.size;
-  for (int64_t i = (int64_t)part * kThreads + threadIdx.x; i < I.size; i += (int64_t)I.nsum * kThreads)
-    put<T>(I, base + i, (float)((double)source_value<T>(I, base + i, mo) * factor), lr, f);
 }
 
 // ---- small matrices -------------------------------------------------------------------------------------------------
@@ -760,18 +832,40 @@ __global__ void __launch_bounds__(kSmallThreads) ns_small_kernel(Items L, Moment
   const int b = w.local / I.strips, strip = w.local % I.strips;
   const int64_t base = b * I.size;
   const float lr = f.lr_dev ? *f.lr_dev : f.lr;
-  if (SINGLE && I.m == 1) {
+  if ((SINGLE || step < 0) && I.m == 1) {
     // X keeps the direction of the vector, S is the number |X|^2: the whole iteration is one factor
+    constexpr int kTurns = 4;                            // a thread's loads on their way at once
+    const T* src = static_cast<const T*>(I.src) + base;
     double s = 0.0;
-    for (int i = tid; i < I.n; i += kSmallThreads) {
-      if (I.mom) I.mom[base + i] = fmaf(mo.mu, I.mom[base + i], (1.0f - mo.mu) * (float)static_cast<const T*>(I.src)[base + i]);
-      const double u = source_value<T>(I, base + i, mo);
-      s = fma(u, u, s);
+    for (int at = tid; at < I.n; at += kTurns * kSmallThreads) {
+      float g[kTurns], m[kTurns];
+#pragma unroll
+      for (int t = 0; t < kTurns; ++t) {
+        const int i = min(at + t * kSmallThreads, I.n - 1);
+        g[t] = (float)src[i];
+        m[t] = I.mom ? I.mom[base + i] : 0.0f;
+      }
+#pragma unroll
+      for (int t = 0; t < kTurns; ++t) {
+        const int i = at + t * kSmallThreads;
+        if (i >= I.n) break;
+        const double u = I.mom ? moved(g[t], m[t], mo) : g[t];
+        s = fma(u, u, s);
+        if (I.mom) I.mom[base + i] = m[t];
+      }
     }
     const double norm = sqrt(block_sum_max(s, 0.0f, red, redf).sum);
     const double factor = vector_factor(norm, eps, kc, steps);
-    for (int i = tid; i < I.n; i += kSmallThreads)
-      put<T>(I, base + i, (float)((double)source_value<T>(I, base + i, mo) * factor), lr, f);
+    for (int at = tid; at < I.n; at += kTurns * kSmallThreads) {
+      float u[kTurns];
+#pragma unroll
+      for (int t = 0; t < kTurns; ++t) u[t] = source_value<T>(I, base + min(at + t * kSmallThreads, I.n - 1), mo);
+#pragma unroll
+      for (int t = 0; t < kTurns; ++t) {
+        const int i = at + t * kSmallThreads;
+        if (i < I.n) put<T>(I, base + i, (float)((double)u[t] * factor), lr, f);
+      }
+    }
     return;
   }
   const int mp = I.mp, width = I.width, rb = mp / 16, mt = mp / 32, wb = width / 16, wt = width / 32, ntri = tri16(mp);
@@ -1090,7 +1184,7 @@ void choose_path(Item& I, Path least) {
   I.width = I.np;
   I.path = kTiles;
   if (I.m == 1) {
-    I.path = I.n <= 65536 ? kSingle : kVector;
+    I.path = I.n <= 65536 && least < kTiles ? kSingle : kVector;
   } else if (I.mp <= kSmallRows && least < kTiles) {
     if (I.np <= widest && least == kSingle) {
       I.path = kSingle;
@@ -1106,7 +1200,8 @@ void choose_path(Item& I, Path least) {
 }
 
 // The matrices of one list.  Those that could go alone in fewer launches join the launches of the others that take more of
-// them: beside those they cost next to nothing, on their own their whole time.
+// them, and vectors beside tiles take part in the launches of the norms and of the pieces: beside those they cost next to
+// nothing, on their own their whole time.
 void make_items(const NsMatrix* mats, int count, Items& L) {
   L.n = 0;
   Path most = kSingle;
@@ -1115,7 +1210,7 @@ void make_items(const NsMatrix* mats, int count, Items& L) {
     if (I.m > 1 && I.path > most) most = (Path)I.path;
   }
   for (int j = 0; j < L.n; ++j)
-    if (L.it[j].m > 1 && L.it[j].path < most) choose_path(L.it[j], most);
+    if (L.it[j].m > 1 ? L.it[j].path < most : most == kTiles) choose_path(L.it[j], most);
 }
 
 int blocks_before(Items& L, int (*count)(const Item&), int times = 1) {
@@ -1126,7 +1221,7 @@ int blocks_before(Items& L, int (*count)(const Item&), int times = 1) {
 }
 int count_sums(const Item& I) { return I.nsum; }
 int count_strips(const Item& I) { return I.strips; }
-int count_split(const Item& I) { return ((I.mp + 63) / 64) * ((I.np + 63) / 64); }
+int count_split(const Item& I) { return I.path == kVector ? I.nsum : ((I.mp + 63) / 64) * ((I.np + 63) / 64); }
 int count_tiles(const Item& I) { return ((I.mp + I.bt - 1) / I.bt) * ((I.np + I.bt - 1) / I.bt); }
 int count_squares(const Item& I) { return tri_squares(I); }
 int count_gram(const Item& I) { return tri_tiles(I) * I.chunks; }
@@ -1274,18 +1369,31 @@ void run_items(const Items& L, const NsPlan& p, hipStream_t st) {
       if (need > lds) lds = need;
     }
   }
+  // vectors take part in the first launch of strips, or the second of tiles (see make_items)
+  Items F = S;
+  if (S.n) {
+    O.n = 0;
+    for (int i = 0; i < L.n; ++i)
+      if (L.it[i].path == kSingle) (L.it[i].m == 1 ? F.it[F.n++] : O.it[O.n++]) = L.it[i];
+  }
   // the small kernels form R, the composed products Q
   const Scales small{p.scale_x, p.scale_s, p.scale_r, p.scale_t, p.scale_p, p.growth};
   launch<kSmallThreads>(ns_small_kernel<T, true>, blocks_before(O, count_strips), lds, st, O, mo, p.eps, p.k, p.steps, 0, small,
                         fin);
   if (S.n)
     for (int k = -1; k < p.steps; ++k)
-      launch<kSmallThreads>(ns_small_kernel<T, false>, blocks_before(S, count_strips), lds, st, S, mo, p.eps, p.k, p.steps, k,
-                            small, fin);
+      launch<kSmallThreads>(ns_small_kernel<T, false>, blocks_before(k < 0 ? F : S, count_strips), lds, st, k < 0 ? F : S, mo, p.eps, p.k,
+                            p.steps, k, small, fin);
   launch(ns_norm_kernel<T>, blocks_before(N, count_sums), 0, st, N, mo);
-  launch(ns_vector_kernel<T>, blocks_before(V, count_sums), 0, st, V, mo, p.eps, p.k, p.steps, fin);
   const Scales sc{p.scale_x, p.scale_s, sizeof(T) == 4 ? p.scale_r : p.scale_q, p.scale_t, p.scale_p, p.growth};
-  for (Items* X : {&M, &B}) launch(ns_split_kernel<T, sizeof(T) == 2>, blocks_before(*X, count_split), 0, st, *X, mo, p.eps, sc);
+  if (!M.n && !B.n) launch(ns_vector_kernel<T>, blocks_before(V, count_sums), 0, st, V, mo, p.eps, p.k, p.steps, fin);
+  for (Items* X : {&M, &B}) {
+    if (!X->n) continue;
+    Items W = *X;
+    for (int i = 0; i < V.n; ++i) W.it[W.n++] = V.it[i];
+    V.n = 0;
+    launch(ns_split_kernel<T, sizeof(T) == 2>, blocks_before(W, count_split), 0, st, W, mo, p.eps, sc, p.k, p.steps, fin);
+  }
   run_products<T, 64>(M, p, sc, fin, st);
   run_products<T, 128>(B, p, sc, fin, st);
 }
