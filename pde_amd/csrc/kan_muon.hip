@@ -11,6 +11,7 @@
 // 8 (l / 16) ..) at 16 l, so a wave loads one operand of one instruction as one contiguous 1 KB, and tiles that follow each
 // other along the inner dimension lie next to each other.
 #include <hip/hip_runtime.h>
+#include <climits>
 #include <cmath>
 #include <cstdint>
 
@@ -49,7 +50,7 @@ struct Item {
 enum Path { kVector, kSingle, kStrips, kTiles };
 struct Items {
   Item it[kItemsMax];
-  int first[kItemsMax + 1];               // first block of each item in this launch
+  int first[kItemsMax + 1];               // first block of each item in this launch, INT_MAX past the last
   int n;
 };
 
@@ -73,11 +74,16 @@ __device__ __host__ inline int64_t item_bytes(const Item& I) {
 template <typename H>
 __device__ __forceinline__ H* at(char* ws, int64_t off) { return reinterpret_cast<H*>(ws + off); }
 
-struct Where { int item, local; };
-__device__ __forceinline__ Where find_item(const Items& L) {
+// The block's matrix, and its number among the blocks of it.  A lone matrix is read with the first kernel arguments, in a list
+// with the second ones: each trip to them takes 0.7 us.
+__device__ __forceinline__ int find_item(const Items& L, Item& I) {
+  I = L.it[0];
+  if (L.n == 1) return (int)blockIdx.x;
   int k = 0;
-  while (k + 1 < L.n && (int)blockIdx.x >= L.first[k + 1]) ++k;
-  return {k, (int)blockIdx.x - L.first[k]};
+#pragma unroll
+  for (int j = 1; j < kItemsMax; ++j) k += (int)blockIdx.x >= L.first[j];
+  I = L.it[k];
+  return (int)blockIdx.x - L.first[k];
 }
 
 // (row, column) of the t-th tile of the upper triangle, columns first: (0,0) (0,1) (1,1) (0,2) ...
@@ -208,9 +214,9 @@ __global__ void __launch_bounds__(kThreads) ns_norm_kernel(Items L, Momentum mo)
   constexpr int kVec = 16 / sizeof(T);
   typedef T Vec __attribute__((ext_vector_type(kVec)));
   __shared__ double red[kThreads / 64];
-  const Where w = find_item(L);
-  const Item& I = L.it[w.item];
-  const int b = w.local / I.nsum, part = w.local % I.nsum;
+  Item I;
+  const int here = find_item(L, I);
+  const int b = here / I.nsum, part = here % I.nsum;
   const int64_t base = b * I.size, per = (I.size + I.nsum - 1) / I.nsum, span = (per + kThreads * kVec - 1) / (kThreads * kVec) * (kThreads * kVec);
   const int64_t lo = part * span, hi = lo + span < I.size ? lo + span : I.size;
   const T* src = static_cast<const T*>(I.src) + base;
@@ -320,8 +326,9 @@ __device__ __forceinline__ void vector_share(const Item& I, int local, const Mom
 template <typename T>
 __global__ void __launch_bounds__(kThreads) ns_vector_kernel(Items L, Momentum mo, float eps, NsCoefficients k, int steps,
                                                              Finish f) {
-  const Where w = find_item(L);
-  vector_share<T>(L.it[w.item], w.local, mo, eps, k, steps, f);
+  Item I;
+  const int here = find_item(L, I);
+  vector_share<T>(I, here, mo, eps, k, steps, f);
 }
 
 // X and X^T of a 64 x 64 tile as pieces, and the vectors of the list; COMPOSED: of U' in one piece (16-bit types: exact).
@@ -330,14 +337,14 @@ __global__ void __launch_bounds__(kThreads) ns_split_kernel(Items L, Momentum mo
                                                             Finish f) {
   constexpr int PX = COMPOSED ? 1 : 2;
   __shared__ float tile[64][65];
-  const Where w = find_item(L);
-  const Item& I = L.it[w.item];
+  Item I;
+  const int here = find_item(L, I);
   if (I.path == kVector) {
-    vector_share<T>(I, w.local, mo, eps, k, steps, f);
+    vector_share<T>(I, here, mo, eps, k, steps, f);
     return;
   }
   const int tm = (I.mp + 63) / 64, tn = (I.np + 63) / 64;
-  const int b = w.local / (tm * tn), t = w.local % (tm * tn), bi = t % tm, bj = t / tm;
+  const int b = here / (tm * tn), t = here % (tm * tn), bi = t % tm, bj = t / tm;
   const int64_t base = b * I.size;
   char* ws = I.ws + b * I.ws_stride;
   // all of a thread's values on their way before the norm is put together
@@ -539,10 +546,10 @@ __device__ __forceinline__ int xcd_order(int local, int count) {
 template <int BT, int PX>
 __global__ void __launch_bounds__(kThreads, BT == 64 ? 3 : 2) ns_gram_kernel(Items L, Scales sc, int step) {
   extern __shared__ char lds[];
-  const Where w = find_item(L);
-  const Item& I = L.it[w.item];
+  Item I;
+  const int here = find_item(L, I);
   const int tiles = tri_tiles(I), per = tiles * I.chunks;
-  const int local = xcd_order(w.local, per * I.batch), b = local / per, rest = local % per, chunk = rest / tiles, t = rest % tiles;
+  const int local = xcd_order(here, per * I.batch), b = local / per, rest = local % per, chunk = rest / tiles, t = rest % tiles;
   int bi, bj;
   tri_tile(t, bi, bj);
   char* ws = I.ws + b * I.ws_stride;
@@ -570,9 +577,9 @@ template <int BT, int GROUPS>
 __global__ void __launch_bounds__(GROUPS * kThreads) ns_gram_sum_kernel(Items L, Scales sc) {
   constexpr int kAcc = BT * BT / 1024, kW = BT / 32;
   __shared__ f32x4 red[GROUPS][kThreads];
-  const Where w = find_item(L);
-  const Item& I = L.it[w.item];
-  const int tiles = tri_tiles(I), b = w.local / (tiles * kAcc), t = w.local / kAcc % tiles, a = w.local % kAcc;
+  Item I;
+  const int here = find_item(L, I);
+  const int tiles = tri_tiles(I), b = here / (tiles * kAcc), t = here / kAcc % tiles, a = here % kAcc;
   int bi, bj;
   tri_tile(t, bi, bj);
   char* ws = I.ws + b * I.ws_stride;
@@ -598,9 +605,9 @@ __global__ void __launch_bounds__(GROUPS * kThreads) ns_gram_sum_kernel(Items L,
 template <int BT>
 __global__ void __launch_bounds__(kThreads, BT == 64 ? 3 : 2) ns_poly_kernel(Items L, Scales sc, NsCoefficients k, int out) {
   extern __shared__ char lds[];
-  const Where w = find_item(L);
-  const Item& I = L.it[w.item];
-  const int tiles = tri_squares(I), local = xcd_order(w.local, tiles * I.batch), b = local / tiles, t = local % tiles;
+  Item I;
+  const int here = find_item(L, I);
+  const int tiles = tri_squares(I), local = xcd_order(here, tiles * I.batch), b = local / tiles, t = local % tiles;
   int bi, bj;
   tri_tile(t, bi, bj);
   char* ws = I.ws + b * I.ws_stride;
@@ -625,9 +632,9 @@ struct SquareJobs { SquareJob j[2]; int n; };
 template <int BT>
 __global__ void __launch_bounds__(kThreads, BT == 64 ? 3 : 2) ns_square_kernel(Items L, SquareJobs jobs) {
   extern __shared__ char lds[];
-  const Where w = find_item(L);
-  const Item& I = L.it[w.item];
-  const int tiles = tri_squares(I), local = xcd_order(w.local, tiles * I.batch * jobs.n);
+  Item I;
+  const int here = find_item(L, I);
+  const int tiles = tri_squares(I), local = xcd_order(here, tiles * I.batch * jobs.n);
   const int b = local / (tiles * jobs.n), t = local % tiles;
   const SquareJob job = jobs.j[local / tiles % jobs.n];
   int bi, bj;
@@ -665,10 +672,10 @@ template <typename T, int BT, int PX, int PN, bool LAST>
 __global__ void __launch_bounds__(kThreads, BT == 64 ? 3 : 2) ns_update_kernel(Items L, Scales sc, float ca, int square, float scale_m, int from,
                                                                 int step, int next_step, Finish f) {
   extern __shared__ char lds[];
-  const Where w = find_item(L);
-  const Item& I = L.it[w.item];
+  Item I;
+  const int here = find_item(L, I);
   const int tm = (I.mp + BT - 1) / BT, tn = (I.np + BT - 1) / BT;
-  const int local = xcd_order(w.local, tm * tn * I.batch), b = local / (tm * tn), t = local % (tm * tn), bi = t % tm, bj = t / tm;
+  const int local = xcd_order(here, tm * tn * I.batch), b = local / (tm * tn), t = local % (tm * tn), bi = t % tm, bj = t / tm;
   char* ws = I.ws + b * I.ws_stride;
   const _Float16* xt = at<const _Float16>(ws, off_xt(I, from));
   const int lane = threadIdx.x & 63, kt = I.mp / 32;
@@ -826,10 +833,10 @@ __global__ void __launch_bounds__(kSmallThreads) ns_small_kernel(Items L, Moment
   extern __shared__ char lds[];
   __shared__ double red[kSmallThreads / 16];
   __shared__ float redf[kSmallThreads / 16];
-  const Where w = find_item(L);
-  const Item& I = L.it[w.item];
+  Item I;
+  const int here = find_item(L, I);
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-  const int b = w.local / I.strips, strip = w.local % I.strips;
+  const int b = here / I.strips, strip = here % I.strips;
   const int64_t base = b * I.size;
   const float lr = f.lr_dev ? *f.lr_dev : f.lr;
   if ((SINGLE || step < 0) && I.m == 1) {
@@ -1216,7 +1223,7 @@ void make_items(const NsMatrix* mats, int count, Items& L) {
 int blocks_before(Items& L, int (*count)(const Item&), int times = 1) {
   int total = 0;
   for (int i = 0; i < L.n; ++i) { L.first[i] = total; total += count(L.it[i]) * L.it[i].batch * times; }
-  L.first[L.n] = total;
+  for (int i = L.n; i <= kItemsMax; ++i) L.first[i] = INT_MAX;
   return total;
 }
 int count_sums(const Item& I) { return I.nsum; }
@@ -1228,7 +1235,7 @@ int count_gram(const Item& I) { return tri_tiles(I) * I.chunks; }
 int count_parts(const Item& I) { return I.chunks > 1 ? tri_tiles(I) * (I.bt * I.bt / 1024) : 0; }
 
 template <int THREADS = kThreads, typename K, typename... A>
-void launch(K kernel, int blocks, size_t lds, hipStream_t st, A... args) {
+void launch(K kernel, int blocks, size_t lds, hipStream_t st, const A&... args) {
   if (!blocks) return;
   ensure_dynamic_lds((const void*)kernel, lds);
   hipLaunchKernelGGL(kernel, dim3(blocks), dim3(THREADS), lds, st, args...);
