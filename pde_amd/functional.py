@@ -349,29 +349,44 @@ def _address(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
 
+def _contiguous(t: Optional[torch.Tensor]):
+    return t if t is None or t.is_contiguous() else t.contiguous()
+
+
+def _group_norm_forward(x, weight, bias, groups, eps, act, keep_stats):
+    """The value and, where the backward wants it, the statistics."""
+    xd, w, b = _contiguous(x), _contiguous(weight), _contiguous(bias)
+    y = torch.empty_like(xd)
+    stats = None
+    n, c = xd.shape[0], xd.shape[-1]
+    if y.numel():
+        s = y.numel() // (n * c)
+        floats, need, _ = _norm_sizes(n, s, c, groups)
+        device = x.device
+        if floats and keep_stats:
+            stats = torch.empty(floats, dtype=torch.float32, device=device)
+        ws = _workspace(need, device) if need else None
+        with _on(device):
+            rc = _lib.load().pdekan_group_norm_forward(xd.data_ptr(), DTYPES[xd.dtype], n, s, c, groups, _address(w),
+                                                       _address(b), eps, act, y.data_ptr(), _address(stats),
+                                                       _address(ws), need, _raw_stream(device))
+        _lib.check(rc)
+    return y, stats
+
+
+def _recorded(*tensors) -> bool:
+    """Whether a call on these leaves a trace: a backward, or a forward derivative."""
+    if torch.autograd.forward_ad._current_level >= 0:
+        return True
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
 class _GroupNormAct(torch.autograd.Function):
     """First-order backward on the kernels; a recorded backward (``create_graph=True``) differentiates the expression."""
 
     @staticmethod
     def forward(ctx, x, weight, bias, groups, eps, act):
-        xd = x if x.is_contiguous() else x.contiguous()
-        w = weight if weight is None or weight.is_contiguous() else weight.contiguous()
-        b = bias if bias is None or bias.is_contiguous() else bias.contiguous()
-        y = torch.empty_like(xd)
-        stats = None
-        n, c = xd.shape[0], xd.shape[-1]
-        if y.numel():
-            s = y.numel() // (n * c)
-            floats, need, _ = _norm_sizes(n, s, c, groups)
-            device = x.device
-            if floats and any(ctx.needs_input_grad):
-                stats = torch.empty(floats, dtype=torch.float32, device=device)
-            ws = _workspace(need, device) if need else None
-            with _on(device):
-                rc = _lib.load().pdekan_group_norm_forward(xd.data_ptr(), DTYPES[xd.dtype], n, s, c, groups, _address(w),
-                                                           _address(b), eps, act, y.data_ptr(), _address(stats),
-                                                           _address(ws), need, _raw_stream(device))
-            _lib.check(rc)
+        y, stats = _group_norm_forward(x, weight, bias, groups, eps, act, any(ctx.needs_input_grad))
         ctx.save_for_backward(x, weight, bias, stats)
         ctx.meta = (groups, eps, act)
         return y
@@ -389,10 +404,10 @@ class _GroupNormAct(torch.autograd.Function):
                 out[i] = g
             return tuple(out)
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        xd = x if x.is_contiguous() else x.contiguous()
-        gd = gy if gy.is_contiguous() else gy.contiguous()
-        w = weight if weight is None or weight.is_contiguous() else weight.contiguous()
-        b = bias if bias is None or bias.is_contiguous() else bias.contiguous()
+        xd = _contiguous(x)
+        gd = _contiguous(gy)
+        w = _contiguous(weight)
+        b = _contiguous(bias)
         n, c = xd.shape[0], xd.shape[-1]
         gx = torch.empty_like(xd)
         gw = torch.empty_like(w) if need_w else None
@@ -433,6 +448,8 @@ def group_norm_act(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] 
     weight = weight if weight is None or weight.dtype == torch.float32 else weight.to(torch.float32)
     bias = bias if bias is None or bias.dtype == torch.float32 else bias.to(torch.float32)
     _same_device(x, weight, bias)
+    if not _recorded(x, weight, bias):
+        return _group_norm_forward(x, weight, bias, int(groups), float(eps), int(act), False)[0]
     return _GroupNormAct.apply(x, weight, bias, int(groups), float(eps), int(act))
 
 
@@ -442,20 +459,23 @@ def _same_device(x, *others) -> None:
             raise RuntimeError(f"pde_amd: tensors on {x.device} and {t.device} in one call")
 
 
+def _group_norm_jet_forward(x_jet, weight, bias, groups, eps, act, n_dir, n_second):
+    xd, w, b = _aligned(_contiguous(x_jet)), _contiguous(weight), _contiguous(bias)
+    n, c, _ = xd.shape
+    y = torch.empty_like(xd)
+    if n:
+        device = x_jet.device
+        with _on(device):
+            rc = _lib.load().pdekan_group_norm_jet_forward(xd.data_ptr(), n, c, groups, n_dir, n_second, _address(w),
+                                                           _address(b), eps, act, y.data_ptr(), _raw_stream(device))
+        _lib.check(rc)
+    return y
+
+
 class _GroupNormActJet(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x_jet, weight, bias, groups, eps, act, n_dir, n_second):
-        xd = _aligned(x_jet if x_jet.is_contiguous() else x_jet.contiguous())
-        w = weight if weight is None or weight.is_contiguous() else weight.contiguous()
-        b = bias if bias is None or bias.is_contiguous() else bias.contiguous()
-        n, c, _ = xd.shape
-        y = torch.empty_like(xd)
-        if n:
-            device = x_jet.device
-            with _on(device):
-                rc = _lib.load().pdekan_group_norm_jet_forward(xd.data_ptr(), n, c, groups, n_dir, n_second, _address(w),
-                                                               _address(b), eps, act, y.data_ptr(), _raw_stream(device))
-            _lib.check(rc)
+        y = _group_norm_jet_forward(x_jet, weight, bias, groups, eps, act, n_dir, n_second)
         ctx.save_for_backward(x_jet, weight, bias)
         ctx.meta = (groups, eps, act, n_dir, n_second)
         return y
@@ -468,10 +488,10 @@ class _GroupNormActJet(torch.autograd.Function):
         x_jet, weight, bias = ctx.saved_tensors
         groups, eps, act, n_dir, n_second = ctx.meta
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        xd = _aligned(x_jet if x_jet.is_contiguous() else x_jet.contiguous())
-        gd = _aligned(gy if gy.is_contiguous() else gy.contiguous())
-        w = weight if weight is None or weight.is_contiguous() else weight.contiguous()
-        b = bias if bias is None or bias.is_contiguous() else bias.contiguous()
+        xd = _aligned(_contiguous(x_jet))
+        gd = _aligned(_contiguous(gy))
+        w = _contiguous(weight)
+        b = _contiguous(bias)
         n, c, _ = xd.shape
         gx = torch.empty_like(xd)
         gw = torch.empty_like(w) if need_w else None
@@ -516,6 +536,8 @@ def group_norm_act_jet(x_jet: torch.Tensor, groups: int, weight: Optional[torch.
     weight = weight if weight is None or weight.dtype == torch.float32 else weight.to(torch.float32)
     bias = bias if bias is None or bias.dtype == torch.float32 else bias.to(torch.float32)
     _same_device(x_jet, weight, bias)
+    if not _recorded(x_jet, weight, bias):
+        return _group_norm_jet_forward(x_jet, weight, bias, int(groups), float(eps), int(act), int(n_dir), int(n_second))
     return _GroupNormActJet.apply(x_jet, weight, bias, int(groups), float(eps), int(act), int(n_dir), int(n_second))
 
 

@@ -402,3 +402,21 @@ def test_under_transforms_of_something_else():
     assert torch.allclose(g, K.group_norm_act(x, 3, w, b), atol=1e-5)
     with pytest.raises(RuntimeError):
         torch.func.vmap(lambda t: K.group_norm_act_jet(t, 2))(torch.ones(3, 2, 4, 4, device="cuda"))
+
+
+def test_outside_of_a_recording():
+    """Calls that leave no trace give the same bits; forward derivatives are refused, not dropped."""
+    import torch.autograd.forward_ad as fwad
+    from pde_amd import functional as K
+    x, w, b, _ = _make((9, 12), torch.float32, 13)
+    jet = torch.randn(9, 12, 4, device="cuda")
+    for f, t in ((lambda t: K.group_norm_act(t, 3, w, b), x), (lambda t: K.group_norm_act_jet(t, 3, w, b), jet)):
+        want = f(t.clone().requires_grad_())
+        assert want.requires_grad
+        with torch.no_grad():
+            got = f(t.clone().requires_grad_())
+        assert not got.requires_grad and torch.equal(got, want)
+        with torch.inference_mode():
+            assert torch.equal(f(t), want)
+        with fwad.dual_level(), pytest.raises(Exception, match="jvp|forward"):
+            f(fwad.make_dual(t, torch.ones_like(t)))
