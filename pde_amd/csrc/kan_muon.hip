@@ -794,14 +794,14 @@ __device__ __forceinline__ SumMax block_sum_max(double s, float v, double* red, 
   v = fmaxf(v, __shfl_xor(v, 32));
   return {s, v};
 }
-// From the sum of squares, in 32 bits: everything over 2^e, so that nothing overflows.  first: 2^e / (|U| + eps);
+// From the sum of squares, in 32 bits (`few` rows, whose errors are few: rounded once): everything over 2^e, so that nothing overflows.  first: 2^e / (|U| + eps);
 // ex: the exponent of (|U| + eps) / |U|, see Scales
 constexpr int kNoExponent = -1000;                             // of a strip of zeros
 struct Start { float first; int ex; };
-__device__ __forceinline__ Start start_of(double squares, float eps, int e) {
+__device__ __forceinline__ Start start_of(double squares, float eps, int e, bool few) {
   const float norm = sqrtf((float)ldexp(squares, -2 * e)), eps_e = ldexpf(eps, -e);
   Start r;
-  r.first = 1.0f / (norm + eps_e);
+  r.first = few ? (float)(1.0 / (sqrt(ldexp(squares, -2 * e)) + ldexp((double)eps, -e))) : 1.0f / (norm + eps_e);
   r.ex = 0;
   if (norm < eps_e && norm > 0.0f) {
     const float small = 1.0f + eps_e / norm;
@@ -810,8 +810,10 @@ __device__ __forceinline__ Start start_of(double squares, float eps, int e) {
   return r;
 }
 
-// 16 x 16 block of P Q^T from tiles of two pieces in LDS: row of tiles `a` of P and `b` of Q, kp and kq inner tiles a row
-__device__ __forceinline__ f32x4 block_product(const _Float16* P, const _Float16* Q, int a, int b, int kt) {
+// 16 x 16 block of P Q^T from tiles of two pieces in LDS: row of tiles `a` of P and `b` of Q, kt inner tiles a row.  `whole`: with
+// lo lo, which is of one sign on the diagonal of S.  In sums of few terms its 2^-24 shows: errors of five steps at 5 x 64 are
+// 1.2e-6 without it and with X apart from its pieces (see below), 0.8e-6 with both; fp32 products 0.7e-6.
+__device__ __forceinline__ f32x4 block_product(const _Float16* P, const _Float16* Q, int a, int b, int kt, bool whole) {
   const int lane = threadIdx.x & 63;
   f32x4 lh = (f32x4){0.0f, 0.0f, 0.0f, 0.0f}, hl = lh, hh = lh;
   const _Float16 *p = P + a * kt * 1024 + lane * 8, *q = Q + b * kt * 1024 + lane * 8;
@@ -819,6 +821,7 @@ __device__ __forceinline__ f32x4 block_product(const _Float16* P, const _Float16
   for (int k = 0; k < kt; ++k) {
     const f16x8 ph = *reinterpret_cast<const f16x8*>(p + k * 1024), pl = *reinterpret_cast<const f16x8*>(p + k * 1024 + 512);
     const f16x8 qh = *reinterpret_cast<const f16x8*>(q + k * 1024), ql = *reinterpret_cast<const f16x8*>(q + k * 1024 + 512);
+    if (whole) lh = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl, ql, lh, 0, 0, 0);
     lh = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl, qh, lh, 0, 0, 0);
     hl = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, ql, hl, 0, 0, 0);
     hh = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, qh, hh, 0, 0, 0);
@@ -876,6 +879,7 @@ __global__ void __launch_bounds__(kSmallThreads) ns_small_kernel(Items L, Moment
     return;
   }
   const int mp = I.mp, width = I.width, rb = mp / 16, mt = mp / 32, wb = width / 16, wt = width / 32, ntri = tri16(mp);
+  const bool few = mp == 32;
   _Float16* xt = reinterpret_cast<_Float16*>(lds);
   _Float16* x = xt + width * mp * 2;
   _Float16* sq = x + width * mp * 2;
@@ -1006,10 +1010,10 @@ __global__ void __launch_bounds__(kSmallThreads) ns_small_kernel(Items L, Moment
     own_e = exps[strip];
     all_e = most;
   }
-  const Start start = start_of(squares, eps, own_e);
+  const Start start = start_of(squares, eps, own_e, few);
   Norm nm;
   nm.factor = 1.0f;
-  nm.ex = SINGLE ? start.ex : start_of(squares, eps, all_e).ex;        // the same in all strips
+  nm.ex = SINGLE ? start.ex : start_of(squares, eps, all_e, few).ex;        // the same in all strips
   const float inv_s = 1.0f / sc.s, inv_q = 1.0f / sc.q;
   if (SINGLE || step < 0) __syncthreads();
 
@@ -1025,13 +1029,13 @@ __global__ void __launch_bounds__(kSmallThreads) ns_small_kernel(Items L, Moment
       if (ta[q] < 0) continue;
       f32x4 r = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
       if constexpr (SINGLE) {
-        r = block_product(x, x, ta[q], tb[q], wt) * (inv_x * inv_x);
+        r = block_product(x, x, ta[q], tb[q], wt, few) * (inv_x * inv_x);
       } else {
         if (k == 0) {
           // a strip's factor by a lane of its own
           const f32x4* part = at<const f32x4>(ws, off_parts(I, 0)) + (wave + q * kSmallWaves) * 64 + lane;
           for (int p0 = 0; p0 < I.strips; p0 += 64) {
-            const float own = p0 + lane < I.strips ? start_of(squares, eps, exps[p0 + lane]).first * (1.0f / kFirst) : 0.0f;
+            const float own = p0 + lane < I.strips ? start_of(squares, eps, exps[p0 + lane], few).first * (1.0f / kFirst) : 0.0f;
             const int n = min(64, I.strips - p0);
             for (int p1 = 0; p1 < n; p1 += kPartsAhead) {
               f32x4 v[kPartsAhead];
@@ -1059,7 +1063,7 @@ __global__ void __launch_bounds__(kSmallThreads) ns_small_kernel(Items L, Moment
 #pragma unroll
     for (int q = 0; q < kTriWave; ++q) {
       if (ta[q] < 0) continue;
-      const f32x4 r = block_product(sq, sq, ta[q], tb[q], mt);
+      const f32x4 r = block_product(sq, sq, ta[q], tb[q], mt, few);
       float o[4];
       load_pieces<2>(sq, tb[q] * 16 + (lane & 15), ta[q] * 16 + 4 * (lane >> 4), mt, o, inv_s);
 #pragma unroll
@@ -1073,7 +1077,9 @@ __global__ void __launch_bounds__(kSmallThreads) ns_small_kernel(Items L, Moment
     // X <- a X + R X, likewise
     const bool last = k + 1 == steps;
     const float next = x_scale(nm, sc, k + 1), unscale = inv_x * inv_q;
-    if (!SINGLE || k == 0) {
+    // (with few rows X is what its pieces hold in every step: R follows from those, and a X + R X of another X is off by |a + R|
+    // times their rounding where the step itself forgets it.  With more the copy in fp32 saves LDS reads)
+    if (!SINGLE || k == 0 || few) {
 #pragma unroll
       for (int q = 0; q < kUpdateWave; ++q) {
         if (ti[q] >= rb) continue;
@@ -1084,7 +1090,7 @@ __global__ void __launch_bounds__(kSmallThreads) ns_small_kernel(Items L, Moment
 #pragma unroll
     for (int q = 0; q < kUpdateWave; ++q) {
       if (ti[q] >= rb) continue;
-      const f32x4 r = block_product(xt, sq, tj[q], ti[q], mt);
+      const f32x4 r = block_product(xt, sq, tj[q], ti[q], mt, few);
 #pragma unroll
       for (int i = 0; i < 4; ++i) xv[q][i] = fmaf(kc.a, xv[q][i], r[i] * unscale);
     }
@@ -1141,7 +1147,7 @@ __global__ void __launch_bounds__(kSmallThreads) ns_small_kernel(Items L, Moment
     f32x4* part = at<f32x4>(ws, off_parts(I, (step + 1) & 1)) + (int64_t)strip * ntri * 64;
 #pragma unroll
     for (int q = 0; q < kTriWave; ++q)
-      if (ta[q] >= 0) part[(wave + q * kSmallWaves) * 64 + lane] = block_product(x, x, ta[q], tb[q], wt);
+      if (ta[q] >= 0) part[(wave + q * kSmallWaves) * 64 + lane] = block_product(x, x, ta[q], tb[q], wt, few);
   }
 }
 
