@@ -347,15 +347,44 @@ __global__ void __launch_bounds__(kThreads) ns_split_kernel(Items L, Momentum mo
   const int b = here / (tm * tn), t = here % (tm * tn), bi = t % tm, bj = t / tm;
   const int64_t base = b * I.size;
   char* ws = I.ws + b * I.ws_stride;
-  // all of a thread's values on their way before the norm is put together
+  // all of a thread's values on their way before the norm is put together, four neighbours at once where all are whole fours
+  typedef T Four __attribute__((ext_vector_type(4)));
+  const T* src = static_cast<const T*>(I.src) + base;
+  const int inner = I.tall ? I.m : I.n;
+  const bool fours = inner % 4 == 0 && (uintptr_t)src % (4 * sizeof(T)) == 0 && !I.mom;
   float raw[16];
-#pragma unroll
-  for (int u = 0; u < 16; ++u) {
-    // neighbouring threads on neighbouring addresses
-    const int k = threadIdx.x + u * kThreads, a = k / 64, c = k % 64;
+  // value u of the thread: row a of memory, value c of it
+  auto place = [&](int u, int& a, int& c) {
+    const int k = fours ? threadIdx.x * 4 + (u & 3) + (u >> 2) * (4 * kThreads) : threadIdx.x + u * kThreads;
+    a = k / 64;
+    c = k % 64;
+  };
+  auto element = [&](int a, int c, bool& in) {
     const int i = bi * 64 + (I.tall ? c : a), j = bj * 64 + (I.tall ? a : c);
-    raw[u] = 0.0f;
-    if (i < I.m && j < I.n) raw[u] = source_value<T>(I, base + (I.tall ? (int64_t)j * I.m + i : (int64_t)i * I.n + j), mo);
+    in = i < I.m && j < I.n;
+    return I.tall ? (int64_t)j * I.m + i : (int64_t)i * I.n + j;
+  };
+  if (fours) {
+#pragma unroll
+    for (int u = 0; u < 16; u += 4) {
+      int a, c;
+      bool in;
+      place(u, a, c);
+      const int64_t e = element(a, c, in);
+      Four v = {};
+      if (in) v = *reinterpret_cast<const Four*>(src + e);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) raw[u + q] = (float)v[q];
+    }
+  } else {
+#pragma unroll
+    for (int u = 0; u < 16; ++u) {
+      int a, c;
+      bool in;
+      place(u, a, c);
+      const int64_t e = element(a, c, in);
+      raw[u] = in ? source_value<T>(I, base + e, mo) : 0.0f;
+    }
   }
   const double norm = matrix_norm(I, b), whole = norm + (double)eps, small = whole / norm;
   Norm nm;
@@ -373,7 +402,8 @@ __global__ void __launch_bounds__(kThreads) ns_split_kernel(Items L, Momentum mo
   const float scx = x_scale(nm, sc, 0);
 #pragma unroll
   for (int u = 0; u < 16; ++u) {
-    const int k = threadIdx.x + u * kThreads, a = k / 64, c = k % 64;
+    int a, c;
+    place(u, a, c);
     tile[I.tall ? c : a][I.tall ? a : c] = raw[u] * scale;
   }
   __syncthreads();

@@ -341,3 +341,20 @@ def test_a_vector_of_two_to_the_30():
         assert torch.allclose(a, -g / norm, rtol=2e-6, atol=0)
     del p
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("shape", [(64, 40), (256, 300), (300, 256), (3, 160, 200), (1, 4096)])
+def test_any_alignment(shape, dtype):
+    """A matrix that starts anywhere gives what the same values at the start of an allocation give."""
+    from pde_amd import functional as K
+    flat = torch.empty(_matrix(shape, 0).numel() + 8, device="cuda", dtype=dtype)
+    want = None
+    for start in (0, 1, 2, 4, 5):
+        g = flat[start:start + flat.numel() - 8].view(shape)
+        g.copy_(_matrix(shape, 21, dtype=dtype))
+        out = K.orthogonalize(g)
+        want = out if want is None else want
+        # the sum of squares is made in another order: 2^-24 of the norm at most, times the steps' slopes
+        _check(out, *_definition(g))
+        assert torch.allclose(out.float(), want.float(), rtol=1e-2, atol=1e-4)
