@@ -207,6 +207,7 @@ __device__ __forceinline__ float moved(float g, float& m, const Momentum& mo) {
   return mo.nesterov ? (1.0f - mo.mu) * g + mo.mu * m : m;
 }
 
+// (2048 x 8192 bf16: 8.4 us, 4.0 TB/s; a step of KAN [2,256,256,256,1], 13 MB of gradients and momentum each: 9.4 us.)
 // Partial sums of squares of U in 64 bits (the squares of gradients as small as 1e-25 vanish in 32), one a block, a block's
 // values contiguous, 16 bytes of G a thread; the optimiser's momentum is updated on the way.
 template <typename T>
@@ -331,6 +332,8 @@ __global__ void __launch_bounds__(kThreads) ns_vector_kernel(Items L, Momentum m
   vector_share<T>(I, here, mo, eps, k, steps, f);
 }
 
+// Bound by what it writes, two planes of pieces: 2048 x 8192 bf16, 33 MB in and 67 MB out, 25 us = 4.1 TB/s; 256 x 5888 fp32, 6 and
+// 12 MB, 8.3 us.
 // X and X^T of a 64 x 64 tile as pieces, and the vectors of the list; COMPOSED: of U' in one piece (16-bit types: exact).
 template <typename T, bool COMPOSED>
 __global__ void __launch_bounds__(kThreads) ns_split_kernel(Items L, Momentum mo, float eps, Scales sc, NsCoefficients k, int steps,
@@ -429,6 +432,11 @@ __global__ void __launch_bounds__(kThreads) ns_split_kernel(Items L, Momentum mo
 
 // ---- products -------------------------------------------------------------------------------------------------------
 
+// What bounds a product: the LDS where a block is 64 (a stage of 16 KB is read 32 KB for 192 cycles of matrix instructions a wave),
+// the latency behind the L2 where it is 128, whose 80 KB hold two stages of two-piece operands.  Alone on the chip 2048 x 2048
+// squares (three matrix instructions a product, the upper triangle) run at 0.62 PFLOP/s of matrix instructions in blocks of 64, 41 us;
+// in blocks of 128, 57 us with four stages and one block a compute unit, more with two, the inner axis split over two to four
+// blocks included.  128 blocks that fill the chip reach 1.0 PFLOP/s (X <- Q X, 2048 x 8192); a large library product 1.2.
 // P Q^T of a BT x BT block over inner tiles [k0, k1), PP and PQ pieces an operand.  Four waves take a quarter each: acc[a][c]
 // is the 16 x 16 block at rows 16 a of P and 16 c of Q; lane l holds Q's row l % 16 and P's rows 4 (l / 16) + r.
 // Operand tiles go from memory to LDS without passing registers, kStages inner tiles of the whole block in a ring, and
@@ -572,6 +580,7 @@ __device__ __forceinline__ int xcd_order(int local, int count) {
   return local < per * 8 ? (local % 8) * per + local / 8 : local;
 }
 
+// 2048 x 8192 bf16, one piece: 52 us, 0.70 PFLOP/s in 128 blocks of four splits; 256 x 5888 fp32: 5.4 us, 46 splits of 10 tiles.
 // S = X X^T: block = (split of the long axis, tile of the upper triangle)
 template <int BT, int PX>
 __global__ void __launch_bounds__(kThreads, BT == 64 ? 3 : 2) ns_gram_kernel(Items L, Scales sc, int step) {
@@ -631,6 +640,7 @@ __global__ void __launch_bounds__(GROUPS * kThreads) ns_gram_sum_kernel(Items L,
   store_symmetric(at<_Float16>(ws, off_sq(I, kS)), I.mp / 32, bi == bj, p0, q0, v, sc.s);
 }
 
+// 2048: 41 us, see Product; 256 (10 blocks): 5.3 us, of which 1.3 until the arguments are there, 2.8 for 8 inner tiles and 1.4 to store.
 // Q = a I + b S + c S S  (a = 0: R, the step less its multiple of one)
 template <int BT>
 __global__ void __launch_bounds__(kThreads, BT == 64 ? 3 : 2) ns_poly_kernel(Items L, Scales sc, NsCoefficients k, int out) {
@@ -696,6 +706,8 @@ __device__ __forceinline__ void put4(const Item& I, int64_t e, const float (&x)[
   *out = v;
 }
 
+// 2048 x 8192 bf16 (128 blocks, three products a value in one and two pieces): 127 us, 1.08 PFLOP/s; 256 x 5888 fp32: 9.2 us, the latency
+// of arguments, eight inner tiles and stores, with 368 blocks in less than two rounds.
 // X <- a X + M X, computed as X^T <- a X^T + X^T M (M symmetric; a = 0: M holds all of the step): block = BT of the long axis x
 // BT of the short; the last one writes the result instead.  PX pieces in, PN out.
 template <typename T, int BT, int PX, int PN, bool LAST>
@@ -1200,13 +1212,18 @@ Item make_item(const NsMatrix& M) {
   // a block of the norm takes at least 4096 values; all matrices together about eight blocks a compute unit
   const int64_t parts = (I.size + kThreads * 16 - 1) / (kThreads * 16), most = kSumsMax / (I.batch < 4 ? I.batch : 4);
   I.nsum = (int)(parts < most ? parts : most);
-  // blocks of 128 x 128 read half as much for a product as blocks of 64 x 64; they need a matrix that gives each of the
-  // 256 compute units one in the products along the long axis
+  // Blocks of 128 x 128 read half as much for a product as blocks of 64 x 64, but need more inner tiles to get going and more
+  // blocks to fill the chip.  Where rows times blocks reach 2^19, us in blocks of 64 and of 128: 2048 x 8192 bf16 1316 and 980, fp32
+  // 2607 and 1854; 2048 x 2048 fp32 803 and 747; 1024 x 16384 bf16 449 and 419; and below it: 4 x 1000 x 771 fp16 297 and 312;
+  // 1024 x 4096 bf16 268 and 283; 512 x 16384 fp32 419 and 431; 256 x 65536 fp32 525 and 561; 100 x 60000 fp32 261 and 320.
+  constexpr int64_t kBigBlocks = 1 << 19;
   const int64_t big = (int64_t)((I.mp + 127) / 128) * ((I.np + 127) / 128) * I.batch;
-  I.bt = I.m > 64 && big >= 192 ? 128 : 64;
-  // among squares only the upper triangle's blocks are computed: 128 x 128 ones where they are two a compute unit
-  const int64_t t128 = (I.mp + 127) / 128;
-  I.bts = t128 * (t128 + 1) / 2 * I.batch >= 512 ? 128 : 64;
+  I.bt = I.m > 64 && I.mp * big >= kBigBlocks ? 128 : 64;
+  // Among squares only the upper triangle's blocks are computed: 128 x 128 ones where they are two a compute unit besides.
+  // 4096 x 4096 bf16 5360 and 4076 us, 4 x 2048 x 2048 bf16 2350 and 2130; 32 x 700 x 700 fp32 1215 and 1257 (2900 x 2900 bf16,
+  // 276 blocks: 2030 and 5000)
+  const int64_t t128 = (I.mp + 127) / 128, tri = t128 * (t128 + 1) / 2 * I.batch;
+  I.bts = tri >= 512 && I.mp * tri >= kBigBlocks ? 128 : 64;
   // splits of the long axis: two blocks a compute unit, at least four inner tiles each
   const int kt = I.np / 32, tiles = tri_tiles(I);
   int64_t chunks = (512 + (int64_t)tiles * I.batch - 1) / ((int64_t)tiles * I.batch);

@@ -29,8 +29,8 @@ def _definition(g, steps=5, eps=1e-7, coefficients=(A, B, C)):
     for _ in range(steps):
         s = x @ x.transpose(-2, -1).contiguous()
         r = b * s + c * (s @ s)
-        top = torch.linalg.matrix_norm(s, ord=2)
-        rn = torch.linalg.matrix_norm(r, ord=2)
+        e = torch.linalg.eigvalsh(s)
+        top, rn = e[..., -1], (b * e + c * e * e).abs().amax(-1)
         step = abs(b) * en * top + abs(c) * (2 * en + em) * top ** 2 + em * rn + U * (abs(a) + rn)
         off = max(abs(a), 1.0) * off + step * fro(x)
         x = a * x + r @ x
@@ -70,6 +70,15 @@ def test_orthogonalize(shape, dtype):
         assert out.dtype == dtype and out.shape == g.shape and torch.equal(g, keep)
         _check(out, *_definition(g))
         assert torch.equal(out, K.orthogonalize(g))              # one summation order
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_blocks_of_128(dtype):
+    """Large enough for the larger blocks: along the long axis (one matrix), among squares too (a stack of four)."""
+    from pde_amd import functional as K
+    g = _matrix((4, 2090, 2049), 5, "low rank", dtype)
+    for out, m in ((K.orthogonalize(g[1]), g[1]), (K.orthogonalize(g)[3], g[3])):
+        _check(out, *_definition(m))
 
 
 def test_singular_values_end_near_one():
@@ -346,15 +355,10 @@ def test_a_vector_of_two_to_the_30():
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
 @pytest.mark.parametrize("shape", [(64, 40), (256, 300), (300, 256), (3, 160, 200), (1, 4096)])
 def test_any_alignment(shape, dtype):
-    """A matrix that starts anywhere gives what the same values at the start of an allocation give."""
+    """A matrix may start anywhere: wide reads where they fit, single ones where not."""
     from pde_amd import functional as K
     flat = torch.empty(_matrix(shape, 0).numel() + 8, device="cuda", dtype=dtype)
-    want = None
     for start in (0, 1, 2, 4, 5):
         g = flat[start:start + flat.numel() - 8].view(shape)
         g.copy_(_matrix(shape, 21, dtype=dtype))
-        out = K.orthogonalize(g)
-        want = out if want is None else want
-        # the sum of squares is made in another order: 2^-24 of the norm at most, times the steps' slopes
-        _check(out, *_definition(g))
-        assert torch.allclose(out.float(), want.float(), rtol=1e-2, atol=1e-4)
+        _check(K.orthogonalize(g), *_definition(g))
