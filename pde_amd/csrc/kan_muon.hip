@@ -118,7 +118,6 @@ template <int PIECES>
 __device__ __forceinline__ int64_t piece_at(int row, int col, int kt) {
   return ((int64_t)(row >> 4) * kt + (col >> 5)) * (512 * PIECES) + ((row & 15) + 16 * ((col & 31) >> 3)) * 8 + (col & 7);
 }
-template <int PIECES>
 __device__ __forceinline__ void store_pieces(_Float16* base, int row, int col, int kt, const float (&v)[4], float scale) {
   f16x4 hi, lo;
 #pragma unroll
@@ -127,9 +126,9 @@ __device__ __forceinline__ void store_pieces(_Float16* base, int row, int col, i
     hi[i] = (_Float16)y;
     lo[i] = (_Float16)(y - (float)hi[i]);
   }
-  _Float16* p = base + piece_at<PIECES>(row, col, kt);
+  _Float16* p = base + piece_at<2>(row, col, kt);
   *reinterpret_cast<f16x4*>(p) = hi;
-  if constexpr (PIECES == 2) *reinterpret_cast<f16x4*>(p + 512) = lo;
+  *reinterpret_cast<f16x4*>(p + 512) = lo;
 }
 // eight values of a row, col % 8 == 0
 template <int PIECES>
@@ -709,8 +708,8 @@ __device__ __forceinline__ void put4(const Item& I, int64_t e, const float (&x)[
 // 2048 x 8192 bf16 (128 blocks, three products a value in one and two pieces): 127 us, 1.08 PFLOP/s; 256 x 5888 fp32: 9.2 us, the latency
 // of arguments, eight inner tiles and stores, with 368 blocks in less than two rounds.
 // X <- a X + M X, computed as X^T <- a X^T + X^T M (M symmetric; a = 0: M holds all of the step): block = BT of the long axis x
-// BT of the short; the last one writes the result instead.  PX pieces in, PN out.
-template <typename T, int BT, int PX, int PN, bool LAST>
+// BT of the short; the last one writes the result instead.  PX pieces in, two out.
+template <typename T, int BT, int PX, bool LAST>
 __global__ void __launch_bounds__(kThreads, BT == 64 ? 3 : 2) ns_update_kernel(Items L, Scales sc, float ca, int square, float scale_m, int from,
                                                                 int step, int next_step, Finish f) {
   extern __shared__ char lds[];
@@ -741,17 +740,11 @@ __global__ void __launch_bounds__(kThreads, BT == 64 ? 3 : 2) ns_update_kernel(I
       for (int r = 0; r < 4; ++r) v[r] += o[r];
     }
     if constexpr (!LAST) {
-      if constexpr (PN == 2) {
-        float p[4];
-        split_pieces(v, next, p);
-        store_packed(at<_Float16>(ws, off_xt(I, from ^ 1)), j, i, kt, p);
-        quad_transpose(p);
-        store_packed(at<_Float16>(ws, 0), i0 + (lane & 15), j0 + 4 * (lane >> 4), I.np / 32, p);
-      } else {
-        store_pieces<1>(at<_Float16>(ws, off_xt(I, from ^ 1)), j, i, kt, v, next);
-        quad_transpose(v);
-        store_pieces<1>(at<_Float16>(ws, 0), i0 + (lane & 15), j0 + 4 * (lane >> 4), I.np / 32, v, next);
-      }
+      float p[4];
+      split_pieces(v, next, p);
+      store_packed(at<_Float16>(ws, off_xt(I, from ^ 1)), j, i, kt, p);
+      quad_transpose(p);
+      store_packed(at<_Float16>(ws, 0), i0 + (lane & 15), j0 + 4 * (lane >> 4), I.np / 32, p);
     } else if (I.tall) {
       if (quads) {
         if (j < I.n && i < I.m) put4<T>(I, b * I.size + (int64_t)j * I.m + i, v, lr, f);
@@ -981,7 +974,7 @@ __global__ void __launch_bounds__(kSmallThreads) ns_small_kernel(Items L, Moment
       for (int j = wave * across4 + jl; j < width; j += kSmallWaves * across4) {
         const float* t = u + j * (mp + 1) + il;
         const float v[4] = {ldexpf(t[0], -e), ldexpf(t[1], -e), ldexpf(t[2], -e), ldexpf(t[3], -e)};
-        store_pieces<2>(xt, j, il, mt, v, kFirst);
+        store_pieces(xt, j, il, mt, v, kFirst);
       }
     }
     if (!apart) __syncthreads();
@@ -990,7 +983,7 @@ __global__ void __launch_bounds__(kSmallThreads) ns_small_kernel(Items L, Moment
         if (apart) {
           const float* t = u + jb * 4 * (mp + 1) + i;
           const float v[4] = {ldexpf(t[0], -e), ldexpf(t[mp + 1], -e), ldexpf(t[2 * (mp + 1)], -e), ldexpf(t[3 * (mp + 1)], -e)};
-          store_pieces<2>(x, i, jb * 4, wt, v, kFirst);
+          store_pieces(x, i, jb * 4, wt, v, kFirst);
         } else {
           _Float16* to = x + piece_at<2>(i, jb * 4, wt);
           const _Float16* from = xt + piece_at<2>(jb * 4, i, mt);        // rows of X^T lie 8 halves apart
@@ -1347,12 +1340,12 @@ struct Steps {
     squares_in<64>(jobs);
     squares_in<128>(jobs);
   }
-  template <int PX, int PN>
+  template <int PX>
   void update(float a, int square, float scale_m, int from, int step, int next) {
     const int blocks = blocks_before(L, count_tiles);
     constexpr int kLds = Product<BT, PX, 2>::kLds;
-    if (next < p.steps) launch(ns_update_kernel<T, BT, PX, PN, false>, blocks, kLds, st, L, sc, a, square, scale_m, from, step, next, fin);
-    else launch(ns_update_kernel<T, BT, PX, PN, true>, blocks, kLds, st, L, sc, a, square, scale_m, from, step, next, fin);
+    if (next < p.steps) launch(ns_update_kernel<T, BT, PX, false>, blocks, kLds, st, L, sc, a, square, scale_m, from, step, next, fin);
+    else launch(ns_update_kernel<T, BT, PX, true>, blocks, kLds, st, L, sc, a, square, scale_m, from, step, next, fin);
   }
 
   // step by step: S = X X^T, R = b S + c S S, X <- a X + R X
@@ -1360,22 +1353,21 @@ struct Steps {
     for (int k = 0; k < p.steps; ++k) {
       gram<2>(k);
       poly(0.0f, kQ);
-      update<2, 2>(p.k.a, kQ, sc.q, k & 1, k, k + 1);
+      update<2>(p.k.a, kQ, sc.q, k & 1, k, k + 1);
     }
   }
 
   // Up to three steps composed in the square matrices, then one product with X: with Q = a I + b S + c S S the step takes X to
   // Q X and S to Q S Q, and all of these commute.  Three products along the long axis for five steps instead of ten.
   // Rounding errors of S in the small singular directions grow by a^2 a step, so three steps cost about a factor 4 in
-  // accuracy over fp32, far below the 2^-9 or 2^-12 of a 16-bit result, and a new S is formed after them.
-  // PN: pieces that X keeps between.  In bf16 one: 2^-12 of each value, of random sign, which the remaining steps multiply by at
-  // most a each in the smallest directions only, against the result's own 2^-9.
-  template <int PN>
+  // accuracy over fp32, far below the 2^-9 or 2^-12 of a 16-bit result, and a new S is formed after them.  X keeps two pieces
+  // between the segments: one (2^-12 of each value) would move one bf16 result in twenty to its neighbour.  2048 x 8192 bf16: 1110 us,
+  // 1007 with one.
   void composed() {
     for (int k = 0, part = 0; k < p.steps; ++part) {
       const int start = k, n = p.steps - k < 3 ? p.steps - k : 3;
       if (part == 0) gram<1>(0);
-      else gram<PN>(start);
+      else gram<2>(start);
       int cur = kP0;                                     // the composed steps so far; the first one is its own Q
       float scale = sc.q;
       for (int i = 0; i < n; ++i, ++k) {
@@ -1396,8 +1388,8 @@ struct Steps {
           squares(next);
         }
       }
-      if (part == 0) update<1, PN>(0.0f, cur, scale, 0, 0, k);
-      else update<PN, PN>(0.0f, cur, scale, part & 1, start, k);
+      if (part == 0) update<1>(0.0f, cur, scale, 0, 0, k);
+      else update<2>(0.0f, cur, scale, part & 1, start, k);
     }
   }
 };
@@ -1407,7 +1399,7 @@ void run_products(Items& L, const NsPlan& p, const Scales& sc, const Finish& fin
   if (!L.n) return;
   Steps<T, BT> s{L, p, sc, fin, st};
   if constexpr (sizeof(T) == 4) s.plain();
-  else s.template composed<__is_same(T, __bf16) ? 1 : 2>();
+  else s.composed();
 }
 
 template <typename T>

@@ -1,0 +1,40 @@
+"""Newton-Schulz orthogonalisation and the Muon step where few bits, large values, long lists or shared memory could tell."""
+import pytest
+import torch
+
+from test_gpu_muon import U, _definition, _matrix
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", [(160, 1000), (1000, 160), (2, 200, 300), (2090, 2300)])
+def test_sixteen_bit_results_are_rounded_once(shape, dtype):
+    """Whatever is held between the steps, a 16-bit result is the 64-bit one rounded, but where fp32's error carries a value over
+    the border between two roundings.
+
+    An error d of a value whose neighbours lie `ulp` apart changes its rounding with probability |d| / ulp, by ulp: the squares
+    of the changes add up to sum |d| ulp + d^2 <= |d| |ulp| + |d|^2 in the mean, and twice that is more than four standard
+    deviations away (dozens of changes at least).  The slopes of (1.5, -0.5, 0) leave `off` at a few 2^-24.  Where steps are
+    composed, their products carry the multiple of one through the sums: five products of at most 3 m / 32 additions each, of
+    which each may be 2 u of the result off: m u."""
+    from pde_amd import functional as K
+    for steps in (4, 5):
+        g = _matrix(shape, steps, "noise", dtype)
+        want, off = _definition(g, steps, 1e-7, (1.5, -0.5, 0.0))
+        out = K.orthogonalize(g, steps=steps, coefficients=(1.5, -0.5, 0.0))
+        fro = lambda t: t.square().sum((-2, -1)).sqrt()
+        off = off + min(shape[-2:]) * U * fro(want)
+        d = fro(out.double() - want.to(dtype).double())
+        tol = (2 * (off * torch.finfo(dtype).eps * fro(want) + off ** 2)).sqrt()
+        assert bool((d <= tol).all()), (steps, float((d / fro(want)).max()), float((tol / fro(want)).max()))
+
+
+@pytest.mark.parametrize("shape,dtype", [((2048, 8192), torch.bfloat16), ((4, 1000, 771), torch.float16), ((256, 5888), torch.float32),
+                                         ((2048, 2048), torch.float32)])
+def test_the_same_bits_every_time(shape, dtype):
+    from pde_amd import functional as K
+    g = _matrix(shape, 31, "low rank", dtype)
+    first = K.orthogonalize(g)
+    for _ in range(4):
+        assert torch.equal(K.orthogonalize(g), first)
