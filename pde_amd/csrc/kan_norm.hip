@@ -536,85 +536,99 @@ struct GridThread {
   }
 };
 
-// Partial statistics of a chunk: per channel the sums of x - k and (x - k)^2 with k the chunk's first value of that
-// channel.  As k is one of the values, the squared deviations are at least about (k - mean)^2, so subtracting the
-// square of the sum loses no more than eps * (positions a chunk) relative, however far the values lie from zero.
+// sum over a wave's 64 lanes, in every lane
+__device__ __forceinline__ double wave_sum64(double v) {
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d);
+  return v;
+}
+// Partial statistics of a chunk: per channel the sums of x - k and (x - k)^2 with k the chunk's first value of that channel,
+// in 64 bits.  k may stand apart from the rest (the boundary value of a field): the sum of squares then loses up to n (k -
+// mean)^2 / M2 <= n, the chunk's positions, to the square of the sum, 24 bits of 53 at most.  In 32 bits the sums of 2^18 positions
+// near 10^4 behind a first one of 0 were 13 % off.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kThreads) norm_grid_stats_kernel(GridMap m, const T* __restrict__ x,
-                                                                   float2* __restrict__ part) {
-  extern __shared__ float chan[];                     // [2][C]: mean and sum of squared deviations of each channel
-  __shared__ float red[2][kThreads][VEC + 1];
+                                                                   double2* __restrict__ part) {
+  extern __shared__ double chan64[];                  // [2][C]: mean and sum of squared deviations of each channel
+  __shared__ double red[kThreads][VEC + 1];
   const GridThread<VEC> t(m, blockIdx.x);
   const T* base = x + t.sample * m.s * m.C;
-  const float cnt = (float)(t.row1 - t.row0);
+  const double cnt = (double)(t.row1 - t.row0);
   for (int tile = 0; tile < t.nv; tile += t.txn) {
     const int vec = tile + t.tx;
     const bool on = t.ty < t.tyn && vec < t.nv;
-    float k[VEC], s1[VEC], s2[VEC];
+    double k[VEC], s1[VEC], s2[VEC];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) k[i] = s1[i] = s2[i] = 0.0f;
+    for (int i = 0; i < VEC; ++i) k[i] = s1[i] = s2[i] = 0.0;
     if (on) {
-      load_vec<T, VEC>(base + t.row0 * m.C + vec * VEC, k);
+      float v[VEC];
+      load_vec<T, VEC>(base + t.row0 * m.C + vec * VEC, v);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) k[i] = v[i];
 #pragma unroll 8
       for (int64_t row = t.row0 + t.ty; row < t.row1; row += t.tyn) {
-        float v[VEC];
         load_vec<T, VEC>(base + row * m.C + vec * VEC, v);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-          const float d = v[i] - k[i];
+          const double d = v[i] - k[i];
           s1[i] += d;
-          s2[i] = fmaf(d, d, s2[i]);
+          s2[i] = fma(d, d, s2[i]);
         }
       }
     }
-    __syncthreads();
+    // the row slots' sums, one kind after the other
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) { red[0][threadIdx.x][i] = s1[i]; red[1][threadIdx.x][i] = s2[i]; }
-    __syncthreads();
+    for (int which = 0; which < 2; ++which) {
+      double(&sum)[VEC] = which ? s2 : s1;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) red[threadIdx.x][i] = sum[i];
+      __syncthreads();
+      if (on && t.ty == 0)
+        for (int j = 1; j < t.tyn; ++j)
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) sum[i] += red[threadIdx.x + j * t.txn][i];
+    }
     if (on && t.ty == 0) {
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        for (int j = 1; j < t.tyn; ++j) {
-          s1[i] += red[0][threadIdx.x + j * t.txn][i];
-          s2[i] += red[1][threadIdx.x + j * t.txn][i];
-        }
-        const float d = s1[i] / cnt;
-        chan[vec * VEC + i] = k[i] + d;
-        chan[m.C + vec * VEC + i] = fmaxf(fmaf(-d, s1[i], s2[i]), 0.0f);
+        const double d = s1[i] / cnt;
+        chan64[vec * VEC + i] = k[i] + d;
+        chan64[m.C + vec * VEC + i] = fmax(0.0, fma(-d, s1[i], s2[i]));
       }
     }
   }
   __syncthreads();
   const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
   for (int g = wave; g < m.G; g += kThreads / 64) {
-    float s = 0.0f, q = 0.0f;
-    for (int c = lane; c < m.cpg; c += 64) s += chan[g * m.cpg + c];
-    const float mean = wave_sum(s) / (float)m.cpg;
+    double s = 0.0, q = 0.0;
+    for (int c = lane; c < m.cpg; c += 64) s += chan64[g * m.cpg + c];
+    const double mean = wave_sum64(s) / m.cpg;
     for (int c = lane; c < m.cpg; c += 64) {
-      const float d = chan[g * m.cpg + c] - mean;
-      q += fmaf(cnt * d, d, chan[m.C + g * m.cpg + c]);
+      const double d = chan64[g * m.cpg + c] - mean;
+      q += fma(cnt * d, d, chan64[m.C + g * m.cpg + c]);
     }
-    q = wave_sum(q);
-    if (lane == 0) part[(int64_t)blockIdx.x * m.G + g] = make_float2(mean, q);
+    q = wave_sum64(q);
+    if (lane == 0) part[(int64_t)blockIdx.x * m.G + g] = make_double2(mean, q);
   }
 }
 
-__device__ __forceinline__ float chunk_rows(const GridMap& m, int chunk) {
+__device__ __forceinline__ double chunk_rows(const GridMap& m, int chunk) {
   const int64_t left = m.s - chunk * m.rows;
-  return (float)(left < m.rows ? left : m.rows);
+  return (double)(left < m.rows ? left : m.rows);
 }
 
 // Sums over a sample's chunks of two numbers a (chunk, group), part [chunks][G], each group's by 256 / G threads (loads of
 // all chunks in flight at once, neighbouring threads on neighbouring groups): term(chunk, value, first chunk's value)
-// adds to s.  take(g, s, first) gets the totals, one thread a group.
-template <typename Term, typename Take>
-__device__ __forceinline__ void merge_chunks(const GridMap& m, const float2* __restrict__ part, float2 (*red), Term term,
-                                             Take take) {
+// adds to s.  take(g, s, first) gets the totals, one thread a group.  Pair: double2 or float2.
+template <typename Pair, typename Term, typename Take>
+__device__ __forceinline__ void merge_chunks(const GridMap& m, const Pair* __restrict__ part, Pair (*red), Term term, Take take) {
   const int gw = m.G < kThreads ? m.G : kThreads, per = kThreads / gw;
   const int gl = threadIdx.x % gw, sub = threadIdx.x / gw;
   for (int g0 = 0; g0 < m.G; g0 += gw) {
     const int g = g0 + gl;
-    float2 s = make_float2(0.0f, 0.0f), first = s;
+    Pair s, first;
+    s.x = s.y = first.x = first.y = 0;
     if (g < m.G && sub < per) {
       first = part[g];
 #pragma unroll 8
@@ -625,7 +639,7 @@ __device__ __forceinline__ void merge_chunks(const GridMap& m, const float2* __r
     __syncthreads();
     if (g < m.G && sub == 0) {
       for (int i = 1; i < per; ++i) {
-        const float2 o = red[gl + i * gw];
+        const Pair o = red[gl + i * gw];
         s.x += o.x;
         s.y += o.y;
       }
@@ -638,10 +652,10 @@ template <typename T, int VEC>
 __global__ void __launch_bounds__(kThreads) norm_grid_apply_kernel(GridMap m, const T* __restrict__ x,
                                                                    const float* __restrict__ w,
                                                                    const float* __restrict__ b, float eps, int act,
-                                                                   const float2* __restrict__ part, T* __restrict__ y,
+                                                                   const double2* __restrict__ part, T* __restrict__ y,
                                                                    float2* stats) {
   extern __shared__ float chan[];                     // [2][G]
-  __shared__ float2 red[kThreads];
+  __shared__ double2 red[kThreads];
   float *mu = chan, *rs = chan + m.G;
   const GridThread<VEC> t(m, blockIdx.x);
   const int64_t base = t.sample * m.s * m.C;
@@ -655,17 +669,17 @@ __global__ void __launch_bounds__(kThreads) norm_grid_apply_kernel(GridMap m, co
     if (first_on && row < t.row1) ahead[j] = *reinterpret_cast<const Raw*>(x + base + row * m.C + t.tx * VEC);
   }
   // mean and r of the sample's groups, about the first chunk's mean (one of the means: see the stats kernel)
-  const float total = (float)m.s, width = (float)m.cpg;
+  const double total = (double)m.s, width = (double)m.cpg;
   merge_chunks(m, part + t.sample * m.chunks * m.G, red,
-               [&](int k, float2 v, float2 first, float2& s) {
-                 const float cnt = chunk_rows(m, k), d = v.x - first.x;
-                 s.x = fmaf(cnt, d, s.x);
-                 s.y += fmaf(cnt * width * d, d, v.y);
+               [&](int k, double2 v, double2 first, double2& s) {
+                 const double cnt = chunk_rows(m, k), d = v.x - first.x;
+                 s.x = fma(cnt, d, s.x);
+                 s.y += fma(cnt * width * d, d, v.y);
                },
-               [&](int g, float2 s, float2 first) {
-                 const float d = s.x / total, var = fmaxf(fmaf(-d * width, s.x, s.y), 0.0f) / (total * width);
-                 mu[g] = first.x + d;
-                 rs[g] = rsqrtf(var + eps);
+               [&](int g, double2 s, double2 first) {
+                 const double d = s.x / total, var = fmax(0.0, fma(-d * width, s.x, s.y)) / (total * width);
+                 mu[g] = (float)(first.x + d);
+                 rs[g] = rsqrtf((float)(var + (double)eps));
                  if (t.chunk == 0 && stats) stats[t.sample * m.G + g] = make_float2(mu[g], rs[g]);
                });
   __syncthreads();
@@ -1011,9 +1025,9 @@ void jet_any(const NormShape& p, int n_dir, const float* x, const float* gy, con
 
 template <typename T, int VEC>
 void grid_forward(const GridMap& m, const T* x, const float* w, const float* b, float eps, int act, T* y, float2* stats,
-                  float2* part, hipStream_t st) {
+                  double2* part, hipStream_t st) {
   const unsigned blocks = (unsigned)(m.n * m.chunks);
-  const size_t lds = 2 * (size_t)m.C * sizeof(float), lds_g = 2 * (size_t)m.G * sizeof(float);
+  const size_t lds = 2 * (size_t)m.C * sizeof(double), lds_g = 2 * (size_t)m.G * sizeof(float);
   ensure_dynamic_lds((const void*)norm_grid_stats_kernel<T, VEC>, lds + kStaticLds);
   ensure_dynamic_lds((const void*)norm_grid_apply_kernel<T, VEC>, lds_g + kStaticLds);
   hipLaunchKernelGGL((norm_grid_stats_kernel<T, VEC>), dim3(blocks), dim3(kThreads), lds, st, m, x, part);
@@ -1062,7 +1076,7 @@ size_t norm_ws_bytes(const NormShape& p, bool backward) {
   }
   const GridMap m = grid_map(p.n, p.s, p.C, p.G);
   const size_t blocks = (size_t)m.n * m.chunks;
-  return blocks * m.G * sizeof(float2) + (backward ? blocks * 2 * m.C * sizeof(float) : 0);
+  return backward ? blocks * m.G * sizeof(float2) + blocks * 2 * m.C * sizeof(float) : blocks * m.G * sizeof(double2);
 }
 
 bool norm_wants_stats(const NormShape& p) { return !rows_kernel_takes(p.s, p.C / p.G); }
@@ -1084,7 +1098,7 @@ void launch_norm_forward(int dtype, const NormShape& p, const void* x, const flo
   }
   const GridMap m = grid_map(p.n, p.s, p.C, p.G);
   const int vec = vec_width(dtype, p.C, x, y, nullptr);
-  float2* part = static_cast<float2*>(ws);
+  double2* part = static_cast<double2*>(ws);
   float2* s2 = reinterpret_cast<float2*>(stats);
   PDEKAN_GRID((grid_forward<T, V>(m, (const T*)x, w, b, eps, act, (T*)y, s2, part, st)));
 }

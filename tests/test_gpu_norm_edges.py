@@ -1,0 +1,52 @@
+"""The norm with an activation where few bits, long sums, wide rows or dependent parameters could tell."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+
+
+def _mean(t):
+    """Over the first dimension, in stages of at most 1024 terms, each of many results: no reduction is split over blocks."""
+    n = t.size(0)
+    while t.size(0) > 1:
+        step = min(1024, t.size(0))
+        t = torch.cat([t, t.new_zeros(-t.size(0) % step, *t.shape[1:])]).view(-1, step, *t.shape[1:]).sum(1)
+    return t[0] / n
+
+
+def _statistics(x, groups, eps=1e-5):
+    """The forward's own (mean, r) of each sample and group."""
+    from pde_amd import functional as K
+    _, stats = K._group_norm_forward(x, None, None, groups, eps, K.ACT_IDENTITY, True)
+    return stats.view(x.size(0), groups, 2)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,s,c,groups,first,rest", [
+    (64, 1 << 21, 8, 2, 0.0, 1e3), (64, 1 << 21, 8, 2, 0.0, 1e4), (512, 1 << 14, 8, 2, 0.0, 1e4), (512, 1 << 18, 4, 1, 0.0, 1e4),
+    (512, 4096, 1024, 8, 30.0, 0.0), (512, 4096, 1024, 8, 1000.0, 0.0), (512, 4096, 257, 1, 1000.0, 0.0), (1, 1 << 20, 6, 3, 0.0, 1e4),
+    (3, 5000, 90, 6, -1e4, 1e4), (600, 100, 24, 3, 1e4, 0.0)])
+def test_a_first_position_far_from_the_rest(n, s, c, groups, first, rest, dtype):
+    """Statistics of samples whose first position (a boundary value, say) stands apart, over chunks of any length.
+
+    The sums are 64-bit: what is left are the roundings of the mean (2^-24) and of r (the variance's two and 2^-23 of the reciprocal
+    root: 3 2^-24)."""
+    gen = torch.Generator(device="cuda").manual_seed(n + s)
+    x = torch.empty(n, s, c, device="cuda", dtype=dtype)
+    for part in x.split(max(1, (1 << 26) // (s * c))):
+        part.copy_(rest + torch.randn(part.shape, device="cuda", generator=gen))
+    x[:, 0] = first
+    got = _statistics(x, groups).double()
+    for i in {0, n // 2, n - 1}:
+        v = x[i].double().view(s, groups, c // groups)
+        mean = _mean(v).mean(1)
+        var = _mean((v - mean[:, None]).square()).mean(1)
+        r = 1 / (var + 1e-5).sqrt()
+        spread = _mean((v - mean[:, None]).abs()).mean(1)
+        assert bool(((got[i, :, 0] - mean).abs() <= 1.1 * U * mean.abs() + 1e-9 * spread).all())
+        rel = (got[i, :, 1] / r - 1).abs()
+        assert bool((rel <= 3.2 * U).all()), (float(rel.max()), float(var.min()))
+    del x
+    torch.cuda.empty_cache()
