@@ -204,7 +204,7 @@ int pdekan_deeponet_step(const PdekanNet* nets, const float* u1, const float* u2
  * pdekan_group_norm_stats_floats is not 0 (NULL: not wanted) and read by the backward.  Backward: gx, and gweight / gbias
  * (fp32, overwritten) summed over all samples in a fixed order; gweight and gbias may be NULL.
  * channels <= 8192.  ws: pdekan_group_norm_workspace_bytes (0 for some shapes: ws may be NULL then); 256-byte aligned.
- * A NaN or infinity stays within its group of its sample, and in gweight / gbias within the channels of its group. */
+ * The group of a sample that holds a NaN or an infinity becomes NaN, and in gweight / gbias the channels of its group. */
 size_t pdekan_group_norm_workspace_bytes(int64_t n, int64_t s, int32_t channels, int32_t groups, int32_t backward);
 int64_t pdekan_group_norm_stats_floats(int64_t n, int64_t s, int32_t channels, int32_t groups);
 int pdekan_group_norm_forward(const void* x, int32_t dtype, int64_t n, int64_t s, int32_t channels, int32_t groups,

@@ -542,6 +542,9 @@ __device__ __forceinline__ double wave_sum64(double v) {
   for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d);
   return v;
 }
+// not below zero; a NaN stays one
+__device__ __forceinline__ double not_negative(double v) { return v < 0.0 ? 0.0 : v; }
+
 // Partial statistics of a chunk: per channel the sums of x - k and (x - k)^2 with k the chunk's first value of that channel,
 // in 64 bits.  k may stand apart from the rest (the boundary value of a field): the sum of squares then loses up to n (k -
 // mean)^2 / M2 <= n, the chunk's positions, to the square of the sum, 24 bits of 53 at most.  In 32 bits the sums of 2^18 positions
@@ -594,7 +597,7 @@ __global__ void __launch_bounds__(kThreads) norm_grid_stats_kernel(GridMap m, co
       for (int i = 0; i < VEC; ++i) {
         const double d = s1[i] / cnt;
         chan64[vec * VEC + i] = k[i] + d;
-        chan64[m.C + vec * VEC + i] = fmax(0.0, fma(-d, s1[i], s2[i]));
+        chan64[m.C + vec * VEC + i] = not_negative(fma(-d, s1[i], s2[i]));
       }
     }
   }
@@ -677,7 +680,7 @@ __global__ void __launch_bounds__(kThreads) norm_grid_apply_kernel(GridMap m, co
                  s.y += fma(cnt * width * d, d, v.y);
                },
                [&](int g, double2 s, double2 first) {
-                 const double d = s.x / total, var = fmax(0.0, fma(-d * width, s.x, s.y)) / (total * width);
+                 const double d = s.x / total, var = not_negative(fma(-d * width, s.x, s.y)) / (total * width);
                  mu[g] = (float)(first.x + d);
                  rs[g] = rsqrtf((float)(var + (double)eps));
                  if (t.chunk == 0 && stats) stats[t.sample * m.G + g] = make_float2(mu[g], rs[g]);

@@ -2,6 +2,8 @@
 import pytest
 import torch
 
+from test_gpu_norm import _kind
+
 pytestmark = pytest.mark.gpu
 
 U = 2.0 ** -24
@@ -50,3 +52,22 @@ def test_a_first_position_far_from_the_rest(n, s, c, groups, first, rest, dtype)
         assert bool((rel <= 3.2 * U).all()), (float(rel.max()), float(var.min()))
     del x
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("act", ["identity", "silu", "tanh"])
+@pytest.mark.parametrize("shape", [(6, 32), (3, 20, 32), (3, 500, 32), (2, 20000, 32), (600, 70, 32)])
+def test_all_of_a_non_finite_group_is_nan(shape, act):
+    """Its mean is not finite, so nothing of the group has a value: no saturated activation stands in for one."""
+    from pde_amd import functional as K
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    x = torch.randn(*shape, device="cuda", generator=gen)
+    for place in (0, -1):
+        for bad in (float("nan"), float("inf"), -float("inf")):
+            z = x.clone()
+            z[(1, *[place] * (len(shape) - 2), 9)] = bad
+            z.requires_grad_()
+            y = K.group_norm_act(z, 4, None, None, 1e-5, _kind(act))
+            gx, = torch.autograd.grad(y, z, torch.ones_like(y))
+            for t in (y, gx):
+                assert bool(t[1, ..., 8:16].isnan().all())
+                assert bool(t[0].isfinite().all()) and bool(t[1, ..., :8].isfinite().all()) and bool(t[1, ..., 16:].isfinite().all())
