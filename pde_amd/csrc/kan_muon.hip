@@ -792,13 +792,6 @@ __device__ __host__ inline int64_t small_bytes(const Item& I) {
   return I.path == kSingle ? 256 : (off_exponents(I) + I.strips * 4 + 255) / 256 * 256;
 }
 
-template <int kCtrl>
-__device__ __forceinline__ double dpp_move64(double v) {
-  const uint64_t u = __builtin_bit_cast(uint64_t, v);
-  const unsigned lo = __builtin_amdgcn_update_dpp(0u, (unsigned)u, kCtrl, 0xf, 0xf, false);
-  const unsigned hi = __builtin_amdgcn_update_dpp(0u, (unsigned)(u >> 32), kCtrl, 0xf, 0xf, false);
-  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
-}
 // sum and maximum (not of NaNs) over the block, in every thread; red: a double and a float a wave
 struct SumMax { double sum; float max; };
 __device__ __forceinline__ SumMax block_sum_max(double s, float v, double* red, float* redf) {

@@ -536,11 +536,17 @@ struct GridThread {
   }
 };
 
-// sum over a wave's 64 lanes, in every lane
-__device__ __forceinline__ double wave_sum64(double v) {
+// the sums of a column of row slots (threads of one vector of channels), in the first of them
+template <int VEC>
+__device__ __forceinline__ void sum_row_slots(const GridThread<VEC>& t, bool on, double (&sum)[VEC], double (*red)[VEC + 1]) {
+  __syncthreads();
 #pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d);
-  return v;
+  for (int i = 0; i < VEC; ++i) red[threadIdx.x][i] = sum[i];
+  __syncthreads();
+  if (on && t.ty == 0)
+    for (int j = 1; j < t.tyn; ++j)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) sum[i] += red[threadIdx.x + j * t.txn][i];
 }
 // not below zero; a NaN stays one
 __device__ __forceinline__ double not_negative(double v) { return v < 0.0 ? 0.0 : v; }
@@ -579,19 +585,8 @@ __global__ void __launch_bounds__(kThreads) norm_grid_stats_kernel(GridMap m, co
         }
       }
     }
-    // the row slots' sums, one kind after the other
-#pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      double(&sum)[VEC] = which ? s2 : s1;
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) red[threadIdx.x][i] = sum[i];
-      __syncthreads();
-      if (on && t.ty == 0)
-        for (int j = 1; j < t.tyn; ++j)
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) sum[i] += red[threadIdx.x + j * t.txn][i];
-    }
+    sum_row_slots<VEC>(t, on, s1, red);
+    sum_row_slots<VEC>(t, on, s2, red);
     if (on && t.ty == 0) {
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
@@ -623,15 +618,16 @@ __device__ __forceinline__ double chunk_rows(const GridMap& m, int chunk) {
 
 // Sums over a sample's chunks of two numbers a (chunk, group), part [chunks][G], each group's by 256 / G threads (loads of
 // all chunks in flight at once, neighbouring threads on neighbouring groups): term(chunk, value, first chunk's value)
-// adds to s.  take(g, s, first) gets the totals, one thread a group.  Pair: double2 or float2.
+// adds to s.  take(g, s, first) gets the totals, one thread a group.  Pair: double2 or float2; added up in 64 bits.
 template <typename Pair, typename Term, typename Take>
-__device__ __forceinline__ void merge_chunks(const GridMap& m, const Pair* __restrict__ part, Pair (*red), Term term, Take take) {
+__device__ __forceinline__ void merge_chunks(const GridMap& m, const Pair* __restrict__ part, double2 (*red), Term term, Take take) {
   const int gw = m.G < kThreads ? m.G : kThreads, per = kThreads / gw;
   const int gl = threadIdx.x % gw, sub = threadIdx.x / gw;
   for (int g0 = 0; g0 < m.G; g0 += gw) {
     const int g = g0 + gl;
-    Pair s, first;
-    s.x = s.y = first.x = first.y = 0;
+    double2 s = make_double2(0.0, 0.0);
+    Pair first;
+    first.x = first.y = 0;
     if (g < m.G && sub < per) {
       first = part[g];
 #pragma unroll 8
@@ -642,7 +638,7 @@ __device__ __forceinline__ void merge_chunks(const GridMap& m, const Pair* __res
     __syncthreads();
     if (g < m.G && sub == 0) {
       for (int i = 1; i < per; ++i) {
-        const Pair o = red[gl + i * gw];
+        const double2 o = red[gl + i * gw];
         s.x += o.x;
         s.y += o.y;
       }
@@ -723,7 +719,9 @@ __global__ void __launch_bounds__(kThreads) norm_grid_apply_kernel(GridMap m, co
 }
 
 // Backward, launch 1: per chunk and channel the sums of p = gy f' and of p z (part_c [n * chunks][2][C], p z first),
-// and per group the sums of w p and w p z (part_g [n * chunks][G])
+// and per group the sums of w p and w p z (part_g [n * chunks][G]).  A thread adds 32 rows in fp32, and what they come to in 64
+// bits: a chunk may have any number of rows.
+constexpr int kChain = 32;
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kThreads) norm_grid_sums_kernel(GridMap m, const T* __restrict__ x,
                                                                   const T* __restrict__ gy, const float* __restrict__ w,
@@ -731,14 +729,15 @@ __global__ void __launch_bounds__(kThreads) norm_grid_sums_kernel(GridMap m, con
                                                                   const float2* __restrict__ stats,
                                                                   float* __restrict__ part_c, float2* __restrict__ part_g) {
   extern __shared__ float chan[];                     // [2][C]: sums of w p z, w p
-  __shared__ float red[2][kThreads][VEC + 1];
+  __shared__ double red[kThreads][VEC + 1];
   const GridThread<VEC> t(m, blockIdx.x);
   const int64_t base = t.sample * m.s * m.C;
   float* mine = part_c + (int64_t)blockIdx.x * 2 * m.C;
   for (int tile = 0; tile < t.nv; tile += t.txn) {
     const int vec = tile + t.tx;
     const bool on = t.ty < t.tyn && vec < t.nv;
-    float s1[VEC], s2[VEC], wv[VEC];
+    double s1[VEC], s2[VEC];
+    float wv[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) s1[i] = s2[i] = wv[i] = 0.0f;
     if (on) {
@@ -754,53 +753,59 @@ __global__ void __launch_bounds__(kThreads) norm_grid_sums_kernel(GridMap m, con
       }
       by_activation(act, [&](auto kind) {
         constexpr int ACT = decltype(kind)::value;
+        for (int64_t row = t.row0 + t.ty; row < t.row1;) {
+          const int64_t left = (t.row1 - row + t.tyn - 1) / t.tyn;
+          const int n = left < kChain ? (int)left : kChain;
+          float c1[VEC], c2[VEC];
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) c1[i] = c2[i] = 0.0f;
 #pragma unroll 2
-        for (int64_t row = t.row0 + t.ty; row < t.row1; row += t.tyn) {
-          float v[VEC], g[VEC];
-          load_vec<T, VEC>(x + base + row * m.C + vec * VEC, v);
-          load_vec<T, VEC>(gy + base + row * m.C + vec * VEC, g);
+          for (int j = 0; j < n; ++j, row += t.tyn) {
+            float v[VEC], g[VEC];
+            load_vec<T, VEC>(x + base + row * m.C + vec * VEC, v);
+            load_vec<T, VEC>(gy + base + row * m.C + vec * VEC, g);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+              const float z = (v[i] - mean[i]) * rs[i];
+              float f[2];
+              activation<ACT, 1>(fmaf(z, wv[i], bv[i]), f);
+              const float p = g[i] * f[1];
+              c1[i] += p;
+              c2[i] = fmaf(p, z, c2[i]);
+            }
+          }
 #pragma unroll
           for (int i = 0; i < VEC; ++i) {
-            const float z = (v[i] - mean[i]) * rs[i];
-            float f[2];
-            activation<ACT, 1>(fmaf(z, wv[i], bv[i]), f);
-            const float p = g[i] * f[1];
-            s1[i] += p;
-            s2[i] = fmaf(p, z, s2[i]);
+            s1[i] += c1[i];
+            s2[i] += c2[i];
           }
         }
       });
     }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) { red[0][threadIdx.x][i] = s1[i]; red[1][threadIdx.x][i] = s2[i]; }
-    __syncthreads();
+    sum_row_slots<VEC>(t, on, s1, red);
+    sum_row_slots<VEC>(t, on, s2, red);
     if (on && t.ty == 0) {
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        for (int j = 1; j < t.tyn; ++j) {
-          s1[i] += red[0][threadIdx.x + j * t.txn][i];
-          s2[i] += red[1][threadIdx.x + j * t.txn][i];
-        }
         const int c = vec * VEC + i;
-        mine[c] = s2[i];
-        mine[m.C + c] = s1[i];
-        chan[c] = wv[i] * s2[i];
-        chan[m.C + c] = wv[i] * s1[i];
+        mine[c] = (float)s2[i];
+        mine[m.C + c] = (float)s1[i];
+        chan[c] = wv[i] * (float)s2[i];
+        chan[m.C + c] = wv[i] * (float)s1[i];
       }
     }
   }
   __syncthreads();
   const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
   for (int g = wave; g < m.G; g += kThreads / 64) {
-    float a = 0.0f, q = 0.0f;
+    double a = 0.0, q = 0.0;
     for (int c = lane; c < m.cpg; c += 64) {
       q += chan[g * m.cpg + c];
       a += chan[m.C + g * m.cpg + c];
     }
-    a = wave_sum(a);
-    q = wave_sum(q);
-    if (lane == 0) part_g[(int64_t)blockIdx.x * m.G + g] = make_float2(a, q);
+    a = wave_sum64(a);
+    q = wave_sum64(q);
+    if (lane == 0) part_g[(int64_t)blockIdx.x * m.G + g] = make_float2((float)a, (float)q);
   }
 }
 
@@ -814,7 +819,7 @@ __global__ void __launch_bounds__(kThreads) norm_grid_grad_kernel(GridMap m, con
                                                                   const float2* __restrict__ part_g, T* __restrict__ gx,
                                                                   float* gw, float* gb, int finish_blocks) {
   extern __shared__ float chan[];                     // [2][G]
-  __shared__ float2 red[kThreads];
+  __shared__ double2 red[kThreads];
   if ((int)blockIdx.x < finish_blocks) {
     finish_columns<kGridFinishCols, kThreads>(blockIdx.x, part_c, m.n * m.chunks, m.C, gw, gb);
     return;
@@ -834,8 +839,8 @@ __global__ void __launch_bounds__(kThreads) norm_grid_grad_kernel(GridMap m, con
   }
   const float inv = 1.0f / ((float)m.s * (float)m.cpg);
   merge_chunks(m, part_g + t.sample * m.chunks * m.G, red,
-               [&](int, float2 v, float2, float2& s) { s.x += v.x; s.y += v.y; },
-               [&](int g, float2 s, float2) { chan[g] = s.x * inv; chan[m.G + g] = s.y * inv; });
+               [&](int, float2 v, float2, double2& s) { s.x += v.x; s.y += v.y; },
+               [&](int g, double2 s, float2) { chan[g] = (float)s.x * inv; chan[m.G + g] = (float)s.y * inv; });
   __syncthreads();
   for (int tile = 0; tile < t.nv; tile += t.txn) {
     const int vec = tile + t.tx;

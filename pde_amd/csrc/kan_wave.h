@@ -5,6 +5,8 @@
 #pragma once
 #include <hip/hip_runtime.h>
 
+#include <cstdint>
+
 namespace pdekan {
 
 // v + (the same value 32 / 16 lanes away), in every lane
@@ -34,6 +36,29 @@ __device__ __forceinline__ float wave_sum(float v) {
   v += dpp_move<0x140>(v);
   v = sum_xor16(v);
   return sum_xor32(v);
+}
+
+template <int kCtrl>
+__device__ __forceinline__ double dpp_move64(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const unsigned lo = __builtin_amdgcn_update_dpp(0u, (unsigned)u, kCtrl, 0xf, 0xf, false);
+  const unsigned hi = __builtin_amdgcn_update_dpp(0u, (unsigned)(u >> 32), kCtrl, 0xf, 0xf, false);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// the same sum of 64-bit values
+__device__ __forceinline__ double wave_sum64(double v) {
+  v += dpp_move64<0xB1>(v);
+  v += dpp_move64<0x4E>(v);
+  v += dpp_move64<0x141>(v);
+  v += dpp_move64<0x140>(v);
+  uint64_t u = __builtin_bit_cast(uint64_t, v);
+  auto lo = __builtin_amdgcn_permlane16_swap((unsigned)u, (unsigned)u, false, false);
+  auto hi = __builtin_amdgcn_permlane16_swap((unsigned)(u >> 32), (unsigned)(u >> 32), false, false);
+  v = __builtin_bit_cast(double, (uint64_t)hi[0] << 32 | lo[0]) + __builtin_bit_cast(double, (uint64_t)hi[1] << 32 | lo[1]);
+  u = __builtin_bit_cast(uint64_t, v);
+  lo = __builtin_amdgcn_permlane32_swap((unsigned)u, (unsigned)u, false, false);
+  hi = __builtin_amdgcn_permlane32_swap((unsigned)(u >> 32), (unsigned)(u >> 32), false, false);
+  return __builtin_bit_cast(double, (uint64_t)hi[0] << 32 | lo[0]) + __builtin_bit_cast(double, (uint64_t)hi[1] << 32 | lo[1]);
 }
 
 // Sums of FOUR values over the 64 lanes for the price of little more than one: a swap of half-waves adds the two

@@ -54,6 +54,36 @@ def test_a_first_position_far_from_the_rest(n, s, c, groups, first, rest, dtype)
     torch.cuda.empty_cache()
 
 
+@pytest.mark.parametrize("n,s,c,groups,dtype", [(512, 8192, 257, 1, torch.float32), (700, 4096, 64, 8, torch.float32),
+                                                (513, 2048, 2048, 16, torch.bfloat16), (2, 1 << 21, 12, 2, torch.float16)])
+def test_long_sums_of_the_backward(n, s, c, groups, dtype):
+    """A constant cotangent, whose roundings all go one way in a long chain of additions: chains of 32 terms, the rest in 64 bits.
+
+    gb is the sum of n s terms, 32 steps off at most in a chain, one more where a chunk's sum and the result are rounded.  gx is
+    r (q - mean q - z mean(q z)) with q constant: nothing but the errors of the means, at most 34 steps of q and |z| times 34 steps
+    of mean |z q|, and a rounding of each operand."""
+    from pde_amd import functional as K
+    gen = torch.Generator(device="cuda").manual_seed(s)
+    x = torch.empty(n, s, c, device="cuda", dtype=dtype)
+    for part in x.split(max(1, (1 << 26) // (s * c))):
+        part.copy_(torch.randn(part.shape, device="cuda", generator=gen))
+    x.requires_grad_()
+    b = torch.zeros(c, device="cuda", requires_grad=True)
+    y = K.group_norm_act(x, groups, None, b, 1e-5, K.ACT_IDENTITY)
+    top = float(y.detach().abs().amax())
+    gy = torch.full((), 0.1, device="cuda", dtype=dtype).expand(y.shape)
+    del y
+    gx, gb = torch.autograd.grad(K.group_norm_act(x, groups, None, b, 1e-5, K.ACT_IDENTITY), (x, b), gy)
+    q = float(gy[0, 0, 0])
+    want = q * n * s
+    assert float((gb.double() - want).abs().max()) <= 36 * U * want
+    # r of N(0, 1) data is 1 within a percent or so (samples of 2048 values at least); half a step of a 16-bit result besides
+    bound = 1.1 * q * U * (40 + 40 * top) * (1 + top) * (1 + torch.finfo(dtype).eps)
+    assert float(gx.abs().amax()) <= bound, (float(gx.abs().amax()), bound)
+    del x, gx, gy
+    torch.cuda.empty_cache()
+
+
 @pytest.mark.parametrize("act", ["identity", "silu", "tanh"])
 @pytest.mark.parametrize("shape", [(6, 32), (3, 20, 32), (3, 500, 32), (2, 20000, 32), (600, 70, 32)])
 def test_all_of_a_non_finite_group_is_nan(shape, act):
