@@ -246,7 +246,8 @@ int pdekan_orthogonalize(const PdekanMatrix* mats, int32_t n_mats, int32_t dtype
 /* One step of the Muon optimiser on fp32 weights [rows][cols] (a vector is a matrix of one row):
  *   momentum <- mu momentum + (1 - mu) grad;  u = nesterov ? (1 - mu) grad + mu momentum : momentum
  *   param <- (1 - lr weight_decay) param - lr gain orthogonalize(u)
- * lr_device, if not NULL, is read on the device instead of lr (a captured step then follows a schedule). */
+ * mu = momentum in 64 bits, from which 1 - mu is formed.  lr_device, if not NULL, is read on the device instead of lr (a
+ * captured step then follows a schedule). */
 typedef struct PdekanMuonParam {
   float* param;
   const float* grad;
@@ -256,7 +257,7 @@ typedef struct PdekanMuonParam {
   int32_t reserved;
 } PdekanMuonParam;
 size_t pdekan_muon_workspace_bytes(const PdekanMuonParam* params, int32_t n_params);
-int pdekan_muon_step(const PdekanMuonParam* params, int32_t n_params, float lr, const float* lr_device, float momentum,
+int pdekan_muon_step(const PdekanMuonParam* params, int32_t n_params, float lr, const float* lr_device, double momentum,
                      int32_t nesterov, float weight_decay, int32_t steps, const float* coefficients, float eps, void* ws,
                      size_t ws_bytes, void* stream);
 

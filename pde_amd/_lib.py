@@ -149,7 +149,7 @@ SIGNATURES = {
                                             ctypes.c_void_p]),
     "pdekan_muon_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(PdekanMuonParam), ctypes.c_int32]),
     "pdekan_muon_step": (ctypes.c_int, [ctypes.POINTER(PdekanMuonParam), ctypes.c_int32, ctypes.c_float, ctypes.c_void_p,
-                                        ctypes.c_float, ctypes.c_int32, ctypes.c_float, ctypes.c_int32, c_float_p,
+                                        ctypes.c_double, ctypes.c_int32, ctypes.c_float, ctypes.c_int32, c_float_p,
                                         ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
     "pdekan_profile_begin": (ctypes.c_int, []),
     "pdekan_profile_end": (ctypes.c_int, []),

@@ -214,7 +214,7 @@ struct NsCoefficients { float a, b, c; };
 struct NsPlan {
   NsCoefficients k;
   int steps;
-  float eps, momentum;
+  float eps, momentum, momentum_rest;       // rest: 1 - momentum
   int nesterov;
   float lr, decay;
   const float* lr_dev;

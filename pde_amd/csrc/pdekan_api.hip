@@ -1290,16 +1290,17 @@ size_t pdekan_muon_workspace_bytes(const PdekanMuonParam* params, int32_t n_para
   return ns_workspace("muon", params, n_params);
 }
 
-int pdekan_muon_step(const PdekanMuonParam* params, int32_t n_params, float lr, const float* lr_device, float momentum,
+int pdekan_muon_step(const PdekanMuonParam* params, int32_t n_params, float lr, const float* lr_device, double momentum,
                      int32_t nesterov, float weight_decay, int32_t steps, const float* coefficients, float eps, void* ws,
                      size_t ws_bytes, void* stream) {
-  if (!(momentum >= 0.0f && momentum < 1.0f)) return fail(PDEKAN_ERR_ARG, "muon_step: momentum must lie in [0, 1)");
+  if (!(momentum >= 0.0 && momentum < 1.0)) return fail(PDEKAN_ERR_ARG, "muon_step: momentum must lie in [0, 1)");
   if (!(weight_decay >= 0.0f && weight_decay < 3.0e38f)) return fail(PDEKAN_ERR_ARG, "muon_step: weight_decay must be finite and not negative");
   if (!lr_device && !(lr >= 0.0f && lr < 3.0e38f)) return fail(PDEKAN_ERR_ARG, "muon_step: lr must be finite and not negative");
   pdekan::NsPlan p{};
   p.steps = steps;
   p.eps = eps;
-  p.momentum = momentum;
+  p.momentum = (float)momentum;
+  p.momentum_rest = (float)(1.0 - momentum);
   p.nesterov = nesterov != 0;
   p.lr = lr;
   p.lr_dev = lr_device;

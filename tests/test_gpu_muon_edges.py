@@ -38,3 +38,16 @@ def test_the_same_bits_every_time(shape, dtype):
     first = K.orthogonalize(g)
     for _ in range(4):
         assert torch.equal(K.orthogonalize(g), first)
+
+
+@pytest.mark.parametrize("mu", [0.5, 0.95, 0.99, 0.999])
+@pytest.mark.parametrize("shape", [(1, 60), (1, 70000), (40, 60), (60, 1000), (200, 140)])
+def test_the_gradient_s_coefficient(shape, mu):
+    """1 - mu comes from 64 bits: the first momentum is (1 - mu) g, two roundings off (the coefficient's and the product's)."""
+    from pde_amd.optim import Muon
+    p = torch.nn.Parameter(torch.zeros(shape, device="cuda"))
+    p.grad = _matrix(shape, 7)
+    opt = Muon([p], lr=0.0, momentum=mu)
+    opt.step()
+    want = (1 - mu) * p.grad.double()
+    assert bool(((opt.state[p]["momentum_buffer"].double() - want).abs() <= 2.1 * U * want.abs()).all())
