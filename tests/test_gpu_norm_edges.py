@@ -101,3 +101,32 @@ def test_all_of_a_non_finite_group_is_nan(shape, act):
             for t in (y, gx):
                 assert bool(t[1, ..., 8:16].isnan().all())
                 assert bool(t[0].isfinite().all()) and bool(t[1, ..., :8].isfinite().all()) and bool(t[1, ..., 16:].isfinite().all())
+
+
+@pytest.mark.parametrize("act", ["silu", "tanh"])
+def test_activations_value_by_value(act):
+    """With weights of zero the value is act(bias) and the bias' gradient its slope, each compared on its own.
+
+    In steps of 2^-24.  tanh: below 0.625 a polynomial (its fit 0.1) with three roundings at the end; above, 1 - q, q =
+    2 / (exp(2|u|) + 1): q is off by 2 of the exponential and 1 of its last rounding, 1 of the sum and of the quotient: 5 of q <=
+    0.45, one of the result >= 0.55: 5 in all.  Its slope q (2 - q): 5 of q, 1 of 2 - q and of the product, 1 - t^2 below: 7.
+    silu: u s, s = 1 / (1 + exp(-u)): exponential 3, sum 1, quotient 2, product 1: 7; the slope s + u s (1 - s) cancels near
+    its zero at -1.28, so it is compared with the magnitudes of its terms: s 6, 1 - s 7 (itself below 0, where it is 1/2 at
+    least, exp(-u) s above: 10), their product 17, the sum 18."""
+    from pde_amd import functional as K
+    b = torch.cat([torch.linspace(-1, 1, 4000), torch.linspace(-12, 12, 2000), torch.linspace(-80, 80, 2000),
+                   torch.logspace(-30, 0, 192)]).cuda().requires_grad_()
+    x = torch.randn(1, b.numel(), device="cuda")
+    y = K.group_norm_act(x, b.numel() // 2, torch.zeros_like(b), b, 1e-5, _kind(act))
+    slope, = torch.autograd.grad(y.sum(), b)
+    u = b.detach().double()
+    t, s = torch.tanh(u), torch.sigmoid(u)
+    if act == "tanh":
+        want, steep, scale, steps = t, 1 / torch.cosh(u) ** 2, 1 / torch.cosh(u) ** 2, (5, 7)
+    else:
+        want, steep, scale, steps = u * s, s + u * s * (1 - s), s + u.abs() * s * torch.sigmoid(-u), (7, 18)
+    tiny = 2.0 ** -121                                            # the slope where exp(2|u|) nearly leaves fp32's range
+    assert bool(((y[0].double() - want).abs() <= steps[0] * U * want.abs() + tiny).all()), \
+        float(((y[0].double() - want).abs() / (U * want.abs() + tiny)).max())
+    assert bool(((slope.double() - steep).abs() <= steps[1] * U * scale + tiny).all()), \
+        float(((slope.double() - steep).abs() / (U * scale + tiny)).max())
