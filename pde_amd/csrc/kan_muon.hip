@@ -429,6 +429,9 @@ __global__ void __launch_bounds__(kThreads) ns_split_kernel(Items L, Momentum mo
   }
 }
 
+// Sums of so few terms that a product takes lo lo too: see block_product.
+__device__ __forceinline__ bool few_rows(const Item& I) { return I.mp == 32; }
+
 // ---- products -------------------------------------------------------------------------------------------------------
 
 // What bounds a product: the LDS where a block is 64 (a stage of 16 KB is read 32 KB for 192 cycles of matrix instructions a wave),
@@ -439,7 +442,7 @@ __global__ void __launch_bounds__(kThreads) ns_split_kernel(Items L, Momentum mo
 // P Q^T of a BT x BT block over inner tiles [k0, k1), PP and PQ pieces an operand.  Four waves take a quarter each: acc[a][c]
 // is the 16 x 16 block at rows 16 a of P and 16 c of Q; lane l holds Q's row l % 16 and P's rows 4 (l / 16) + r.
 // Operand tiles go from memory to LDS without passing registers, kStages inner tiles of the whole block in a ring, and
-// from LDS to registers as contiguous 1 KB reads.
+// from LDS to registers as contiguous 1 KB reads.  `whole`: with lo lo, for matrices of few rows (see block_product).
 template <int BT, int PP, int PQ>
 struct Product {
   static constexpr int kW = BT / 32;                           // 16-row tiles a wave takes of either operand
@@ -452,7 +455,7 @@ struct Product {
   f32x4 v[kW][kW];
 
   __device__ __forceinline__ void run(const _Float16* P, const _Float16* Q, int bp, int bq, int prows, int qrows, int kt,
-                                      int k0, int k1, char* lds) {
+                                      int k0, int k1, char* lds, bool whole) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const _Float16* src[kLoads];
     int step[kLoads];
@@ -500,6 +503,13 @@ struct Product {
     };
     // one kind of product over all blocks, then the next: instructions on one accumulator stand kW^2 apart
     auto multiply = [&](const Regs& r) {
+      if constexpr (BT == 64 && PP == 2 && PQ == 2) {
+        if (whole)
+#pragma unroll
+          for (int a = 0; a < kW; ++a)
+#pragma unroll
+            for (int c = 0; c < kW; ++c) v[a][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(r.p[a][1], r.q[c][1], v[a][c], 0, 0, 0);
+      }
 #pragma unroll
       for (int kind = 0; kind < 3; ++kind) {
         const int hp = kind == 0, hq = kind == 1;
@@ -594,7 +604,7 @@ __global__ void __launch_bounds__(kThreads, BT == 64 ? 3 : 2) ns_gram_kernel(Ite
   const _Float16* x = at<const _Float16>(ws, 0);
   const int kt = I.np / 32, k0 = chunk * I.kchunk, k1 = min(k0 + I.kchunk, kt);
   Product<BT, PX, PX> acc;
-  acc.run(x, x, bi, bj, I.mp, I.mp, kt, k0, k1, lds);
+  acc.run(x, x, bi, bj, I.mp, I.mp, kt, k0, k1, lds, few_rows(I));
   const Norm nm = *norm_slot(I, ws);
   const float scx = x_scale(nm, sc, step), factor = step ? 1.0f : nm.factor, unscale = factor / scx * (factor / scx);
   if (I.chunks == 1) {
@@ -653,7 +663,7 @@ __global__ void __launch_bounds__(kThreads, BT == 64 ? 3 : 2) ns_poly_kernel(Ite
   const _Float16* s = at<const _Float16>(ws, off_sq(I, kS));
   const int lane = threadIdx.x & 63, kt = I.mp / 32;
   Product<BT, 2, 2> acc;
-  acc.run(s, s, bi, bj, I.mp, I.mp, kt, 0, kt, lds);
+  acc.run(s, s, bi, bj, I.mp, I.mp, kt, 0, kt, lds, few_rows(I));
   const float unscale = 1.0f / sc.s;
   acc.each(bi, bj, I.mp, I.mp, [&](int p0, int q0, float (&v)[4]) {
     const int q = q0 + (lane & 15), p = p0 + 4 * (lane >> 4);
@@ -682,7 +692,7 @@ __global__ void __launch_bounds__(kThreads, BT == 64 ? 3 : 2) ns_square_kernel(I
   const int kt = I.mp / 32;
   Product<BT, 2, 2> acc;
   acc.run(at<const _Float16>(ws, off_sq(I, job.left)), at<const _Float16>(ws, off_sq(I, job.right)), bi, bj, I.mp, I.mp, kt, 0,
-          kt, lds);
+          kt, lds, few_rows(I));
   acc.each(bi, bj, I.mp, I.mp, [&](int p0, int q0, float (&v)[4]) {
     store_symmetric(at<_Float16>(ws, off_sq(I, job.out)), kt, bi == bj, p0, q0, v, job.scale);
   });
@@ -721,7 +731,7 @@ __global__ void __launch_bounds__(kThreads, BT == 64 ? 3 : 2) ns_update_kernel(I
   const _Float16* xt = at<const _Float16>(ws, off_xt(I, from));
   const int lane = threadIdx.x & 63, kt = I.mp / 32;
   Product<BT, PX, 2> acc;
-  acc.run(xt, at<const _Float16>(ws, off_sq(I, square)), bj, bi, I.np, I.mp, kt, 0, kt, lds);
+  acc.run(xt, at<const _Float16>(ws, off_sq(I, square)), bj, bi, I.np, I.mp, kt, 0, kt, lds, few_rows(I));
   const Norm nm = *norm_slot(I, ws);
   const float scx = x_scale(nm, sc, step), next = x_scale(nm, sc, next_step);
   const float factor = step ? 1.0f : nm.factor, unscale = factor / scx / scale_m, own = ca * factor / scx;
@@ -907,7 +917,7 @@ __global__ void __launch_bounds__(kSmallThreads) ns_small_kernel(Items L, Moment
     return;
   }
   const int mp = I.mp, width = I.width, rb = mp / 16, mt = mp / 32, wb = width / 16, wt = width / 32, ntri = tri16(mp);
-  const bool few = mp == 32;
+  const bool few = few_rows(I);
   _Float16* xt = reinterpret_cast<_Float16*>(lds);
   _Float16* x = xt + width * mp * 2;
   _Float16* sq = x + width * mp * 2;
