@@ -68,8 +68,12 @@ __device__ __host__ inline int64_t off_sums(const Item& I) {
   if (I.path == kVector) return 0;        // a vector has nothing else
   return off_part(I) + (I.chunks > 1 ? (int64_t)I.chunks * tri_tiles(I) * I.bt * I.bt * 4 : 0);
 }
+// What the first kernels find out about a matrix.  X = factor U' with U' = U 2^-e: the composed form keeps U' itself, whose
+// entries are those of U to the last bit, in the pieces, and applies the factor to the products; the other form has 1.
+struct Norm { float factor; int ex; };
+__device__ __host__ inline int64_t off_norm(const Item& I) { return off_sums(I) + I.nsum * (int64_t)sizeof(double); }
 __device__ __host__ inline int64_t item_bytes(const Item& I) {
-  return (off_sums(I) + kSumsMax * (int64_t)sizeof(double) + 16 + 255) / 256 * 256;
+  return (off_norm(I) + (int64_t)sizeof(Norm) + 255) / 256 * 256;
 }
 template <typename H>
 __device__ __forceinline__ H* at(char* ws, int64_t off) { return reinterpret_cast<H*>(ws + off); }
@@ -101,11 +105,8 @@ __device__ __forceinline__ void tri_tile(int t, int& bi, int& bj) {
 // k it is 2^max(0, ex - growth k).
 struct Scales { float x, s, q, t, p; int growth; };    // what the entries of X, S, Q (or R), T = Q S, P are multiplied by
 
-// What the first kernels find out about a matrix.  X = factor U' with U' = U 2^-e: the composed form keeps U' itself, whose
-// entries are those of U to the last bit, in the pieces, and applies the factor to the products; the other form has 1.
-struct Norm { float factor; int ex; };
 __device__ __forceinline__ Norm* norm_slot(const Item& I, char* ws) {
-  return at<Norm>(ws, off_sums(I) + kSumsMax * (int64_t)sizeof(double));
+  return at<Norm>(ws, off_norm(I));
 }
 __device__ __forceinline__ float x_scale(const Norm& n, const Scales& sc, int step) {
   const int ex = n.ex - sc.growth * step;
@@ -1252,21 +1253,29 @@ void choose_path(Item& I, Path least) {
       if ((int64_t)strips * tri16(I.mp) <= 1024) { I.path = kStrips; I.width = width; I.strips = strips; }
     }
   }
-  I.ws_stride = I.path == kVector ? (int64_t)kSumsMax * (int64_t)sizeof(double) : I.path == kTiles ? item_bytes(I) : small_bytes(I);
+  I.ws_stride = I.path == kVector ? (I.nsum * (int64_t)sizeof(double) + 255) / 256 * 256 : I.path == kTiles ? item_bytes(I) : small_bytes(I);
 }
 
 // The matrices of one list.  Those that could go alone in fewer launches join the launches of the others that take more of
 // them, and vectors beside tiles take part in the launches of the norms and of the pieces: beside those they cost next to
-// nothing, on their own their whole time.
+// nothing, on their own their whole time.  Matrices that one block does alone join only where all of them are at most kSinglesJoin:
+// more take longer than a launch of their own, and far more workspace.  Beside 60 x 1000, us with them and apart: 128 of 64 x 64 63
+// and 78, 256 108 and 78, 4096 851 and 390; beside 300 x 300: 128 of 4 x 6 128 and 133, 256 134 and 132, 4096 398 and 327, 128
+// of 64 x 64 142 and 141.  Strips beside tiles gain in any number (256 of 40 x 900: 349 and 900), vectors too (4096 of 50: 128 and 146).
+constexpr int64_t kSinglesJoin = 128;
 void make_items(const NsMatrix* mats, int count, Items& L) {
   L.n = 0;
   Path most = kSingle;
+  int64_t singles = 0;
   for (int j = 0; j < count && j < kItemsMax; ++j) {
     const Item& I = L.it[L.n++] = make_item(mats[j]);
     if (I.m > 1 && I.path > most) most = (Path)I.path;
+    if (I.m > 1 && I.path == kSingle) singles += I.batch;
   }
-  for (int j = 0; j < L.n; ++j)
-    if (L.it[j].m > 1 ? L.it[j].path < most : most == kTiles) choose_path(L.it[j], most);
+  for (int j = 0; j < L.n; ++j) {
+    Item& I = L.it[j];
+    if (I.m == 1 ? most == kTiles : I.path < most && (I.path != kSingle || singles <= kSinglesJoin)) choose_path(I, most);
+  }
 }
 
 int blocks_before(Items& L, int (*count)(const Item&), int times = 1) {

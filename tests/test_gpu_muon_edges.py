@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from test_gpu_muon import U, _definition, _matrix
+from test_gpu_muon import U, _check, _definition, _matrix
 
 pytestmark = pytest.mark.gpu
 
@@ -70,3 +70,18 @@ def test_small_matrices_beside_larger_ones():
             out = K.orthogonalize(mats[i:i + 15] + [_matrix(other, 5)])
             beside += sum(_error(o, g) for o, g in zip(out, mats[i:i + 15])) / 60
         assert beside <= 1.2 * alone, (other, beside, alone)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_long_stacks_beside_a_larger_matrix(dtype):
+    """Large stacks of small matrices and of vectors in one list with larger ones: no workspace beyond their kind, the same results."""
+    from pde_amd import functional as K
+    mats = [_matrix(s, i, dtype=dtype) for i, s in enumerate([(20000, 4, 6), (300, 300), (30000, 1, 50), (600, 40, 900), (7, 5, 9)])]
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    out = K.orthogonalize(mats)
+    kept = sum(o.numel() * o.element_size() for o in out)
+    assert torch.cuda.max_memory_allocated() - before - kept < 1 << 30
+    for g, o in zip(mats, out):
+        _check(o, *_definition(g))
