@@ -393,21 +393,18 @@ __global__ void __launch_bounds__(kThreads) ns_split_kernel(Items L, Momentum mo
   Norm nm;
   // at most 2^96: entries below 2^-96 |X| lose their low bits; (NaN and 0 norms: no shift)
   nm.ex = small > 1.0 && norm > 0.0 ? (small < 7.9e28 ? ilogb(small) : 96) : 0;
-  nm.factor = 1.0f;
-  float scale = (float)(1.0 / whole);
-  if constexpr (COMPOSED) {
-    // U 2^-e with 2^e >= |U| + eps: entries within [-1, 1]; an infinite or NaN norm makes everything NaN
-    const int e = whole < 1.0e300 ? ilogb(whole) + 1 : 0;
-    nm.factor = whole < 1.0e300 ? (float)ldexp(1.0 / whole, e) : __builtin_nanf("");
-    scale = ldexpf(1.0f, -e);
-  }
+  // U 2^-e with 2^e >= |U| + eps: entries within [-1, 1], whatever their size; an infinite or NaN norm makes everything NaN
+  const int e = whole < 1.0e300 ? ilogb(whole) + 1 : 0;
+  const float factor = whole < 1.0e300 ? (float)ldexp(1.0 / whole, e) : __builtin_nanf("");
+  nm.factor = COMPOSED ? factor : 1.0f;
   if (t == 0 && threadIdx.x == 0) *norm_slot(I, ws) = nm;
   const float scx = x_scale(nm, sc, 0);
 #pragma unroll
   for (int u = 0; u < 16; ++u) {
     int a, c;
     place(u, a, c);
-    tile[I.tall ? c : a][I.tall ? a : c] = raw[u] * scale;
+    const float v = ldexpf(raw[u], -e);
+    tile[I.tall ? c : a][I.tall ? a : c] = COMPOSED ? v : v * factor;
   }
   __syncthreads();
   _Float16 *x = at<_Float16>(ws, 0), *xt = at<_Float16>(ws, off_xt(I, 0));
@@ -972,7 +969,7 @@ __global__ void __launch_bounds__(kSmallThreads) ns_small_kernel(Items L, Moment
     const SumMax all = block_sum_max(s, big, red, redf);
     s = all.sum;
     big = all.max;
-    const int e = big > 0.0f ? (big < 3.4e38f ? ilogbf(big) + 1 : 0) : kNoExponent;
+    const int e = big > 0.0f ? (big < INFINITY ? ilogbf(big) + 1 : 0) : kNoExponent;
     const int per = mp / 4, across4 = 64 / per, jl = lane / per, il = (lane - jl * per) * 4;       // lanes a column of X, columns a wave
     if (jl < across4) {
       for (int j = wave * across4 + jl; j < width; j += kSmallWaves * across4) {

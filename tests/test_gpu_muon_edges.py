@@ -85,3 +85,30 @@ def test_long_stacks_beside_a_larger_matrix(dtype):
     assert torch.cuda.max_memory_allocated() - before - kept < 1 << 30
     for g, o in zip(mats, out):
         _check(o, *_definition(g))
+
+
+@pytest.mark.parametrize("kind", ["1e38", "largest", "one largest"])
+@pytest.mark.parametrize("shape", [(1, 300), (20, 30), (100, 90), (60, 1000), (200, 140), (140, 200)])
+def test_the_largest_values(shape, kind):
+    """Entries up to the largest fp32 number, whose norm fp32 does not hold: as accurate as any others."""
+    from pde_amd import functional as K
+    g = _matrix(shape, 9) * 1e3
+    big = torch.finfo(torch.float32).max
+    if kind == "one largest":
+        g[0, 3] = -big                                           # the rest vanishes beside it
+    else:
+        g = (g / g.abs().max()).clamp(-1, 1).double() * (1e38 if kind == "1e38" else big)
+        g = g.float()
+    assert bool(g.isfinite().all())
+    _check(K.orthogonalize(g), *_definition(g))
+
+
+def test_the_largest_values_in_a_step():
+    from pde_amd.optim import Muon
+    big = torch.finfo(torch.float32).max
+    for shape in ((1, 300), (20, 30), (60, 1000), (200, 140)):
+        p = torch.nn.Parameter(torch.zeros(shape, device="cuda"))
+        g = _matrix(shape, 9)
+        p.grad = (g / g.abs().max()).clamp(-1, 1) * big
+        Muon([p], lr=1.0, momentum=0.0, adjust_lr="none").step()
+        _check(-p.detach(), *_definition(p.grad))
