@@ -907,7 +907,7 @@ constexpr int kRowBlocks = 2048;       // 8 blocks of 4 waves a compute unit: al
 // Forward and backward of 8 x 4096 x 320 bf16 with 256, 384, 512, 768, 1024 blocks: 74, 70, 63, 80, 80 us; of 2 x 16384 x 512 with
 // at most 64, 128, 256 chunks a sample: 136, 86, 79 us.
 constexpr int kGridBlocks = 512, kChunksMax = 256;
-constexpr size_t kStaticLds = 20 * 1024;   // at least what the grid kernels declare besides the per-channel sums
+constexpr size_t kStaticLds = 20 * 1024, kLds = 160 * 1024;    // at least what the grid kernels declare besides the per-channel sums; all there is
 
 int pow2_at_least(int v) { int p = 1; while (p < v) p *= 2; return p; }
 
@@ -948,6 +948,10 @@ int vec_width(int dtype, int unit, const void* a, const void* b, const void* c) 
   }
   return 1;
 }
+
+// The limit to raise a grid kernel's dynamic LDS to: with what it declares it counts against 64 KB until raised, and against all
+// there is then.
+size_t lds_limit(size_t dynamic) { return dynamic + kStaticLds < kLds - kStaticLds ? dynamic + kStaticLds : kLds - kStaticLds; }
 
 GridMap grid_map(int64_t n, int64_t s, int C, int G) {
   GridMap m;
@@ -1050,8 +1054,8 @@ void grid_forward(const GridMap& m, const T* x, const float* w, const float* b, 
                   double2* part, hipStream_t st) {
   const unsigned blocks = (unsigned)(m.n * m.chunks);
   const size_t lds = 2 * (size_t)m.C * sizeof(double), lds_g = 2 * (size_t)m.G * sizeof(float);
-  ensure_dynamic_lds((const void*)norm_grid_stats_kernel<T, VEC>, lds + kStaticLds);
-  ensure_dynamic_lds((const void*)norm_grid_apply_kernel<T, VEC>, lds_g + kStaticLds);
+  ensure_dynamic_lds((const void*)norm_grid_stats_kernel<T, VEC>, lds_limit(lds));
+  ensure_dynamic_lds((const void*)norm_grid_apply_kernel<T, VEC>, lds_limit(lds_g));
   hipLaunchKernelGGL((norm_grid_stats_kernel<T, VEC>), dim3(blocks), dim3(kThreads), lds, st, m, x, part);
   hipLaunchKernelGGL((norm_grid_apply_kernel<T, VEC>), dim3(blocks), dim3(kThreads), lds_g, st, m, x, w, b, eps, act,
                      part, y, stats);
@@ -1061,8 +1065,8 @@ void grid_backward(const GridMap& m, const T* x, const T* gy, const float* w, co
                    const float2* stats, T* gx, float* gw, float* gb, float* part_c, float2* part_g, hipStream_t st) {
   const unsigned blocks = (unsigned)(m.n * m.chunks);
   const size_t lds = 2 * (size_t)m.C * sizeof(float), lds_g = 2 * (size_t)m.G * sizeof(float);
-  ensure_dynamic_lds((const void*)norm_grid_sums_kernel<T, VEC>, lds + kStaticLds);
-  ensure_dynamic_lds((const void*)norm_grid_grad_kernel<T, VEC>, lds_g + kStaticLds);
+  ensure_dynamic_lds((const void*)norm_grid_sums_kernel<T, VEC>, lds_limit(lds));
+  ensure_dynamic_lds((const void*)norm_grid_grad_kernel<T, VEC>, lds_limit(lds_g));
   hipLaunchKernelGGL((norm_grid_sums_kernel<T, VEC>), dim3(blocks), dim3(kThreads), lds, st, m, x, gy, w, b, act, stats,
                      part_c, part_g);
   const unsigned extra = gw || gb ? (2 * m.C + kGridFinishCols - 1) / kGridFinishCols : 0;

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from test_gpu_norm import _kind
+from test_gpu_norm import _definition, _kind
 
 pytestmark = pytest.mark.gpu
 
@@ -130,3 +130,21 @@ def test_activations_value_by_value(act):
         float(((y[0].double() - want).abs() / (U * want.abs() + tiny)).max())
     assert bool(((slope.double() - steep).abs() <= steps[1] * U * scale + tiny).all()), \
         float(((slope.double() - steep).abs() / (U * scale + tiny)).max())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("c,groups", [(8192, 1), (8192, 8192), (8191, 1), (7810, 2), (6000, 5)])
+def test_the_widest_channels(c, groups, dtype):
+    """Up to 8192 channels at every alignment: the statistics' 16 bytes a channel and the kernel's own LDS fit together."""
+    from pde_amd import functional as K
+    for shape in ((3, c), (2, 40, c)):
+        x = torch.randn(*shape, device="cuda", generator=torch.Generator(device="cuda").manual_seed(c)).to(dtype).requires_grad_()
+        y = K.group_norm_act(x, groups)
+        gx, = torch.autograd.grad(y, x, torch.ones_like(y))
+        ones, zeros = torch.ones(c, device="cuda").double(), torch.zeros(c, device="cuda").double()
+        want = _definition(x.detach().double(), ones, zeros, groups, 1e-5, "identity")
+        # half a step of the type, the roundings of the mean, the deviation, r and the product, of N(0, 1) data: 8 2^-24 of the scale
+        assert float((y.detach().double() - want).abs().max()) <= (8 * U + torch.finfo(dtype).eps / 2) * max(1.0, float(want.abs().max()))
+        # (a constant cotangent gives no gradient: r times the roundings of the means, 40 2^-24 each and |z| times that; r is near 1,
+        # 316 where a group is a single value)
+        assert float(gx.abs().max()) <= 2 * 80 * U * (1 + float(want.abs().max())) ** 2 * (1 if groups < c else 400)
