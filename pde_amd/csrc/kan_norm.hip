@@ -530,7 +530,11 @@ __global__ void __launch_bounds__(1024) norm_finish_kernel(const float* __restri
 constexpr int kAhead = 4;              // rows a thread of the second launches loads before the sums are merged
 
 // A block takes one chunk of positions of one sample and all its channels: thread = (vector of channels, row slot).
-struct GridMap { int64_t n, s, rows; int C, G, cpg, chunks; };   // rows: positions a chunk (the last may have fewer)
+struct GridMap {
+  int64_t n, s, rows;                  // rows: positions a chunk (the last may have fewer)
+  int64_t sums;                        // blocks of the backward's sums, of `per` samples each (the last may have fewer)
+  int C, G, cpg, chunks, per;          // per: 1 where a sample has more than one chunk, a block takes one of those
+};
 
 template <int VEC>
 struct GridThread {
@@ -550,17 +554,81 @@ struct GridThread {
   }
 };
 
-// the sums of a column of row slots (threads of one vector of channels), in the first of them
+// body(raw x[N], raw y[N], rows) for the rows of a thread, up to N at a time, whose loads are on their way at once; TWO: y too
+template <typename T, int VEC, int N, bool TWO, typename F>
+__device__ __forceinline__ void for_rows(const GridMap& m, const GridThread<VEC>& t, const T* __restrict__ x, const T* __restrict__ y, F&& body) {
+  typedef typename VecOf<T, VEC>::type Raw;
+  Raw rx[N], ry[N];
+  int64_t row = t.row0 + t.ty;
+  for (; row + (N - 1) * t.tyn < t.row1; row += N * t.tyn) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      rx[j] = *reinterpret_cast<const Raw*>(x + (row + j * t.tyn) * m.C);
+      if constexpr (TWO) ry[j] = *reinterpret_cast<const Raw*>(y + (row + j * t.tyn) * m.C);
+    }
+    body(rx, ry, IntC<N>{});
+  }
+  for (; row < t.row1; row += t.tyn) {
+    rx[0] = *reinterpret_cast<const Raw*>(x + row * m.C);
+    if constexpr (TWO) ry[0] = *reinterpret_cast<const Raw*>(y + row * m.C);
+    body(rx, ry, IntC<1>{});
+  }
+}
+
+// bytes of LDS ahead of the per-channel numbers: two sums and a number a thread and channel where a channel's rows are spread
+// over several threads
 template <int VEC>
-__device__ __forceinline__ void sum_row_slots(const GridThread<VEC>& t, bool on, double (&sum)[VEC], double (*red)[VEC + 1]) {
-  __syncthreads();
+__device__ __host__ constexpr int red_bytes(int C) { return C / VEC > kThreads / 2 ? 0 : kThreads * VEC * 20; }
+
+// own(c, sum of s1, sum of s2, k) once for each channel c of the tile: over the threads of its row slots, through red [2][threads x
+// VEC], where there are several (all channels are one tile then).  With more than eight slots every thread adds up a part first.
+template <int VEC, typename Own>
+__device__ __forceinline__ void channel_sums(const GridThread<VEC>& t, int tile, bool on, const double (&s1)[VEC], const double (&s2)[VEC],
+                                             const float (&k)[VEC], double* red, Own own) {
+  const int slots = t.row1 - t.row0 < t.tyn ? (int)(t.row1 - t.row0) : t.tyn;
+  if (slots == 1) {
+    if (on && t.ty == 0) {
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) red[threadIdx.x][i] = sum[i];
+      for (int i = 0; i < VEC; ++i) own((tile + t.tx) * VEC + i, s1[i], s2[i], k[i]);
+    }
+    return;
+  }
+  const int cols = t.txn * VEC;
+  double* red2 = red + kThreads * VEC;
+  float* redk = reinterpret_cast<float*>(red2 + kThreads * VEC);
   __syncthreads();
-  if (on && t.ty == 0)
-    for (int j = 1; j < t.tyn; ++j)
+  if (on && t.ty < slots) {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) sum[i] += red[threadIdx.x + j * t.txn][i];
+    for (int i = 0; i < VEC; ++i) {
+      red[t.ty * cols + i * t.txn + t.tx] = s1[i];
+      red2[t.ty * cols + i * t.txn + t.tx] = s2[i];
+      if (t.ty == 0) redk[i * t.txn + t.tx] = k[i];
+    }
+  }
+  __syncthreads();
+  int parts = slots;
+  if (slots > 8) {
+    parts = kThreads / (2 * cols) > 1 ? kThreads / (2 * cols) : 1;
+    if (parts > slots) parts = slots;
+    // (a thread's sum takes the place of its first term)
+    for (int job = threadIdx.x; job < 2 * cols * parts; job += kThreads) {
+      const int part = job / (2 * cols), col = job - part * 2 * cols;
+      double* at = col < cols ? red + col : red2 + col - cols;
+      double s = at[part * cols];
+      for (int y = part + parts; y < slots; y += parts) s += at[y * cols];
+      at[part * cols] = s;
+    }
+    __syncthreads();
+  }
+  for (int col = threadIdx.x; col < cols; col += kThreads) {
+    double a = red[col], b = red2[col];
+    for (int y = 1; y < parts; ++y) {
+      a += red[y * cols + col];
+      b += red2[y * cols + col];
+    }
+    const int i = col / t.txn;
+    own((col - i * t.txn) * VEC + i, a, b, redk[col]);
+  }
 }
 // not below zero; a NaN stays one
 __device__ __forceinline__ double not_negative(double v) { return v < 0.0 ? 0.0 : v; }
@@ -570,52 +638,48 @@ __device__ __forceinline__ double not_negative(double v) { return v < 0.0 ? 0.0 
 // mean)^2 / M2 <= n, the chunk's positions, to the square of the sum, 24 bits of 53 at most.  In 32 bits the sums of 2^18 positions
 // near 10^4 behind a first one of 0 were 13 % off.
 template <typename T, int VEC>
-__global__ void __launch_bounds__(kThreads) norm_grid_stats_kernel(GridMap m, const T* __restrict__ x,
+__global__ void __launch_bounds__(kThreads, VEC >= 2 ? 4 : 6) norm_grid_stats_kernel(GridMap m, const T* __restrict__ x,
                                                                    double2* __restrict__ part) {
-  extern __shared__ double chan64[];                  // [2][C]: mean and sum of squared deviations of each channel
-  __shared__ double red[kThreads][VEC + 1];
+  extern __shared__ double lds64[];                   // see red_bytes;  [2][C]: mean and sum of squared deviations of each channel
+  double* chan64 = lds64 + red_bytes<VEC>(m.C) / 8;
   const GridThread<VEC> t(m, blockIdx.x);
   const T* base = x + t.sample * m.s * m.C;
-  const double cnt = (double)(t.row1 - t.row0);
+  const double cnt = (double)(t.row1 - t.row0), inv = 1.0 / cnt, inv_cpg = 1.0 / m.cpg;
   for (int tile = 0; tile < t.nv; tile += t.txn) {
     const int vec = tile + t.tx;
     const bool on = t.ty < t.tyn && vec < t.nv;
-    double k[VEC], s1[VEC], s2[VEC];
+    float k[VEC];
+    double s1[VEC], s2[VEC];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) k[i] = s1[i] = s2[i] = 0.0;
+    for (int i = 0; i < VEC; ++i) k[i] = s1[i] = s2[i] = 0.0f;
     if (on) {
-      float v[VEC];
-      load_vec<T, VEC>(base + t.row0 * m.C + vec * VEC, v);
+      load_vec<T, VEC>(base + t.row0 * m.C + vec * VEC, k);
+      for_rows<T, VEC, VEC >= 4 ? 4 : 8, false>(m, t, base + vec * VEC, nullptr, [&](const auto& rx, const auto&, auto rows) {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) k[i] = v[i];
-#pragma unroll 8
-      for (int64_t row = t.row0 + t.ty; row < t.row1; row += t.tyn) {
-        load_vec<T, VEC>(base + row * m.C + vec * VEC, v);
+        for (int j = 0; j < decltype(rows)::value; ++j) {
+          float v[VEC];
+          widen<T, VEC>(rx[j], v);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const double d = v[i] - k[i];
-          s1[i] += d;
-          s2[i] = fma(d, d, s2[i]);
+          for (int i = 0; i < VEC; ++i) {
+            const double d = (double)v[i] - (double)k[i];
+            s1[i] += d;
+            s2[i] = fma(d, d, s2[i]);
+          }
         }
-      }
+      });
     }
-    sum_row_slots<VEC>(t, on, s1, red);
-    sum_row_slots<VEC>(t, on, s2, red);
-    if (on && t.ty == 0) {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const double d = s1[i] / cnt;
-        chan64[vec * VEC + i] = k[i] + d;
-        chan64[m.C + vec * VEC + i] = not_negative(fma(-d, s1[i], s2[i]));
-      }
-    }
+    channel_sums<VEC>(t, tile, on, s1, s2, k, lds64, [&](int c, double a, double b, float first) {
+      const double d = a * inv;
+      chan64[c] = (double)first + d;
+      chan64[m.C + c] = not_negative(fma(-d, a, b));
+    });
   }
   __syncthreads();
   const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
   for (int g = wave; g < m.G; g += kThreads / 64) {
     double s = 0.0, q = 0.0;
     for (int c = lane; c < m.cpg; c += 64) s += chan64[g * m.cpg + c];
-    const double mean = wave_sum64(s) / m.cpg;
+    const double mean = wave_sum64(s) * inv_cpg;
     for (int c = lane; c < m.cpg; c += 64) {
       const double d = chan64[g * m.cpg + c] - mean;
       q += fma(cnt * d, d, chan64[m.C + g * m.cpg + c]);
@@ -635,6 +699,16 @@ __device__ __forceinline__ double chunk_rows(const GridMap& m, int chunk) {
 // adds to s.  take(g, s, first) gets the totals, one thread a group.  Pair: double2 or float2; added up in 64 bits.
 template <typename Pair, typename Term, typename Take>
 __device__ __forceinline__ void merge_chunks(const GridMap& m, const Pair* __restrict__ part, double2 (*red), Term term, Take take) {
+  if (m.chunks == 1) {
+    for (int g = threadIdx.x; g < m.G; g += kThreads) {
+      const Pair v = part[g];
+      double2 s = make_double2(0.0, 0.0);
+      term(0, v, v, s);
+      take(g, s, v);
+    }
+    return;
+  }
+  constexpr int kBatch = 8;                           // loads of a thread on their way at once
   const int gw = m.G < kThreads ? m.G : kThreads, per = kThreads / gw;
   const int gl = threadIdx.x % gw, sub = threadIdx.x / gw;
   for (int g0 = 0; g0 < m.G; g0 += gw) {
@@ -644,8 +718,14 @@ __device__ __forceinline__ void merge_chunks(const GridMap& m, const Pair* __res
     first.x = first.y = 0;
     if (g < m.G && sub < per) {
       first = part[g];
-#pragma unroll 8
-      for (int k = sub; k < m.chunks; k += per) term(k, part[(int64_t)k * m.G + g], first, s);
+      for (int k0 = sub; k0 < m.chunks; k0 += kBatch * per) {
+        Pair v[kBatch];
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) v[j] = part[(int64_t)min(k0 + j * per, m.chunks - 1) * m.G + g];
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j)
+          if (k0 + j * per < m.chunks) term(k0 + j * per, v[j], first, s);
+      }
     }
     __syncthreads();
     red[threadIdx.x] = s;
@@ -682,7 +762,7 @@ __global__ void __launch_bounds__(kThreads) norm_grid_apply_kernel(GridMap m, co
     if (first_on && row < t.row1) ahead[j] = *reinterpret_cast<const Raw*>(x + base + row * m.C + t.tx * VEC);
   }
   // mean and r of the sample's groups, about the first chunk's mean (one of the means: see the stats kernel)
-  const double total = (double)m.s, width = (double)m.cpg;
+  const double width = (double)m.cpg, inv_s = 1.0 / (double)m.s, inv_all = inv_s / width;
   merge_chunks(m, part + t.sample * m.chunks * m.G, red,
                [&](int k, double2 v, double2 first, double2& s) {
                  const double cnt = chunk_rows(m, k), d = v.x - first.x;
@@ -690,7 +770,7 @@ __global__ void __launch_bounds__(kThreads) norm_grid_apply_kernel(GridMap m, co
                  s.y += fma(cnt * width * d, d, v.y);
                },
                [&](int g, double2 s, double2 first) {
-                 const double d = s.x / total, var = not_negative(fma(-d * width, s.x, s.y)) / (total * width);
+                 const double d = s.x * inv_s, var = not_negative(fma(-d * width, s.x, s.y)) * inv_all;
                  mu[g] = (float)(first.x + d);
                  rs[g] = rsqrtf((float)(var + (double)eps));
                  if (t.chunk == 0 && stats) stats[t.sample * m.G + g] = make_float2(mu[g], rs[g]);
@@ -732,94 +812,101 @@ __global__ void __launch_bounds__(kThreads) norm_grid_apply_kernel(GridMap m, co
   }
 }
 
-// Backward, launch 1: per chunk and channel the sums of p = gy f' and of p z (part_c [n * chunks][2][C], p z first),
-// and per group the sums of w p and w p z (part_g [n * chunks][G]).  A thread adds 32 rows in fp32, and what they come to in 64
-// bits: a chunk may have any number of rows.
+// Backward, launch 1: per chunk and group the sums of w p and w p z with p = gy f' (part_g [n * chunks][G]), and per block and
+// channel those of p z and p (part_c [sums][2][C], not wanted: nullptr).  A thread adds 32 rows in fp32, and what they come to
+// in 64 bits: a chunk may have any number of rows.  A block adds up to 64 samples in its row of part_c, which stays in the L2: a
+// row a sample would be 8 bytes a value where samples are single wide points.
 constexpr int kChain = 32;
 template <typename T, int VEC>
-__global__ void __launch_bounds__(kThreads) norm_grid_sums_kernel(GridMap m, const T* __restrict__ x,
+__global__ void __launch_bounds__(kThreads, VEC == 8 ? 2 : VEC == 4 ? 4 : 5) norm_grid_sums_kernel(GridMap m, const T* __restrict__ x,
                                                                   const T* __restrict__ gy, const float* __restrict__ w,
                                                                   const float* __restrict__ b, int act,
                                                                   const float2* __restrict__ stats,
                                                                   float* __restrict__ part_c, float2* __restrict__ part_g) {
-  extern __shared__ float chan[];                     // [2][C]: sums of w p z, w p
-  __shared__ double red[kThreads][VEC + 1];
-  const GridThread<VEC> t(m, blockIdx.x);
-  const int64_t base = t.sample * m.s * m.C;
-  float* mine = part_c + (int64_t)blockIdx.x * 2 * m.C;
-  for (int tile = 0; tile < t.nv; tile += t.txn) {
-    const int vec = tile + t.tx;
-    const bool on = t.ty < t.tyn && vec < t.nv;
-    double s1[VEC], s2[VEC];
-    float wv[VEC];
+  extern __shared__ double lds64[];                   // see red_bytes;  [2][C]: sums of w p z, w p
+  float* chan = reinterpret_cast<float*>(lds64 + red_bytes<VEC>(m.C) / 8);
+  float* mine = part_c ? part_c + (int64_t)blockIdx.x * 2 * m.C : nullptr;
+  const int64_t first = (int64_t)blockIdx.x * m.per, all = m.n * m.chunks, end = first + m.per < all ? first + m.per : all;
+  for (int64_t item = first; item < end; ++item) {
+    const GridThread<VEC> t(m, item);
+    const int64_t base = t.sample * m.s * m.C;
+    for (int tile = 0; tile < t.nv; tile += t.txn) {
+      const int vec = tile + t.tx;
+      const bool on = t.ty < t.tyn && vec < t.nv;
+      double s1[VEC], s2[VEC];
+      float wv[VEC];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) s1[i] = s2[i] = wv[i] = 0.0f;
-    if (on) {
-      float bv[VEC], mean[VEC], rs[VEC];
+      for (int i = 0; i < VEC; ++i) s1[i] = s2[i] = wv[i] = 0.0f;
+      if (on) {
+        float bv[VEC], mean[VEC], rs[VEC];
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const int c = vec * VEC + i;
-        const float2 st = stats[t.sample * m.G + c / m.cpg];
-        wv[i] = w ? w[c] : 1.0f;
-        bv[i] = b ? b[c] : 0.0f;
-        mean[i] = st.x;
-        rs[i] = st.y;
-      }
-      by_activation(act, [&](auto kind) {
-        constexpr int ACT = decltype(kind)::value;
-        for (int64_t row = t.row0 + t.ty; row < t.row1;) {
-          const int64_t left = (t.row1 - row + t.tyn - 1) / t.tyn;
-          const int n = left < kChain ? (int)left : kChain;
+        for (int i = 0; i < VEC; ++i) {
+          const int c = vec * VEC + i;
+          const float2 st = stats[t.sample * m.G + c / m.cpg];
+          wv[i] = w ? w[c] : 1.0f;
+          bv[i] = b ? b[c] : 0.0f;
+          mean[i] = st.x;
+          rs[i] = st.y;
+        }
+        by_activation(act, [&](auto kind) {
+          constexpr int ACT = decltype(kind)::value;
           float c1[VEC], c2[VEC];
 #pragma unroll
           for (int i = 0; i < VEC; ++i) c1[i] = c2[i] = 0.0f;
-#pragma unroll 2
-          for (int j = 0; j < n; ++j, row += t.tyn) {
-            float v[VEC], g[VEC];
-            load_vec<T, VEC>(x + base + row * m.C + vec * VEC, v);
-            load_vec<T, VEC>(gy + base + row * m.C + vec * VEC, g);
+          int terms = 0;
+          auto fold = [&]() {
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
-              const float z = (v[i] - mean[i]) * rs[i];
-              float f[2];
-              activation<ACT, 1, sizeof(T) == 4>(fmaf(z, wv[i], bv[i]), f);
-              const float p = g[i] * f[1];
-              c1[i] += p;
-              c2[i] = fmaf(p, z, c2[i]);
+              s1[i] += c1[i];
+              s2[i] += c2[i];
+              c1[i] = c2[i] = 0.0f;
             }
-          }
+            terms = 0;
+          };
+          for_rows<T, VEC, VEC >= 4 ? 2 : 4, true>(m, t, x + base + vec * VEC, gy + base + vec * VEC, [&](const auto& rx, const auto& ry, auto rows) {
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            s1[i] += c1[i];
-            s2[i] += c2[i];
-          }
+            for (int j = 0; j < decltype(rows)::value; ++j) {
+              float v[VEC], g[VEC];
+              widen<T, VEC>(rx[j], v);
+              widen<T, VEC>(ry[j], g);
+#pragma unroll
+              for (int i = 0; i < VEC; ++i) {
+                const float z = (v[i] - mean[i]) * rs[i];
+                float f[2];
+                activation<ACT, 1, sizeof(T) == 4>(fmaf(z, wv[i], bv[i]), f);
+                const float p = g[i] * f[1];
+                c1[i] += p;
+                c2[i] = fmaf(p, z, c2[i]);
+              }
+            }
+            terms += decltype(rows)::value;
+            if (terms > kChain - 4) fold();
+          });
+          fold();
+        });
+      }
+      channel_sums<VEC>(t, tile, on, s1, s2, wv, lds64, [&](int c, double a, double q, float wc) {
+        if (mine) {
+          mine[c] = (item > first ? mine[c] : 0.0f) + (float)q;
+          mine[m.C + c] = (item > first ? mine[m.C + c] : 0.0f) + (float)a;
         }
+        chan[c] = wc * (float)q;
+        chan[m.C + c] = wc * (float)a;
       });
     }
-    sum_row_slots<VEC>(t, on, s1, red);
-    sum_row_slots<VEC>(t, on, s2, red);
-    if (on && t.ty == 0) {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const int c = vec * VEC + i;
-        mine[c] = (float)s2[i];
-        mine[m.C + c] = (float)s1[i];
-        chan[c] = wv[i] * (float)s2[i];
-        chan[m.C + c] = wv[i] * (float)s1[i];
+    __syncthreads();
+    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+    for (int g = wave; g < m.G; g += kThreads / 64) {
+      double a = 0.0, q = 0.0;
+      for (int c = lane; c < m.cpg; c += 64) {
+        q += chan[g * m.cpg + c];
+        a += chan[m.C + g * m.cpg + c];
       }
+      a = wave_sum64(a);
+      q = wave_sum64(q);
+      if (lane == 0) part_g[item * m.G + g] = make_float2((float)a, (float)q);
     }
-  }
-  __syncthreads();
-  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
-  for (int g = wave; g < m.G; g += kThreads / 64) {
-    double a = 0.0, q = 0.0;
-    for (int c = lane; c < m.cpg; c += 64) {
-      q += chan[g * m.cpg + c];
-      a += chan[m.C + g * m.cpg + c];
-    }
-    a = wave_sum64(a);
-    q = wave_sum64(q);
-    if (lane == 0) part_g[(int64_t)blockIdx.x * m.G + g] = make_float2((float)a, (float)q);
+    __syncthreads();                                   // (the next sample's sums take chan's place)
   }
 }
 
@@ -835,7 +922,7 @@ __global__ void __launch_bounds__(kThreads) norm_grid_grad_kernel(GridMap m, con
   extern __shared__ float chan[];                     // [2][G]
   __shared__ double2 red[kThreads];
   if ((int)blockIdx.x < finish_blocks) {
-    finish_columns<kGridFinishCols, kThreads>(blockIdx.x, part_c, m.n * m.chunks, m.C, gw, gb);
+    finish_columns<kGridFinishCols, kThreads>(blockIdx.x, part_c, m.sums, m.C, gw, gb);
     return;
   }
   const GridThread<VEC> t(m, blockIdx.x - finish_blocks);
@@ -906,8 +993,8 @@ constexpr int kRowBlocks = 2048;       // 8 blocks of 4 waves a compute unit: al
 // Two blocks a compute unit: each merges all chunks of its sample, which more blocks have more of, and fewer leave it idle.
 // Forward and backward of 8 x 4096 x 320 bf16 with 256, 384, 512, 768, 1024 blocks: 74, 70, 63, 80, 80 us; of 2 x 16384 x 512 with
 // at most 64, 128, 256 chunks a sample: 136, 86, 79 us.
-constexpr int kGridBlocks = 512, kChunksMax = 256;
-constexpr size_t kStaticLds = 20 * 1024, kLds = 160 * 1024;    // at least what the grid kernels declare besides the per-channel sums; all there is
+constexpr int kGridBlocks = 512, kChunksMax = 256, kSamplesMax = 64;
+constexpr size_t kStaticLds = 8 * 1024, kLds = 160 * 1024;     // at least what the grid kernels declare themselves; all there is
 
 int pow2_at_least(int v) { int p = 1; while (p < v) p *= 2; return p; }
 
@@ -964,6 +1051,10 @@ GridMap grid_map(int64_t n, int64_t s, int C, int G) {
   if (chunks < 1) chunks = 1;
   m.rows = (s + chunks - 1) / chunks;
   m.chunks = (int)((s + m.rows - 1) / m.rows);
+  // blocks of the backward's sums: as many as the chip holds, more where that would be more than 64 samples each
+  const int64_t per = m.chunks > 1 ? 1 : (n + kRowBlocks - 1) / kRowBlocks;
+  m.per = (int)(per < kSamplesMax ? per : kSamplesMax);
+  m.sums = (n * m.chunks + m.per - 1) / m.per;
   return m;
 }
 
@@ -1053,7 +1144,7 @@ template <typename T, int VEC>
 void grid_forward(const GridMap& m, const T* x, const float* w, const float* b, float eps, int act, T* y, float2* stats,
                   double2* part, hipStream_t st) {
   const unsigned blocks = (unsigned)(m.n * m.chunks);
-  const size_t lds = 2 * (size_t)m.C * sizeof(double), lds_g = 2 * (size_t)m.G * sizeof(float);
+  const size_t lds = red_bytes<VEC>(m.C) + 2 * (size_t)m.C * sizeof(double), lds_g = 2 * (size_t)m.G * sizeof(float);
   ensure_dynamic_lds((const void*)norm_grid_stats_kernel<T, VEC>, lds_limit(lds));
   ensure_dynamic_lds((const void*)norm_grid_apply_kernel<T, VEC>, lds_limit(lds_g));
   hipLaunchKernelGGL((norm_grid_stats_kernel<T, VEC>), dim3(blocks), dim3(kThreads), lds, st, m, x, part);
@@ -1064,11 +1155,11 @@ template <typename T, int VEC>
 void grid_backward(const GridMap& m, const T* x, const T* gy, const float* w, const float* b, int act,
                    const float2* stats, T* gx, float* gw, float* gb, float* part_c, float2* part_g, hipStream_t st) {
   const unsigned blocks = (unsigned)(m.n * m.chunks);
-  const size_t lds = 2 * (size_t)m.C * sizeof(float), lds_g = 2 * (size_t)m.G * sizeof(float);
+  const size_t lds = red_bytes<VEC>(m.C) + 2 * (size_t)m.C * sizeof(float), lds_g = 2 * (size_t)m.G * sizeof(float);
   ensure_dynamic_lds((const void*)norm_grid_sums_kernel<T, VEC>, lds_limit(lds));
   ensure_dynamic_lds((const void*)norm_grid_grad_kernel<T, VEC>, lds_limit(lds_g));
-  hipLaunchKernelGGL((norm_grid_sums_kernel<T, VEC>), dim3(blocks), dim3(kThreads), lds, st, m, x, gy, w, b, act, stats,
-                     part_c, part_g);
+  hipLaunchKernelGGL((norm_grid_sums_kernel<T, VEC>), dim3((unsigned)m.sums), dim3(kThreads), lds, st, m, x, gy, w, b, act,
+                     stats, gw || gb ? part_c : nullptr, part_g);
   const unsigned extra = gw || gb ? (2 * m.C + kGridFinishCols - 1) / kGridFinishCols : 0;
   hipLaunchKernelGGL((norm_grid_grad_kernel<T, VEC>), dim3(blocks + extra), dim3(kThreads), lds_g, st, m, x, gy, w, b,
                      act, stats, part_c, part_g, gx, gw, gb, (int)extra);
@@ -1102,7 +1193,7 @@ size_t norm_ws_bytes(const NormShape& p, bool backward) {
   }
   const GridMap m = grid_map(p.n, p.s, p.C, p.G);
   const size_t blocks = (size_t)m.n * m.chunks;
-  return backward ? blocks * m.G * sizeof(float2) + blocks * 2 * m.C * sizeof(float) : blocks * m.G * sizeof(double2);
+  return backward ? blocks * m.G * sizeof(float2) + (size_t)m.sums * 2 * m.C * sizeof(float) : blocks * m.G * sizeof(double2);
 }
 
 bool norm_wants_stats(const NormShape& p) { return !rows_kernel_takes(p.s, p.C / p.G); }

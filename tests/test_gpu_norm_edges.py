@@ -148,3 +148,32 @@ def test_the_widest_channels(c, groups, dtype):
         # (a constant cotangent gives no gradient: r times the roundings of the means, 40 2^-24 each and |z| times that; r is near 1,
         # 316 where a group is a single value)
         assert float(gx.abs().max()) <= 2 * 80 * U * (1 + float(want.abs().max())) ** 2 * (1 if groups < c else 400)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape,groups", [((5000, 1536), 2), ((2049, 4100), 1), ((3000, 2, 384), 1), ((2500, 33, 40), 5), ((2048, 600), 1),
+                                          ((20, 8192), 1), ((9000, 3, 257), 1)])
+def test_wide_rows_and_many_samples(shape, groups, dtype):
+    """More samples than the backward's blocks: each block adds up those it takes.  All gradients against the definition."""
+    from pde_amd import functional as K
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    c = shape[-1]
+    x = torch.randn(*shape, device="cuda", generator=gen).to(dtype).requires_grad_()
+    gy = torch.randn(*shape, device="cuda", generator=gen).to(dtype)
+    w = (1 + 0.2 * torch.randn(c, device="cuda", generator=gen)).requires_grad_()
+    b = (0.2 * torch.randn(c, device="cuda", generator=gen)).requires_grad_()
+    y = K.group_norm_act(x, groups, w, b, 1e-5, K.ACT_TANH)
+    gx, gw, gb = torch.autograd.grad(y, (x, w, b), gy)
+    leaves = [t.detach().double().requires_grad_() for t in (x, w, b)]
+    want = _definition(*leaves, groups, 1e-5, "tanh")
+    ex, ew, eb = torch.autograd.grad(want, leaves, gy.double())
+    half = torch.finfo(dtype).eps / 2
+    # N(0, 1) data: each value and each term of a sum a few steps of magnitudes of at most a few; in the 2-norm 16 steps
+    for got, e in ((y, want.detach()), (gx, ex)):
+        assert float((got.double() - e).norm() / e.norm()) <= 16 * U + half
+    for got, e in ((gw, ew), (gb, eb)):
+        assert float((got.double() - e).norm() / e.norm()) <= 32 * U
+    alone, = torch.autograd.grad(K.group_norm_act(x, groups, w.detach(), b.detach(), 1e-5, K.ACT_TANH), x, gy)
+    assert torch.equal(alone, gx)                                 # without the parameters' gradients: the same
+    only, = torch.autograd.grad(K.group_norm_act(x, groups, w.detach(), b, 1e-5, K.ACT_TANH), b, gy)
+    assert torch.equal(only, gb)
