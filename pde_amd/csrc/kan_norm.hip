@@ -72,20 +72,31 @@ __device__ __forceinline__ float exp_times(float u) {
 
 // f and its first ORDER derivatives at u.
 //   tanh: 1 - q with q = 2 / (exp(2|u|) + 1), slope q (2 - q), which keeps its bits where tanh is nearly 1; below 0.625, where 1 - q
-//   loses some, u + u^3 p(u^2) with p a polynomial of degree 4 fitted for the least relative error (5e-9)
+//   loses some, u + u^3 p(u^2) with p a polynomial fitted for the least relative error: of degree 4 (5e-9), or for tensors of 16 bits,
+//   which take the slope as 1 - t^2 too, of degree 3 (1.4e-7)
 //   silu: u s, s = 1 / (1 + exp(-u)); 1 - s = exp(-u) s where s is nearly 1
 template <int ACT, int ORDER, bool FULL>
 __device__ __forceinline__ void activation(float u, float (&f)[ORDER + 1]) {
   if constexpr (ACT == kNormActTanh) {
-    const float a = fabsf(u), u2 = u * u;
-    const float d = exp_times<2, FULL>(a > 43.0f ? 43.0f : a) + 1.0f;               // (finite; a NaN stays one)
-    float q = __builtin_amdgcn_rcpf(d);
-    q = 2.0f * (FULL ? fmaf(fmaf(-d, q, 1.0f), q, q) : q);
-    const float poly = fmaf(u2, fmaf(u2, fmaf(u2, fmaf(u2, -0.00571705587f, 0.0206505991f), -0.0537435003f), 0.133314908f), -0.333332837f);
+    const float u2 = u * u, a = fabsf(u);
+    const float poly = FULL ? fmaf(u2, fmaf(u2, fmaf(u2, fmaf(u2, -0.00571705587f, 0.0206505991f), -0.0537435003f), 0.133314908f), -0.333332837f)
+                            : fmaf(u2, fmaf(u2, fmaf(u2, 0.0152269052f, -0.0519716218f), 0.133087143f), -0.333323747f);
+    const float inner = fmaf(u * u2, poly, u);
     const bool near = a < 0.625f;
-    const float t = near ? fmaf(u * u2, poly, u) : copysignf(1.0f - q, u);
+    float t, slope;
+    if constexpr (FULL) {
+      // (43: finite; a NaN stays one.  The value alone loses at most half a step without the exponential's rest, the slope more)
+      const float d = exp_times<2, (ORDER > 0)>(a > 43.0f ? 43.0f : a) + 1.0f;
+      float q = __builtin_amdgcn_rcpf(d);
+      q = 2.0f * fmaf(fmaf(-d, q, 1.0f), q, q);
+      t = near ? inner : copysignf(1.0f - q, u);
+      slope = near ? fmaf(-t, t, 1.0f) : q * (2.0f - q);
+    } else {
+      t = near ? inner : fmaf(-2.0f, __builtin_amdgcn_rcpf(exp_times<2, false>(u) + 1.0f), 1.0f);
+      slope = fmaf(-t, t, 1.0f);
+    }
     f[0] = t;
-    if constexpr (ORDER >= 1) f[1] = near ? fmaf(-t, t, 1.0f) : q * (2.0f - q);
+    if constexpr (ORDER >= 1) f[1] = slope;
     if constexpr (ORDER >= 2) f[2] = -2.0f * t * f[1];
     if constexpr (ORDER >= 3) f[3] = f[1] * (6.0f * t * t - 2.0f);
   } else if constexpr (ACT == kNormActSilu) {
