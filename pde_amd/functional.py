@@ -396,9 +396,11 @@ class _GroupNormAct(torch.autograd.Function):
         x, weight, bias, stats = ctx.saved_tensors
         groups, eps, act = ctx.meta
         if torch.is_grad_enabled():                    # this backward is being recorded (create_graph=True)
-            y = _group_norm_expression(x, groups, weight, bias, eps, act)
+            # of views: where one input was computed from another, each derivative is that of the norm alone
+            own = [t if t is None else t.view_as(t) for t in (x, weight, bias)]
+            y = _group_norm_expression(own[0], groups, own[1], own[2], eps, act)
             wanted = [i for i in range(3) if ctx.needs_input_grad[i]]
-            got = torch.autograd.grad(y, [(x, weight, bias)[i] for i in wanted], gy, create_graph=True, allow_unused=True)
+            got = torch.autograd.grad(y, [own[i] for i in wanted], gy, create_graph=True, allow_unused=True)
             out = [None] * 6
             for i, g in zip(wanted, got):
                 out[i] = g

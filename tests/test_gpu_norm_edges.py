@@ -177,3 +177,22 @@ def test_wide_rows_and_many_samples(shape, groups, dtype):
     assert torch.equal(alone, gx)                                 # without the parameters' gradients: the same
     only, = torch.autograd.grad(K.group_norm_act(x, groups, w.detach(), b, 1e-5, K.ACT_TANH), b, gy)
     assert torch.equal(only, gb)
+
+
+def test_a_recorded_backward_of_parameters_that_depend_on_each_other():
+    """weight and bias computed from x: a recorded backward hands on the norm's own derivatives, and the rest of the graph adds theirs."""
+    from pde_amd import functional as K
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    x0 = torch.randn(5, 12, device="cuda", generator=gen)
+
+    def grads(x, norm):
+        w = 1 + 0.3 * x.mean(0)
+        y = norm(x, w, 0.5 * w * x.sum(0))
+        g, = torch.autograd.grad(y.square().sum(), x, create_graph=True)
+        h, = torch.autograd.grad(g.square().sum(), x)
+        return g.detach().double(), h.double()
+
+    got = grads(x0.clone().requires_grad_(), lambda x, w, b: K.group_norm_act(x, 3, w, b, 1e-5, K.ACT_TANH))
+    want = grads(x0.double().requires_grad_(), lambda x, w, b: _definition(x, w, b, 3, 1e-5, "tanh"))
+    for a, e in zip(got, want):
+        assert float((a - e).norm() / e.norm()) < 1e-5            # groups of four of spread 1: a few r^3 of 2^-24 (second order: r^5)
