@@ -177,6 +177,9 @@ class _KanLayerJet(torch.autograd.Function):
                 "KAN.forward_jet already returns the input derivatives that nested gradients would form, and its "
                 "first-order backward gives their parameter gradients")
         with torch.enable_grad():
+            # of views: where one input was computed from another, each derivative is that of the layer alone
+            x_jet, base_weight, spline_weight, spline_scaler = (
+                t if t is None else t.view_as(t) for t in (x_jet, base_weight, spline_weight, spline_scaler))
             y = _dense_layer(x_jet.squeeze(-1), grid, base_weight, spline_weight, spline_scaler, act_kind, grid_size,
                              spline_order).unsqueeze(-1)
             wanted = [(i, t) for i, t in ((0, x_jet), (2, base_weight), (3, spline_weight), (4, spline_scaler))
