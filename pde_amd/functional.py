@@ -9,6 +9,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import functools
+import math
 from typing import Optional, Sequence, Tuple, Union
 
 import torch
@@ -326,7 +327,7 @@ def _norm_check(channels: int, groups: int, weight, bias, eps: float, act: int) 
 
 def _group_norm_expression(x, groups, weight, bias, eps, act):
     """``group_norm_act`` as its defining expression, differentiable to any order and under ``torch.func``."""
-    v = x.reshape(x.size(0), -1, groups, x.size(-1) // groups)
+    v = x.reshape(x.size(0), math.prod(x.shape[1:-1]), groups, x.size(-1) // groups)        # (0 samples leave no -1 to infer)
     if v.dtype in (torch.bfloat16, torch.float16):
         v = v.float()
     v = v - v.mean((1, 3), keepdim=True)

@@ -196,3 +196,13 @@ def test_a_recorded_backward_of_parameters_that_depend_on_each_other():
     want = grads(x0.double().requires_grad_(), lambda x, w, b: _definition(x, w, b, 3, 1e-5, "tanh"))
     for a, e in zip(got, want):
         assert float((a - e).norm() / e.norm()) < 1e-5            # groups of four of spread 1: a few r^3 of 2^-24 (second order: r^5)
+
+
+def test_empty_batches_in_tensor_code():
+    """The defining expression takes what the kernels take: no samples, no positions."""
+    from pde_amd import functional as K
+    for shape in ((0, 8), (0, 5, 8), (3, 0, 8)):
+        x = torch.empty(shape, device="cuda", requires_grad=True)
+        w = torch.ones(8, device="cuda", requires_grad=True)
+        gx, gw = torch.autograd.grad(K.group_norm_act(x, 2, w).square().sum(), (x, w), create_graph=True)
+        assert gx.shape == x.shape and not gw.any()
