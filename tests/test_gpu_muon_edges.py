@@ -1,8 +1,10 @@
 """Newton-Schulz orthogonalisation and the Muon step where few bits, large values, long lists or shared memory could tell."""
+import ctypes
+
 import pytest
 import torch
 
-from test_gpu_muon import U, _check, _definition, _matrix
+from test_gpu_muon import A, B, C, U, _check, _definition, _matrix
 
 pytestmark = pytest.mark.gpu
 
@@ -112,3 +114,41 @@ def test_the_largest_values_in_a_step():
         p.grad = (g / g.abs().max()).clamp(-1, 1) * big
         Muon([p], lr=1.0, momentum=0.0, adjust_lr="none").step()
         _check(-p.detach(), *_definition(p.grad))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", [(3, 40, 70), (3, 70, 40), (3, 1, 50), (3, 1, 70000), (3, 200, 140), (3, 60, 1000), (3, 1100, 50)])
+def test_all_of_a_non_finite_matrix_is_nan(shape, dtype):
+    from pde_amd import functional as K
+    g = _matrix(shape, 4, dtype=dtype)
+    clean = K.orthogonalize(g)
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        g[2, 0, 3] = bad
+        out = K.orthogonalize(g)
+        assert torch.equal(out[:2], clean[:2]) and bool(out[2].isnan().all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_a_result_in_its_matrix_s_place(dtype):
+    """`out` may be `g`, on every path and in a list of all of them: the bits of a result in a place of its own."""
+    from pde_amd import _lib, functional as K
+    lib = _lib.load()
+    coefficients = (ctypes.c_float * 3)(A, B, C)
+
+    def run(mats, outs):
+        desc = (_lib.PdekanMatrix * len(mats))()
+        for d, g, o in zip(desc, mats, outs):
+            rows, cols = g.shape[-2:]
+            d.g, d.out, d.rows, d.cols, d.batch = g.data_ptr(), o.data_ptr(), rows, cols, g.numel() // (rows * cols)
+        need = lib.pdekan_orthogonalize_workspace_bytes(desc, len(mats))
+        ws = K._workspace(need, "cuda")
+        _lib.check(lib.pdekan_orthogonalize(desc, len(mats), K.DTYPES[dtype], 5, coefficients, 1e-7, ws.data_ptr(), need,
+                                            K._raw_stream(mats[0].device)))
+
+    shapes = [(1, 500), (1, 70000), (40, 60), (60, 40), (60, 1000), (1000, 60), (200, 140), (140, 200), (3, 50, 70), (2, 2100, 2050)]
+    for group in [[s] for s in shapes] + [shapes[:6], shapes[:9]]:
+        mats = [_matrix(s, 40 + i, dtype=dtype) for i, s in enumerate(group)]
+        apart = [torch.empty_like(g) for g in mats]
+        run(mats, apart)
+        run(mats, mats)
+        assert all(torch.equal(g, o) for g, o in zip(mats, apart)), group
