@@ -1207,17 +1207,19 @@ Item make_item(const NsMatrix& M) {
   const int64_t parts = (I.size + kThreads * 16 - 1) / (kThreads * 16), most = kSumsMax / (I.batch < 4 ? I.batch : 4);
   I.nsum = (int)(parts < most ? parts : most);
   // Blocks of 128 x 128 read half as much for a product as blocks of 64 x 64, but need more inner tiles to get going and more
-  // blocks to fill the chip.  Where rows times blocks reach 2^19, us in blocks of 64 and of 128: 2048 x 8192 bf16 1316 and 980, fp32
-  // 2607 and 1854; 2048 x 2048 fp32 803 and 747; 1024 x 16384 bf16 449 and 419; and below it: 4 x 1000 x 771 fp16 297 and 312;
-  // 1024 x 4096 bf16 268 and 283; 512 x 16384 fp32 419 and 431; 256 x 65536 fp32 525 and 561; 100 x 60000 fp32 261 and 320.
+  // blocks to fill the chip.  Where rows times blocks reach 2^19, us in blocks of 64 and of 128: 2048 x 8192 bf16 1417 and 1120, fp32
+  // 2533 and 1859; 2048 x 2048 fp32 794 and 753; 1024 x 8192 bf16 364 and 357; 512 x 32768 fp32 727 and 721; and below it: 1500 x
+  // 3000 bf16 473 and 486; 1024 x 4096 bf16 287 and 302; 512 x 16384 fp32 419 and 429; 4 x 1000 x 771 fp16 294 and 311.
   constexpr int64_t kBigBlocks = 1 << 19;
   const int64_t big = (int64_t)((I.mp + 127) / 128) * ((I.np + 127) / 128) * I.batch;
   I.bt = I.m > 64 && I.mp * big >= kBigBlocks ? 128 : 64;
-  // Among squares only the upper triangle's blocks are computed: 128 x 128 ones where they are two a compute unit besides.
-  // 4096 x 4096 bf16 5360 and 4076 us, 4 x 2048 x 2048 bf16 2350 and 2130; 32 x 700 x 700 fp32 1215 and 1257 (2900 x 2900 bf16,
-  // 276 blocks: 2030 and 5000)
+  // Among squares only the upper triangle's blocks are computed: 128 x 128 ones where rows times those reach 600000.  In blocks of 64 and
+  // of 128: 2600 x 2600 bf16 1457 and 1243 us, 2900 x 2900 2113 and 1901, 4096 x 4096 5540 and 4286, 4 x 2048 x 2048 2477 and 2290,
+  // 2900 x 2900 fp32 1992 and 1941; below it 2300 x 2300 bf16 985 and 1032, 2 x 2048 x 2048 1310 and 1367, 8 x 1024 x 1024 742 and 812,
+  // 32 x 700 x 700 fp32 1223 and 1279.
+  constexpr int64_t kBigSquares = 600000;
   const int64_t t128 = (I.mp + 127) / 128, tri = t128 * (t128 + 1) / 2 * I.batch;
-  I.bts = tri >= 512 && I.mp * tri >= kBigBlocks ? 128 : 64;
+  I.bts = I.mp * tri >= kBigSquares ? 128 : 64;
   // splits of the long axis: two blocks a compute unit, at least four inner tiles each
   const int kt = I.np / 32, tiles = tri_tiles(I);
   int64_t chunks = (512 + (int64_t)tiles * I.batch - 1) / ((int64_t)tiles * I.batch);
@@ -1312,11 +1314,12 @@ struct Steps {
     S.n = 0;
     for (int i = 0; i < L.n; ++i)
       if (L.it[i].chunks > 1) S.it[S.n++] = L.it[i];
-    // with many splits four groups of waves share them (46 splits of 256 x 5888: 7.0 -> 6.1 us; 4 splits: 11 -> 17 us)
+    // With many splits four groups of waves share them: fp32 matrices by one group and by four, 8 splits (256 x 1024) 110 and 114 us, 16
+    // 118 and 122, 32 137 and 139, 40 151 and 156; 46 164 and 161, 156 (150 x 20000) 195 and 189.
     int most = 0;
     for (int i = 0; i < S.n; ++i) most = S.it[i].chunks > most ? S.it[i].chunks : most;
     const int sums = blocks_before(S, count_parts);
-    if (most >= 16) launch<4 * kThreads>(ns_gram_sum_kernel<BT, 4>, sums, 0, st, S, sc);
+    if (most >= 44) launch<4 * kThreads>(ns_gram_sum_kernel<BT, 4>, sums, 0, st, S, sc);
     else launch(ns_gram_sum_kernel<BT, 1>, sums, 0, st, S, sc);
   }
   // go(the matrices whose squares go in blocks of `bts`, their number of blocks), for each block size there is
