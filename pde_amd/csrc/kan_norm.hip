@@ -11,6 +11,7 @@
 //   grids (norm_grid_*): samples of many positions.  Launch 1 leaves partial statistics per chunk of positions, launch 2
 //     merges them (Chan's formula) and applies; the second reading of x comes mostly from the caches.
 #include <hip/hip_runtime.h>
+#include <algorithm>
 #include <cstdint>
 
 #include "kan_launch.h"
@@ -1047,9 +1048,11 @@ int vec_width(int dtype, int unit, const void* a, const void* b, const void* c) 
   return 1;
 }
 
-// The limit to raise a grid kernel's dynamic LDS to: with what it declares it counts against 64 KB until raised, and against all
-// there is then.
-size_t lds_limit(size_t dynamic) { return dynamic + kStaticLds < kLds - kStaticLds ? dynamic + kStaticLds : kLds - kStaticLds; }
+// A launch may ask for 64 KB of LDS with what the kernel declares itself; beyond, the limit of its dynamic part is raised first, up
+// to what is left of all there is.
+void ensure_lds(const void* kernel, size_t dynamic) {
+  if (dynamic + kStaticLds > 64 * 1024) ensure_dynamic_lds(kernel, std::min(dynamic + kStaticLds, kLds - kStaticLds));
+}
 
 GridMap grid_map(int64_t n, int64_t s, int C, int G) {
   GridMap m;
@@ -1156,8 +1159,8 @@ void grid_forward(const GridMap& m, const T* x, const float* w, const float* b, 
                   double2* part, hipStream_t st) {
   const unsigned blocks = (unsigned)(m.n * m.chunks);
   const size_t lds = red_bytes<VEC>(m.C) + 2 * (size_t)m.C * sizeof(double), lds_g = 2 * (size_t)m.G * sizeof(float);
-  ensure_dynamic_lds((const void*)norm_grid_stats_kernel<T, VEC>, lds_limit(lds));
-  ensure_dynamic_lds((const void*)norm_grid_apply_kernel<T, VEC>, lds_limit(lds_g));
+  ensure_lds((const void*)norm_grid_stats_kernel<T, VEC>, lds);
+  ensure_lds((const void*)norm_grid_apply_kernel<T, VEC>, lds_g);
   hipLaunchKernelGGL((norm_grid_stats_kernel<T, VEC>), dim3(blocks), dim3(kThreads), lds, st, m, x, part);
   hipLaunchKernelGGL((norm_grid_apply_kernel<T, VEC>), dim3(blocks), dim3(kThreads), lds_g, st, m, x, w, b, eps, act,
                      part, y, stats);
@@ -1167,8 +1170,8 @@ void grid_backward(const GridMap& m, const T* x, const T* gy, const float* w, co
                    const float2* stats, T* gx, float* gw, float* gb, float* part_c, float2* part_g, hipStream_t st) {
   const unsigned blocks = (unsigned)(m.n * m.chunks);
   const size_t lds = red_bytes<VEC>(m.C) + 2 * (size_t)m.C * sizeof(float), lds_g = 2 * (size_t)m.G * sizeof(float);
-  ensure_dynamic_lds((const void*)norm_grid_sums_kernel<T, VEC>, lds_limit(lds));
-  ensure_dynamic_lds((const void*)norm_grid_grad_kernel<T, VEC>, lds_limit(lds_g));
+  ensure_lds((const void*)norm_grid_sums_kernel<T, VEC>, lds);
+  ensure_lds((const void*)norm_grid_grad_kernel<T, VEC>, lds_g);
   hipLaunchKernelGGL((norm_grid_sums_kernel<T, VEC>), dim3((unsigned)m.sums), dim3(kThreads), lds, st, m, x, gy, w, b, act,
                      stats, gw || gb ? part_c : nullptr, part_g);
   const unsigned extra = gw || gb ? (2 * m.C + kGridFinishCols - 1) / kGridFinishCols : 0;

@@ -206,3 +206,30 @@ def test_empty_batches_in_tensor_code():
         w = torch.ones(8, device="cuda", requires_grad=True)
         gx, gw = torch.autograd.grad(K.group_norm_act(x, 2, w).square().sum(), (x, w), create_graph=True)
         assert gx.shape == x.shape and not gw.any()
+
+
+@pytest.mark.parametrize("shape,groups", [((3, 3000, 40), 5), ((600, 300, 24), 3), ((5000, 2, 384), 1)])
+def test_captured_and_replayed(shape, groups):
+    """Forward and backward of samples with several chunks, one, and many samples a block, captured without an eager call of the shape
+    before and replayed on new values between eager work: the eager bits each time."""
+    from pde_amd import functional as K
+    gen = torch.Generator(device="cuda").manual_seed(11)
+    rand = lambda *s: torch.randn(*s, device="cuda", generator=gen)
+    leaves = [rand(*shape), 1 + 0.2 * rand(shape[-1]), 0.2 * rand(shape[-1])]
+    gy = rand(*shape)
+
+    def both(leaves):
+        leaves = [t.detach().requires_grad_() for t in leaves]
+        y = K.group_norm_act(leaves[0], groups, leaves[1], leaves[2], 1e-5, K.ACT_SILU)
+        return (y.detach(), *torch.autograd.grad(y, leaves, gy))
+
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        held = both(leaves)
+    for _ in range(4):
+        for t in leaves:
+            t.copy_(rand(*t.shape))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, both(leaves)))
