@@ -566,12 +566,13 @@ struct GridThread {
   }
 };
 
-// body(raw x[N], raw y[N], rows) for the rows of a thread, up to N at a time, whose loads are on their way at once; TWO: y too
+// body(raw x[N], raw y[N], N) for a thread's rows from `row`, N at a time, whose loads are on their way at once, then half as many and
+// so on down to one; TWO: y too.  (Loads with a condition each would wait for one another.)
 template <typename T, int VEC, int N, bool TWO, typename F>
-__device__ __forceinline__ void for_rows(const GridMap& m, const GridThread<VEC>& t, const T* __restrict__ x, const T* __restrict__ y, F&& body) {
+__device__ __forceinline__ void for_rows(const GridMap& m, const GridThread<VEC>& t, int64_t row, const T* __restrict__ x, const T* __restrict__ y,
+                                         F&& body) {
   typedef typename VecOf<T, VEC>::type Raw;
   Raw rx[N], ry[N];
-  int64_t row = t.row0 + t.ty;
   for (; row + (N - 1) * t.tyn < t.row1; row += N * t.tyn) {
 #pragma unroll
     for (int j = 0; j < N; ++j) {
@@ -580,11 +581,7 @@ __device__ __forceinline__ void for_rows(const GridMap& m, const GridThread<VEC>
     }
     body(rx, ry, IntC<N>{});
   }
-  for (; row < t.row1; row += t.tyn) {
-    rx[0] = *reinterpret_cast<const Raw*>(x + row * m.C);
-    if constexpr (TWO) ry[0] = *reinterpret_cast<const Raw*>(y + row * m.C);
-    body(rx, ry, IntC<1>{});
-  }
+  if constexpr (N > 1) for_rows<T, VEC, N / 2, TWO>(m, t, row, x, y, body);
 }
 
 // bytes of LDS ahead of the per-channel numbers: two sums and a number a thread and channel where a channel's rows are spread
@@ -650,7 +647,7 @@ __device__ __forceinline__ double not_negative(double v) { return v < 0.0 ? 0.0 
 // mean)^2 / M2 <= n, the chunk's positions, to the square of the sum, 24 bits of 53 at most.  In 32 bits the sums of 2^18 positions
 // near 10^4 behind a first one of 0 were 13 % off.
 template <typename T, int VEC>
-__global__ void __launch_bounds__(kThreads, VEC >= 2 ? 4 : 6) norm_grid_stats_kernel(GridMap m, const T* __restrict__ x,
+__global__ void __launch_bounds__(kThreads, VEC == 8 ? 3 : VEC >= 2 ? 4 : 6) norm_grid_stats_kernel(GridMap m, const T* __restrict__ x,
                                                                    double2* __restrict__ part) {
   extern __shared__ double lds64[];                   // see red_bytes;  [2][C]: mean and sum of squared deviations of each channel
   double* chan64 = lds64 + red_bytes<VEC>(m.C) / 8;
@@ -666,7 +663,7 @@ __global__ void __launch_bounds__(kThreads, VEC >= 2 ? 4 : 6) norm_grid_stats_ke
     for (int i = 0; i < VEC; ++i) k[i] = s1[i] = s2[i] = 0.0f;
     if (on) {
       load_vec<T, VEC>(base + t.row0 * m.C + vec * VEC, k);
-      for_rows<T, VEC, VEC >= 4 ? 4 : 8, false>(m, t, base + vec * VEC, nullptr, [&](const auto& rx, const auto&, auto rows) {
+      for_rows<T, VEC, VEC >= 4 ? 4 : 8, false>(m, t, t.row0 + t.ty, base + vec * VEC, nullptr, [&](const auto& rx, const auto&, auto rows) {
 #pragma unroll
         for (int j = 0; j < decltype(rows)::value; ++j) {
           float v[VEC];
@@ -830,7 +827,7 @@ __global__ void __launch_bounds__(kThreads) norm_grid_apply_kernel(GridMap m, co
 // row a sample would be 8 bytes a value where samples are single wide points.
 constexpr int kChain = 32;
 template <typename T, int VEC>
-__global__ void __launch_bounds__(kThreads, VEC == 8 ? 2 : VEC == 4 ? 4 : 5) norm_grid_sums_kernel(GridMap m, const T* __restrict__ x,
+__global__ void __launch_bounds__(kThreads, VEC == 8 ? 2 : 4) norm_grid_sums_kernel(GridMap m, const T* __restrict__ x,
                                                                   const T* __restrict__ gy, const float* __restrict__ w,
                                                                   const float* __restrict__ b, int act,
                                                                   const float2* __restrict__ stats,
@@ -875,7 +872,7 @@ __global__ void __launch_bounds__(kThreads, VEC == 8 ? 2 : VEC == 4 ? 4 : 5) nor
             }
             terms = 0;
           };
-          for_rows<T, VEC, VEC >= 4 ? 2 : 4, true>(m, t, x + base + vec * VEC, gy + base + vec * VEC, [&](const auto& rx, const auto& ry, auto rows) {
+          for_rows<T, VEC, VEC >= 4 ? 2 : 4, true>(m, t, t.row0 + t.ty, x + base + vec * VEC, gy + base + vec * VEC, [&](const auto& rx, const auto& ry, auto rows) {
 #pragma unroll
             for (int j = 0; j < decltype(rows)::value; ++j) {
               float v[VEC], g[VEC];
