@@ -199,8 +199,8 @@ int pdekan_deeponet_step(const PdekanNet* nets, const float* u1, const float* u2
  * next layer's knots (no counterpart in the reference).  x [n][s][channels] of `dtype`; the statistics of a group run
  * over the s positions and the channels / groups channels of one sample:
  *   z = (x - mean) / sqrt(var + eps) (biased variance),  y = f(weight[c] z + bias[c])
- * weight and bias are fp32 [channels] or NULL (1 and 0).  Sums and statistics are fp32 whatever dtype; y is rounded
- * once.  `stats` [n][groups][2] (mean, 1 / sqrt(var + eps)) is written by the forward where
+ * weight and bias are fp32 [channels] or NULL (1 and 0).  Sums and statistics are fp32 whatever dtype, 64-bit where a
+ * sample has many positions (mean within 2^-24 of itself, r within 3 2^-24); y is rounded once.  `stats` [n][groups][2] (mean, 1 / sqrt(var + eps)) is written by the forward where
  * pdekan_group_norm_stats_floats is not 0 (NULL: not wanted) and read by the backward.  Backward: gx, and gweight / gbias
  * (fp32, overwritten) summed over all samples in a fixed order; gweight and gbias may be NULL.
  * channels <= 8192.  ws: pdekan_group_norm_workspace_bytes (0 for some shapes: ws may be NULL then); 256-byte aligned.
@@ -231,7 +231,9 @@ int pdekan_group_norm_jet_backward(const float* x_jet, const float* gy_jet, int6
  *   steps times:  S = X X^T,  X <- c[0] X + (c[1] S + c[2] S S) X
  * out = X, so every singular value of g well above |g|_F c[0]^-steps is carried close to 1.  coefficients: 3 floats on
  * the HOST ((3.4445, -4.7750, 2.0315) are the usual ones); refused if they carry singular values of [0, 1] past 64.
- * Products have fp32 accuracy, the norm is summed in 64 bits; out is rounded to dtype once.  1 <= steps <= 100,
+ * Products are of two 11-bit pieces an operand, summed in fp32, the norm in 64 bits: fp32 results are within 0.6 to 1.5
+ * times the error of fp32 products.  Steps on large 16-bit matrices are composed, which leaves about 5e-6 of X before it is
+ * rounded to dtype, once.  1 <= steps <= 100,
  * eps >= 1e-30.  A stack of `batch` contiguous matrices [batch][rows][cols] counts as one entry; `out` may be `g`.  A matrix
  * that holds a NaN or an infinity becomes NaN, the others are not touched by it; one of zeros stays zero. */
 typedef struct PdekanMatrix {

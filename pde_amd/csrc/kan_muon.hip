@@ -6,7 +6,7 @@
 //
 // Products run on the fp16 matrix instructions with fp32 accuracy: an operand is two fp16 pieces, x = hi + lo (22 bits and a
 // sign, of values scaled so that nothing overflows), a product three matrix instructions, hi hi + hi lo + lo hi, summed in
-// fp32; what is left out is 2^-24 of a term.  Operands lie in memory in the order of the instruction's registers: a tile of
+// fp32; what is left out is 2^-24 of a term (matrices of at most 32 rows take lo lo too).  Operands lie in memory in the order of the instruction's registers: a tile of
 // 16 rows x 32 inner values is 1 KB of hi pieces and 1 KB of lo pieces, lane l's 8 values (row l % 16, inner values
 // 8 (l / 16) ..) at 16 l, so a wave loads one operand of one instruction as one contiguous 1 KB, and tiles that follow each
 // other along the inner dimension lie next to each other.
@@ -207,7 +207,8 @@ __device__ __forceinline__ float moved(float g, float& m, const Momentum& mo) {
   return mo.nesterov ? mo.rest * g + mo.mu * m : m;
 }
 
-// (2048 x 8192 bf16: 8.4 us, 4.0 TB/s; a step of KAN [2,256,256,256,1], 13 MB of gradients and momentum each: 9.4 us.)
+// (Times here and below: mean of 20 calls under the profiler, the best in brackets.  2048 x 8192 bf16: 10.4 us (9.8), 3.2 TB/s; a step
+// of KAN [2,256,256,256,1], 13 MB of gradients and momentum each: 10.8 (9.6).)
 // Partial sums of squares of U in 64 bits (the squares of gradients as small as 1e-25 vanish in 32), one a block, a block's
 // values contiguous, 16 bytes of G a thread; the optimiser's momentum is updated on the way.
 template <typename T>
@@ -332,8 +333,8 @@ __global__ void __launch_bounds__(kThreads) ns_vector_kernel(Items L, Momentum m
   vector_share<T>(I, here, mo, eps, k, steps, f);
 }
 
-// Bound by what it writes, two planes of pieces: 2048 x 8192 bf16, 33 MB in and 67 MB out, 25 us = 4.1 TB/s; 256 x 5888 fp32, 6 and
-// 12 MB, 8.3 us.
+// Bound by what it writes, two planes of pieces: 2048 x 8192 bf16, 33 MB in and 67 MB out, 28 us (27) = 3.6 TB/s; 256 x 5888 fp32, 6
+// and 12 MB, 11.3 (9.1).
 // X and X^T of a 64 x 64 tile as pieces, and the vectors of the list; COMPOSED: of U' in one piece (16-bit types: exact).
 template <typename T, bool COMPOSED>
 __global__ void __launch_bounds__(kThreads) ns_split_kernel(Items L, Momentum mo, float eps, Scales sc, NsCoefficients k, int steps,
@@ -434,9 +435,9 @@ __device__ __forceinline__ bool few_rows(const Item& I) { return I.mp == 32; }
 
 // What bounds a product: the LDS where a block is 64 (a stage of 16 KB is read 32 KB for 192 cycles of matrix instructions a wave),
 // the latency behind the L2 where it is 128, whose 80 KB hold two stages of two-piece operands.  Alone on the chip 2048 x 2048
-// squares (three matrix instructions a product, the upper triangle) run at 0.62 PFLOP/s of matrix instructions in blocks of 64, 41 us;
-// in blocks of 128, 57 us with four stages and one block a compute unit, more with two, the inner axis split over two to four
-// blocks included.  128 blocks that fill the chip reach 1.0 PFLOP/s (X <- Q X, 2048 x 8192); a large library product 1.2.
+// squares (three matrix instructions a product, the upper triangle) run at 0.60 PFLOP/s of matrix instructions in blocks of 64, 45 us
+// (41); in blocks of 128, 57 us with four stages and one block a compute unit, more with two, the inner axis split over two to four
+// blocks included.  128 blocks that fill the chip reach 1.06 PFLOP/s (X <- Q X, 2048 x 8192); a large library product 1.2.
 // P Q^T of a BT x BT block over inner tiles [k0, k1), PP and PQ pieces an operand.  Four waves take a quarter each: acc[a][c]
 // is the 16 x 16 block at rows 16 a of P and 16 c of Q; lane l holds Q's row l % 16 and P's rows 4 (l / 16) + r.
 // Operand tiles go from memory to LDS without passing registers, kStages inner tiles of the whole block in a ring, and
@@ -587,7 +588,8 @@ __device__ __forceinline__ int xcd_order(int local, int count) {
   return local < per * 8 ? (local % 8) * per + local / 8 : local;
 }
 
-// 2048 x 8192 bf16, one piece: 52 us, 0.70 PFLOP/s in 128 blocks of four splits; 256 x 5888 fp32: 5.4 us, 46 splits of 10 tiles.
+// 2048 x 8192 bf16 in 128 blocks of four splits: one piece 57 us (52), 0.64 PFLOP/s, two 127 (117), 0.86; 256 x 5888 fp32: 8.0 (5.6), 46
+// splits of 10 tiles.
 // S = X X^T: block = (split of the long axis, tile of the upper triangle)
 template <int BT, int PX>
 __global__ void __launch_bounds__(kThreads, BT == 64 ? 3 : 2) ns_gram_kernel(Items L, Scales sc, int step) {
@@ -647,7 +649,8 @@ __global__ void __launch_bounds__(GROUPS * kThreads) ns_gram_sum_kernel(Items L,
   store_symmetric(at<_Float16>(ws, off_sq(I, kS)), I.mp / 32, bi == bj, p0, q0, v, sc.s);
 }
 
-// 2048: 41 us, see Product; 256 (10 blocks): 5.3 us, of which 1.3 until the arguments are there, 2.8 for 8 inner tiles and 1.4 to store.
+// 2048: 45 us (41), see Product; 256 (10 blocks): 6.4 (5.2), of which 1.3 until the arguments are there, 2.8 for 8 inner tiles and 1.4 to
+// store.
 // Q = a I + b S + c S S  (a = 0: R, the step less its multiple of one)
 template <int BT>
 __global__ void __launch_bounds__(kThreads, BT == 64 ? 3 : 2) ns_poly_kernel(Items L, Scales sc, NsCoefficients k, int out) {
@@ -713,8 +716,8 @@ __device__ __forceinline__ void put4(const Item& I, int64_t e, const float (&x)[
   *out = v;
 }
 
-// 2048 x 8192 bf16 (128 blocks, three products a value in one and two pieces): 127 us, 1.08 PFLOP/s; 256 x 5888 fp32: 9.2 us, the latency
-// of arguments, eight inner tiles and stores, with 368 blocks in less than two rounds.
+// 2048 x 8192 bf16 in 128 blocks: of one piece (two matrix instructions a product) 149 us (139), 0.92 PFLOP/s, of two (three) 194 (184),
+// 1.06; 256 x 5888 fp32: 11.4 (9.6), the latency of arguments, eight inner tiles and stores, with 368 blocks in less than two rounds.
 // X <- a X + M X, computed as X^T <- a X^T + X^T M (M symmetric; a = 0: M holds all of the step): block = BT of the long axis x
 // BT of the short; the last one writes the result instead.  PX pieces in, two out.
 template <typename T, int BT, int PX, bool LAST>
@@ -848,7 +851,7 @@ __device__ __forceinline__ Start start_of(double squares, float eps, int e, bool
 
 // 16 x 16 block of P Q^T from tiles of two pieces in LDS: row of tiles `a` of P and `b` of Q, kt inner tiles a row.  `whole`: with
 // lo lo, which is of one sign on the diagonal of S.  In sums of few terms its 2^-24 shows: errors of five steps at 5 x 64 are
-// 1.2e-6 without it and with X apart from its pieces (see below), 0.8e-6 with both; fp32 products 0.7e-6.
+// 1.2e-6 without it and with X apart from its pieces (see below), 0.9e-6 with both; fp32 products 0.7e-6.
 __device__ __forceinline__ f32x4 block_product(const _Float16* P, const _Float16* Q, int a, int b, int kt, bool whole) {
   const int lane = threadIdx.x & 63;
   f32x4 lh = (f32x4){0.0f, 0.0f, 0.0f, 0.0f}, hl = lh, hh = lh;
@@ -1371,9 +1374,10 @@ struct Steps {
 
   // Up to three steps composed in the square matrices, then one product with X: with Q = a I + b S + c S S the step takes X to
   // Q X and S to Q S Q, and all of these commute.  Three products along the long axis for five steps instead of ten.
-  // Rounding errors of S in the small singular directions grow by a^2 a step, so three steps cost about a factor 4 in
-  // accuracy over fp32, far below the 2^-9 or 2^-12 of a 16-bit result, and a new S is formed after them.  X keeps two pieces
-  // between the segments: one (2^-12 of each value) would move one bf16 result in twenty to its neighbour.  2048 x 8192 bf16: 1110 us,
+  // Rounding errors of S in the small singular directions grow by a^2 a step, and Q and its products carry their multiple of one
+  // through the sums of the matrix instructions: X is 4e-6 (4 x 1000 x 771) to 6e-6 (2048 x 8192) off before it is rounded, against
+  // the 2^-9 or 2^-12 of a 16-bit result, and a new S is formed after three steps.  X keeps two pieces
+  // between the segments: one (2^-12 of each value) would move one bf16 result in twenty to its neighbour.  2048 x 8192 bf16: 1096 us,
   // 1007 with one.
   void composed() {
     for (int k = 0, part = 0; k < p.steps; ++part) {

@@ -1,6 +1,7 @@
 // Group norm followed by an activation, channels last: on plain values [n][s][C] in fp32, bf16 or fp16 (statistics of a
 // group run over the s positions and the C / groups channels of a sample) and on derivative jets [n][C][J] in fp32
-// (statistics per point).  Sums, statistics and every intermediate are fp32; a 16-bit tensor is rounded once, at the store.
+// (statistics per point).  Sums, statistics and every intermediate are fp32, sums over a sample's positions 64-bit beyond 32 rows (the
+// statistics' throughout); a 16-bit tensor is rounded once, at the store.
 //
 //   z = (x - mean) r,  r = (var + eps)^-1/2,  y = f(w z + b)
 //   backward: p = gy f',  gb = sum p,  gw = sum p z,  q = w p,  gx = r (q - mean(q) - z mean(q z))
@@ -61,7 +62,7 @@ __device__ __forceinline__ float group_sum(float v) {
 }
 
 // exp(S u), S = -1 or 2: 2^p with p = S u log2(e) rounded, for FULL (fp32 tensors) times what the rounding left out: |p| steps of
-// 2^-24, which results of 16 bits do not show (8 x 4096 x 320 bf16 SiLU, sums 23 us with and 19 without)
+// 2^-24, which results of 16 bits do not show (8 x 4096 x 320 bf16 SiLU, all four launches 70 us with and 64 without)
 template <int S, bool FULL>
 __device__ __forceinline__ float exp_times(float u) {
   constexpr float kHi = S * 1.44269502162933349609375f, kLo = S * 1.9259629911266e-8f;      // log2(e) in two parts
@@ -171,8 +172,8 @@ __device__ __forceinline__ void row_grad_out(const RowMap& m, const RowPlace& r,
 
 // Points (and samples of up to 512 values a group): a group in the registers of L lanes, so x (and gy) is read once and y (gx)
 // written once, with 16-byte accesses where the tensors allow them.  HBM bounds it.  2^19 x 256 fp32, groups of 32, tanh:
-// forward 195 us (1.07 GB, 5.5 TB/s), backward 358 us (1.61 GB, 4.5 TB/s); a large copy reaches 5.0 TB/s.  10000 x 64: 4.2 us of
-// launch and latency.
+// forward 212 us (best of 20: 193; 1.07 GB, 5.1 TB/s), backward 368 (360; 1.61 GB, 4.4 TB/s); bf16 135 and 199 (4.0 TB/s); a large copy
+// reaches 5.0 TB/s.  10000 x 64: 5.1 us of launch and latency.
 template <typename T, int VEC, int L, int K, bool BWD>
 __global__ void __launch_bounds__(kThreads) norm_rows_kernel(RowMap m, const T* __restrict__ x, const T* __restrict__ gy,
                                                              const float* __restrict__ w, const float* __restrict__ b,
@@ -293,8 +294,9 @@ __global__ void __launch_bounds__(kThreads) norm_rows_kernel(RowMap m, const T* 
 //   ge = r h + 2 e gV / M + sum_d (r' h' + r'' h'' + (f gA + s gB) / M),  gf = r h' + 2 r' h'' + (e gA + 2 f gB) / M,
 //   gs = r h'' + e gB / M, each less its mean over the group (the means of e, f, s vanish: only h's remain)
 // A lane holds a channel's whole jet (J = 4 or 12 floats, 16-byte accesses), a group sits in L lanes: the five sums of the
-// forward and the backward's cross the lanes in registers.  HBM bounds the 4-slot form: 2^19 x 64 x 4, forward 190 us (1.07 GB,
-// 5.6 TB/s), backward 360 us (1.61 GB, 4.5 TB/s); 12 slots: 30011 x 128 x 12, 77 us (369 MB, 4.8 TB/s) and 113 us (553 MB, 4.9 TB/s).
+// forward and the backward's cross the lanes in registers.  HBM bounds it: 2^19 x 64 x 4, forward 208 us (best of 20: 193;
+// 1.07 GB, 5.2 TB/s), backward 369 (361; 1.61 GB, 4.4 TB/s); 12 slots: 30011 x 128 x 12, 81 us (77; 369 MB, 4.6 TB/s) and 125 (113;
+// 553 MB, 4.4 TB/s).
 template <int ND, int NS, int L, int K, bool BWD>
 __global__ void __launch_bounds__(kThreads) norm_jet_kernel(RowMap m, const float* __restrict__ x,
                                                             const float* __restrict__ gy, const float* __restrict__ w,
@@ -537,7 +539,7 @@ __global__ void __launch_bounds__(1024) norm_finish_kernel(const float* __restri
 // ---- samples of many positions ------------------------------------------------------------------------------------
 
 // Four launches for forward and backward; each reads its rows with VEC channels a thread, 8 x 4096 x 320 bf16 (21 MB a tensor): statistics
-// 12 us, apply 14, sums 19, gradient 19.  A third of that is the arithmetic (SiLU and its slope: about 25 vector instructions a
+// 11.5 us, apply 15, sums 20, gradient 19.  A third of that is the arithmetic (SiLU and its slope: about 25 vector instructions a
 // value), the rest latency: chunks are short, and every block first reduces or merges.
 constexpr int kAhead = 4;              // rows a thread of the second launches loads before the sums are merged
 
@@ -1000,8 +1002,8 @@ __global__ void __launch_bounds__(kThreads) norm_grid_grad_kernel(GridMap m, con
 
 constexpr int kRowBlocks = 2048;       // 8 blocks of 4 waves a compute unit: all that fit, so that a block's channels stay with it
 // Two blocks a compute unit: each merges all chunks of its sample, which more blocks have more of, and fewer leave it idle.
-// Forward and backward of 8 x 4096 x 320 bf16 with 256, 384, 512, 768, 1024 blocks: 74, 70, 63, 80, 80 us; of 2 x 16384 x 512 with
-// at most 64, 128, 256 chunks a sample: 136, 86, 79 us.
+// All four launches of 8 x 4096 x 320 bf16 with 256, 384, 512, 768, 1024 blocks: 65, 69, 64, 78, 88 us, of 32 x 1024 x 640 102, 100, 91,
+// 103, 109; of 2 x 16384 x 512 with at most 64, 128, 256 chunks a sample: 128, 84, 83 us.
 constexpr int kGridBlocks = 512, kChunksMax = 256, kSamplesMax = 64;
 constexpr size_t kStaticLds = 8 * 1024, kLds = 160 * 1024;     // at least what the grid kernels declare themselves; all there is
 
