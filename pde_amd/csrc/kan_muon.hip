@@ -6,10 +6,10 @@
 //
 // Products run on the fp16 matrix instructions with fp32 accuracy: an operand is two fp16 pieces, x = hi + lo (22 bits and a
 // sign, of values scaled so that nothing overflows), a product three matrix instructions, hi hi + hi lo + lo hi, summed in
-// fp32; what is left out is 2^-24 of a term (matrices of at most 32 rows take lo lo too).  Operands lie in memory in the order of the instruction's registers: a tile of
-// 16 rows x 32 inner values is 1 KB of hi pieces and 1 KB of lo pieces, lane l's 8 values (row l % 16, inner values
-// 8 (l / 16) ..) at 16 l, so a wave loads one operand of one instruction as one contiguous 1 KB, and tiles that follow each
-// other along the inner dimension lie next to each other.
+// fp32; what is left out is 2^-24 of a term (matrices of at most 32 rows take lo lo too).  Operands lie in memory in the order of the
+// instruction's registers: a tile of 16 rows x 32 inner values is 1 KB of hi pieces and 1 KB of lo pieces, lane l's 8 values (row
+// l % 16, inner values 8 (l / 16) ..) at 16 l, so a wave loads one operand of one instruction as one contiguous 1 KB, and tiles that
+// follow each other along the inner dimension lie next to each other.
 #include <hip/hip_runtime.h>
 #include <climits>
 #include <cmath>
@@ -1216,13 +1216,14 @@ Item make_item(const NsMatrix& M) {
   constexpr int64_t kBigBlocks = 1 << 19;
   const int64_t big = (int64_t)((I.mp + 127) / 128) * ((I.np + 127) / 128) * I.batch;
   I.bt = I.m > 64 && I.mp * big >= kBigBlocks ? 128 : 64;
-  // Among squares only the upper triangle's blocks are computed: 128 x 128 ones where rows times those reach 600000.  In blocks of 64 and
-  // of 128: 2600 x 2600 bf16 1457 and 1243 us, 2900 x 2900 2113 and 1901, 4096 x 4096 5540 and 4286, 4 x 2048 x 2048 2477 and 2290,
-  // 2900 x 2900 fp32 1992 and 1941; below it 2300 x 2300 bf16 985 and 1032, 2 x 2048 x 2048 1310 and 1367, 8 x 1024 x 1024 742 and 812,
-  // 32 x 700 x 700 fp32 1223 and 1279.
+  // Among squares only the upper triangle's blocks are computed: 128 x 128 ones where rows times those reach 600000 and a matrix has four
+  // rows of them, of which the diagonal's are half wasted.  In blocks of 64 and of 128: 2600 x 2600 bf16 1457 and 1243 us, 4096 x 4096
+  // 5540 and 4286, 3 x 2048 x 2048 1841 and 1601, 40 x 1000 x 1000 3555 and 3041, 64 x 700 x 700 fp32 2315 and 2297; and otherwise:
+  // 2300 x 2300 bf16 985 and 1032, 2 x 2048 x 2048 1310 and 1367, 8 x 1024 x 1024 742 and 812, 32 x 700 x 700 fp32 1223 and 1279, 2000 x
+  // 129 x 129 2918 and 3118.
   constexpr int64_t kBigSquares = 600000;
   const int64_t t128 = (I.mp + 127) / 128, tri = t128 * (t128 + 1) / 2 * I.batch;
-  I.bts = I.mp * tri >= kBigSquares ? 128 : 64;
+  I.bts = t128 >= 4 && I.mp * tri >= kBigSquares ? 128 : 64;
   // splits of the long axis: two blocks a compute unit, at least four inner tiles each
   const int kt = I.np / 32, tiles = tri_tiles(I);
   int64_t chunks = (512 + (int64_t)tiles * I.batch - 1) / ((int64_t)tiles * I.batch);
@@ -1376,9 +1377,8 @@ struct Steps {
   // Q X and S to Q S Q, and all of these commute.  Three products along the long axis for five steps instead of ten.
   // Rounding errors of S in the small singular directions grow by a^2 a step, and Q and its products carry their multiple of one
   // through the sums of the matrix instructions: X is 4e-6 (4 x 1000 x 771) to 6e-6 (2048 x 8192) off before it is rounded, against
-  // the 2^-9 or 2^-12 of a 16-bit result, and a new S is formed after three steps.  X keeps two pieces
-  // between the segments: one (2^-12 of each value) would move one bf16 result in twenty to its neighbour.  2048 x 8192 bf16: 1096 us,
-  // 1007 with one.
+  // the 2^-9 or 2^-12 of a 16-bit result, and a new S is formed after three steps.  X keeps two pieces between the segments: one
+  // (2^-12 of each value) would move one bf16 result in twenty to its neighbour.  2048 x 8192 bf16: 1096 us, 1007 with one.
   void composed() {
     for (int k = 0, part = 0; k < p.steps; ++part) {
       const int start = k, n = p.steps - k < 3 ? p.steps - k : 3;
