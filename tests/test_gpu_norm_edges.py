@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from test_gpu_norm import _definition, _kind
+from test_gpu_norm import _definition, _kind, _repeats_match, _with_gradients
 
 pytestmark = pytest.mark.gpu
 
@@ -233,3 +233,25 @@ def test_captured_and_replayed(shape, groups):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(held, both(leaves)))
+
+
+def test_many_samples_beyond_32_bits():
+    """2^22 samples of 33 positions, 2^32 values and more, 64 samples a block of the backward's sums: a block of samples over and over
+    has the same bits everywhere, and its parameters' gradients as many times.
+
+    Those are sums of one sign: chains of 32 rows and of 64 samples, two roundings besides, the base's own alike: 2 (32 + 64 + 2)."""
+    from pde_amd import functional as K
+    gen = torch.Generator(device="cuda").manual_seed(12)
+    x = torch.randn(1 << 12, 33, 32, device="cuda", generator=gen).bfloat16()
+    gy = torch.rand(1 << 12, 33, 32, device="cuda", generator=gen).bfloat16()
+    w, b = torch.ones(32, device="cuda"), torch.zeros(32, device="cuda", requires_grad=True)
+    copies = (1 << 10) + 1
+    f = lambda t: K.group_norm_act(t, 2, w, b.detach(), 1e-5, K.ACT_TANH)
+    want = [t.clone() for t in _with_gradients(f, x, gy)]
+    got = _with_gradients(f, x.repeat(copies, 1, 1), gy.repeat(copies, 1, 1))
+    assert got[0].numel() > 1 << 32
+    assert all(_repeats_match(a, e) for a, e in zip(got, want))
+    del got
+    sums = [torch.autograd.grad(K.group_norm_act(x.repeat(c, 1, 1), 2, w, b), b, gy.repeat(c, 1, 1))[0].double() for c in (1, copies)]
+    assert torch.allclose(sums[1], copies * sums[0], rtol=2 * 98 * U, atol=0)
+    torch.cuda.empty_cache()
